@@ -46,6 +46,7 @@ extern "C" {
 /* ---- dtype / layout / flag codes --------------------------------------- */
 #define TL_F32 0
 #define TL_F16 1
+#define TL_E4M3 2 /* pages of a cache only: 8 bits a value, and a power of two to a row (tl_pages) */
 
 #define TL_X_ROW_MAJOR 0 /* X is [M][ldx], K contiguous (what the nn.Module callers pass)      */
 #define TL_X_K_MAJOR 1   /* X is [K][ldx], M contiguous (what the reference kernel itself reads, */
@@ -597,6 +598,84 @@ int tl_spmm_gated(const tl_layout_header* header, const void* blob_dev,
                   void* Y, int y_dtype, int64_t ldy, int y_layout,
                   const void* scale, int scale_dtype,
                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ======================================================================== */
+/* Serving from a paged cache: sequences of different lengths in one pass.  */
+/* ======================================================================== */
+
+/* The pages of one layer's keys and values.  Slot `s` of page `p` holds a token: key head h's head_dim values lie side by side at element
+ * p * page_stride + h * head_stride + s * slot_stride of k, and the values' at that of v.
+ *   dtype      TL_F16, or TL_E4M3: a value is code * 2^(exponent - 127), the codes finite numbers of sign, 4 bits of exponent (bias 7) and 3 of
+ *              fraction, the exponents one byte to a row, [pages][kv_heads][page_size] (NULL for TL_F16)
+ *   page_size  a power of two, 16 to 1024;  strides in elements, addresses and strides whole 16-byte pieces */
+typedef struct tl_pages {
+    void *k, *v;
+    void *k_exponents, *v_exponents;
+    int64_t page_stride, head_stride, slot_stride;
+    int64_t pages;
+    int32_t page_size, kv_heads, head_dim, dtype;
+} tl_pages;
+
+/* A ragged batch of sequences, on the device.  Sequence b's rows are starts[b] .. starts[b + 1] - 1 of the operands, the LAST n of its lengths[b]
+ * tokens; token j of it lies in slot j % page_size of page table[b * table_stride + j / page_size].  What the device finds wrong is never followed:
+ * a row of no sequence is left as it was, a page number that is no page's, or a length that the table does not hold, writes nothing and makes what
+ * reads it NaN. */
+typedef struct tl_page_batch {
+    const int32_t* table;    /* [seqs][table_stride], the first table_pages of each are read */
+    const int32_t* starts;   /* [seqs + 1], not falling */
+    const int32_t* lengths;  /* [seqs] */
+    int64_t table_stride;
+    int32_t table_pages, seqs;
+} tl_page_batch;
+
+/* Heads of queries and keys (and values, on their way into pages): element (token t, head h, value d) of x at t * x_token + h * x_head + d. */
+typedef struct tl_head_rows {
+    const void* x;
+    int64_t x_token, x_head;
+    void* y;                 /* where they go; NULL for keys and values that go into pages */
+    int64_t y_token, y_head;
+    const void* norm_weight; /* NULL, or [head_dim] of the rows' type: x * rsqrt(mean(x^2) + eps) * norm_weight first */
+    int32_t heads;
+} tl_head_rows;
+
+/* How heads are rotated: pair i < pairs of a head, its values (i, i + pairs) or, interleaved, (2 i, 2 i + 1), by the angle position * frequencies[i]
+ * (64 bits), cosine and sine times factor; values from 2 * pairs on are left alone.  pairs == 0: none. */
+typedef struct tl_rotation {
+    const double* frequencies;
+    const int64_t* positions; /* [tokens], or NULL with a batch: a token's index in its sequence */
+    int32_t pairs, interleaved;
+    float factor, eps;        /* eps: of the norms */
+} tl_rotation;
+
+/* RMSNorm of every head, where there is a weight, and the rotation of its first values, in one pass (TernaryLLM/TernaryAttn.py:91-93; the norms
+ * are what models do that keep queries and keys in range).  Held in fp32 from the input to the one rounding of the result.  dtype TL_F32 or TL_F16;
+ * q or k may have no heads; y may be x.  head_dim a multiple of 8 up to 512; addresses and strides whole 16-byte pieces. */
+int tl_rope_heads(const tl_head_rows* q, const tl_head_rows* k, int dtype, int64_t tokens, int head_dim, const tl_rotation* rotation, void* stream);
+
+/* tl_rope_heads whose keys go into the pages of their sequence, the values beside them (TernaryLLM/TernaryAttn.py:93-98).  k and v have
+ * pages->kv_heads heads, q may have none.  Pages of TL_E4M3: a row's exponent is the least integer e from -32 to 8 with max|x| <= 448 * 2^e
+ * (what is not a number left out), its codes x / 2^e rounded to the nearest (even), no larger than 448, or 240 for e = 8, so that each stands
+ * for a finite fp16 number. */
+int tl_rope_to_pages(const tl_head_rows* q, const tl_head_rows* k, const tl_head_rows* v, int dtype, int64_t tokens, const tl_rotation* rotation,
+                     const tl_pages* pages, const tl_page_batch* batch, void* stream);
+
+/* The keys and values of a batch's rows out of their pages, as `dtype` (TL_F32 or TL_F16): k_out, v_out at t * out_token + h * out_head.
+ * Either may be NULL. */
+int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, int64_t tokens, int dtype, void* k_out, void* v_out, int64_t out_token,
+                  int64_t out_head, void* stream);
+
+/* Causal softmax attention of a batch's rows over everything their sequences have in the pages (TernaryLLM/TernaryAttn.py:100-113 with the
+ * causal mask): row i of sequence b's n sees its tokens 0 .. lengths[b] - n + i; a row that sees none gives 0.  fp16 queries, head_dim 64, 128
+ * or 256, scores, softmax and sums in fp32, probabilities rounded to fp16 for the product with the values.  Query head h reads key head
+ * h / (heads / kv_heads).
+ *   q          element (t, h, 0) at t * q_token + h * q_head
+ *   most_rows  the most rows that a sequence has: it chooses the kernel, nothing else
+ *   out        [tokens][heads * head_dim]
+ *   workspace  device, 16-byte aligned, of tl_paged_attention_workspace bytes at least; calls that share it must not overlap
+ * Work is shared out on the device by the lengths that stand there, in equal parts whatever they are, parts of a row's keys among them. */
+int tl_paged_attention_workspace(int heads, const tl_pages* pages, int64_t most_rows, int64_t* bytes);
+int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
+                       const tl_page_batch* batch, int64_t most_rows, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ import numpy as np
 _DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_DIR, "libternary_spmm.so")
 
-TL_F32, TL_F16 = 0, 1
+TL_F32, TL_F16, TL_E4M3 = 0, 1, 2
 TL_X_ROW_MAJOR, TL_X_K_MAJOR = 0, 1
 TL_ACT_SILU_GATE = 1
 TL_PRODUCER_NONE, TL_PRODUCER_SILU_GATE, TL_PRODUCER_ADD_RMSNORM, TL_PRODUCER_RMSNORM, TL_PRODUCER_RMSNORM_SUMS = 0, 1, 2, 3, 4
@@ -31,6 +31,31 @@ class Chain(ctypes.Structure):
     _fields_ = [("residual", ctypes.c_void_p), ("residual_ld", ctypes.c_int64), ("next_norm_weight", ctypes.c_void_p),
                 ("image_out", ctypes.c_void_p), ("image_ld", ctypes.c_int64), ("squares_out", ctypes.c_void_p),
                 ("squares_in", ctypes.c_void_p), ("squares_blocks", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class Pages(ctypes.Structure):
+    """Mirror of tl_pages."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exponents", ctypes.c_void_p), ("v_exponents", ctypes.c_void_p),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class PageBatch(ctypes.Structure):
+    """Mirror of tl_page_batch."""
+    _fields_ = [("table", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("table_pages", ctypes.c_int32), ("seqs", ctypes.c_int32)]
+
+
+class HeadRows(ctypes.Structure):
+    """Mirror of tl_head_rows."""
+    _fields_ = [("x", ctypes.c_void_p), ("x_token", ctypes.c_int64), ("x_head", ctypes.c_int64), ("y", ctypes.c_void_p), ("y_token", ctypes.c_int64),
+                ("y_head", ctypes.c_int64), ("norm_weight", ctypes.c_void_p), ("heads", ctypes.c_int32)]
+
+
+class Rotation(ctypes.Structure):
+    """Mirror of tl_rotation."""
+    _fields_ = [("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("pairs", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("factor", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
 class LayoutHeader(ctypes.Structure):
@@ -53,6 +78,7 @@ assert ctypes.sizeof(LayoutHeader) == 256
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HDRP = ctypes.POINTER(LayoutHeader)
+_PAGESP, _BATCHP, _ROWSP, _ROTP = (ctypes.POINTER(t) for t in (Pages, PageBatch, HeadRows, Rotation))
 _VP = ctypes.c_void_p
 _INT = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -111,6 +137,11 @@ SIGNATURES = {
     "tl_add_rmsnorm": (_INT, [_VP, _VP, _VP, _INT, _I64, _INT, ctypes.c_float, _VP, _VP, _I64, _VP]),
     "tl_silu_mul": (_INT, [_VP, _INT, _I64, _INT, _VP, _I64, _VP]),
     "tl_silu_mul_pairs": (_INT, [_VP, _INT, _I64, _INT, _VP, _I64, _VP]),
+    "tl_rope_heads": (_INT, [_ROWSP, _ROWSP, _INT, _I64, _INT, _ROTP, _VP]),
+    "tl_rope_to_pages": (_INT, [_ROWSP, _ROWSP, _ROWSP, _INT, _I64, _ROTP, _PAGESP, _BATCHP, _VP]),
+    "tl_read_pages": (_INT, [_PAGESP, _BATCHP, _I64, _INT, _VP, _VP, _I64, _I64, _VP]),
+    "tl_paged_attention_workspace": (_INT, [_INT, _PAGESP, _I64, _I64P]),
+    "tl_paged_attention": (_INT, [_VP, _I64, _I64, _INT, _I64, _INT, _PAGESP, _BATCHP, _I64, ctypes.c_float, _VP, _VP, _I64, _VP]),
 }
 
 _lib = None

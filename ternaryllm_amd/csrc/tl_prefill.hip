@@ -79,16 +79,6 @@ struct PrefillAttn {
     float scale_log2;                          // 1 / sqrt(head_dim) * log2(e)
 };
 
-// f over the four lanes with the same number modulo 16, on the vector unit (16 x 512 of 16 heads took 48.4 us with shuffles, 47.6).
-template <typename F>
-__device__ __forceinline__ float with_other_rows(float v, F f)
-{
-    const auto near = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = f(__uint_as_float(near[0]), __uint_as_float(near[1]));
-    const auto far = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return f(__uint_as_float(far[0]), __uint_as_float(far[1]));
-}
-
 // Causal attention: query i of a batch row sees keys 0 .. i + (kv_len - q_len).  A workgroup of four waves owns 64 * QF
 // queries of one head, a wave QF fragments of 16; it walks the keys that its queries see in tiles of 64, one pass, with a
 // running maximum, sum and weighted sum in fp32 (rescaled when the maximum moves).

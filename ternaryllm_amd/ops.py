@@ -3,6 +3,8 @@
 torch is used for device memory and streams only; every product runs in libternary_spmm.so.
 """
 import ctypes
+import math
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
@@ -616,6 +618,204 @@ def prefill_attention(q, k, v, tables=None):
                                              sin.data_ptr() if sin is not None else None, _code(q.dtype, "q"), B, heads, k.shape[1], hd, S, k.shape[2],
                                              steps, out.data_ptr(), _stream_ptr(q.device))
     _lib.check(rc)
+    return out
+
+
+class Pages(NamedTuple):
+    """One layer's keys and values in pages: k, v [pages, kv_heads, page_size, head_dim], float16 (any strides of whole 16-byte pieces, the
+    same for both) or float8_e4m3fn with exponents, uint8 [pages, kv_heads, page_size]: a row's values are code * 2^(exponent - 127)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exponents: Optional[torch.Tensor] = None
+    v_exponents: Optional[torch.Tensor] = None
+
+
+class PageBatch(NamedTuple):
+    """Sequences of different lengths in one pass.  Sequence b's rows are starts[b] .. starts[b + 1] - 1 of the operands, the last ones of its
+    lengths[b] tokens; token j of it lies in page table[b, j // page_size].  All int32 on the device: table [seqs, pages of the longest], starts
+    [seqs + 1], lengths [seqs].  most_rows: the most rows that one sequence has, as far as the host knows (it chooses the attention's kernel,
+    results do not depend on it).  Rows of no sequence -- behind the last, before the first -- are left as they are."""
+    table: torch.Tensor
+    starts: torch.Tensor
+    lengths: torch.Tensor
+    most_rows: int
+
+
+_PAGE_CODE = {torch.float16: _lib.TL_F16, torch.float8_e4m3fn: _lib.TL_E4M3}
+
+
+def _page_args(pages, batch, device):
+    """The library's structures for pages and batch, which must lie on `device`."""
+    k, v, ke, ve = pages
+    if k.dim() != 4 or k.shape != v.shape or k.dtype not in _PAGE_CODE or v.dtype != k.dtype or k.stride() != v.stride() or k.stride(3) != 1:
+        raise ValueError("pages must be [pages, kv_heads, page_size, head_dim], float16 or float8_e4m3fn, keys and values alike")
+    if (ke is None) != (k.dtype == torch.float16) or (ve is None) != (ke is None):
+        raise ValueError("pages of float8_e4m3fn have exponents, others have none")
+    for t in (k, v) if ke is None else (k, v, ke, ve):
+        if t.device != device:
+            raise RuntimeError(f"the pages are on {t.device}, the rows on {device}")
+    for t in () if ke is None else (ke, ve):
+        if t.shape != k.shape[:3] or t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError("exponents must be contiguous uint8 [pages, kv_heads, page_size]")
+    for t, dims, what in ((batch.table, 2, "table"), (batch.starts, 1, "starts"), (batch.lengths, 1, "lengths")):
+        if t.dim() != dims or t.dtype != torch.int32 or (t.numel() > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{what} must be an int32 tensor of {dims} dimension(s)")
+        if t.device != device:
+            raise RuntimeError(f"{what} is on {t.device}, the rows on {device}")
+    seqs, columns = batch.table.shape
+    if batch.starts.numel() != seqs + 1 or batch.lengths.numel() != seqs:
+        raise ValueError("starts has one entry more than the table has rows, lengths as many")
+    # (a dimension of one entry has no stride of its own: whatever torch says, any will do)
+    steps = [t if n > 1 else k.shape[2] * k.shape[3] for t, n in zip(k.stride()[:3], k.shape[:3])]
+    p = _lib.Pages(k.data_ptr(), v.data_ptr(), *((None, None) if ke is None else (ke.data_ptr(), ve.data_ptr())), *steps, k.shape[0],
+                   k.shape[2], k.shape[1], k.shape[3], _PAGE_CODE[k.dtype])
+    return p, _lib.PageBatch(batch.table.data_ptr() or None, batch.starts.data_ptr(), batch.lengths.data_ptr() or None,
+                             batch.table.stride(0) if seqs > 1 else columns, columns, seqs)
+
+
+def _overlap(x, y):
+    """Whether [tokens, heads, head_dim] tensors x and y share memory (views of one row after the other, such as parts of one product's
+    rows, do not)."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    (x0, xr, xs), (y0, yr, ys) = ((t.data_ptr(), (1 + (t.shape[1] - 1) * _steps(t, (1,))[0] + t.shape[2] - 1) * t.element_size(),
+                                   _steps(t, (0,))[0] * t.element_size()) for t in (x, y))
+    if x0 >= y0 + (y.shape[0] - 1) * ys + yr or y0 >= x0 + (x.shape[0] - 1) * xs + xr:
+        return False
+    return not (xs == ys >= max(xr, yr) and xr <= (y0 - x0) % xs <= xs - yr)
+
+
+def _same_place(x, y):
+    return x.data_ptr() == y.data_ptr() and x.shape == y.shape and _steps(x, (0, 1)) == _steps(y, (0, 1))
+
+
+def _head_rows(x, y, norm, what, others=()):
+    """tl_head_rows of x [tokens, heads, head_dim] and where it goes: to itself, or apart from it and the other operands."""
+    if x.dim() != 3 or (x.stride(2) != 1 and x.shape[2] > 1):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with unit last stride")
+    if norm is not None and (norm.shape != x.shape[2:] or norm.dtype != x.dtype or norm.device != x.device or not norm.is_contiguous()):
+        raise ValueError(f"the norm's weight of {what} must be a contiguous [head_dim] tensor of its type and device")
+    if y is not None:
+        if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(2) != 1:
+            raise ValueError(f"the output of {what} must be of its shape, type and device, with unit last stride")
+        if (not _same_place(x, y) and _overlap(x, y)) or any(_overlap(t, y) for t in others):
+            raise ValueError(f"the output of {what} must be {what} itself or lie apart from the operands")
+    return _lib.HeadRows(x.data_ptr(), *_steps(x, (0, 1)), None if y is None else y.data_ptr(), *((0, 0) if y is None else _steps(y, (0, 1))),
+                         None if norm is None else norm.data_ptr(), x.shape[1])
+
+
+def _rotation(frequencies, positions, tokens, factor, interleaved, eps, like):
+    if frequencies is None:
+        return _lib.Rotation(None, None, 0, 0, 1.0, float(eps))
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or frequencies.device != like.device or not frequencies.is_contiguous():
+        raise ValueError("frequencies must be a contiguous float64 tensor of one dimension on the rows' device")
+    if positions is not None and (positions.shape != (tokens,) or positions.dtype != torch.int64 or positions.device != like.device or not positions.is_contiguous()):
+        raise ValueError("positions must be a contiguous int64 [tokens] tensor on the rows' device")
+    return _lib.Rotation(frequencies.data_ptr(), None if positions is None else positions.data_ptr(), frequencies.numel(), int(bool(interleaved)),
+                         float(factor), float(eps))
+
+
+def _cuda(x, what):
+    if x.device.type != "cuda":
+        raise RuntimeError(f"{what} is on {x.device}: the kernels run on a GPU only")
+
+
+def rope_heads(q, k, positions, frequencies, *, factor=1.0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
+    """Queries and keys [tokens, heads, head_dim], each head normalised (RMSNorm by the weights q_norm, k_norm [head_dim], where there are) and
+    its first 2 * len(frequencies) values rotated: by positions[token] * frequencies[i] the pair (i, i + len(frequencies)), or, interleaved,
+    (2 i, 2 i + 1); cosine and sine are multiplied by factor (attention.rope_frequencies gives both for a model's scaling).  positions: int64
+    [tokens]; frequencies: float64 on the device, None: no rotation.  k may be None.  Returns (q, k) rotated, new tensors or q_out, k_out,
+    which may be q and k themselves.  float16 or float32, head_dim a multiple of 8, strides of whole 16-byte pieces."""
+    if k is not None and (k.dim() != 3 or k.shape[::2] != q.shape[::2] or k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("k must have q's tokens, head_dim, type and device")
+    if frequencies is not None and positions is None:
+        raise ValueError("a rotation needs positions")
+    code = _code(q.dtype, "q")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    rows = [_head_rows(q, q_out, q_norm, "q", () if k is None else (k,))]
+    if k is not None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        rows.append(_head_rows(k, k_out, k_norm, "k", (q, q_out)))
+    rotation = _rotation(frequencies, positions, q.shape[0], factor, interleaved, eps, q)
+    _cuda(q, "q")
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().tl_rope_heads(rows[0], rows[1] if k is not None else None, code, q.shape[0], q.shape[2], rotation, _stream_ptr(q.device)))
+    return q_out, (k_out if k is not None else None)
+
+
+def rope_to_pages(q, k, v, pages, batch, frequencies=None, positions=None, *, factor=1.0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6,
+                  q_out=None):
+    """rope_heads for the rows of a batch, the keys going into the pages of their sequences with the values v [tokens, kv_heads, head_dim] beside
+    them.  positions None: each row's index in its sequence.  q may be None.  Returns the rotated queries.  Pages of float8_e4m3fn: a row's
+    exponent is the least that keeps it within 448, its codes are rounded to the nearest; they saturate at the largest value that is a finite
+    float16."""
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one type and device")
+    if q is not None and (q.dim() != 3 or q.shape[::2] != k.shape[::2] or q.dtype != k.dtype or q.device != k.device):
+        raise ValueError("q must have k's tokens, head_dim, type and device")
+    if pages.k.dim() != 4 or pages.k.shape[1::2] != k.shape[1:]:
+        raise ValueError("the pages must have k's heads and head_dim")
+    code = _code(k.dtype, "k")
+    p, b = _page_args(pages, batch, k.device)
+    first = None
+    if q is not None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        first = _head_rows(q, q_out, q_norm, "q", (k, v))
+    rows = _head_rows(k, None, k_norm, "k"), _head_rows(v, None, None, "v")
+    rotation = _rotation(frequencies, positions, k.shape[0], factor, interleaved, eps, k)
+    _cuda(k, "k")
+    with torch.cuda.device(k.device):
+        _lib.check(_lib.lib().tl_rope_to_pages(first, *rows, code, k.shape[0], rotation, p, b, _stream_ptr(k.device)))
+    return q_out if q is not None else None
+
+
+def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=None):
+    """The keys and values of a batch's `tokens` rows out of the pages, [tokens, kv_heads, head_dim] each, float16 (which every 8-bit row fits
+    exactly) or float32: new tensors (rows of no sequence are not written there either), or k_out and v_out of the same strides.  A row whose
+    page is none is NaN."""
+    if pages.k.dim() != 4:
+        raise ValueError("pages must be [pages, kv_heads, page_size, head_dim]")
+    device, (_, heads, _, hd) = pages.k.device, pages.k.shape
+    p, b = _page_args(pages, batch, device)
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out go together")
+    if k_out is None:
+        k_out, v_out = torch.empty((2, tokens, heads, hd), dtype=dtype, device=device).unbind(0)
+    for t in (k_out, v_out):
+        if t.shape != (tokens, heads, hd) or t.device != device or t.stride(2) != 1 or t.dtype != k_out.dtype or _steps(t, (0, 1)) != _steps(k_out, (0, 1)):
+            raise ValueError("k_out and v_out must be [tokens, kv_heads, head_dim] of one type, of the same strides, on the pages' device")
+    code = _code(k_out.dtype, "the output")
+    _cuda(pages.k, "pages")
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().tl_read_pages(p, b, tokens, code, k_out.data_ptr(), v_out.data_ptr(), *_steps(k_out, (0, 1)), _stream_ptr(device)))
+    return k_out, v_out
+
+
+def paged_attention(q, pages, batch, *, scale=None, out=None):
+    """Causal attention of a batch's rows q [tokens, heads, head_dim] over everything their sequences have in the pages (their own keys and values
+    among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
+    rows of no sequence are not written, a row that sees nothing is 0, rows of a sequence with a page that is none are NaN.  float16, head_dim 64,
+    128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim)."""
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
+    tokens, heads, hd = q.shape
+    if pages.k.dim() != 4 or pages.k.shape[3] != hd:
+        raise ValueError("the pages must have q's head_dim")
+    code = _code(q.dtype, "q")
+    p, b = _page_args(pages, batch, q.device)
+    if out is None:
+        out = torch.empty((tokens, heads * hd), dtype=q.dtype, device=q.device)
+    elif out.shape != (tokens, heads * hd) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [tokens, heads * head_dim] tensor of q's type and device")
+    _cuda(q, "q")
+    need = ctypes.c_int64(0)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().tl_paged_attention_workspace(heads, p, batch.most_rows, ctypes.byref(need)))
+        # (of the call's own: kept for the next, it would be shared by graphs that were captured on one stream and are replayed on several)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        _lib.check(_lib.lib().tl_paged_attention(q.data_ptr(), *_steps(q, (0, 1)), code, tokens, heads, p, b, batch.most_rows,
+                                                 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                 _stream_ptr(q.device)))
     return out
 
 

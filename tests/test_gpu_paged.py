@@ -1,0 +1,306 @@
+"""The operators of a paged cache against float64 on the CPU (tests/paged.py): sizes at the edges of pages, tiles, fragments and parts."""
+import math
+
+import pytest
+import torch
+
+from ternaryllm_amd import ops
+
+from tests import paged
+
+pytestmark = pytest.mark.gpu
+
+
+def frequencies(pairs, theta=10000.0):
+    return theta ** (-torch.arange(pairs, dtype=torch.float64) / max(pairs, 1))
+
+
+def random(shape, seed, dtype=torch.float16):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def fresh_pages(seqs, kv, hd, kind, seed=0, spoiled=True):
+    """Pages on the CPU of random rows; where no sequence has a row, values that are not finite."""
+    shape = (seqs.pages, kv, seqs.page_size, hd)
+    k, v = random(shape, seed + 1), random(shape, seed + 2)
+    ke = ve = None
+    if kind == "e4m3":
+        k, v = ((100 * t.float()).clamp(-448, 448).to(torch.float8_e4m3fn) for t in (k, v))
+        ke, ve = (torch.randint(118, 123, shape[:3], generator=torch.Generator().manual_seed(seed + i), dtype=torch.uint8) for i in (3, 4))
+    if spoiled:
+        used = torch.zeros(shape[0], shape[2], dtype=torch.bool)
+        for b, (_, length) in enumerate(seqs.both):
+            for j in range(length):
+                used[int(seqs.table[b, j // seqs.page_size]), j % seqs.page_size] = True
+        for t, bad in ((k, math.nan), (v, math.inf if kind != "e4m3" else math.nan)):
+            where = (~used)[:, None, :, None].expand(shape)
+            if kind == "e4m3":
+                t.view(torch.uint8)[where] = 0x7f
+            else:
+                t[where] = bad
+    return ops.Pages(k, v, ke, ve)
+
+
+def on_gpu(pages):
+    return ops.Pages(*(None if t is None else t.cuda() for t in pages))
+
+
+# ---------------------------------------------------------------- rotated heads
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,kv,hd,pairs,norm", [
+    (1, 1, 1, 8, 4, True), (1, 32, 32, 128, 64, False), (3, 5, 1, 64, 32, True), (7, 12, 4, 96, 20, True), (5, 3, 3, 80, 5, False), (2, 64, 8, 128, 64, True),
+    (2, 2, 1, 256, 1, True), (2, 3, 2, 512, 256, True), (3, 2, 2, 192, 0, True), (65, 9, 3, 128, 31, True)])
+def test_rope_heads(dtype, interleaved, tokens, heads, kv, hd, pairs, norm):
+    qkv = random((tokens, heads + 2 * kv, hd), tokens * hd + pairs, dtype)
+    q, k = qkv[:, :heads], qkv[:, heads:heads + kv]
+    weights = [1 + 0.2 * random((hd,), 7 + i, torch.float32) for i in range(2)] if norm else [None, None]
+    weights = [None if w is None else w.to(dtype) for w in weights]
+    positions = torch.randint(0, 1 << 20, (tokens,), generator=torch.Generator().manual_seed(pairs))
+    positions[0] = 0 if tokens == 1 else 1048575
+    f, factor, eps = frequencies(pairs), 1.25, 1e-5
+    dev = qkv.cuda()
+    dq, dk = dev[:, :heads], dev[:, heads:heads + kv]
+    on = [None if w is None else w.cuda() for w in weights]
+    how = dict(factor=factor, interleaved=interleaved, q_norm=on[0], k_norm=on[1], eps=eps)
+    got = ops.rope_heads(dq, dk, positions.cuda(), f.cuda(), **how)
+    for x, w, y in zip((q, k), weights, got):
+        x = paged.normed(x, w, eps)
+        want = paged.rotated(x, positions, f, interleaved, factor)
+        assert y.dtype == dtype and y.is_contiguous()
+        assert ((y.cpu().double() - want).abs() <= paged.rope_bound(x, paged.partners(x, pairs, interleaved), max(1.0, factor), dtype, want)).all()
+    # the same bits in place, and of one operand alone
+    alone = ops.rope_heads(dq, None, positions.cuda(), f.cuda(), **how)
+    assert alone[1] is None and torch.equal(alone[0], got[0])
+    ops.rope_heads(dq, dk, positions.cuda(), f.cuda(), q_out=dq, k_out=dk, **how)
+    assert torch.equal(dq, got[0]) and torch.equal(dk, got[1]) and torch.equal(dev[:, heads + kv:].cpu(), qkv[:, heads + kv:])
+
+
+def test_rope_heads_without_tokens():
+    q, k = ops.rope_heads(torch.zeros((0, 4, 64), device="cuda"), torch.zeros((0, 2, 64), device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"),
+                          frequencies(32).cuda())
+    assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
+
+
+def test_rope_heads_keeps_what_is_not_finite_in_its_own_head():
+    q = torch.randn((3, 4, 64)).half()
+    q[1, 2, 5], q[2, 0, 3] = math.nan, math.inf
+    y, _ = ops.rope_heads(q.cuda(), None, torch.arange(3, device="cuda"), frequencies(32).cuda(), q_norm=torch.ones(64).half().cuda())
+    bad = ~torch.isfinite(y.cpu())
+    assert bad[1, 2].any() and bad[2, 0].any()
+    bad[1, 2] = bad[2, 0] = False
+    assert not bad.any()
+
+
+# ---------------------------------------------------------------- into pages and back
+BATCHES = [
+    ([(1, 1)], 16), ([(1, 17)], 16), ([(3, 3), (0, 5), (1, 40), (16, 16), (17, 33)], 16), ([(2, 130), (0, 0), (5, 64)], 64), ([(40, 40), (1, 257)], 256),
+    ([(5, 3), (2, 2)], 32)]  # (the last: more rows than tokens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("both,page", BATCHES)
+@pytest.mark.parametrize("heads,kv,hd,pairs,interleaved,norm", [(4, 2, 128, 64, False, True), (3, 3, 64, 32, True, False), (2, 1, 256, 24, False, True), (1, 1, 80, 3, False, False)])
+def test_rope_to_pages_and_back(dtype, kind, both, page, heads, kv, hd, pairs, interleaved, norm):
+    seqs = paged.Sequences(both, page, front=2, behind=3, seed=len(both))
+    q, k, v = random((seqs.tokens, heads + 2 * kv, hd), hd + page, dtype).split((heads, kv, kv), dim=1)
+    v = (v * torch.exp2(torch.arange(seqs.tokens)[:, None, None] % 9 - 4.0)).to(dtype)
+    weight = (1 + 0.2 * random((hd,), 5, torch.float32)).to(dtype) if norm else None
+    f = frequencies(pairs)
+    pages = on_gpu(fresh_pages(seqs, kv, hd, kind, seed=3, spoiled=False))
+    before = ops.Pages(*(None if t is None else t.clone() for t in pages))
+    q_out = torch.full((seqs.tokens, heads, hd), 7.0, dtype=dtype, device="cuda")
+    on = None if weight is None else weight.cuda()
+    how = dict(interleaved=interleaved, q_norm=on, k_norm=on)
+    batch = seqs.batch(ops)
+    got = ops.rope_to_pages(q.cuda(), k.cuda(), v.cuda(), pages, batch, f.cuda(), q_out=q_out, **how)
+    assert got is q_out
+    positions = torch.zeros(seqs.tokens, dtype=torch.int64)
+    inside = torch.zeros(seqs.tokens, dtype=torch.bool)
+    for b, (n, length) in enumerate(both):
+        first = int(seqs.starts[b])
+        positions[first:first + n] = torch.arange(length - n, length)
+        inside[first:first + n] = True
+    xq, xk = (paged.normed(t, weight, 1e-6) for t in (q, k))
+    want_q, want_k = (paged.rotated(t, positions, f, interleaved, 1.0) for t in (xq, xk))
+    q_bound = paged.rope_bound(xq, paged.partners(xq, pairs, interleaved), 1.0, dtype, want_q)
+    assert ((q_out.cpu().double() - want_q).abs() <= q_bound)[inside].all() and (q_out[~inside.cuda()] == 7).all()
+    # what the pages hold: the rows that have a place, and everything else as it was
+    held = paged.values(pages.k.cpu(), None if pages.k_exponents is None else pages.k_exponents.cpu()), \
+        paged.values(pages.v.cpu(), None if pages.v_exponents is None else pages.v_exponents.cpu())
+    slack = paged.rope_bound(xk, paged.partners(xk, pairs, interleaved), 1.0, torch.float32, want_k)
+    touched = torch.zeros((seqs.pages, page), dtype=torch.bool)
+    for row, b, at, number, slot in seqs.rows():
+        touched[number, slot] = True
+        if kind == "float16":
+            assert ((held[0][number, :, slot] - want_k[row]).abs() <= slack[row] + 2.0 ** -11 * want_k[row].abs()).all()
+            assert torch.equal(held[1][number, :, slot], v[row].half().double())
+        else:
+            # a value is off by half a step of three bits, or of the row's smallest: 2^-4 of it, 2^-10 of the power of two
+            grain = 2.0 ** (paged.exponents_of(want_k[row])[:, None] - 10)
+            assert ((held[0][number, :, slot] - want_k[row]).abs() <= torch.maximum(want_k[row].abs() * 2.0 ** -4, 2 * grain) + slack[row]).all()
+            assert torch.equal(held[1][number, :, slot], paged.byte_values(v[row].double()))
+    for now, then in zip(pages, before):
+        if now is not None:
+            now, then = (t.cpu().view(torch.uint8).transpose(1, 2) for t in (now, then))
+            assert torch.equal(now[~touched], then[~touched])
+    # and read back, into new tensors and into a cache of another layout
+    for out in (torch.float16, torch.float32):
+        back = [torch.full((kv, seqs.tokens, hd), 5.0, dtype=out, device="cuda").transpose(0, 1) for _ in range(2)]
+        ops.read_pages(pages, batch, seqs.tokens, k_out=back[0], v_out=back[1])
+        fresh = ops.read_pages(pages, batch, seqs.tokens, out)
+        rows = {row for row, *_ in seqs.rows()}
+        for row in range(seqs.tokens):
+            if not inside[row]:
+                assert (back[0][row] == 5).all() and (back[1][row] == 5).all()
+            elif row not in rows:
+                assert torch.isnan(back[0][row]).all() and torch.isnan(back[1][row]).all()
+        for row, b, at, number, slot in seqs.rows():
+            for t, n, h in zip(back, fresh, held):
+                assert torch.equal(t[row].cpu(), h[number, :, slot].to(out)) and torch.equal(n[row], t[row])
+
+
+@pytest.mark.parametrize("positions", [None, "given"])
+def test_rope_to_pages_without_queries_and_with_positions(positions):
+    seqs = paged.Sequences([(4, 9)], 16)
+    k, v = random((4, 2, 64), 1), random((4, 2, 64), 2)
+    where = None if positions is None else torch.tensor([5, 900000, 0, 17])
+    pages = on_gpu(fresh_pages(seqs, 2, 64, "float16", spoiled=False))
+    assert ops.rope_to_pages(None, k.cuda(), v.cuda(), pages, seqs.batch(ops), frequencies(32).cuda(), None if where is None else where.cuda()) is None
+    at = torch.arange(5, 9) if where is None else where
+    alone, _ = ops.rope_heads(k.cuda(), None, at.cuda(), frequencies(32).cuda())
+    back = ops.read_pages(pages, seqs.batch(ops), 4)
+    assert torch.equal(back[0], alone) and torch.equal(back[1].cpu(), v)
+
+
+def test_bytes_at_the_ends_of_their_range():
+    """Rows of zeros, of the smallest and largest numbers, of infinities and NaN."""
+    rows = torch.zeros((9, 1, 64), dtype=torch.float32)
+    rows[1, 0, 3] = 1e-30
+    rows[2] = torch.linspace(-65504, 65504, 64)
+    rows[3, 0, :3] = torch.tensor([math.inf, -math.inf, 1.0])
+    rows[4, 0, :2] = torch.tensor([math.nan, 3.0])
+    rows[5, 0, :4] = torch.tensor([448.0, 447.0, -8.5, 0.0146484375])
+    rows[6, 0, :2] = torch.tensor([448.0001, 1.0])
+    rows[7] = 6e-8
+    rows[8, 0, :2] = torch.tensor([3e38, -70000.0])
+    seqs = paged.Sequences([(9, 9)], 16)
+    pages = on_gpu(fresh_pages(seqs, 1, 64, "e4m3", spoiled=False))
+    ops.rope_to_pages(None, rows.cuda(), rows.cuda(), pages, seqs.batch(ops))
+    want = paged.byte_values(rows.double())
+    for got in ops.read_pages(pages, seqs.batch(ops), 9, torch.float32):
+        assert torch.equal(torch.nan_to_num(got.cpu().double(), nan=-1.0), torch.nan_to_num(want, nan=-1.0))
+        assert torch.isfinite(got[:4]).all() and torch.isnan(got[4, 0, 0]) and got[4, 0, 1] == 3
+    for got in ops.read_pages(pages, seqs.batch(ops), 9):   # every value is a finite fp16 number
+        assert torch.isfinite(got[[0, 1, 2, 3, 5, 6, 7, 8]]).all()
+
+
+# ---------------------------------------------------------------- attention
+def attention_bound(q, k, v, want, longest, scale):
+    """Probabilities are rounded to 11 bits (2^-11 of the largest value, and 2^-25 a key below fp16's normal range), the result once more; a score
+    is a sum of head_dim exact products in fp32, off by head_dim * 2^-24 of the largest sum of magnitudes, which the softmax takes twice; the
+    exponentials, their sum and the rescaling of sums have a few steps of fp32 each."""
+    k, v = (torch.nan_to_num(t, nan=0.0, posinf=0.0, neginf=0.0) for t in (k, v))
+    score = 2 * scale * q.shape[-1] * 2.0 ** -24 * (q.double().norm(dim=-1).max() * k.norm(dim=-1).max())
+    return (2.0 ** -11 + longest * 2.0 ** -25 + score + 64 * 2.0 ** -24) * v.abs().max() + 2.0 ** -11 * want.abs() + 2.0 ** -25
+
+
+def check_attention(both, heads, kv, hd, page, kind, *, front=0, behind=0, most=None, scale=None, seed=1):
+    seqs = paged.Sequences(both, page, front=front, behind=behind, seed=seed)
+    pages = fresh_pages(seqs, kv, hd, kind, seed=seed)
+    q = random((seqs.tokens, heads + 3, hd), seed + 9)[:, 1:1 + heads]
+    out = torch.full((seqs.tokens, heads * hd), 3.0, dtype=torch.float16, device="cuda")
+    wide = random((seqs.tokens, heads + 3, hd), seed + 9).cuda()
+    ops.paged_attention(wide[:, 1:1 + heads], on_gpu(pages), seqs.batch(ops, most=most), scale=scale, out=out)
+    got = out.cpu().view(seqs.tokens, heads, hd)
+    s = 1 / math.sqrt(hd) if scale is None else scale
+    k, v = paged.values(pages.k, pages.k_exponents), paged.values(pages.v, pages.v_exponents)
+    want = paged.attention(q, k, v, seqs, s)
+    inside = torch.zeros(seqs.tokens, dtype=torch.bool)
+    inside[front:seqs.tokens - behind if behind else None] = True
+    assert (got[~inside] == 3).all()
+    bound = attention_bound(q, k, v, want, max(length for _, length in both), s)
+    assert ((got.double() - want).abs() <= bound)[inside].all()
+
+
+SHAPES = [(1, 1, 128), (8, 2, 128), (14, 2, 64), (4, 4, 256), (3, 1, 64), (40, 2, 128), (5, 5, 64)]
+
+
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("both,page", [
+    ([(1, 1)], 16), ([(1, 15), (1, 16), (1, 17)], 16), ([(1, 700), (1, 63), (1, 64), (1, 65), (0, 30), (1, 1)], 32), ([(1, 1300)], 256)])
+def test_one_row_of_each_sequence(kind, heads, kv, hd, both, page):
+    check_attention(both, heads, kv, hd, page, kind)
+
+
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("both,page", [
+    ([(2, 2)], 16), ([(5, 130), (16, 16), (0, 0), (1, 90), (17, 63)], 16), ([(64, 64), (65, 400)], 64), ([(130, 131), (1, 257), (3, 3)], 128)])
+def test_chunks(kind, heads, kv, hd, both, page):
+    check_attention(both, heads, kv, hd, page, kind, front=1, behind=2)
+
+
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_rows_that_see_nothing(kind, hd):
+    """More rows than tokens: the first see nothing and are 0."""
+    check_attention([(5, 2), (3, 0), (70, 66), (2, 2)], 2, 1, hd, 16, kind)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (2, 2, 64), (4, 1, 256)])
+def test_a_long_sequence_is_shared_out(heads, kv, hd):
+    check_attention([(1, 9000), (1, 100), (3, 5000)], heads, kv, hd, 64, "float16")
+
+
+def test_many_sequences():
+    both = [(i % 3, (i * 37) % 90 + 2) for i in range(1500)]
+    check_attention(both, 2, 1, 64, 16, "float16")
+
+
+@pytest.mark.parametrize("most", [0, 1, 3, 100])
+def test_the_hint_changes_no_result(most):
+    check_attention([(3, 200), (1, 80), (40, 300)], 8, 2, 128, 16, "float16", most=most)
+
+
+def test_scale():
+    check_attention([(3, 200), (1, 80)], 8, 2, 128, 16, "float16", scale=0.3)
+    check_attention([(3, 200), (1, 80)], 8, 2, 128, 16, "e4m3", scale=1e-3)
+
+
+@pytest.mark.parametrize("most", [1, 70])
+def test_pages_and_lengths_that_are_none(most):
+    """A page number out of range, or a length that the table does not hold: the sequence is NaN, nothing else is touched."""
+    seqs = paged.Sequences([(1, 300), (1, 40), (2, 300)], 16)
+    pages = on_gpu(fresh_pages(seqs, 2, 64, "float16"))
+    q = random((4, 4, 64), 3).cuda()
+    good = ops.paged_attention(q, pages, seqs.batch(ops, most=most))
+    for number in (-1, seqs.pages, 1 << 30):
+        batch = seqs.batch(ops, most=most)
+        batch.table[2, 11] = number
+        got = ops.paged_attention(q, pages, batch)
+        assert torch.equal(got[:2], good[:2]) and torch.isnan(got[2:]).all()
+        k, v = random((4, 2, 64), 5).cuda(), random((4, 2, 64), 6).cuda()
+        then = [t.clone() for t in pages[:2]]
+        batch.table[2, 18] = number                 # the page of the sequence's last two rows
+        ops.rope_to_pages(None, k, v, ops.Pages(*then), batch)
+        kept = ops.read_pages(ops.Pages(*then), batch, 4)
+        assert torch.equal(kept[0][:2], k[:2]) and torch.isnan(kept[0][2:]).all()
+    batch = seqs.batch(ops, most=most)
+    batch.lengths[2] = 19 * 16 + 1
+    got = ops.paged_attention(q, pages, batch)
+    assert torch.equal(got[:2], good[:2]) and torch.isnan(got[2:]).all()
+
+
+def test_no_sequences_and_no_rows():
+    pages = ops.Pages(*(torch.zeros((2, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    none = ops.PageBatch(torch.zeros((0, 1), **i32), torch.zeros(1, **i32), torch.zeros(0, **i32), 0)
+    assert ops.paged_attention(torch.zeros((0, 1, 64), dtype=torch.float16, device="cuda"), pages, none).shape == (0, 64)
+    out = torch.full((2, 64), 3.0, dtype=torch.float16, device="cuda")
+    ops.paged_attention(torch.zeros((2, 1, 64), dtype=torch.float16, device="cuda"), pages, none, out=out)
+    empty = ops.PageBatch(torch.zeros((3, 1), **i32), torch.zeros(4, **i32), torch.zeros(3, **i32), 0)
+    ops.paged_attention(torch.zeros((2, 1, 64), dtype=torch.float16, device="cuda"), pages, empty, out=out)
+    assert (out == 3).all()

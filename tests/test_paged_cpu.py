@@ -1,0 +1,206 @@
+"""What the operators of a paged cache refuse, without a GPU: the tensor-level checks, and the library's own in front of a launch."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests import paged
+from ternaryllm_amd import _lib, ops
+
+
+def parts(kind="float16", kv=2, page=16, hd=64, seqs=2, tokens=3, heads=4):
+    dtype = torch.float16 if kind == "float16" else torch.float8_e4m3fn
+    k, v = (torch.zeros((5, kv, page, hd)).to(dtype) for _ in range(2))
+    exps = (None, None) if kind == "float16" else (torch.zeros((5, kv, page), dtype=torch.uint8), torch.zeros((5, kv, page), dtype=torch.uint8))
+    batch = ops.PageBatch(torch.zeros((seqs, 2), dtype=torch.int32), torch.zeros(seqs + 1, dtype=torch.int32), torch.zeros(seqs, dtype=torch.int32), 1)
+    return torch.zeros((tokens, heads, hd), dtype=torch.float16), torch.zeros((tokens, kv, hd), dtype=torch.float16), ops.Pages(k, v, *exps), batch
+
+
+def test_nothing_runs_without_a_gpu():
+    q, k, pages, batch = parts()
+    with pytest.raises(RuntimeError):
+        ops.rope_heads(q, k, torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64))
+    with pytest.raises(RuntimeError):
+        ops.rope_to_pages(q, k, k, pages, batch)
+    with pytest.raises(RuntimeError):
+        ops.read_pages(pages, batch, 3)
+    with pytest.raises(RuntimeError):
+        ops.paged_attention(q, pages, batch)
+
+
+@pytest.mark.parametrize("change", [
+    lambda p: p._replace(v=p.v[:4]), lambda p: p._replace(v=p.v.float()), lambda p: p._replace(k=p.k.float(), v=p.v.float()),
+    lambda p: p._replace(k_exponents=torch.zeros((5, 2, 16), dtype=torch.uint8)), lambda p: p._replace(v=p.v.transpose(1, 2).contiguous().transpose(1, 2)),
+    lambda p: p._replace(k=p.k[0], v=p.v[0]), lambda p: p._replace(k=p.k.to(torch.float8_e4m3fn), v=p.v.to(torch.float8_e4m3fn))])
+def test_pages_that_are_none(change):
+    q, k, pages, batch = parts()
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, change(pages), batch)
+    with pytest.raises(ValueError):
+        ops.read_pages(change(pages), batch, 3)
+    with pytest.raises(ValueError):
+        ops.rope_to_pages(q, k, k, change(pages), batch)
+
+
+@pytest.mark.parametrize("change", [
+    lambda p: p._replace(k_exponents=None), lambda p: p._replace(v_exponents=None), lambda p: p._replace(k_exponents=p.k_exponents[:4]),
+    lambda p: p._replace(k_exponents=p.k_exponents.int()), lambda p: p._replace(v_exponents=p.v_exponents.transpose(1, 2).contiguous().transpose(1, 2))])
+def test_exponents_that_are_none(change):
+    q, _, pages, batch = parts("e4m3")
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, change(pages), batch)
+
+
+@pytest.mark.parametrize("change", [
+    lambda b: b._replace(table=b.table.long()), lambda b: b._replace(starts=b.starts.long()), lambda b: b._replace(lengths=b.lengths.long()),
+    lambda b: b._replace(starts=b.starts[:-1]), lambda b: b._replace(lengths=b.lengths[:-1]), lambda b: b._replace(table=b.table[0]),
+    lambda b: b._replace(table=b.table.t().contiguous().t()), lambda b: b._replace(starts=torch.zeros(6, dtype=torch.int32)[::2])])
+def test_batches_that_are_none(change):
+    q, k, pages, batch = parts()
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, pages, change(batch))
+    with pytest.raises(ValueError):
+        ops.rope_to_pages(q, k, k, pages, change(batch))
+
+
+def test_heads_and_outputs_that_do_not_fit():
+    q, k, pages, batch = parts()
+    at, f = torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    bad = [
+        lambda: ops.rope_heads(q[0], None, at, f), lambda: ops.rope_heads(q, k[:2], at, f), lambda: ops.rope_heads(q, k.float(), at, f),
+        lambda: ops.rope_heads(q, k, None, f), lambda: ops.rope_heads(q, k, at.int(), f), lambda: ops.rope_heads(q, k, at[:2], f),
+        lambda: ops.rope_heads(q, k, at, f.float()), lambda: ops.rope_heads(q, k, at, f[None]), lambda: ops.rope_heads(q.bfloat16(), None, at, f),
+        lambda: ops.rope_heads(q, k, at, f, q_norm=torch.ones(64)), lambda: ops.rope_heads(q, k, at, f, k_norm=torch.ones(32).half()),
+        lambda: ops.rope_heads(q, k, at, f, q_out=k), lambda: ops.rope_heads(q, k, at, f, q_out=q.float()),
+        lambda: ops.rope_heads(q.transpose(1, 2), None, at, f), lambda: ops.rope_to_pages(q, k, k[:2], pages, batch),
+        lambda: ops.rope_to_pages(q[:2], k, k, pages, batch), lambda: ops.rope_to_pages(q, k[:, :1], k[:, :1], pages, batch),
+        lambda: ops.rope_to_pages(q, q, q, pages, batch), lambda: ops.read_pages(pages, batch, 3, torch.bfloat16),
+        lambda: ops.read_pages(pages, batch, 3, k_out=k), lambda: ops.read_pages(pages, batch, 3, k_out=k, v_out=k.float()),
+        lambda: ops.read_pages(pages, batch, 2, k_out=k, v_out=k.clone()), lambda: ops.paged_attention(q[..., :32], pages, batch),
+        lambda: ops.paged_attention(q[0], pages, batch), lambda: ops.paged_attention(q, pages, batch, out=q), lambda: ops.paged_attention(q.bfloat16(), pages, batch),
+        lambda: ops.paged_attention(q, pages, batch, out=torch.zeros((3, 256)))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_outputs_that_overlap_operands():
+    at, f = torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    rows = torch.zeros((5, 6, 64), dtype=torch.float16)
+    q, k = rows[:3, :4], rows[:3, 4:]
+    for out in (rows[1:4, :4], rows[:3, 1:5], rows[:3, 2:]):
+        with pytest.raises(ValueError):
+            ops.rope_heads(q, k, at, f, q_out=out)
+    with pytest.raises(ValueError):
+        ops.rope_heads(q, k, at, f, q_out=q, k_out=q[:, 2:])
+    # taken, up to the GPU that is not there: in place, and beside each other in other rows
+    other = torch.zeros((3, 6, 64), dtype=torch.float16)
+    for outs in ({"q_out": q, "k_out": k}, {"q_out": other[:, :4], "k_out": other[:, 4:]}):
+        with pytest.raises(RuntimeError):
+            ops.rope_heads(q, k, at, f, **outs)
+
+
+class Raw:
+    """The library's structures over addresses that are never followed: every call here is refused before a launch."""
+
+    def __init__(self, **changes):
+        at = 1 << 20
+        self.pages = _lib.Pages(at, at, None, None, 2 * 16 * 64, 16 * 64, 64, 5, 16, 2, 64, _lib.TL_F16)
+        self.batch = _lib.PageBatch(at, at, at, 2, 2, 2)
+        self.q = _lib.HeadRows(at, 256, 64, at, 256, 64, None, 4)
+        self.k = _lib.HeadRows(at, 128, 64, at, 128, 64, None, 2)
+        self.v = _lib.HeadRows(at, 128, 64, None, 0, 0, None, 2)
+        self.rotation = _lib.Rotation(at, at, 32, 0, 1.0, 1e-6)
+        self.args = {"dtype": _lib.TL_F16, "tokens": 3, "head_dim": 64, "scale": 0.125, "out": at, "workspace": at, "bytes": 1 << 40, "heads": 4, "most": 1,
+                     "q_token": 256, "k_out": at, "out_token": 128}
+        for name, value in changes.items():
+            where, _, field = name.partition("__")
+            if field:
+                setattr(getattr(self, where), field, value)
+            elif where in self.args:
+                self.args[where] = value
+            else:
+                setattr(self, where, value)
+
+    def heads(self):
+        return _lib.lib().tl_rope_heads(self.q, self.k, self.args["dtype"], self.args["tokens"], self.args["head_dim"], self.rotation, None)
+
+    def to_pages(self):
+        return _lib.lib().tl_rope_to_pages(self.q, self.k, self.v, self.args["dtype"], self.args["tokens"], self.rotation, self.pages, self.batch, None)
+
+    def read(self):
+        return _lib.lib().tl_read_pages(self.pages, self.batch, self.args["tokens"], self.args["dtype"], self.args["k_out"], self.args["out"],
+                                        self.args["out_token"], 64, None)
+
+    def attend(self):
+        a = self.args
+        return _lib.lib().tl_paged_attention(1 << 20, a["q_token"], 64, a["dtype"], a["tokens"], a["heads"], self.pages, self.batch, a["most"], a["scale"],
+                                             a["out"], a["workspace"], a["bytes"], None)
+
+
+ARG, SHAPE, DTYPE, ALIGN, UNSUPPORTED, SIZE = -1, -2, -3, -4, -5, -8
+
+
+@pytest.mark.parametrize("call,changes,code", [
+    ("heads", {"dtype": 2}, DTYPE), ("heads", {"head_dim": 60}, UNSUPPORTED), ("heads", {"head_dim": 520}, UNSUPPORTED), ("heads", {"head_dim": 0}, UNSUPPORTED),
+    ("heads", {"tokens": -1}, SHAPE), ("heads", {"tokens": 1 << 40}, SHAPE), ("heads", {"rotation": None}, ARG), ("heads", {"rotation__pairs": 33}, SHAPE),
+    ("heads", {"rotation__pairs": -1}, SHAPE), ("heads", {"rotation__frequencies": None}, ARG), ("heads", {"rotation__positions": None}, ARG),
+    ("heads", {"q__x": None}, ARG), ("heads", {"q__y": None}, ARG), ("heads", {"k__heads": -1}, SHAPE), ("heads", {"q__x": (1 << 20) + 8}, ALIGN),
+    ("heads", {"q__x_token": 257}, ALIGN), ("heads", {"k__y_head": 4}, ALIGN), ("heads", {"q__norm_weight": 8}, ALIGN),
+    ("to_pages", {"dtype": 7}, DTYPE), ("to_pages", {"pages": None}, ARG), ("to_pages", {"batch": None}, ARG), ("to_pages", {"pages__k": None}, ARG),
+    ("to_pages", {"k__heads": 3}, SHAPE), ("to_pages", {"v__heads": 0}, SHAPE), ("to_pages", {"v__norm_weight": 16}, ARG), ("to_pages", {"rotation__pairs": 33}, SHAPE),
+    ("to_pages", {"batch__starts": None}, ARG), ("to_pages", {"batch__lengths": None}, ARG), ("to_pages", {"batch__table": None}, ARG),
+    ("read", {"dtype": 2}, DTYPE), ("read", {"out_token": 129}, ALIGN), ("read", {"k_out": 8}, ALIGN), ("read", {"tokens": -3}, SHAPE),
+    ("read", {"pages__page_size": 8}, SHAPE), ("read", {"pages__page_size": 48}, SHAPE), ("read", {"pages__page_size": 2048}, SHAPE), ("read", {"pages__pages": 0}, SHAPE),
+    ("read", {"pages__pages": 1 << 40}, SHAPE), ("read", {"pages__kv_heads": 0}, SHAPE), ("read", {"pages__head_dim": 72}, SHAPE), ("read", {"pages__head_dim": 528}, SHAPE),
+    ("read", {"pages__slot_stride": 32}, SHAPE), ("read", {"pages__page_stride": 0}, SHAPE), ("read", {"pages__head_stride": -64}, SHAPE),
+    ("read", {"pages__slot_stride": 1 << 28}, SHAPE), ("read", {"pages__head_stride": 1025}, ALIGN), ("read", {"pages__v": 24}, ALIGN),
+    ("read", {"pages__dtype": 0}, DTYPE), ("read", {"pages__dtype": 2}, ARG), ("read", {"pages__k_exponents": 16}, None), ("read", {"batch__seqs": -1}, SHAPE),
+    ("read", {"batch__table_stride": 1}, SHAPE), ("read", {"batch__table_pages": -1}, SHAPE), ("read", {"batch__table_pages": 1 << 30, "batch__table_stride": 1 << 30}, SHAPE),
+    ("attend", {"dtype": 0}, UNSUPPORTED), ("attend", {"dtype": 2}, DTYPE), ("attend", {"heads": 3}, SHAPE), ("attend", {"heads": 0}, SHAPE),
+    ("attend", {"pages__head_dim": 96, "pages__slot_stride": 96}, UNSUPPORTED), ("attend", {"out": None}, ARG), ("attend", {"workspace": None}, ARG),
+    ("attend", {"workspace": 8}, ALIGN), ("attend", {"bytes": 100}, SIZE), ("attend", {"scale": 0.0}, ARG), ("attend", {"scale": -1.0}, ARG),
+    ("attend", {"scale": math.nan}, ARG), ("attend", {"scale": math.inf}, ARG), ("attend", {"most": -1}, ARG), ("attend", {"q_token": 100}, ALIGN),
+    ("attend", {"out": (1 << 20) + 2}, ALIGN)])
+def test_the_library_refuses(call, changes, code):
+    if code is None:                                # exponents beside fp16 pages: one alone is refused as well
+        changes = {**changes, "pages__v_exponents": 16}
+        code = ARG
+    raw = Raw(**changes)
+    assert getattr(raw, call)() == code
+    assert _lib.lib().tl_last_error()
+
+
+@pytest.mark.parametrize("call", ["heads", "to_pages", "read", "attend"])
+def test_no_rows_need_no_addresses(call):
+    raw = Raw(tokens=0, q__x=None, q__y=None, k__x=None, k__y=None, v__x=None, rotation__positions=None, k_out=None, out=None, workspace=None)
+    assert getattr(raw, call)() == 0
+    if call != "heads":
+        assert getattr(Raw(batch__seqs=0, batch__table=None, batch__lengths=None, batch__starts=None), call)() == 0
+
+
+def test_workspace_size():
+    need = ctypes.c_int64(0)
+    raw = Raw()
+    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, 1, ctypes.byref(need)) == 0 and need.value > 0
+    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, 1, None) == ARG
+    assert _lib.lib().tl_paged_attention_workspace(3, raw.pages, 1, ctypes.byref(need)) == SHAPE
+    assert _lib.lib().tl_paged_attention_workspace(4, None, 1, ctypes.byref(need)) == ARG
+    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, -1, ctypes.byref(need)) == ARG
+
+
+def test_what_the_plain_forms_hold():
+    """The 8-bit grid of the plain form is torch's, row exponents are the least, and a sequence's rows come out of any order of pages."""
+    x = torch.randn((50, 64), generator=torch.Generator().manual_seed(1), dtype=torch.float64) * torch.exp2(torch.arange(50.0))[:, None].double() * 2.0 ** -30
+    e = paged.exponents_of(x)
+    assert ((x.abs().amax(-1) <= 448 * 2.0 ** e) | (e == 8)).all() and ((x.abs().amax(-1) > 448 * 2.0 ** (e - 1)) | (e == -32)).all()
+    small = e < 8
+    codes = (x / 2.0 ** e[:, None]).float().to(torch.float8_e4m3fn).double()
+    assert torch.equal(paged.byte_values(x)[small], (codes * 2.0 ** e[:, None])[small])
+    seqs = paged.Sequences([(2, 40), (1, 16), (0, 0)], 16)
+    pool = torch.zeros((seqs.pages, 1, 16, 1))
+    for _, b, at, page, slot in seqs.rows():
+        pool[page, 0, slot, 0] = 100 * b + at
+    assert seqs.held(0, pool)[38:].flatten().tolist() == [38, 39] and seqs.held(1, pool)[15].item() == 115 and seqs.held(2, pool).shape == (0, 1, 1)
