@@ -13,6 +13,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+
 #include "ternary_spmm.h"
 
 namespace {
@@ -22,6 +24,11 @@ decltype(&tl_spmm) g_spmm;
 decltype(&tl_spmm_workspace) g_workspace;
 decltype(&tl_mlp_gate_up) g_gate_up;
 decltype(&tl_mlp_gate_up_few) g_gate_up_few;
+decltype(&tl_rope_heads) g_rope_heads;
+decltype(&tl_rope_to_pages) g_rope_to_pages;
+decltype(&tl_read_pages) g_read_pages;
+decltype(&tl_paged_attention_workspace) g_attention_workspace;
+decltype(&tl_paged_attention) g_attention;
 PyObject* g_workspaces;  // {(device index, stream): uint8 tensor}: the scratch of ops
 
 int type_code(const at::Tensor& t)
@@ -172,15 +179,250 @@ PyObject* gate_up(PyObject*, PyObject* const* args, Py_ssize_t count)
     END_HANDLE_TH_ERRORS
 }
 
-// init(addresses of tl_spmm, tl_spmm_workspace, tl_mlp_gate_up, tl_mlp_gate_up_few, the scratch dict)
+// ---- a paged cache: what ops.rope_heads, rope_to_pages, read_pages and paged_attention do for plain calls.  One token's heads
+// rotated took 36 us through Python's checks and structures.
+
+int64_t step(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+bool absent(PyObject* o) { return o == Py_None; }
+
+// x [tokens, heads, head_dim] on `device`, of type `type`, its rows' last dimension in one piece; y where it goes (null: pages).
+bool head_rows(const at::Tensor& x, const at::Tensor* y, PyObject* norm, tl_head_rows* r)
+{
+    if (x.dim() != 3 || x.stride(2) != 1 || x.numel() == 0) return false;
+    const at::Tensor* w = nullptr;
+    if (!absent(norm)) {
+        w = plain(norm);
+        if (!w || w->dim() != 1 || w->size(0) != x.size(2) || w->scalar_type() != x.scalar_type() || w->device() != x.device() || !w->is_contiguous()) return false;
+    }
+    *r = tl_head_rows{x.data_ptr(), step(x, 0), step(x, 1), y ? y->data_ptr() : nullptr, y ? step(*y, 0) : 0, y ? step(*y, 1) : 0,
+                      w ? w->data_ptr() : nullptr, (int32_t)x.size(1)};
+    return true;
+}
+
+// An output that is not given, or is the operand itself.
+bool output_rows(PyObject* given, PyObject* operand, const at::Tensor& x, at::Tensor* y)
+{
+    if (given == operand) *y = x;
+    else if (absent(given)) *y = at::empty(x.sizes(), x.options().requires_grad(false));
+    else return false;
+    return true;
+}
+
+bool rotation(PyObject* frequencies, PyObject* positions, PyObject* factor, PyObject* interleaved, PyObject* eps, const at::Tensor& like, tl_rotation* r)
+{
+    const double f = PyFloat_AsDouble(factor), e = PyFloat_AsDouble(eps);
+    const int pairs_side_by_side = PyObject_IsTrue(interleaved);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    *r = tl_rotation{nullptr, nullptr, 0, 0, (float)f, (float)e};
+    if (absent(frequencies)) return true;
+    const at::Tensor* t = plain(frequencies);
+    if (!t || t->dim() != 1 || t->scalar_type() != at::kDouble || t->device() != like.device() || !t->is_contiguous()) return false;
+    r->frequencies = static_cast<const double*>(t->data_ptr());
+    r->pairs = (int32_t)t->numel();
+    r->interleaved = pairs_side_by_side;
+    if (absent(positions)) return true;
+    const at::Tensor* p = plain(positions);
+    if (!p || p->dim() != 1 || p->size(0) != like.size(0) || p->scalar_type() != at::kLong || p->device() != like.device() || !p->is_contiguous()) return false;
+    r->positions = static_cast<const int64_t*>(p->data_ptr());
+    return true;
+}
+
+const at::Tensor* member(PyObject* tuple, int i) { return absent(PyTuple_GET_ITEM(tuple, i)) ? nullptr : plain(PyTuple_GET_ITEM(tuple, i)); }
+
+// ops.Pages and ops.PageBatch as the library's structures.
+bool pages_and_batch(PyObject* pages, PyObject* batch, c10::Device device, tl_pages* p, tl_page_batch* b, int64_t* most_rows)
+{
+    if (!PyTuple_Check(pages) || PyTuple_GET_SIZE(pages) != 4 || !PyTuple_Check(batch) || PyTuple_GET_SIZE(batch) != 4) return false;
+    const at::Tensor *k = member(pages, 0), *v = member(pages, 1), *ke = member(pages, 2), *ve = member(pages, 3);
+    if (!k || !v || k->dim() != 4 || k->numel() == 0 || k->sizes() != v->sizes() || k->strides() != v->strides() || k->stride(3) != 1 ||
+        k->scalar_type() != v->scalar_type() || k->device() != device || v->device() != device)
+        return false;
+    const bool bytes = k->scalar_type() == at::kFloat8_e4m3fn;
+    if (!bytes && k->scalar_type() != at::kHalf) return false;
+    if (bytes) {
+        for (const at::Tensor* e : {ke, ve})
+            if (!e || e->dim() != 3 || e->sizes() != k->sizes().slice(0, 3) || e->scalar_type() != at::kByte || !e->is_contiguous() || e->device() != device) return false;
+    } else if (!absent(PyTuple_GET_ITEM(pages, 2)) || !absent(PyTuple_GET_ITEM(pages, 3))) {
+        return false;
+    }
+    const at::Tensor *table = member(batch, 0), *starts = member(batch, 1), *lengths = member(batch, 2);
+    for (const at::Tensor* t : {table, starts, lengths})
+        if (!t || t->scalar_type() != at::kInt || t->device() != device || t->numel() == 0) return false;
+    if (table->dim() != 2 || starts->dim() != 1 || lengths->dim() != 1 || starts->size(0) != table->size(0) + 1 || lengths->size(0) != table->size(0) ||
+        step(*table, 1) > 1 || step(*starts, 0) > 1 || step(*lengths, 0) > 1)
+        return false;
+    *most_rows = PyLong_AsLongLong(PyTuple_GET_ITEM(batch, 3));
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    const int64_t any = k->size(2) * k->size(3);   // (a dimension of one entry has no stride of its own)
+    auto stride = [&](int d) { return k->size(d) > 1 ? k->stride(d) : any; };
+    *p = tl_pages{k->data_ptr(), v->data_ptr(), bytes ? ke->data_ptr() : nullptr, bytes ? ve->data_ptr() : nullptr, stride(0), stride(1), stride(2), k->size(0),
+                  (int32_t)k->size(2), (int32_t)k->size(1), (int32_t)k->size(3), bytes ? TL_E4M3 : TL_F16};
+    *b = tl_page_batch{static_cast<const int32_t*>(table->data_ptr()), static_cast<const int32_t*>(starts->data_ptr()),
+                       static_cast<const int32_t*>(lengths->data_ptr()), table->size(0) > 1 ? table->stride(0) : table->size(1), (int32_t)table->size(1),
+                       (int32_t)table->size(0)};
+    return true;
+}
+
+PyObject* pair_of(at::Tensor a, at::Tensor b)
+{
+    PyObject* both = PyTuple_New(2);
+    if (!both) throw python_error();
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(a)));
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(b)));
+    return both;
+}
+
+// rope_heads(q, k, positions, frequencies, factor, interleaved, q_norm, k_norm, eps, q_out, k_out) -> (q, k) or None
+PyObject* rope_heads(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+    HANDLE_TH_ERRORS
+    if (count != 11) {
+        PyErr_SetString(PyExc_TypeError, "rope_heads takes eleven arguments");
+        return nullptr;
+    }
+    const at::Tensor *q = plain(a[0]), *k = plain(a[1]);
+    tl_rotation turn;
+    if (!q || !k || q->dim() != 3 || k->dim() != 3 || type_code(*q) < 0 || k->scalar_type() != q->scalar_type() || k->device() != q->device() ||
+        k->size(0) != q->size(0) || k->size(2) != q->size(2) || (!absent(a[3]) && absent(a[2])) || !rotation(a[3], a[2], a[4], a[5], a[8], *q, &turn))
+        Py_RETURN_NONE;
+    const c10::DeviceGuard guard(q->device());
+    at::Tensor q_out, k_out;
+    tl_head_rows qr, kr;
+    if (a[0] == a[1] || !output_rows(a[9], a[0], *q, &q_out) || !output_rows(a[10], a[1], *k, &k_out) || !head_rows(*q, &q_out, a[6], &qr) || !head_rows(*k, &k_out, a[7], &kr))
+        Py_RETURN_NONE;
+    // (in place on one of two views of the same rows: Python looks at where they lie)
+    if ((a[9] == a[0] || a[10] == a[1]) && q->storage().data() == k->storage().data()) Py_RETURN_NONE;
+    void* stream = current_stream(q->device());
+    int rc;
+    {
+        const pybind11::gil_scoped_release no_gil;
+        rc = g_rope_heads(&qr, &kr, type_code(*q), q->size(0), (int)q->size(2), &turn, stream);
+    }
+    if (rc != TL_OK) Py_RETURN_NONE;
+    return pair_of(std::move(q_out), std::move(k_out));
+    END_HANDLE_TH_ERRORS
+}
+
+// rope_to_pages(q, k, v, pages, batch, frequencies, positions, factor, interleaved, q_norm, k_norm, eps) -> q or None
+PyObject* rope_to_pages(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+    HANDLE_TH_ERRORS
+    if (count != 12) {
+        PyErr_SetString(PyExc_TypeError, "rope_to_pages takes twelve arguments");
+        return nullptr;
+    }
+    const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]);
+    tl_rotation turn;
+    tl_pages p;
+    tl_page_batch b;
+    int64_t most;
+    if (!q || !k || !v || q->dim() != 3 || k->dim() != 3 || type_code(*k) < 0 || q->scalar_type() != k->scalar_type() || v->scalar_type() != k->scalar_type() ||
+        q->device() != k->device() || v->device() != k->device() || q->size(0) != k->size(0) || q->size(2) != k->size(2) || v->sizes() != k->sizes() ||
+        !rotation(a[5], a[6], a[7], a[8], a[11], *k, &turn) || !pages_and_batch(a[3], a[4], k->device(), &p, &b, &most) || p.kv_heads != k->size(1) ||
+        p.head_dim != k->size(2))
+        Py_RETURN_NONE;
+    const c10::DeviceGuard guard(k->device());
+    at::Tensor q_out = at::empty(q->sizes(), q->options().requires_grad(false));
+    tl_head_rows qr, kr, vr;
+    if (!head_rows(*q, &q_out, a[9], &qr) || !head_rows(*k, nullptr, a[10], &kr) || !head_rows(*v, nullptr, Py_None, &vr)) Py_RETURN_NONE;
+    void* stream = current_stream(k->device());
+    int rc;
+    {
+        const pybind11::gil_scoped_release no_gil;
+        rc = g_rope_to_pages(&qr, &kr, &vr, type_code(*k), k->size(0), &turn, &p, &b, stream);
+    }
+    if (rc != TL_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(q_out));
+    END_HANDLE_TH_ERRORS
+}
+
+// read_pages(pages, batch, tokens, fp16) -> (k, v) or None
+PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+    HANDLE_TH_ERRORS
+    if (count != 4) {
+        PyErr_SetString(PyExc_TypeError, "read_pages takes four arguments");
+        return nullptr;
+    }
+    const at::Tensor* k = PyTuple_Check(a[0]) && PyTuple_GET_SIZE(a[0]) == 4 ? member(a[0], 0) : nullptr;
+    const int64_t tokens = PyLong_AsLongLong(a[2]);
+    if (PyErr_Occurred()) PyErr_Clear();
+    tl_pages p;
+    tl_page_batch b;
+    int64_t most;
+    if (!k || tokens <= 0 || !pages_and_batch(a[0], a[1], k->device(), &p, &b, &most)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(k->device());
+    const bool half = a[3] == Py_True;
+    at::Tensor both = at::empty({2, tokens, p.kv_heads, p.head_dim}, k->options().dtype(half ? at::kHalf : at::kFloat).requires_grad(false));
+    at::Tensor k_out = both.select(0, 0), v_out = both.select(0, 1);
+    void* stream = current_stream(k->device());
+    int rc;
+    {
+        const pybind11::gil_scoped_release no_gil;
+        rc = g_read_pages(&p, &b, tokens, half ? TL_F16 : TL_F32, k_out.data_ptr(), v_out.data_ptr(), (int64_t)p.kv_heads * p.head_dim, p.head_dim, stream);
+    }
+    if (rc != TL_OK) Py_RETURN_NONE;
+    return pair_of(std::move(k_out), std::move(v_out));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, pages, batch, scale or None, out or None) -> out or None
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+    HANDLE_TH_ERRORS
+    if (count != 5) {
+        PyErr_SetString(PyExc_TypeError, "paged_attention takes five arguments");
+        return nullptr;
+    }
+    const at::Tensor* q = plain(a[0]);
+    tl_pages p;
+    tl_page_batch b;
+    int64_t most, need;
+    if (!q || q->dim() != 3 || q->numel() == 0 || q->stride(2) != 1 || q->scalar_type() != at::kHalf || !pages_and_batch(a[1], a[2], q->device(), &p, &b, &most) ||
+        p.head_dim != q->size(2))
+        Py_RETURN_NONE;
+    const int64_t tokens = q->size(0), width = q->size(1) * q->size(2);
+    const double scale = absent(a[3]) ? 1.0 / std::sqrt((double)q->size(2)) : PyFloat_AsDouble(a[3]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const c10::DeviceGuard guard(q->device());
+    const at::Tensor* given = absent(a[4]) ? nullptr : plain(a[4]);
+    if (!absent(a[4]) && (!given || given->dim() != 2 || given->size(0) != tokens || given->size(1) != width || given->scalar_type() != at::kHalf ||
+                          given->device() != q->device() || !given->is_contiguous() || given->storage().data() == q->storage().data()))
+        Py_RETURN_NONE;
+    if (g_attention_workspace((int)q->size(1), &p, most, &need) != TL_OK) Py_RETURN_NONE;
+    at::Tensor out = given ? *given : at::empty({tokens, width}, q->options().requires_grad(false));
+    at::Tensor ws = at::empty({need}, q->options().dtype(at::kByte).requires_grad(false));
+    void* stream = current_stream(q->device());
+    int rc;
+    {
+        const pybind11::gil_scoped_release no_gil;
+        rc = g_attention(q->data_ptr(), step(*q, 0), step(*q, 1), TL_F16, tokens, (int)q->size(1), &p, &b, most, (float)scale, out.data_ptr(), ws.data_ptr(), need,
+                         stream);
+    }
+    if (rc != TL_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// init(addresses of the library's entry points in the order of g_*, the scratch dict)
 PyObject* init(PyObject*, PyObject* args)
 {
-    PyObject *spmm, *space, *both, *few, *dict;
-    if (!PyArg_ParseTuple(args, "OOOOO!", &spmm, &space, &both, &few, &PyDict_Type, &dict)) return nullptr;
-    g_spmm = reinterpret_cast<decltype(g_spmm)>(PyLong_AsVoidPtr(spmm));
-    g_workspace = reinterpret_cast<decltype(g_workspace)>(PyLong_AsVoidPtr(space));
-    g_gate_up = reinterpret_cast<decltype(g_gate_up)>(PyLong_AsVoidPtr(both));
-    g_gate_up_few = reinterpret_cast<decltype(g_gate_up_few)>(PyLong_AsVoidPtr(few));
+    PyObject *at[9], *dict;
+    if (!PyArg_ParseTuple(args, "OOOOOOOOOO!", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8], &PyDict_Type, &dict)) return nullptr;
+    int i = 0;
+    auto take = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(PyLong_AsVoidPtr(at[i++])); };
+    take(g_spmm), take(g_workspace), take(g_gate_up), take(g_gate_up_few);
+    take(g_rope_heads), take(g_rope_to_pages), take(g_read_pages), take(g_attention_workspace), take(g_attention);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(dict);
     g_workspaces = dict;
@@ -191,6 +433,10 @@ PyMethodDef g_methods[] = {
     {"init", init, METH_VARARGS, "addresses of the library's entry points, and the scratch buffers"},
     {"product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product)), METH_FASTCALL, "x @ W * scale, or None"},
     {"gate_up", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gate_up)), METH_FASTCALL, "silu(x @ Wg) * (x @ Wu), or None"},
+    {"rope_heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope_heads)), METH_FASTCALL, "heads normalised and rotated, or None"},
+    {"rope_to_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope_to_pages)), METH_FASTCALL, "the same into pages, or None"},
+    {"read_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(read_pages)), METH_FASTCALL, "rows out of pages, or None"},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, "attention over pages, or None"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tl_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

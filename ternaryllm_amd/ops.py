@@ -726,6 +726,9 @@ def rope_heads(q, k, positions, frequencies, *, factor=1.0, interleaved=False, q
     (2 i, 2 i + 1); cosine and sine are multiplied by factor (attention.rope_frequencies gives both for a model's scaling).  positions: int64
     [tokens]; frequencies: float64 on the device, None: no rotation.  k may be None.  Returns (q, k) rotated, new tensors or q_out, k_out,
     which may be q and k themselves.  float16 or float32, head_dim a multiple of 8, strides of whole 16-byte pieces."""
+    both = _short().rope_heads(q, k, positions, frequencies, factor, interleaved, q_norm, k_norm, eps, q_out, k_out)
+    if both is not None:
+        return both
     if k is not None and (k.dim() != 3 or k.shape[::2] != q.shape[::2] or k.dtype != q.dtype or k.device != q.device):
         raise ValueError("k must have q's tokens, head_dim, type and device")
     if frequencies is not None and positions is None:
@@ -749,6 +752,10 @@ def rope_to_pages(q, k, v, pages, batch, frequencies=None, positions=None, *, fa
     them.  positions None: each row's index in its sequence.  q may be None.  Returns the rotated queries.  Pages of float8_e4m3fn: a row's
     exponent is the least that keeps it within 448, its codes are rounded to the nearest; they saturate at the largest value that is a finite
     float16."""
+    if q_out is None:
+        rotated = _short().rope_to_pages(q, k, v, pages, batch, frequencies, positions, factor, interleaved, q_norm, k_norm, eps)
+        if rotated is not None:
+            return rotated
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one type and device")
     if q is not None and (q.dim() != 3 or q.shape[::2] != k.shape[::2] or q.dtype != k.dtype or q.device != k.device):
@@ -773,6 +780,10 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
     """The keys and values of a batch's `tokens` rows out of the pages, [tokens, kv_heads, head_dim] each, float16 (which every 8-bit row fits
     exactly) or float32: new tensors (rows of no sequence are not written there either), or k_out and v_out of the same strides.  A row whose
     page is none is NaN."""
+    if k_out is None and v_out is None and (dtype is torch.float16 or dtype is torch.float32):
+        both = _short().read_pages(pages, batch, tokens, dtype is torch.float16)
+        if both is not None:
+            return both
     if pages.k.dim() != 4:
         raise ValueError("pages must be [pages, kv_heads, page_size, head_dim]")
     device, (_, heads, _, hd) = pages.k.device, pages.k.shape
@@ -796,6 +807,9 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
     among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
     rows of no sequence are not written, a row that sees nothing is 0, rows of a sequence with a page that is none are NaN.  float16, head_dim 64,
     128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim)."""
+    y = _short().paged_attention(q, pages, batch, scale, out)
+    if y is not None:
+        return y
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
     tokens, heads, hd = q.shape
@@ -807,6 +821,8 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
         out = torch.empty((tokens, heads * hd), dtype=q.dtype, device=q.device)
     elif out.shape != (tokens, heads * hd) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise ValueError("out must be a contiguous [tokens, heads * head_dim] tensor of q's type and device")
+    elif _overlap(q, out.view(tokens, heads, hd)):
+        raise ValueError("out must lie apart from q")
     _cuda(q, "q")
     need = ctypes.c_int64(0)
     with torch.cuda.device(q.device):

@@ -304,3 +304,34 @@ def test_no_sequences_and_no_rows():
     empty = ops.PageBatch(torch.zeros((3, 1), **i32), torch.zeros(4, **i32), torch.zeros(3, **i32), 0)
     ops.paged_attention(torch.zeros((2, 1, 64), dtype=torch.float16, device="cuda"), pages, empty, out=out)
     assert (out == 3).all()
+
+
+class _NoShortWay:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_the_short_way_and_the_general_one(monkeypatch):
+    """The same bits, whichever of the two takes a call."""
+    seqs = paged.Sequences([(2, 30), (1, 70), (5, 5)], 16)
+    qkv = random((seqs.tokens, 8, 64), 1).cuda()
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    w, f, at = random((64,), 2).cuda(), frequencies(32).cuda(), torch.arange(seqs.tokens, device="cuda")
+
+    def all_of_them():
+        got = []
+        for kind in ("float16", "e4m3"):
+            pages = on_gpu(fresh_pages(seqs, 2, 64, kind, spoiled=False))
+            got += ops.rope_heads(q, k, at, f, q_norm=w, factor=1.5)
+            got.append(ops.rope_to_pages(q, k, v, pages, seqs.batch(ops), f, interleaved=True, k_norm=w))
+            got.append(ops.rope_to_pages(q, k, v, pages, seqs.batch(ops), f, at, k_norm=w))
+            got += [t.view(torch.uint8) for t in pages if t is not None]
+            got += ops.read_pages(pages, seqs.batch(ops), seqs.tokens) + ops.read_pages(pages, seqs.batch(ops), seqs.tokens, torch.float32)
+            got.append(ops.paged_attention(q, pages, seqs.batch(ops)))
+            got.append(ops.paged_attention(q, pages, seqs.batch(ops), scale=0.5, out=torch.empty((seqs.tokens, 256), dtype=torch.float16, device="cuda")))
+        return got
+
+    short = all_of_them()
+    monkeypatch.setattr(ops, "_short", _NoShortWay)
+    general = all_of_them()
+    assert len(short) == len(general) and all(torch.equal(a, b) for a, b in zip(short, general))
