@@ -673,7 +673,7 @@ int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, int64_t tok
  *   out        [tokens][heads * head_dim]
  *   workspace  device, 16-byte aligned, of tl_paged_attention_workspace bytes at least; calls that share it must not overlap
  * Work is shared out on the device by the lengths that stand there, in equal parts whatever they are, parts of a row's keys among them. */
-int tl_paged_attention_workspace(int heads, const tl_pages* pages, int64_t most_rows, int64_t* bytes);
+int tl_paged_attention_workspace(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows, int64_t* bytes);
 int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
                        const tl_page_batch* batch, int64_t most_rows, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 

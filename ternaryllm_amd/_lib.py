@@ -140,7 +140,7 @@ SIGNATURES = {
     "tl_rope_heads": (_INT, [_ROWSP, _ROWSP, _INT, _I64, _INT, _ROTP, _VP]),
     "tl_rope_to_pages": (_INT, [_ROWSP, _ROWSP, _ROWSP, _INT, _I64, _ROTP, _PAGESP, _BATCHP, _VP]),
     "tl_read_pages": (_INT, [_PAGESP, _BATCHP, _I64, _INT, _VP, _VP, _I64, _I64, _VP]),
-    "tl_paged_attention_workspace": (_INT, [_INT, _PAGESP, _I64, _I64P]),
+    "tl_paged_attention_workspace": (_INT, [_I64, _INT, _PAGESP, _BATCHP, _I64, _I64P]),
     "tl_paged_attention": (_INT, [_VP, _I64, _I64, _INT, _I64, _INT, _PAGESP, _BATCHP, _I64, ctypes.c_float, _VP, _VP, _I64, _VP]),
 }
 

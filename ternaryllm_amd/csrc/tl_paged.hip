@@ -35,10 +35,17 @@ struct PagedAttn {
     int heads, group;
     int tile_heads, blocks, tile_tokens;         // query heads and tokens of a unit, units that a group's heads are shared out among
     float scale_log2;                            // of the scores, times log2(e)
+    int fixed;                                   // cost of a unit beside its keys
     int least;                                   // cost of a workgroup's part, 1 or more
     float* pieces;                               // [workgroups][2][rows][head_dim + 4]
     Shared* shared;                              // [workgroups]
 };
+
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long scalar(long long v)
+{
+    return (long long)(((unsigned long long)(uint32_t)scalar((int)(v >> 32)) << 32) | (uint32_t)scalar((int)v));
+}
 
 // A sequence as the walk over the units takes it.
 struct Seq {
@@ -61,10 +68,16 @@ __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
     return s;
 }
 
-// Cost of a key head's first `tiles` units: unit i costs before + (i + 1) * tile_tokens.
+// The same for a sequence that all lanes look at.
+__device__ __forceinline__ Seq scalar(Seq s)
+{
+    return Seq{scalar(s.start), scalar(s.n), scalar(s.length), scalar(s.tiles), scalar(s.before), scalar((int)s.wrong) != 0};
+}
+
+// Cost of a key head's first `tiles` units: unit i costs fixed + before + (i + 1) * tile_tokens.
 __device__ __forceinline__ long long tiles_cost(const PagedAttn& a, int before, int tiles)
 {
-    return (long long)tiles * before + (long long)a.tile_tokens * tiles * (tiles + 1ll) / 2;
+    return (long long)tiles * (a.fixed + before) + (long long)a.tile_tokens * tiles * (tiles + 1ll) / 2;
 }
 
 __device__ __forceinline__ long long seq_cost(const PagedAttn& a, int b)
@@ -82,12 +95,6 @@ struct Walk {
     int b, head, tile;                           // the unit: sequence, key head and block of query heads, rows
     Seq s;
 };
-
-__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ long long scalar(long long v)
-{
-    return (long long)(((unsigned long long)(uint32_t)scalar((int)(v >> 32)) << 32) | (uint32_t)scalar((int)v));
-}
 
 // By a whole workgroup of 256 threads.  False where it has no part.
 __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
@@ -153,7 +160,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     __syncthreads();
     w.b = scalar(found_b);
     w.at = scalar(found_at);
-    w.s = sequence(a, w.b);
+    w.s = scalar(sequence(a, w.b));
     const long long head_cost = tiles_cost(a, w.s.before, w.s.tiles);
     w.head = (int)((w.from - w.at) / head_cost);
     w.at += w.head * head_cost;
@@ -179,7 +186,7 @@ __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long
     w.head = 0;
     do {
         if (++w.b >= a.batch.seqs) return false;
-        w.s = sequence(a, w.b);
+        w.s = scalar(sequence(a, w.b));
     } while (w.s.tiles == 0);
     return true;
 }
@@ -197,7 +204,7 @@ template <int ROWS, int HD>
 __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
 {
     Unit u;
-    u.cost = (long long)w.s.before + (w.tile + 1ll) * a.tile_tokens;
+    u.cost = a.fixed + (long long)w.s.before + (w.tile + 1ll) * a.tile_tokens;
     u.first_token = w.tile * a.tile_tokens;
     u.kv_head = w.head / a.blocks;
     u.first_head = (w.head - u.kv_head * a.blocks) * a.tile_heads;
@@ -205,7 +212,8 @@ __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
     u.begins = w.at >= w.from;
     const bool ends = w.at + u.cost <= w.to;
     u.whole = u.begins && ends;
-    auto cut = [&](long long at) { return (int)min((at - w.at + kRound - 1) / kRound * kRound, (long long)seen); };
+    // (its keys in proportion to its cost)
+    auto cut = [&](long long at) { return min((int)((at - w.at) * seen / u.cost + kRound - 1) / kRound * kRound, seen); };
     u.first_key = u.begins ? 0 : cut(w.from);
     u.end_key = ends ? seen : cut(w.to);
     u.piece = a.pieces + ((long long)w.wg * 2 + (u.begins ? 1 : 0)) * ROWS * (HD + 4);
@@ -264,55 +272,94 @@ __device__ __forceinline__ void sixteen_halves(u32x4 codes, float scale, u32x4* 
     }
 }
 
-// The running softmax of one fragment of 16 rows over COUNT fragments of 16 keys: scores in, probabilities out (as the operand of the
-// product with the values), the sums so far shrunk where the maximum moved.
-template <int COUNT, int DF>
-__device__ __forceinline__ void softmax_step(f32x4 (&sc)[COUNT], float scale_log2, float& top, float& sum, f32x4 (&o)[DF], u32x4 (&px)[COUNT / 2])
+// The running softmax of a row: its reference is a maximum that it has seen (in units of the scores), which probabilities are taken
+// against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, 8 in the exponent of 2: a
+// probability is then 256 at most, as exact in fp16 as one of 1, and the sums, which are fp32, hardly ever have to be scaled.
+struct Running {
+    float top, limit, base, sum;                 // base: top as an exponent of 2 (0 while there is none); sum: of this lane's keys
+};
+
+constexpr Running kNothing{kNone, kNone, 0.f, 0.f};
+
+// Scores of QF rows and COUNT fragments of 16 keys in, probabilities out (as the operand of the product with the values).
+template <int QF, int COUNT, int DF>
+__device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale_log2, Running (&run)[QF], f32x4 (&o)[QF][DF], u32x4 (&px)[QF][COUNT / 2])
 {
-    float most = sc[0][0];
+    float most[QF];
+    bool past = false;
 #pragma unroll
-    for (int n = 0; n < COUNT; ++n)
+    for (int f = 0; f < QF; ++f) {
+        most[f] = sc[f][0][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most = fmaxf(most, sc[n][i]);
-    most = with_other_rows(most, [](float x, float y) { return fmaxf(x, y); });
-    const float now = fmaxf(top, most);
-    const float base = now == kNone ? 0.f : now * scale_log2;      // (nothing but -inf so far)
-    const float shrink = __builtin_amdgcn_exp2f(fmaf(top, scale_log2, -base));
-    top = now;
-    float part = 0.f;
+        for (int n = 0; n < COUNT; ++n)
 #pragma unroll
-    for (int n = 0; n < COUNT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float2v e;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(sc[n][2 * i + j], scale_log2, -base));
-            part += e[0];
-            part += e[1];
-            px[n >> 1][(n & 1) * 2 + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, half2v));
-        }
-    sum = fmaf(sum, shrink, part);
-    if (__builtin_amdgcn_ballot_w64(shrink != 1.0f) != 0) {
-#pragma unroll
-        for (int d = 0; d < DF; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] *= shrink;
+            for (int i = 0; i < 4; ++i) most[f] = fmaxf(most[f], sc[f][n][i]);
+        past |= most[f] > run[f].limit;
     }
+    if (__builtin_amdgcn_ballot_w64(past) != 0) {
+        const float slack = 8.0f / scale_log2;
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+            const float now = fmaxf(run[f].top, with_other_rows(most[f], [](float x, float y) { return fmaxf(x, y); }));
+            const float base = now == kNone ? 0.f : now * scale_log2;             // (nothing but -inf so far)
+            const float shrink = __builtin_amdgcn_exp2f(fmaf(run[f].top, scale_log2, -base));
+            run[f].top = now;
+            run[f].limit = now + slack;
+            run[f].base = base;
+            run[f].sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < DF; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[f][d][i] *= shrink;
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < QF; ++f)
+#pragma unroll
+        for (int n = 0; n < COUNT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float2v e;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(sc[f][n][2 * i + j], scale_log2, -run[f].base));
+                const half2v two = __builtin_convertvector(e, half2v);
+                run[f].sum = __builtin_amdgcn_fdot2(two, half2v{(_Float16)1.0f, (_Float16)1.0f}, run[f].sum, false);
+                px[f][n >> 1][(n & 1) * 2 + i] = __builtin_bit_cast(uint32_t, two);
+            }
+}
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is a register that the compiler reserves; named all the same, as this writes it)
+// 16 bytes per lane from a buffer's byte `offset` + `more` into LDS at `lds` + 16 * lane, zeros past the buffer's end.  (As assembly, because the
+// compiler would wait for all such loads before any read of LDS; here they are waited for by hand.)
+__device__ __forceinline__ void buffer_to_lds(uint32_t lds, u32x4 buffer, uint32_t offset, uint32_t more)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(offset), "s"(buffer), "s"(more) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// The description of a buffer of `bytes` bytes for such loads.
+__device__ __forceinline__ u32x4 buffer_at(const void* base, int bytes)
+{
+    const unsigned long long at = reinterpret_cast<unsigned long long>(base);
+    return u32x4{(uint32_t)scalar((int)(uint32_t)at), (uint32_t)scalar((int)(uint32_t)(at >> 32) & 0xffff), (uint32_t)scalar(bytes), 0x00020000u};
 }
 
 // A workgroup of four waves holds 64 * QF rows, a wave QF fragments of 16, and walks its units' keys in tiles of KT, one pass.
 // The scores are computed transposed, keys x rows: a lane then holds, for ONE row (lane % 16), four neighbouring keys of every
-// fragment -- the maximum and sum take two cross-lane steps a tile, and what it holds is already its operand of the second product
-// (values^T x probabilities).  The values lie in LDS as they come, rows of a key, and are read by columns (column_read).
+// fragment -- what it holds is already its operand of the second product (values^T x probabilities), and no probability crosses lanes.
+// The values lie in LDS as they come, rows of a key, and are read by columns (column_read).
 // LDS: two buffers of a tile of keys (pieces of 16 bytes swizzled so that the 16 keys of a read hit all banks) and of values (32-byte
-// pairs swizzled so that the eight keys of a read do).  8-bit rows are turned into fp16 between the load and LDS, exactly.  The next
-// tile is on its way into registers while this one is worked on; one barrier a tile.
+// pairs swizzled so that the eight keys of a read do); one barrier a tile.  A wave brings a quarter of a tile's keys, which share a page.
+// fp16 rows go from memory into LDS by themselves, from lane offsets that do not change: a tile costs a wave a page number and two
+// buffer descriptions, and what lies past the sequence's end, outside the buffer, is zero (a key there weighs 0, which would make NaN of a value
+// that is not finite).  8-bit rows pass through registers, where they become fp16, exactly.
 template <int HD, int QF, bool BYTES>
 __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 {
     constexpr int ROWS = 64 * QF, KT = HD == 256 ? 32 : 64, NF = KT / 16, KS = HD / 32, DF = HD / 16;
-    constexpr int KB = KT * HD * 2, BUF = 2 * KB;
-    constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, KL = KT * PIECES / 256;    // of 16 bytes in the pages
+    constexpr int KB = KT * HD * 2, BUF = 2 * KB, KW = KT / 4;    // KW: keys that a wave brings
+    constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, KL = KW * PIECES / 64, KEYS = 64 / PIECES;   // of a load
     __shared__ __align__(16) unsigned char lds[2 * BUF];
     __shared__ int wrong_somewhere;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
@@ -321,70 +368,86 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     if (!begin_walk(a, w)) return;
     auto key_place = [](int key, int p) { return HD == 64 ? p ^ ((key >> 1) & 7) : p ^ (key & 15); };
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
+    const int mask = (1 << a.pages.shift) - 1;
+    // fp16: this lane's bytes within the wave's keys, for each load: where what comes to its place in LDS lies in the page
+    uint32_t key_from[KL], value_from[KL];
+    if constexpr (!BYTES) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+            const int key = wave * KW + i * KEYS + lane / PIECES, p = lane % PIECES;
+            key_from[i] = (uint32_t)(lane / PIECES) * (uint32_t)a.pages.slot_stride * 2u + (uint32_t)key_place(key, p) * 16u;
+            value_from[i] = (uint32_t)(lane / PIECES) * (uint32_t)a.pages.slot_stride * 2u + (uint32_t)(value_place(key, p >> 1) * 2 + (p & 1)) * 16u;
+        }
+    }
+    const uint32_t lds_at = (uint32_t)(uintptr_t)lds;             // (the low half of such an address is the offset in LDS)
     for (;;) {
         const Unit u = unit_of<ROWS, HD>(a, w);
         const int first_tile = (u.first_key + KT - 1) / KT, tiles = (u.end_key + KT - 1) / KT;   // (a share may be empty)
         bool wrong = w.s.wrong;
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
-        const int* ids = a.batch.table + w.b * a.batch.table_stride;
+        const const_u32_ptr ids = as_const(reinterpret_cast<const uint32_t*>(a.batch.table + w.b * a.batch.table_stride));
+        int ahead = 0;                                            // page of this wave's keys of the tile after the next
+        auto ask = [&](int t) { ahead = (int)ids[min(t * KT + wave * KW, w.s.length - 1) >> a.pages.shift]; };
         u32x4 kreg[KL], vreg[KL];
         int kexp[KL], vexp[KL];
-        auto fetch = [&](int t) {
+        auto fetch = [&](int t, int buf) {
+            const bool known = (unsigned)ahead < a.pages.pages;
+            wrong |= !known;
+            const int page = known ? ahead : 0, first = t * KT + wave * KW;
+            const long long at = page * a.pages.page_stride + head_at;
+            if constexpr (BYTES) {
+                const long long exp_at = ((long long)page * a.pages.kv_heads + u.kv_head) << a.pages.shift;
 #pragma unroll
-            for (int i = 0; i < KL; ++i) {
-                const int group_key = t * KT + (i * 256 + wave * 64) / PIECES;              // a wave's rows of one i share a page
-                int page = ids[min(group_key, w.s.length - 1) >> a.pages.shift];
-                page = scalar(page);
-                const bool known = (unsigned)page < a.pages.pages;
-                wrong |= !known;
-                page = known ? page : 0;
-                const int key = group_key + lane / PIECES, slot = min(key, w.s.length - 1) & ((1 << a.pages.shift) - 1);
-                const long long at = page * a.pages.page_stride + head_at;
-                const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)(lane % PIECES) * VALUES;
-                const bool there = key < w.s.length;
-                if constexpr (BYTES) {
+                for (int i = 0; i < KL; ++i) {
+                    const int key = first + i * KEYS + lane / PIECES, slot = min(key, w.s.length - 1) & mask;
+                    const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)(lane % PIECES) * VALUES;
                     kreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.k) + at + within);
-                    vreg[i] = there ? *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.v) + at + within) : u32x4{0u, 0u, 0u, 0u};
-                    const long long e = (((long long)page * a.pages.kv_heads + u.kv_head) << a.pages.shift) + slot;
-                    kexp[i] = a.pages.k_exp[e];
-                    vexp[i] = a.pages.v_exp[e];
-                } else {
-                    kreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const __half*>(a.pages.k) + at + within);
-                    // (a key past the end weighs 0, which would make NaN of a value that is not finite)
-                    vreg[i] = there ? *reinterpret_cast<const u32x4*>(static_cast<const __half*>(a.pages.v) + at + within) : u32x4{0u, 0u, 0u, 0u};
+                    vreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.v) + at + within);
+                    kexp[i] = a.pages.k_exp[exp_at + slot];
+                    vexp[i] = a.pages.v_exp[exp_at + slot];
+                }
+            } else {
+                const int there = min(max(w.s.length - first, 0), KW), step = (int)a.pages.slot_stride * 2;
+                const long long from = (at + (long long)(there ? first & mask : 0) * a.pages.slot_stride) * 2;
+                const u32x4 kbuf = buffer_at(static_cast<const char*>(a.pages.k) + from, there * step), vbuf = buffer_at(static_cast<const char*>(a.pages.v) + from, there * step);
+                const uint32_t to = (uint32_t)scalar((int)(lds_at + buf * BUF + wave * KW * HD * 2));
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    buffer_to_lds(to + i * 1024, kbuf, key_from[i], (uint32_t)(i * KEYS * step));
+                    buffer_to_lds(to + KB + i * 1024, vbuf, value_from[i], (uint32_t)(i * KEYS * step));
                 }
             }
         };
-        auto put = [&](int buf) {
-            unsigned char* kd = lds + buf * BUF;
-            unsigned char* vd = kd + KB;
+        auto put = [&](int t, int buf) {                          // what fetch has asked for is in LDS
+            if constexpr (BYTES) {
+                unsigned char* kd = lds + buf * BUF;
+                unsigned char* vd = kd + KB;
 #pragma unroll
-            for (int i = 0; i < KL; ++i) {
-                const int id = i * 256 + tid, key = id / PIECES, p = id % PIECES;
-                if constexpr (BYTES) {
+                for (int i = 0; i < KL; ++i) {
+                    const int key = wave * KW + i * KEYS + lane / PIECES, p = lane % PIECES;
                     u32x4 lo, hi;
                     sixteen_halves(kreg[i], __uint_as_float((uint32_t)kexp[i] << 23), &lo, &hi);
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p) * 16) = lo;
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p + 1) * 16) = hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
+                    if (t * KT + key >= w.s.length) lo = hi = u32x4{0u, 0u, 0u, 0u};
                     u32x4* v = reinterpret_cast<u32x4*>(vd + key * HD * 2 + value_place(key, p) * 32);
                     v[0] = lo;
                     v[1] = hi;
-                } else {
-                    *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, p) * 16) = kreg[i];
-                    *reinterpret_cast<u32x4*>(vd + key * HD * 2 + value_place(key, p >> 1) * 32 + (p & 1) * 16) = vreg[i];
                 }
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
         };
-        if (first_tile < tiles) fetch(first_tile);
+        if (first_tile < tiles) ask(first_tile);
 
         // ---- the wave's rows ----
         u32x4 qx[QF][KS];
         int last[QF];                                             // the last key that this lane's row sees
-        int wave_last = -1;
+        int wave_last = -1, wave_first = INT_MAX;                 // ... any of the wave's, and all of them
         f32x4 o[QF][DF];
-        float top[QF], sum[QF];
+        Running run[QF];
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const Row x = row_of(a, w, u, wave * 16 * QF + f * 16 + r16);
@@ -392,25 +455,27 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             const __half* row = a.q + (long long)(w.s.start + x.token) * a.q_t + x.head * a.q_h + g * 8;
 #pragma unroll
             for (int s = 0; s < KS; ++s) qx[f][s] = x.there ? *reinterpret_cast<const u32x4*>(row + s * 32) : u32x4{0u, 0u, 0u, 0u};
-            top[f] = kNone;
-            sum[f] = 0.f;
+            run[f] = kNothing;
 #pragma unroll
             for (int d = 0; d < DF; ++d) o[f][d] = f32x4{0.f, 0.f, 0.f, 0.f};
             wave_last = max(wave_last, last[f]);
+            wave_first = min(wave_first, last[f]);
         }
 #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) wave_last = max(wave_last, __shfl_xor(wave_last, off, 64));
+        for (int off = 1; off < 16; off <<= 1) {
+            wave_last = max(wave_last, __shfl_xor(wave_last, off, 64));
+            wave_first = min(wave_first, __shfl_xor(wave_first, off, 64));
+        }
         wave_last = scalar(wave_last);
-        int wave_first = INT_MAX;                                 // the last key that all its rows see
-#pragma unroll
-        for (int f = 0; f < QF; ++f) wave_first = min(wave_first, last[f]);
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) wave_first = min(wave_first, __shfl_xor(wave_first, off, 64));
         wave_first = scalar(wave_first);
 
         __syncthreads();                                          // the unit before is done with LDS
         if (tid == 0) wrong_somewhere = 0;
-        if (first_tile < tiles) put(0);
+        if (first_tile < tiles) {
+            fetch(first_tile, 0);
+            if (first_tile + 1 < tiles) ask(first_tile + 1);
+            put(first_tile, 0);
+        }
         __syncthreads();
 #pragma unroll
         for (int f = 0; f < QF; ++f)
@@ -418,8 +483,12 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qx[f][s]));   // (here before the loop: waited for inside it, the next tile's loads are too)
 
         for (int t = first_tile; t < tiles; ++t) {
-            if (t + 1 < tiles) fetch(t + 1);
-            const unsigned char* ks = lds + ((t - first_tile) & 1) * BUF;
+            const int buf = (t - first_tile) & 1;
+            if (t + 1 < tiles) {
+                fetch(t + 1, buf ^ 1);
+                if (t + 2 < tiles) ask(t + 2);
+            }
+            const unsigned char* ks = lds + buf * BUF;
             const unsigned char* vs = ks + KB;
             if (t * KT <= wave_last) {                            // (a tile of which the wave's rows see nothing is skipped)
                 f32x4 sc[QF][NF];
@@ -441,8 +510,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     }
                 }
                 u32x4 px[QF][NF / 2];
-#pragma unroll
-                for (int f = 0; f < QF; ++f) softmax_step(sc[f], a.scale_log2, top[f], sum[f], o[f], px[f]);
+                softmax_step(sc, a.scale_log2, run, o, px);
 #pragma unroll
                 for (int s = 0; s < NF / 2; ++s)
 #pragma unroll
@@ -456,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     }
             }
             if (t + 1 < tiles) {
-                put((t + 1 - first_tile) & 1);                    // (read last before the barrier of the turn before)
+                put(t + 1, buf ^ 1);                              // (read last before the barrier of the turn before)
                 __syncthreads();
             }
         }
@@ -467,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         for (int f = 0; f < QF; ++f) {
             const int r = wave * 16 * QF + f * 16 + r16;
             const Row x = row_of(a, w, u, r);
-            float all = with_other_rows(sum[f], [](float v, float y) { return v + y; });
+            float all = with_other_rows(run[f].sum, [](float v, float y) { return v + y; });
             if (wrong) all = __builtin_nanf("");
             if (!x.there) continue;
             if (u.whole) {
@@ -484,7 +552,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 float* row = u.piece + r * (HD + 4);
 #pragma unroll
                 for (int d = 0; d < DF; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + g * 4) = o[f][d];
-                if (g == 0) row[HD] = top[f], row[HD + 1] = all;
+                if (g == 0) row[HD] = run[f].top, row[HD + 1] = all;
             }
         }
         if (last_unit(w, u)) {
@@ -492,6 +560,212 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             return;
         }
         if (!next_unit(a, w, u.cost)) return;
+    }
+}
+
+// 16 rows: single tokens, or the few of a group of query heads.  Bound by the pages' bytes.  A workgroup's four waves share out a unit's
+// keys, tile by tile of 32 each, every wave with a softmax of its own; at the unit's end they meet in LDS.  No wave waits for another
+// before: a wave's keys go from memory straight into the registers that its products want, its values through LDS of its own (to be read
+// by columns).  The next tile is asked for as soon as this one's registers are free.  8-bit rows are loaded 16 values to a lane, and
+// the order of the values within a score is free: the queries are loaded to match.
+template <int HD, bool BYTES>
+__global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
+{
+    constexpr int ROWS = 16, KT = 32, KS = HD / 32, DF = HD / 16;
+    constexpr int KL = BYTES ? HD / 64 : KS;                      // 16-byte pieces of a key that a lane loads
+    constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, VL = KT * PIECES / 64, VKEYS = 64 / PIECES;   // keys of one load of values
+    constexpr int LD = HD + 4;
+    __shared__ __align__(16) unsigned char lds[4 * ROWS * LD * 4];                                              // >= 4 * KT * HD * 2
+    __shared__ float tops[4][ROWS], sums[4][ROWS];
+    __shared__ int wrong_somewhere;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    Walk w;
+    if (!begin_walk(a, w)) return;
+    unsigned char* own = lds + wave * KT * HD * 2;
+    auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
+    for (;;) {
+        const Unit u = unit_of<ROWS, HD>(a, w);
+        const int tiles = (u.end_key + KT - 1) / KT, first_tile = (u.first_key + KT - 1) / KT + wave;
+        bool wrong = w.s.wrong;
+        const long long head_at = u.kv_head * a.pages.head_stride;
+        const int* ids = a.batch.table + w.b * a.batch.table_stride;
+        u32x4 kreg[2][KL], vreg[VL];
+        int kexp[2], vexp[VL];
+        int ahead[2];                                             // pages of the next tile's keys
+        auto ask = [&](int t) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) ahead[n] = (int)as_const(reinterpret_cast<const uint32_t*>(ids))[scalar(min(t * KT + n * 16, w.s.length - 1) >> a.pages.shift)];
+        };
+        auto fetch = [&](int t) {
+            long long at[2], exp_at[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const bool known = (unsigned)ahead[n] < a.pages.pages;
+                wrong |= !known;
+                const int page = known ? ahead[n] : 0;
+                at[n] = page * a.pages.page_stride + head_at;
+                exp_at[n] = ((long long)page * a.pages.kv_heads + u.kv_head) << a.pages.shift;
+            }
+            const int mask = (1 << a.pages.shift) - 1;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int slot = min(t * KT + n * 16 + r16, w.s.length - 1) & mask;
+                const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)g * VALUES;
+#pragma unroll
+                for (int s = 0; s < KL; ++s) {
+                    if constexpr (BYTES) kreg[n][s] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.k) + at[n] + within + s * 64);
+                    else kreg[n][s] = *reinterpret_cast<const u32x4*>(static_cast<const __half*>(a.pages.k) + at[n] + within + s * 32);
+                }
+                if constexpr (BYTES) kexp[n] = a.pages.k_exp[exp_at[n] + slot];
+            }
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int n = i * VKEYS / 16, slot = min(t * KT + i * VKEYS + lane / PIECES, w.s.length - 1) & mask;
+                const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)(lane % PIECES) * VALUES;
+                if constexpr (BYTES) {
+                    vreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.v) + at[n] + within);
+                    vexp[i] = a.pages.v_exp[exp_at[n] + slot];
+                } else {
+                    vreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const __half*>(a.pages.v) + at[n] + within);
+                }
+            }
+        };
+        if (first_tile < tiles) {
+            ask(first_tile);
+            fetch(first_tile);
+            if (first_tile + 4 < tiles) ask(first_tile + 4);
+        }
+        const Row x = row_of(a, w, u, r16);
+        const int last = x.there ? w.s.length - w.s.n + x.token : -1;
+        u32x4 qx[KS];
+        const __half* row = a.q + (long long)(w.s.start + x.token) * a.q_t + x.head * a.q_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = BYTES ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
+            qx[s] = x.there ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0u, 0u, 0u, 0u};
+        }
+        f32x4 o[1][DF];
+        Running run[1] = {kNothing};
+#pragma unroll
+        for (int d = 0; d < DF; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
+
+        for (int t = first_tile; t < tiles; t += 4) {
+            const bool ends = t * KT + KT > w.s.length;
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int key = i * VKEYS + lane / PIECES, p = lane % PIECES;
+                // (a key past the end weighs 0, which would make NaN of a value that is not finite)
+                if (ends && t * KT + key >= w.s.length) vreg[i] = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (BYTES) {
+                    u32x4 lo, hi;
+                    sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
+                    u32x4* v = reinterpret_cast<u32x4*>(own + key * HD * 2 + value_place(key, p) * 32);
+                    v[0] = lo;
+                    v[1] = hi;
+                } else {
+                    *reinterpret_cast<u32x4*>(own + key * HD * 2 + value_place(key, p >> 1) * 32 + (p & 1) * 16) = vreg[i];
+                }
+            }
+            f32x4 sc[1][2];
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    u32x4 kx;
+                    if constexpr (BYTES) {
+                        u32x4 both[2];
+                        if (s % 2 == 0) sixteen_halves(kreg[n][s / 2], __uint_as_float((uint32_t)kexp[n] << 23), &both[0], &both[1]), kreg[n][s / 2] = both[1], kx = both[0];
+                        else kx = kreg[n][s / 2];
+                    } else {
+                        kx = kreg[n][s];
+                    }
+                    sc[0][n] = matrix_step<false>(kx, qx[s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[0][n]);
+                }
+            if (t + 4 < tiles) {
+                fetch(t + 4);
+                if (t + 8 < tiles) ask(t + 8);
+            }
+            if (t * KT + KT - 1 > all_see) {
+                const int seen = last - t * KT - g * 4;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[0][n][i] = n * 16 + i <= seen ? sc[0][n][i] : kNone;
+            }
+            u32x4 px[1][1];
+            softmax_step(sc, a.scale_log2, run, o, px);
+#pragma unroll
+            for (int d = 0; d < DF; ++d) {
+                const int key = g * 4 + (r16 >> 2);
+                const unsigned char* from = own + key * HD * 2 + value_place(key, d) * 32 + (r16 & 3) * 8;
+                const uint2 lo = column_read(from), hi = column_read(from + 16 * HD * 2);   // (16 keys on: the same swizzle)
+                o[0][d] = matrix_step<false>(u32x4{lo.x, lo.y, hi.x, hi.y}, px[0][0], o[0][d]);
+            }
+        }
+        // ---- the waves meet ----
+        const float sum = with_other_rows(run[0].sum, [](float v, float y) { return v + y; });
+        if (tid == 0) wrong_somewhere = 0;
+        __syncthreads();                                          // every wave is done with its values
+        float* mine = reinterpret_cast<float*>(lds) + (wave * ROWS + r16) * LD;
+        if (x.there) {
+#pragma unroll
+            for (int d = 0; d < DF; ++d) *reinterpret_cast<f32x4*>(mine + d * 16 + g * 4) = o[0][d];
+            if (g == 0) tops[wave][r16] = run[0].top, sums[wave][r16] = sum;
+        }
+        if (wrong && lane == 0) wrong_somewhere = 1;
+        __syncthreads();
+        {
+            constexpr int EACH = HD / 16;                         // values of a thread
+            const int r = tid >> 4, d = (tid & 15) * 4;           // four values, and those 64 on
+            const Row y = row_of(a, w, u, r);
+            if (y.there) {
+                float most = tops[0][r];
+#pragma unroll
+                for (int i = 1; i < 4; ++i) most = fmaxf(most, tops[i][r]);
+                const float base = most == kNone ? 0.f : most * a.scale_log2;
+                f32x4 v[EACH / 4];
+#pragma unroll
+                for (int j = 0; j < EACH / 4; ++j) v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                float all = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float weight = __builtin_amdgcn_exp2f(fmaf(tops[i][r], a.scale_log2, -base));
+                    all = fmaf(sums[i][r], weight, all);
+                    const float* theirs = reinterpret_cast<const float*>(lds) + (i * ROWS + r) * LD + d;
+#pragma unroll
+                    for (int j = 0; j < EACH / 4; ++j) {
+                        const f32x4 z = *reinterpret_cast<const f32x4*>(theirs + j * 64);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[j][e] = fmaf(z[e], weight, v[j][e]);
+                    }
+                }
+                if (wrong_somewhere) all = __builtin_nanf("");
+                if (u.whole) {
+                    const float inv = all == 0.f ? 0.f : 1.0f / all;   // (no key: 0)
+                    __half* to = a.out + ((long long)(w.s.start + y.token) * a.heads + y.head) * HD + d;
+#pragma unroll
+                    for (int j = 0; j < EACH / 4; ++j) {
+                        __half h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) h[e] = __float2half(v[j][e] * inv);
+                        *reinterpret_cast<uint2*>(to + j * 64) = *reinterpret_cast<const uint2*>(h);
+                    }
+                } else {
+                    float* to = u.piece + r * LD;
+#pragma unroll
+                    for (int j = 0; j < EACH / 4; ++j) *reinterpret_cast<f32x4*>(to + d + j * 64) = v[j];
+                    if (d == 0) to[HD] = most, to[HD + 1] = all;
+                }
+            }
+        }
+        if (last_unit(w, u)) {
+            if (tid == 0) tell_shared(a, w, u);
+            return;
+        }
+        if (!next_unit(a, w, u.cost)) return;
+        __syncthreads();                                          // the unit is done with LDS
     }
 }
 
@@ -553,13 +827,19 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
 
 // What a call takes: rows of a unit, workgroups at most, and the cost below which a part is not cut.
 struct Plan {
-    int rows, workgroups, least;
+    int rows, workgroups, fixed, least;
 };
 
-Plan plan_of(int heads, const tl_pages* pages, int64_t most_rows)
+Plan plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows)
 {
-    (void)heads, (void)pages, (void)most_rows;
-    return Plan{64, (int)ceil_div(2 * compute_units(), 8) * 8, 512};
+    const int group = heads / pages->kv_heads, workgroups = (int)ceil_div(2 * compute_units(), 8) * 8;
+    if (most_rows * group <= 16) return Plan{16, workgroups, 128, 128};
+    // 128 rows to a workgroup read half as much from LDS for a product, 64 have twice as many units: from 2048 keys of 128 rows to a workgroup on, as
+    // far as the host can tell (us with 128 / 64: 4096 rows over 4096, 32 heads on 8: 520 / 617; 723 rows of 8 sequences of up to 3500, 14
+    // heads of 64 on 2: 57 / 43).
+    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;
+    const bool tall = pages->head_dim < 256 && most_rows * group >= 128 && tokens * heads / 128 * keys >= workgroups * 2048ll;
+    return Plan{tall ? 128 : 64, workgroups, 128, 512};
 }
 
 int64_t workspace_of(const Plan& p, int hd)
@@ -578,17 +858,30 @@ int check_heads(int heads, const tl_pages* pages)
 template <int HD, bool BYTES>
 void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
-    hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES>), dim3((unsigned)p.workgroups), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((tl_paged_join<HD, 64>), dim3((unsigned)p.workgroups, 8), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)p.workgroups), block(256);
+    if (p.rows == 16) {
+        hipLaunchKernelGGL((tl_paged_few<HD, BYTES>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((tl_paged_join<HD, 16>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
+        return;
+    }
+    if constexpr (HD < 256) {
+        if (p.rows == 128) {
+            hipLaunchKernelGGL((tl_paged_rows<HD, 2, BYTES>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((tl_paged_join<HD, 128>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((tl_paged_join<HD, 64>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
 }
 
 }  // namespace
 
-extern "C" int tl_paged_attention_workspace(int heads, const tl_pages* pages, int64_t most_rows, int64_t* bytes)
+extern "C" int tl_paged_attention_workspace(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows, int64_t* bytes)
 {
     if (int rc = check_heads(heads, pages)) return rc;
-    if (!bytes || most_rows < 0) return fail(TL_ERR_ARG, "bytes is null or most_rows negative");
-    *bytes = workspace_of(plan_of(heads, pages, most_rows), pages->head_dim);
+    if (!bytes || !batch || most_rows < 0 || tokens < 0) return fail(TL_ERR_ARG, "a pointer is null, or tokens or most_rows negative");
+    *bytes = workspace_of(plan_of(tokens, heads, pages, batch, most_rows), pages->head_dim);
     return TL_OK;
 }
 
@@ -605,7 +898,7 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
     if (most_rows < 0) return fail(TL_ERR_ARG, "most_rows is negative");
     if (!(scale > 0.f) || scale > 3e38f) return fail(TL_ERR_ARG, "scale=%g is not a positive number", (double)scale);
     if (!in_pieces(q, {q_token, q_head}, 2) || !in_pieces(out, {}, 2) || !in_pieces(workspace, {}, 1)) return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
-    const Plan p = plan_of(heads, pages, most_rows);
+    const Plan p = plan_of(tokens, heads, pages, batch, most_rows);
     if (workspace_bytes < workspace_of(p, pages->head_dim))
         return fail(TL_ERR_SIZE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)workspace_of(p, pages->head_dim));
     a.q = static_cast<const __half*>(q), a.q_t = q_token, a.q_h = q_head;
@@ -615,6 +908,7 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
     a.blocks = (int)ceil_div(a.group, a.tile_heads);
     a.tile_tokens = p.rows / a.tile_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
+    a.fixed = p.fixed;
     a.least = p.least;
     a.shared = static_cast<Shared*>(workspace);
     a.pieces = reinterpret_cast<float*>(a.shared + p.workgroups);

@@ -399,7 +399,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
     if (!absent(a[4]) && (!given || given->dim() != 2 || given->size(0) != tokens || given->size(1) != width || given->scalar_type() != at::kHalf ||
                           given->device() != q->device() || !given->is_contiguous() || given->storage().data() == q->storage().data()))
         Py_RETURN_NONE;
-    if (g_attention_workspace((int)q->size(1), &p, most, &need) != TL_OK) Py_RETURN_NONE;
+    if (g_attention_workspace(tokens, (int)q->size(1), &p, &b, most, &need) != TL_OK) Py_RETURN_NONE;
     at::Tensor out = given ? *given : at::empty({tokens, width}, q->options().requires_grad(false));
     at::Tensor ws = at::empty({need}, q->options().dtype(at::kByte).requires_grad(false));
     void* stream = current_stream(q->device());

@@ -826,7 +826,7 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
     _cuda(q, "q")
     need = ctypes.c_int64(0)
     with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().tl_paged_attention_workspace(heads, p, batch.most_rows, ctypes.byref(need)))
+        _lib.check(_lib.lib().tl_paged_attention_workspace(tokens, heads, p, b, batch.most_rows, ctypes.byref(need)))
         # (of the call's own: kept for the next, it would be shared by graphs that were captured on one stream and are replayed on several)
         ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
         _lib.check(_lib.lib().tl_paged_attention(q.data_ptr(), *_steps(q, (0, 1)), code, tokens, heads, p, b, batch.most_rows,

@@ -206,8 +206,8 @@ def attention_bound(q, k, v, want, longest, scale):
     return (2.0 ** -11 + longest * 2.0 ** -25 + score + 64 * 2.0 ** -24) * v.abs().max() + 2.0 ** -11 * want.abs() + 2.0 ** -25
 
 
-def check_attention(both, heads, kv, hd, page, kind, *, front=0, behind=0, most=None, scale=None, seed=1):
-    seqs = paged.Sequences(both, page, front=front, behind=behind, seed=seed)
+def check_attention(both, heads, kv, hd, page, kind, *, front=0, behind=0, most=None, scale=None, seed=1, widest=None):
+    seqs = paged.Sequences(both, page, front=front, behind=behind, seed=seed, widest=widest)
     pages = fresh_pages(seqs, kv, hd, kind, seed=seed)
     q = random((seqs.tokens, heads + 3, hd), seed + 9)[:, 1:1 + heads]
     out = torch.full((seqs.tokens, heads * hd), 3.0, dtype=torch.float16, device="cuda")
@@ -241,6 +241,13 @@ def test_one_row_of_each_sequence(kind, heads, kv, hd, both, page):
     ([(2, 2)], 16), ([(5, 130), (16, 16), (0, 0), (1, 90), (17, 63)], 16), ([(64, 64), (65, 400)], 64), ([(130, 131), (1, 257), (3, 3)], 128)])
 def test_chunks(kind, heads, kv, hd, both, page):
     check_attention(both, heads, kv, hd, page, kind, front=1, behind=2)
+
+
+# 128 rows to a workgroup: a table with room for 64 K tokens, and rows enough for the host to expect as much work
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("heads,kv,hd,page", [(16, 2, 128, 256), (14, 2, 64, 256), (16, 16, 128, 64), (32, 1, 64, 16)])
+def test_tall_workgroups(kind, heads, kv, hd, page):
+    check_attention([(130, 131), (1, 257), (0, 5), (129, 400), (9, 5)], heads, kv, hd, page, kind, front=1, behind=1, widest=65536 // page)
 
 
 @pytest.mark.parametrize("kind", ["float16", "e4m3"])

@@ -182,13 +182,14 @@ def test_no_rows_need_no_addresses(call):
 
 
 def test_workspace_size():
-    need = ctypes.c_int64(0)
-    raw = Raw()
-    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, 1, ctypes.byref(need)) == 0 and need.value > 0
-    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, 1, None) == ARG
-    assert _lib.lib().tl_paged_attention_workspace(3, raw.pages, 1, ctypes.byref(need)) == SHAPE
-    assert _lib.lib().tl_paged_attention_workspace(4, None, 1, ctypes.byref(need)) == ARG
-    assert _lib.lib().tl_paged_attention_workspace(4, raw.pages, -1, ctypes.byref(need)) == ARG
+    need, raw = ctypes.c_int64(0), Raw()
+
+    def ask(tokens=3, heads=4, pages=raw.pages, batch=raw.batch, most=1, to=ctypes.byref(need)):
+        return _lib.lib().tl_paged_attention_workspace(tokens, heads, pages, batch, most, to)
+
+    assert ask() == 0 and need.value > 0
+    assert ask(to=None) == ask(pages=None) == ask(batch=None) == ask(most=-1) == ask(tokens=-1) == ARG
+    assert ask(heads=3) == SHAPE
 
 
 def test_what_the_plain_forms_hold():
