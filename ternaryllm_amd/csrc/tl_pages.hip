@@ -58,28 +58,43 @@ struct RopeHeads {
 
 enum Where { kRows, kHalfPages, kBytePages };   // where keys and values go
 
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// Eight neighbouring values as they lie, and as fp32.
 template <typename T>
-struct EightOf {
-    float v[8];
-    __device__ __forceinline__ void load(const T* p)
-    {
-        if constexpr (sizeof(T) == 2) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+struct Raw {
+    u32x4 a[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> raw_eight(const T* p)
+{
+    Raw<T> r;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f(__builtin_bit_cast(__half, (unsigned short)(a[i >> 1] >> (i & 1) * 16)));
-        } else {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.a[i] = reinterpret_cast<const u32x4*>(p)[i];
+    return r;
+}
+
+struct Eight {
+    float v[8];
+    template <typename T>
+    __device__ __forceinline__ void set(const Raw<T>& r)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 2) v[i] = to_f(__builtin_bit_cast(__half, (unsigned short)(r.a[0][i >> 1] >> (i & 1) * 16)));
+            else v[i] = __uint_as_float(r.a[i >> 2][i & 3]);
         }
     }
     template <typename U>
     __device__ __forceinline__ void store(U* p) const
     {
         if constexpr (sizeof(U) == 2) {
-            __half h[8];
+            u32x4 h;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = from_f<__half>(settled(v[i]));
-            *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(h);
+            for (int i = 0; i < 4; ++i) h[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{settled(v[2 * i]), settled(v[2 * i + 1])}), half2v));
+            *reinterpret_cast<u32x4*>(p) = h;
         } else {
             reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -87,11 +102,26 @@ struct EightOf {
     }
 };
 
-// f over the 2^bits neighbouring lanes that share a head.
+// f over the 2^bits neighbouring lanes that share a head, on the vector unit: lanes a step apart, then mirrored groups, whose values are alike
+// by then.
 template <typename F>
 __device__ __forceinline__ float over_lanes(float x, int bits, F f)
 {
-    for (int off = 1 << bits >> 1; off > 0; off >>= 1) x = f(x, __shfl_xor(x, off, 64));
+    auto with = [&](auto control) {
+        return f(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(control)::value, 0xf, 0xf, true)));
+    };
+    if (bits > 0) x = with(std::integral_constant<int, 0xb1>{});      // 1, 0, 3, 2
+    if (bits > 1) x = with(std::integral_constant<int, 0x4e>{});      // 2, 3, 0, 1
+    if (bits > 2) x = with(std::integral_constant<int, 0x141>{});     // eight lanes mirrored
+    if (bits > 3) x = with(std::integral_constant<int, 0x140>{});     // sixteen
+    if (bits > 4) {
+        const auto near = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(near[0]), __uint_as_float(near[1]));
+    }
+    if (bits > 5) {
+        const auto far = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(far[0]), __uint_as_float(far[1]));
+    }
     return x;
 }
 
@@ -103,16 +133,17 @@ __device__ __forceinline__ int row_exponent(float most)
     return min(max(e, -32), 8);
 }
 
-// Eight codes of x / 2^e.  The conversion rounds to the nearest, ties to even; what is too large for it is held at the largest
-// code that stands for a finite fp16 number, what is not a number stays that.
+// Eight codes of x / 2^e.  The conversion rounds to the nearest, ties to even.  Only in rows of the largest exponent can a value be too large
+// for it: it is held at the largest code that stands for a finite fp16 number.  What is not a number stays that.
 __device__ __forceinline__ uint2 byte_codes(const float* x, int e)
 {
-    const float bound = e == 8 ? 240.0f : 448.0f, scale = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
     float c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = x[i] * scale;
-        c[i] = y != y ? y : fminf(fmaxf(y, -bound), bound);
+    for (int i = 0; i < 8; ++i) c[i] = x[i] * scale;
+    if (e == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = c[i] != c[i] ? c[i] : fminf(fmaxf(c[i], -240.0f), 240.0f);
     }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
@@ -121,22 +152,52 @@ __device__ __forceinline__ uint2 byte_codes(const float* x, int e)
     return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
-// A workgroup takes a token, 2^bits lanes one of its heads, a lane eight neighbouring values.  The token's cosines and sines
-// are made once, for all its heads: the angle in 64 bits, taken modulo a turn there (at position 10^6 an fp32 angle is off by
-// 0.06), its sine and cosine in 32.  A value's partner is another lane's unless pairs are neighbours: rows cross in LDS, within
-// their wave.  Everything is fp32 from the load to the one rounding of the result.
+// A workgroup takes a token, 2^bits lanes one of its heads, a lane eight neighbouring values, a wave at a time heads of queries, of keys or of
+// values.  The token's cosines and sines are made once, for all its heads: the angle in 64 bits, taken modulo a turn there (at position
+// 10^6 an fp32 angle is off by 0.06), its sine and cosine in 32.  A value's partner is another lane's unless pairs are neighbours: rows
+// cross in LDS, within their wave.  Everything is fp32 from the load to the one rounding of the result.
+// Bound by memory, for few tokens by the trips to it in a row (the first kTurns heads of a group of lanes are asked for before the place and the
+// angles are looked for), and nearly by the vector unit: with 280 instructions for eight values, addresses of 64 bits and a kind of head
+// to each lane, 8192 tokens of 32 / 8 / 8 heads into pages of 8 bits took 72 us.
+constexpr int kTurns = 4;
+
 template <typename T, Where W>
 __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
 {
-    __shared__ float turn[2 * kHalf];
-    __shared__ __align__(16) float cross[256 * 8];
-    const int tid = (int)threadIdx.x, token = (int)blockIdx.x;
+    // the cosine and sine of pair i: float4 i / 8 of plane i % 8 / 2; a lane's eight values: half of them in each plane (lanes side by side hit all banks)
+    __shared__ float4 turn[4][kHalf / 8];
+    __shared__ float4 cross[2][256];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), token = (int)blockIdx.x;
+    const int p = lane & ((1 << bits) - 1), d = p * 8, each = 64 >> bits, sub = lane >> bits;   // each: heads of a wave at a time
+    const bool inside = d < a.hd;
+    const int gq = (a.q.heads + each - 1) / each, gk = gq + (a.k.heads + each - 1) / each, groups = gk + (a.v.heads + each - 1) / each;
+    // group g of heads: its kind, this lane's head and the first value's place behind the token's
+    auto kind_of = [&](int g) { return g < gq ? 0 : g < gk ? 1 : 2; };
+    auto head_of = [&](int g) { return (g - (g < gq ? 0 : g < gk ? gq : gk)) * each + sub; };
+    const T* const from[3] = {static_cast<const T*>(a.q.x) + token * a.q.x_t, static_cast<const T*>(a.k.x) + token * a.k.x_t, static_cast<const T*>(a.v.x) + token * a.v.x_t};
+    Raw<T> raw[kTurns];
+    auto ask = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            const int g = first + 4 * i;
+            if (g >= groups) continue;
+            const int h = head_of(g);
+            const unsigned at = (unsigned)h * (unsigned)(g < gq ? a.q.x_h : g < gk ? a.k.x_h : a.v.x_h) + (unsigned)d;
+            if (inside && h < (g < gq ? a.q.heads : g < gk ? a.k.heads : a.v.heads)) raw[i] = raw_eight((g < gq ? from[0] : g < gk ? from[1] : from[2]) + at);
+        }
+    };
+    ask(wave);
+    Raw<T> weight[2];
+    if (inside && a.q.w) weight[0] = raw_eight(static_cast<const T*>(a.q.w) + d);
+    if (inside && a.k.w) weight[1] = raw_eight(static_cast<const T*>(a.k.w) + d);
     Place at{0, 0};
     Slot slot{-1, 0};
     if constexpr (W != kRows) {
         at = place_of(a.batch, token);
         if (at.seq < 0) return;                                 // (the same for every wave)
         slot = slot_of(a.pages, a.batch, at);
+        slot.page = __builtin_amdgcn_readfirstlane(slot.page);
+        slot.slot = __builtin_amdgcn_readfirstlane(slot.slot);
     }
     if (a.pairs) {
         const long long position = a.positions ? a.positions[token] : (long long)at.index;
@@ -145,82 +206,106 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
             turns -= rint(turns);
             float s, c;
             sincospif(2.0f * (float)turns, &s, &c);
-            turn[2 * i] = c * a.factor;
-            turn[2 * i + 1] = s * a.factor;
+            reinterpret_cast<float2*>(&turn[(i & 7) >> 1][i >> 3])[i & 1] = make_float2(c * a.factor, s * a.factor);
         }
         __syncthreads();
     }
-    const int p = tid & ((1 << bits) - 1), d = p * 8, per_pass = 256 >> bits;
-    const bool inside = d < a.hd;
-    const int rows = a.q.heads + a.k.heads + a.v.heads;
-    float* own = cross + (tid & ~((1 << bits) - 1)) * 8;        // this head's row
-    for (int row = tid >> bits; row < rows; row += per_pass) {
-        const int kind = row < a.q.heads ? 0 : row < a.q.heads + a.k.heads ? 1 : 2;
-        const Rows& r = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-        const int h = row - (kind > 0 ? a.q.heads : 0) - (kind > 1 ? a.k.heads : 0);
-        EightOf<T> x;
-        if (inside) x.load(static_cast<const T*>(r.x) + token * r.x_t + h * r.x_h + d);
-        else
+    const int row = tid - p;                                    // this head's first lane, among all
+    const bool whole = (a.pairs & 7) == 0;                      // the halves of a head are whole lanes
+    const float part = 1.0f / (float)a.hd;
+    for (int first = wave; first < groups; first += 4 * kTurns) {
+        if (first > wave) ask(first);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x.v[i] = 0.f;
-        if (kind < 2) {
-            if (r.w) {
+        for (int i = 0; i < kTurns; ++i) {
+            const int g = first + 4 * i;
+            if (g >= groups) break;
+            const int kind = kind_of(g), h = head_of(g);
+            const bool there = inside && h < (kind == 0 ? a.q.heads : kind == 1 ? a.k.heads : a.v.heads);
+            Eight x;
+            if (there) x.set(raw[i]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x.v[j] = 0.f;
+            if (kind < 2 && (kind == 0 ? a.q.w : a.k.w)) {
                 float squares = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) squares = fmaf(x.v[i], x.v[i], squares);
+                for (int j = 0; j < 8; ++j) squares = fmaf(x.v[j], x.v[j], squares);
                 squares = over_lanes(squares, bits, [](float u, float v) { return u + v; });
-                const float inv = 1.0f / sqrtf(squares / (float)a.hd + a.eps);
-                EightOf<T> w;
-                if (inside) {
-                    w.load(static_cast<const T*>(r.w) + d);
+                const float inv = rsqrtf(fmaf(squares, part, a.eps));
+                Eight w;
+                w.set(kind == 0 ? weight[0] : weight[1]);
+                if (there) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x.v[i] = x.v[i] * inv * w.v[i];
+                    for (int j = 0; j < 8; ++j) x.v[j] *= inv * w.v[j];
                 }
             }
-            if (a.interleaved) {
+            if (kind < 2 && a.interleaved) {
+                if (d < 2 * a.pairs) {
+                    const float4 t[2] = {turn[p & 1 ? 2 : 0][p >> 1], turn[p & 1 ? 3 : 1][p >> 1]};
+                    const float cs[8] = {t[0].x, t[0].y, t[0].z, t[0].w, t[1].x, t[1].y, t[1].z, t[1].w};
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const int pair = (d + i) >> 1;
-                    if (pair < a.pairs) {
-                        const float c = turn[2 * pair], s = turn[2 * pair + 1], lo = x.v[i], hi = x.v[i + 1];
-                        x.v[i] = lo * c - hi * s;
-                        x.v[i + 1] = hi * c + lo * s;
+                    for (int j = 0; j < 8; j += 2) {
+                        if (d + j < 2 * a.pairs) {
+                            const float c = cs[j], s = cs[j + 1], lo = x.v[j], hi = x.v[j + 1];
+                            x.v[j] = fmaf(lo, c, -(hi * s));
+                            x.v[j + 1] = fmaf(hi, c, lo * s);
+                        }
                     }
                 }
-            } else if (a.pairs) {
-                reinterpret_cast<float4*>(own + d)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
-                reinterpret_cast<float4*>(own + d)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+            } else if (kind < 2 && a.pairs) {
+                cross[0][tid] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+                cross[1][tid] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
+                if (whole) {
+                    if (d < 2 * a.pairs) {
+                        const bool low = d < a.pairs;
+                        const int other = low ? d + a.pairs : d - a.pairs, chunk = (low ? d : other) >> 3;
+                        const float4 y0 = cross[0][row + (other >> 3)], y1 = cross[1][row + (other >> 3)];
+                        const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+                        const uint32_t sign = low ? 0x80000000u : 0u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool low = d + i < a.pairs;
-                    const int pair = low ? d + i : d + i - a.pairs;
-                    if (pair < a.pairs) {
-                        const float c = turn[2 * pair], s = turn[2 * pair + 1], other = own[low ? pair + a.pairs : pair];
-                        x.v[i] = low ? x.v[i] * c - other * s : x.v[i] * c + other * s;
+                        for (int j = 0; j < 4; ++j) {
+                            const float4 t = turn[j][chunk];
+                            x.v[2 * j] = fmaf(x.v[2 * j], t.x, __uint_as_float(__float_as_uint(y[2 * j] * t.y) ^ sign));
+                            x.v[2 * j + 1] = fmaf(x.v[2 * j + 1], t.z, __uint_as_float(__float_as_uint(y[2 * j + 1] * t.w) ^ sign));
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool low = d + j < a.pairs;
+                        const int pair = low ? d + j : d + j - a.pairs;
+                        if (pair < a.pairs) {
+                            const int other = low ? pair + a.pairs : pair;
+                            const float2 t = reinterpret_cast<const float2*>(&turn[(pair & 7) >> 1][pair >> 3])[pair & 1];
+                            const float y = reinterpret_cast<const float*>(&cross[(other & 7) >> 2][row + (other >> 3)])[other & 3] * t.y;
+                            x.v[j] = fmaf(x.v[j], t.x, low ? -y : y);
+                        }
                     }
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
             }
-        }
-        if (W == kRows || kind == 0) {
-            if (inside) x.store(static_cast<T*>(r.y) + token * r.y_t + h * r.y_h + d);
-        } else if constexpr (W != kRows) {
-            const long long to = slot.page * a.pages.page_stride + h * a.pages.head_stride + slot.slot * a.pages.slot_stride + d;
-            void* base = kind == 1 ? a.pages.k : a.pages.v;
-            if constexpr (W == kHalfPages) {
-                if (inside && slot.page >= 0) x.store(static_cast<__half*>(base) + to);
-            } else {
-                float most = 0.f;
+            if (W == kRows || kind == 0) {
+                T* to = kind == 0 ? static_cast<T*>(a.q.y) + token * a.q.y_t : static_cast<T*>(a.k.y) + token * a.k.y_t;
+                if (there) x.store(to + ((unsigned)h * (unsigned)(kind == 0 ? a.q.y_h : a.k.y_h) + (unsigned)d));
+            } else if constexpr (W != kRows) {
+                const long long page = slot.page * a.pages.page_stride + slot.slot * a.pages.slot_stride;
+                void* base = kind == 1 ? a.pages.k : a.pages.v;
+                const long long to = page + h * a.pages.head_stride + d;
+                if constexpr (W == kHalfPages) {
+                    if (there && slot.page >= 0) x.store(static_cast<__half*>(base) + to);
+                } else {
+                    float most = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x.v[i]));
-                most = over_lanes(most, bits, [](float u, float v) { return fmaxf(u, v); });
-                const int e = row_exponent(most);
-                if (inside && slot.page >= 0) {
-                    *reinterpret_cast<uint2*>(static_cast<unsigned char*>(base) + to) = byte_codes(x.v, e);
-                    if (p == 0) (kind == 1 ? a.pages.k_exp : a.pages.v_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot] = (unsigned char)(e + 127);
+                    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x.v[j]));
+                    most = over_lanes(most, bits, [](float u, float v) { return fmaxf(u, v); });
+                    const int e = row_exponent(most);
+                    if (there && slot.page >= 0) {
+                        *reinterpret_cast<uint2*>(static_cast<unsigned char*>(base) + to) = byte_codes(x.v, e);
+                        if (p == 0) (kind == 1 ? a.pages.k_exp : a.pages.v_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot] = (unsigned char)(e + 127);
+                    }
                 }
             }
         }
@@ -234,47 +319,63 @@ struct ReadPages {
     long long out_t, out_h;
 };
 
-// A workgroup takes a token, 2^bits lanes one of its rows, a lane eight values.  Bound by memory.
+// A wave takes a token, 2^bits lanes one of its rows, a lane 16 bytes of it in the pages; its rows are asked for several at a time.  Bound by
+// memory: while a workgroup took a token, four of these waves of a row of the trips to memory that find its page, 65536 tokens of 8 heads in
+// 8 bits were 104 us.
 template <typename T, bool BYTES>
 __global__ __launch_bounds__(256) void tl_read_pages_k(ReadPages a, int bits)
 {
-    const int tid = (int)threadIdx.x, token = (int)blockIdx.x;
+    constexpr int VALUES = BYTES ? 16 : 8, TURNS = 4;
+    const int lane = (int)threadIdx.x & 63, token = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
+    if (token >= a.batch.tokens) return;
     const Place at = place_of(a.batch, token);
     if (at.seq < 0) return;
     const Slot slot = slot_of(a.pages, a.batch, at);
-    const int d = (tid & ((1 << bits) - 1)) * 8;
+    const int d = (lane & ((1 << bits) - 1)) * VALUES, per_turn = 64 >> bits, rows = 2 * a.pages.kv_heads;
     if (d >= a.pages.hd) return;
-    for (int row = tid >> bits; row < 2 * a.pages.kv_heads; row += 256 >> bits) {
-        const int which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
-        T* out = static_cast<T*>(which ? a.v_out : a.k_out);
-        if (!out) continue;
-        EightOf<__half> x;
-        if (slot.page < 0) {
+    for (int first = lane >> bits; first < rows; first += TURNS * per_turn) {
+        u32x4 raw[TURNS];
+        int e[TURNS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x.v[i] = __builtin_nanf("");
-        } else {
+        for (int i = 0; i < TURNS; ++i) {
+            const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
+            if (row >= rows || slot.page < 0) continue;
             const long long from = slot.page * a.pages.page_stride + h * a.pages.head_stride + slot.slot * a.pages.slot_stride + d;
-            const void* base = which ? a.pages.v : a.pages.k;
-            if constexpr (BYTES) {
-                const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(base) + from);
-                const int e = (which ? a.pages.v_exp : a.pages.k_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot];
-                const float scale = ldexpf(1.0f, e - 127);
-                const auto a0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false), a1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
-                const auto a2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false), a3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
-                x.v[0] = a0[0] * scale, x.v[1] = a0[1] * scale, x.v[2] = a1[0] * scale, x.v[3] = a1[1] * scale;
-                x.v[4] = a2[0] * scale, x.v[5] = a2[1] * scale, x.v[6] = a3[0] * scale, x.v[7] = a3[1] * scale;
-            } else {
-                x.load(static_cast<const __half*>(base) + from);
-            }
+            raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(which ? a.pages.v : a.pages.k) + from * (BYTES ? 1 : 2));
+            if constexpr (BYTES) e[i] = (which ? a.pages.v_exp : a.pages.k_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot];
         }
-        x.store(out + token * a.out_t + h * a.out_h + d);
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
+            T* out = static_cast<T*>(which ? a.v_out : a.k_out);
+            if (row >= rows || !out) continue;
+            out += token * a.out_t + h * a.out_h + d;
+            Eight x[VALUES / 8];
+            if (slot.page < 0) {
+#pragma unroll
+                for (int j = 0; j < VALUES; ++j) x[j / 8].v[j % 8] = __builtin_nanf("");
+            } else if constexpr (BYTES) {
+                const float scale = ldexpf(1.0f, e[i] - 127);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], true);
+                    float* v = x[j / 2].v + j % 2 * 4;
+                    v[0] = lo[0] * scale, v[1] = lo[1] * scale, v[2] = hi[0] * scale, v[3] = hi[1] * scale;
+                }
+            } else {
+                x[0].set(Raw<__half>{{raw[i]}});
+            }
+#pragma unroll
+            for (int j = 0; j < VALUES / 8; ++j) x[j].store(out + j * 8);
+        }
     }
 }
 
-int lane_bits(int hd)
+// Lanes of a head of which each has `values`, as a power of two.
+int lane_bits(int hd, int values)
 {
     int bits = 0;
-    while (8 << bits < hd) ++bits;
+    while (values << bits < hd) ++bits;
     return bits;
 }
 
@@ -288,6 +389,8 @@ int take_rows(const tl_head_rows* r, int64_t es, int64_t tokens, bool out, Rows*
     if (tokens > 0 && (!r->x || (out && !r->y))) return fail(TL_ERR_ARG, "device pointer is null");
     if (!in_pieces(r->x, {r->x_token, r->x_head}, es) || (out && !in_pieces(r->y, {r->y_token, r->y_head}, es)) || !in_pieces(r->norm_weight, {}, es))
         return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
+    const int64_t reach = std::max(r->x_head, out ? r->y_head : 0);
+    if (r->x_head < 0 || (out && r->y_head < 0) || reach * r->heads > INT32_MAX) return fail(TL_ERR_SHAPE, "a token's heads must lie within 2^31 elements, in order");
     *to = Rows{r->x, r->x_token, r->x_head, r->y, r->y_token, r->y_head, r->norm_weight, r->heads};
     return TL_OK;
 }
@@ -311,7 +414,7 @@ template <typename T>
 void launch_rope(const RopeHeads& a, Where where, int64_t tokens, hipStream_t st)
 {
     const dim3 grid((unsigned)tokens), block(256);
-    const int bits = lane_bits(a.hd);
+    const int bits = lane_bits(a.hd, 8);
     if (where == kRows) hipLaunchKernelGGL((tl_rope_heads_k<T, kRows>), grid, block, 0, st, a, bits);
     else if (where == kHalfPages) hipLaunchKernelGGL((tl_rope_heads_k<T, kHalfPages>), grid, block, 0, st, a, bits);
     else hipLaunchKernelGGL((tl_rope_heads_k<T, kBytePages>), grid, block, 0, st, a, bits);
@@ -366,10 +469,10 @@ extern "C" int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, 
     if (!in_pieces(k_out, {out_token, out_head}, es) || !in_pieces(v_out, {}, es)) return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
     a.k_out = k_out, a.v_out = v_out, a.out_t = out_token, a.out_h = out_head;
     if (tokens == 0 || a.batch.seqs == 0 || (!k_out && !v_out)) return TL_OK;
-    const dim3 grid((unsigned)tokens), block(256);
-    const int bits = lane_bits(a.pages.hd);
-    hipStream_t st = static_cast<hipStream_t>(stream);
     const bool bytes = pages->dtype == TL_E4M3;
+    const dim3 grid((unsigned)ceil_div(tokens, 4)), block(256);
+    const int bits = lane_bits(a.pages.hd, bytes ? 16 : 8);
+    hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == TL_F16) {
         if (bytes) hipLaunchKernelGGL((tl_read_pages_k<__half, true>), grid, block, 0, st, a, bits);
         else hipLaunchKernelGGL((tl_read_pages_k<__half, false>), grid, block, 0, st, a, bits);
