@@ -770,36 +770,56 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
 }
 
 // Joins the pieces of the units that were shared out: blockIdx.x is the workgroup in which one begins.  HD / 4 lanes take a row, four
-// values each, and 1024 / HD of them at a time its pieces.
+// values each.  Of a unit of a few pieces 1024 / HD rows are joined at a time; where they are many, as of a single long sequence, one row by as many
+// groups of lanes, which share the pieces out.
 template <int HD, int ROWS>
 __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
 {
-    constexpr int LANES = HD / 4, AT_ONCE = 256 / LANES;
+    constexpr int LANES = HD / 4, AT_ONCE = 256 / LANES, FEW = 6;
     __shared__ float4 part[256];
     __shared__ float tops[AT_ONCE], sums[AT_ONCE];
-    const Shared sh = a.shared[blockIdx.x];
+    Shared sh = a.shared[blockIdx.x];
+    sh.last = scalar(sh.last);
     if (sh.last < 0) return;
     Walk w{};
-    w.b = sh.seq, w.head = sh.head, w.tile = sh.tile;
-    w.s = sequence(a, w.b);
+    w.b = scalar(sh.seq), w.head = scalar(sh.head), w.tile = scalar(sh.tile);
+    w.s = scalar(sequence(a, w.b));
     const Unit u = unit_of<ROWS, HD>(a, w);
     const int first = (int)blockIdx.x, count = sh.last - first + 1;
     const int lane = (int)threadIdx.x % LANES, own = (int)threadIdx.x / LANES;
+    float4 o;
+    float top, sum;
+    auto start = [&] { o = make_float4(0.f, 0.f, 0.f, 0.f), top = kNone, sum = 0.f; };
+    auto add = [&](int i, int r) {
+        const float* piece = a.pieces + (((long long)(first + i) * 2 + (i == 0 ? 1 : 0)) * ROWS + r) * (HD + 4);
+        const float m = piece[HD], l = piece[HD + 1];
+        const float4 v = *reinterpret_cast<const float4*>(piece + lane * 4);
+        const float now = fmaxf(top, m), base = now == kNone ? 0.f : now * a.scale_log2;
+        const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -base));
+        o = make_float4(o.x * old + v.x * fresh, o.y * old + v.y * fresh, o.z * old + v.z * fresh, o.w * old + v.w * fresh);
+        sum = sum * old + l * fresh;
+        top = now;
+    };
+    auto finish = [&](const Row& x) {
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;          // (no key: 0)
+        const __half h[4] = {__float2half(o.x * inv), __float2half(o.y * inv), __float2half(o.z * inv), __float2half(o.w * inv)};
+        *reinterpret_cast<uint2*>(a.out + ((long long)(w.s.start + x.token) * a.heads + x.head) * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
+    };
+    if (count <= FEW) {
+        for (int r = (int)blockIdx.y * AT_ONCE + own; r < ROWS; r += (int)gridDim.y * AT_ONCE) {
+            const Row x = row_of(a, w, u, r);
+            if (!x.there) continue;
+            start();
+            for (int i = 0; i < count; ++i) add(i, r);
+            finish(x);
+        }
+        return;
+    }
     for (int r = (int)blockIdx.y; r < ROWS; r += (int)gridDim.y) {
         const Row x = row_of(a, w, u, r);
         if (!x.there) continue;                                   // (the same for all)
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float top = kNone, sum = 0.f;
-        for (int i = own; i < count; i += AT_ONCE) {
-            const float* piece = a.pieces + (((long long)(first + i) * 2 + (i == 0 ? 1 : 0)) * ROWS + r) * (HD + 4);
-            const float m = piece[HD], l = piece[HD + 1];
-            const float4 v = *reinterpret_cast<const float4*>(piece + lane * 4);
-            const float now = fmaxf(top, m), base = now == kNone ? 0.f : now * a.scale_log2;
-            const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -base));
-            o = make_float4(o.x * old + v.x * fresh, o.y * old + v.y * fresh, o.z * old + v.z * fresh, o.w * old + v.w * fresh);
-            sum = sum * old + l * fresh;
-            top = now;
-        }
+        start();
+        for (int i = own; i < count; i += AT_ONCE) add(i, r);
         __syncthreads();                                          // the row before is done with LDS
         part[threadIdx.x] = o;
         if (lane == 0) tops[own] = top, sums[own] = sum;
@@ -809,18 +829,15 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
 #pragma unroll
             for (int i = 1; i < AT_ONCE; ++i) most = fmaxf(most, tops[i]);
             const float base = most == kNone ? 0.f : most * a.scale_log2;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            float all = 0.f;
+            start();
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
                 const float weight = __builtin_amdgcn_exp2f(fmaf(tops[i], a.scale_log2, -base));
                 const float4 v = part[i * LANES + lane];
-                y = make_float4(y.x + v.x * weight, y.y + v.y * weight, y.z + v.z * weight, y.w + v.w * weight);
-                all += sums[i] * weight;
+                o = make_float4(o.x + v.x * weight, o.y + v.y * weight, o.z + v.z * weight, o.w + v.w * weight);
+                sum += sums[i] * weight;
             }
-            const float inv = all == 0.f ? 0.f : 1.0f / all;
-            const __half h[4] = {__float2half(y.x * inv), __float2half(y.y * inv), __float2half(y.z * inv), __float2half(y.w * inv)};
-            *reinterpret_cast<uint2*>(a.out + ((long long)(w.s.start + x.token) * a.heads + x.head) * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
+            finish(x);
         }
     }
 }
