@@ -33,6 +33,45 @@ def rope_tables(positions, head_dim, theta, dtype, device):
     return ang.cos().to(dtype), ang.sin().to(dtype)
 
 
+def rope_frequencies(rotary_dim, theta, scaling=None, device=None):
+    """(frequencies, factor) for ops.rope_heads and ops.rope_to_pages: theta^(-2 i / rotary_dim), float64 [rotary_dim / 2], and what cosines and
+    sines are multiplied by, as scaled for long contexts by `scaling`, a dictionary with the names of a `transformers` configuration's
+    rope_parameters -- rope_type
+      "default"  nothing;
+      "linear"   positions divided by factor;
+      "llama3"   frequencies whose wave is longer than original_max_position_embeddings / low_freq_factor divided by factor, those shorter than
+                 original_max_position_embeddings / high_freq_factor kept, between the two a mean weighted by the number of waves;
+      "yarn"     divided by factor where fewer than beta_slow (1) waves fit the original length, kept from beta_fast (32) on, a ramp over the
+                 dimensions between (Peng et al. 2023), and attention_factor, 0.1 ln(factor) + 1, on cosines and sines."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim={rotary_dim} must be positive and even")
+    scaling = scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    f = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    factor = 1.0
+    if kind == "linear":
+        f = f / scaling["factor"]
+    elif kind == "llama3":
+        waves = scaling["original_max_position_embeddings"] * f / (2 * math.pi)
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        kept = ((waves - low) / (high - low)).clamp(0, 1)
+        f = kept * f + (1 - kept) * f / scaling["factor"]
+    elif kind == "yarn":
+        def dimension(waves):   # the pair of which so many waves fit the original length
+            return rotary_dim * math.log(scaling["original_max_position_embeddings"] / (2 * math.pi * waves)) / (2 * math.log(theta))
+
+        low = max(math.floor(dimension(scaling.get("beta_fast") or 32)), 0)
+        high = min(math.ceil(dimension(scaling.get("beta_slow") or 1)), rotary_dim - 1)
+        kept = 1 - ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        f = kept * f + (1 - kept) * f / scaling["factor"]
+        factor = scaling.get("attention_factor")
+        if factor is None:
+            factor = 0.1 * math.log(scaling["factor"]) + 1 if scaling["factor"] > 1 else 1.0
+    elif kind != "default":
+        raise ValueError(f"rope_type {kind!r} is not known")
+    return f.to(device), float(factor)
+
+
 def apply_rope(x, cos, sin):
     """x: [batch, heads, seq, head_dim]; cos/sin: [seq, head_dim] or [batch, seq, head_dim]."""
     half = x.shape[-1] // 2
@@ -232,5 +271,5 @@ def replace_linear_layers(layers, attn, sparsity=0.8, *, generator=None, referen
     torch.cuda.empty_cache()
 
 
-__all__ = ["LlamaTernaryAttention", "TwoResultAttention", "rope_tables", "apply_rope", "collect_attn_linear_layers",
+__all__ = ["LlamaTernaryAttention", "TwoResultAttention", "rope_tables", "rope_frequencies", "apply_rope", "collect_attn_linear_layers",
            "replace_linear_layers"]

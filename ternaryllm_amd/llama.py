@@ -21,7 +21,9 @@ import torch
 from torch import nn
 
 from . import _lib, ops, packing
+from .attention import rope_frequencies
 from .linear import TernaryLinear
+from .paged import PagedCache
 
 
 def _draw_ternary(K, N, sparsity, generator, device):
@@ -446,6 +448,75 @@ class TernaryLlamaDecoder(nn.Module):
                 break
             self.decode_once(st, use_graph)
         return out
+
+    # -- sequences of different lengths over pages ----------------------------------------------
+    def paged_cache(self, pages, page_size=64, dtype=torch.float16):
+        """A PagedCache for this decoder: `pages` pages in every layer, float16 or float8_e4m3fn."""
+        c = self.config
+        return PagedCache(c.num_hidden_layers, pages, c.num_attention_heads, c.head_dim, page_size, dtype, self.embed_tokens.device)
+
+    @torch.no_grad()
+    def extend(self, cache, chunks):
+        """A pass over new tokens of sequences of any lengths: chunks = [(sequence of `cache`, LongTensor of its new tokens, one or more), ...].
+        Their keys and values go into the cache; returns the logits of each chunk's last token, [chunks, vocab]."""
+        if not chunks or any(t.dim() != 1 or t.numel() == 0 for _, t in chunks):
+            raise ValueError("every chunk is a sequence and a one-dimensional tensor of one or more new tokens")
+        if any(cache.length(s) + t.numel() > self.max_seq_len for s, t in chunks):
+            raise ValueError("a sequence would be longer than max_seq_len")
+        batch = cache.extend([(s, t.numel()) for s, t in chunks])
+        return self.extend_batch(cache, torch.cat([t for _, t in chunks]).to(self.embed_tokens.device), batch)
+
+    @torch.no_grad()
+    def extend_batch(self, cache, tokens, batch):
+        """extend for an ops.PageBatch that the caller keeps (cache.extend makes one): tokens [rows].  No part of it is done on the host, so it
+        can be captured in a graph; the batch's tensors may then hold other sequences and lengths at every replay, for as many rows and
+        sequences.  Rows of no sequence are computed and mean nothing."""
+        c = self.config
+        nh, hd = c.num_attention_heads, c.head_dim
+        if self.dtype != torch.float16 or hd not in (64, 128, 256) or c.hidden_size != nh * hd:
+            raise RuntimeError("sequences over pages need a float16 decoder with heads of 64, 128 or 256")
+        f = getattr(self, "_frequencies", None)
+        if f is None or f.device != tokens.device:
+            f = self._frequencies = rope_frequencies(hd, c.rope_theta, device=tokens.device)[0]
+        fused = self._norms_as_built()
+
+        def add_norm(x, y, norm):
+            if fused:
+                return ops.add_rmsnorm(x, y, norm.weight, norm.eps)
+            x = x if y is None else x + y
+            return x, norm(x)
+
+        # (rows of no sequence: what an attention leaves there must not be what the memory held, which the products behind it may not take)
+        a = torch.zeros((tokens.shape[0], c.hidden_size), dtype=self.dtype, device=tokens.device)
+        x = self.embed_tokens[tokens]
+        _, h = add_norm(x, None, self.layers[0].input_layernorm)
+        for li, layer in enumerate(self.layers):
+            q, k, v = layer.qkv_proj(h).view(-1, 3, nh, hd).unbind(1)
+            pages = cache.layer(li)
+            q = ops.rope_to_pages(q, k, v, pages, batch, f)
+            ops.paged_attention(q, pages, batch, out=a)
+            x, h = add_norm(x, layer.o_proj(a), layer.post_attention_layernorm)
+            y = self._mlp(layer, h)
+            x, h = add_norm(x, y, self.layers[li + 1].input_layernorm if li + 1 < len(self.layers) else self.norm)
+        last = (batch.starts[1:].long() - 1).clamp(min=0)
+        return self.lm_head(h.index_select(0, last))
+
+    @torch.no_grad()
+    def adopt(self, cache, sequences):
+        """Copies sequences of one length out of a PagedCache into the decoder's own cache, as a batch: `generate`'s single-token steps
+        (decode_once) can go on from there.  Returns the length."""
+        lengths = {cache.length(s) for s in sequences}
+        if len(lengths) != 1 or max(lengths) > self.max_seq_len:
+            raise ValueError("the sequences must be of one length that the decoder's cache holds")
+        n, B = lengths.pop(), len(sequences)
+        if self._cache is None or self._cache.shape[2] != B:
+            self.allocate_cache(B)
+        for b, s in enumerate(sequences if n else ()):
+            batch = cache.whole([s])
+            for li in range(len(self.layers)):
+                k, v = (self._cache[li, w, b, :, :n].transpose(0, 1) for w in (0, 1))
+                ops.read_pages(cache.layer(li), batch, n, self.dtype, k_out=k, v_out=v)
+        return n
 
     def _decode_state(self, B):
         dev = self.embed_tokens.device

@@ -205,3 +205,112 @@ def test_what_the_plain_forms_hold():
     for _, b, at, page, slot in seqs.rows():
         pool[page, 0, slot, 0] = 100 * b + at
     assert seqs.held(0, pool)[38:].flatten().tolist() == [38, 39] and seqs.held(1, pool)[15].item() == 115 and seqs.held(2, pool).shape == (0, 1, 1)
+
+
+# ---------------------------------------------------------------- what the host keeps
+def test_sequences_hold_the_pages_that_they_need():
+    from ternaryllm_amd import PagedCache
+    cache = PagedCache(2, 6, 2, 64, 16, device="cpu")
+    a, b = cache.open(), cache.open()
+    batch = cache.extend([(a, 17), (b, 3)])
+    assert batch.starts.tolist() == [0, 17, 20] and batch.lengths.tolist() == [17, 3] and batch.most_rows == 17 and batch.table.shape == (2, 2)
+    assert all(t.dtype == torch.int32 for t in batch[:3]) and cache.free_pages == 3
+    held = set(batch.table[0].tolist()) | {batch.table[1, 0].item()}
+    assert len(held) == 3 and held <= set(range(6))
+    again = cache.extend([(b, 1), (a, 15)])                      # b first; both within their pages
+    assert again.lengths.tolist() == [4, 32] and cache.free_pages == 3 and again.table[1].tolist() == batch.table[0].tolist()
+    with pytest.raises(RuntimeError):
+        cache.extend([(a, 48), (b, 13)])                          # four pages of three; nothing changes
+    assert cache.free_pages == 3 and cache.length(a) == 32 and cache.length(b) == 4
+    cache.truncate(a, 16)
+    assert cache.free_pages == 4 and cache.length(a) == 16
+    whole = cache.whole([a, b])
+    assert whole.starts.tolist() == [0, 16, 20] and whole.lengths.tolist() == [16, 4]
+    cache.close(a)
+    assert cache.free_pages == 5
+    c = cache.open()
+    assert c not in (a, b) and cache.length(c) == 0 and cache.extend([(c, 0), (b, 0)]).most_rows == 0
+    for bad in ([], [(a, 1)], [(b, 1), (b, 1)], [(b, -1)]):
+        with pytest.raises(ValueError):
+            cache.extend(bad)
+    for length in (-1, 5):
+        with pytest.raises(ValueError):
+            cache.truncate(b, length)
+    assert cache.length(b) == 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float8_e4m3fn])
+def test_layers_of_a_paged_cache(dtype):
+    from ternaryllm_amd import PagedCache
+    cache = PagedCache(3, 4, 2, 32, 32, dtype, device="cpu")
+    layers = [cache.layer(i) for i in range(3)]
+    for p in layers:
+        assert p.k.dtype == p.v.dtype == dtype and p.k.shape == p.v.shape == (4, 2, 32, 32) and (p.k_exponents is None) == (dtype == torch.float16)
+        if p.k_exponents is not None:
+            assert p.k_exponents.shape == p.v_exponents.shape == (4, 2, 32) and p.k_exponents.is_contiguous()
+    assert len({p.k.data_ptr() for p in layers} | {p.v.data_ptr() for p in layers}) == 6
+
+
+@pytest.mark.parametrize("change", [{"dtype": torch.float32}, {"page_size": 24}, {"page_size": 8}, {"page_size": 2048}, {"pages": 0}, {"layers": 0}, {"head_dim": 40}])
+def test_paged_caches_that_are_refused(change):
+    from ternaryllm_amd import PagedCache
+    with pytest.raises(ValueError):
+        PagedCache(**{**dict(layers=1, pages=2, kv_heads=1, head_dim=64, device="cpu"), **change})
+
+
+SCALINGS = [
+    None, {"rope_type": "default"}, {"rope_type": "linear", "factor": 4.0},
+    {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 8192},
+    {"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096},
+    {"rope_type": "yarn", "factor": 2.5, "original_max_position_embeddings": 1000, "beta_fast": 20, "beta_slow": 2, "attention_factor": 0.75}]
+
+
+@pytest.mark.parametrize("scaling", SCALINGS)
+@pytest.mark.parametrize("rotary,theta", [(128, 10000.0), (64, 500000.0), (20, 10000.0)])
+def test_rope_frequencies(scaling, rotary, theta):
+    from ternaryllm_amd.attention import rope_frequencies
+    got, factor = rope_frequencies(rotary, theta, scaling)
+    assert got.dtype == torch.float64 and got.shape == (rotary // 2,)
+    kind = (scaling or {}).get("rope_type", "default")
+    for i in range(rotary // 2):                                  # dimension by dimension, from the definition
+        f = theta ** (-2 * i / rotary)
+        if kind == "linear":
+            f /= scaling["factor"]
+        if kind == "llama3":
+            length, wave = scaling["original_max_position_embeddings"], 2 * math.pi / f
+            if wave > length / scaling["low_freq_factor"]:
+                f /= scaling["factor"]
+            elif wave >= length / scaling["high_freq_factor"]:
+                part = (length / wave - scaling["low_freq_factor"]) / (scaling["high_freq_factor"] - scaling["low_freq_factor"])
+                f = (1 - part) * f / scaling["factor"] + part * f
+        if kind == "yarn":
+            edges = [rotary * math.log(scaling["original_max_position_embeddings"] / (2 * math.pi * n)) / (2 * math.log(theta))
+                     for n in (scaling.get("beta_fast", 32), scaling.get("beta_slow", 1))]
+            low, high = max(math.floor(edges[0]), 0), min(math.ceil(edges[1]), rotary - 1)
+            ramp = min(max((i - low) / (high - low), 0.0), 1.0)
+            f = f / scaling["factor"] * ramp + f * (1 - ramp)
+        assert abs(got[i].item() / f - 1) < 1e-12
+    assert factor == (1.0 if kind != "yarn" else scaling.get("attention_factor") or 0.1 * math.log(scaling["factor"]) + 1)
+
+
+@pytest.mark.parametrize("scaling", [s for s in SCALINGS if s and s["rope_type"] != "default"])
+def test_rope_frequencies_are_those_of_transformers(scaling):
+    utils = pytest.importorskip("transformers.modeling_rope_utils")
+    transformers = pytest.importorskip("transformers")
+    from ternaryllm_amd.attention import rope_frequencies
+    try:
+        cfg = transformers.LlamaConfig(hidden_size=1024, num_attention_heads=8, max_position_embeddings=65536, rope_parameters={"rope_theta": 10000.0, **scaling})
+        cfg.rope_parameters
+    except Exception:
+        pytest.skip("a release whose configurations have no rope_parameters")
+    want, factor = utils.ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")
+    got, mine = rope_frequencies(128, 10000.0, scaling)
+    # theirs are fp32 throughout: a power, a quotient and a weighted mean
+    assert (got / want.double() - 1).abs().max() < 2.0 ** -20 and abs(mine - factor) < 1e-6
+
+
+def test_rope_frequencies_refuses():
+    from ternaryllm_amd.attention import rope_frequencies
+    for args in ((0, 1e4), (7, 1e4), (8, 1e4, {"rope_type": "no such"})):
+        with pytest.raises(ValueError):
+            rope_frequencies(*args)
