@@ -37,6 +37,7 @@ struct PagedAttn {
     float scale_log2;                            // of the scores, times log2(e)
     int fixed;                                   // cost of a unit beside its keys
     int least;                                   // cost of a workgroup's part, 1 or more
+    int uncut;                                   // units go to one workgroup whole
     float* pieces;                               // [workgroups][2][rows][head_dim + 4]
     Shared* shared;                              // [workgroups]
 };
@@ -80,13 +81,6 @@ __device__ __forceinline__ long long tiles_cost(const PagedAttn& a, int before, 
     return (long long)tiles * (a.fixed + before) + (long long)a.tile_tokens * tiles * (tiles + 1ll) / 2;
 }
 
-__device__ __forceinline__ long long seq_cost(const PagedAttn& a, int b)
-{
-    if (b >= a.batch.seqs) return 0;
-    const Seq s = sequence(a, b);
-    return tiles_cost(a, s.before, s.tiles) * (a.pages.kv_heads * a.blocks);
-}
-
 // The workgroup's part of the list, and where it stands in it.
 struct Walk {
     int wg, wgs;                                 // this workgroup, and how many have a part
@@ -96,35 +90,56 @@ struct Walk {
     Seq s;
 };
 
+__device__ __forceinline__ long long unit_cost(const PagedAttn& a, const Walk& w) { return a.fixed + (long long)w.s.before + (w.tile + 1ll) * a.tile_tokens; }
+
+// a * b / c rounded down, for a * b < 2^53 (exact then: a quotient below an integer by 1 / c at least does not round to it; a division of 64-bit
+// integers takes several times as long).
+__device__ __forceinline__ long long share_of(long long a, long long b, long long c) { return (long long)((double)(a * b) / (double)c); }
+
+__device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long cost);
+
 // By a whole workgroup of 256 threads.  False where it has no part.
 __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
 {
     __shared__ long long sums[4];
     __shared__ long long found_at;
     __shared__ int found_b;
+    __shared__ Seq found;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr int kPass = 256 * kSeqsOfThread;
-    const int seqs = a.batch.seqs;
+    const int seqs = a.batch.seqs, heads = a.pages.kv_heads * a.blocks;
+    Seq s[kSeqsOfThread];
     long long cost[kSeqsOfThread], upto = 0, total = 0, pass = 0;
-    // costs of this thread's sequences from `first` on, and the sum of all before and of its own
+    // this thread's sequences from `first` on, what they cost, and the sum of all before and of its own
     auto look = [&](int first) {
         long long own = 0;
 #pragma unroll
-        for (int i = 0; i < kSeqsOfThread; ++i) own += cost[i] = seq_cost(a, first + tid * kSeqsOfThread + i);
-        upto = own;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const long long below = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += below;
+        for (int i = 0; i < kSeqsOfThread; ++i) {
+            const int b = first + tid * kSeqsOfThread + i;
+            cost[i] = 0;
+            if (b < seqs) {
+                s[i] = sequence(a, b);
+                cost[i] = tiles_cost(a, s[i].before, s[i].tiles) * heads;
+            }
+            own += cost[i];
         }
-        __syncthreads();
-        if (lane == 63) sums[wave] = upto;
-        __syncthreads();
-        pass = 0;
+        upto = own;
+        if (seqs - first > kSeqsOfThread) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i < wave) upto += sums[i];
-            pass += sums[i];
+            for (int off = 1; off < 64; off <<= 1) {
+                const long long below = __shfl_up(upto, off, 64);
+                if (lane >= off) upto += below;
+            }
+        }
+        if (seqs > kPass) __syncthreads();       // the pass before is done with the sums
+        if (lane == 63) sums[wave] = upto;
+        if (tid == 0 && seqs - first <= kSeqsOfThread) sums[0] = upto;
+        __syncthreads();
+        pass = sums[0];
+        if (seqs - first > 64 * kSeqsOfThread) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) upto += i < wave ? sums[i] : 0;
+            pass += sums[1] + sums[2] + sums[3];
         }
     };
     for (int first = 0; first < seqs; first += kPass) {
@@ -134,7 +149,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     total = scalar(total);
     // as many parts as there are workgroups, but none of less than `least`; neighbours of the list stay in one part of the chip, whose
     // cache they share
-    w.wgs = (int)min((total + a.least - 1) / a.least, (long long)gridDim.x);
+    w.wgs = (int)min(share_of(total + a.least - 1, 1, a.least), (long long)gridDim.x);
     const int eighth = (w.wgs + 7) / 8, inside = (int)blockIdx.x / 8;
     w.wg = inside < eighth ? ((int)blockIdx.x & 7) * eighth + inside : (int)blockIdx.x;
     if (w.wg >= w.wgs) {
@@ -142,8 +157,8 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
         return false;
     }
     w.total = total;
-    w.from = total * w.wg / w.wgs;
-    w.to = total * (w.wg + 1) / w.wgs;
+    w.from = scalar(share_of(total, w.wg, w.wgs));
+    w.to = scalar(share_of(total, w.wg + 1, w.wgs));
     long long below = 0;
     for (int first = 0;; first += kPass) {
         if (seqs > kPass) look(first);
@@ -152,7 +167,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
         for (int i = kSeqsOfThread - 1; i >= 0; --i) {
             const long long ends = begins;
             begins -= cost[i];
-            if (begins <= w.from && w.from < ends) found_b = first + tid * kSeqsOfThread + i, found_at = begins;
+            if (begins <= w.from && w.from < ends) found_b = first + tid * kSeqsOfThread + i, found_at = begins, found = s[i];
         }
         below += pass;
         if (w.from < below) break;               // (the same for all: the list ends behind the part)
@@ -160,9 +175,9 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     __syncthreads();
     w.b = scalar(found_b);
     w.at = scalar(found_at);
-    w.s = scalar(sequence(a, w.b));
+    w.s = scalar(found);
     const long long head_cost = tiles_cost(a, w.s.before, w.s.tiles);
-    w.head = (int)((w.from - w.at) / head_cost);
+    w.head = scalar((int)((double)(w.from - w.at) / (double)head_cost));
     w.at += w.head * head_cost;
     int low = 0, high = w.s.tiles - 1;           // the last unit that begins no later
     while (low < high) {
@@ -172,7 +187,8 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     }
     w.tile = low;
     w.at += tiles_cost(a, w.s.before, low);
-    return true;
+    // units that are not cut belong to the part in which they begin
+    return !(a.uncut && w.at < w.from) || next_unit(a, w, unit_cost(a, w));
 }
 
 // On to the next unit; false behind the last of the part.
@@ -191,6 +207,12 @@ __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long
     return true;
 }
 
+// A walk as it was put into LDS, for all lanes alike: it is needed between units only, and would fill the scalar registers while one is worked on.
+__device__ __forceinline__ Walk scalar(const Walk& k)
+{
+    return Walk{scalar(k.wg), scalar(k.wgs), scalar(k.total), scalar(k.from), scalar(k.to), scalar(k.at), scalar(k.b), scalar(k.head), scalar(k.tile), scalar(k.s)};
+}
+
 // The present unit as one workgroup has it.
 struct Unit {
     long long cost;
@@ -204,16 +226,16 @@ template <int ROWS, int HD>
 __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
 {
     Unit u;
-    u.cost = a.fixed + (long long)w.s.before + (w.tile + 1ll) * a.tile_tokens;
+    u.cost = unit_cost(a, w);
     u.first_token = w.tile * a.tile_tokens;
     u.kv_head = w.head / a.blocks;
     u.first_head = (w.head - u.kv_head * a.blocks) * a.tile_heads;
     const int seen = max(w.s.length - w.s.n + min(u.first_token + a.tile_tokens, w.s.n), 0);   // by its last row
-    u.begins = w.at >= w.from;
-    const bool ends = w.at + u.cost <= w.to;
+    u.begins = a.uncut || w.at >= w.from;
+    const bool ends = a.uncut || w.at + u.cost <= w.to;
     u.whole = u.begins && ends;
     // (its keys in proportion to its cost)
-    auto cut = [&](long long at) { return min((int)((at - w.at) * seen / u.cost + kRound - 1) / kRound * kRound, seen); };
+    auto cut = [&](long long at) { return min((int)(share_of(at - w.at, seen, u.cost) + kRound - 1) / kRound * kRound, seen); };
     u.first_key = u.begins ? 0 : cut(w.from);
     u.end_key = ends ? seen : cut(w.to);
     u.piece = a.pieces + ((long long)w.wg * 2 + (u.begins ? 1 : 0)) * ROWS * (HD + 4);
@@ -224,7 +246,12 @@ __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
 __device__ __forceinline__ void tell_shared(const PagedAttn& a, const Walk& w, const Unit& u)
 {
     Shared s{w.b, w.head, w.tile, -1};
-    if (u.begins && !u.whole) s.last = (int)(((w.at + u.cost) * w.wgs + w.total - 1) / w.total) - 1;
+    if (u.begins && !u.whole) {
+        const long long end = w.at + u.cost;
+        s.last = (int)share_of(end, w.wgs, w.total);              // or one beside it: the last whose part begins before the unit's end
+        while (s.last + 1 < w.wgs && share_of(w.total, s.last + 1, w.wgs) < end) ++s.last;
+        while (share_of(w.total, s.last, w.wgs) >= end) --s.last;
+    }
     a.shared[w.wg] = s;
 }
 
@@ -281,6 +308,20 @@ struct Running {
 
 constexpr Running kNothing{kNone, kNone, 0.f, 0.f};
 
+// Eight sums times `by` where `moves` says so.  (As assembly with a branch of its own: around a branch of the compiler's it keeps the sums in two
+// sets of registers and copies all of them from the one to the other at every tile.  The matrix products that made the sums are done: the scores
+// that moved the reference come from later ones.  Those that follow want two steps between a write and their read.)
+__device__ __forceinline__ void scale_if(int moves, float by, f32x4& x, f32x4& y)
+{
+    float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    asm volatile("s_cmp_eq_u32 %8, 0\n\ts_cbranch_scc1 .Lkeep%=\n\t"
+                 "v_mul_f32 %0, %9, %0\n\tv_mul_f32 %1, %9, %1\n\tv_mul_f32 %2, %9, %2\n\tv_mul_f32 %3, %9, %3\n\t"
+                 "v_mul_f32 %4, %9, %4\n\tv_mul_f32 %5, %9, %5\n\tv_mul_f32 %6, %9, %6\n\tv_mul_f32 %7, %9, %7\n.Lkeep%=:\n\ts_nop 1"
+                 : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]) : "s"(moves), "v"(by) : "scc");
+    x = f32x4{v[0], v[1], v[2], v[3]};
+    y = f32x4{v[4], v[5], v[6], v[7]};
+}
+
 // Scores of QF rows and COUNT fragments of 16 keys in, probabilities out (as the operand of the product with the values).
 template <int QF, int COUNT, int DF>
 __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale_log2, Running (&run)[QF], f32x4 (&o)[QF][DF], u32x4 (&px)[QF][COUNT / 2])
@@ -296,23 +337,27 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
             for (int i = 0; i < 4; ++i) most[f] = fmaxf(most[f], sc[f][n][i]);
         past |= most[f] > run[f].limit;
     }
-    if (__builtin_amdgcn_ballot_w64(past) != 0) {
+    const int moves = scalar((int)__popcll(__builtin_amdgcn_ballot_w64(past)));
+    float shrink[QF];
+#pragma unroll
+    for (int f = 0; f < QF; ++f) shrink[f] = 1.0f;
+    if (moves) {
         const float slack = 8.0f / scale_log2;
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const float now = fmaxf(run[f].top, with_other_rows(most[f], [](float x, float y) { return fmaxf(x, y); }));
             const float base = now == kNone ? 0.f : now * scale_log2;             // (nothing but -inf so far)
-            const float shrink = __builtin_amdgcn_exp2f(fmaf(run[f].top, scale_log2, -base));
+            shrink[f] = __builtin_amdgcn_exp2f(fmaf(run[f].top, scale_log2, -base));
             run[f].top = now;
             run[f].limit = now + slack;
             run[f].base = base;
-            run[f].sum *= shrink;
-#pragma unroll
-            for (int d = 0; d < DF; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[f][d][i] *= shrink;
+            run[f].sum *= shrink[f];
         }
     }
+#pragma unroll
+    for (int f = 0; f < QF; ++f)
+#pragma unroll
+        for (int d = 0; d < DF; d += 2) scale_if(moves, shrink[f], o[f][d], o[f][d + 1]);
 #pragma unroll
     for (int f = 0; f < QF; ++f)
 #pragma unroll
@@ -362,6 +407,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, KL = KW * PIECES / 64, KEYS = 64 / PIECES;   // of a load
     __shared__ __align__(16) unsigned char lds[2 * BUF];
     __shared__ int wrong_somewhere;
+    __shared__ Walk kept;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
@@ -381,26 +427,29 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     }
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;             // (the low half of such an address is the offset in LDS)
     for (;;) {
-        const Unit u = unit_of<ROWS, HD>(a, w);
+        Unit u = unit_of<ROWS, HD>(a, w);
         const int first_tile = (u.first_key + KT - 1) / KT, tiles = (u.end_key + KT - 1) / KT;   // (a share may be empty)
         bool wrong = w.s.wrong;
+        const int length = w.s.length;
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
-        const const_u32_ptr ids = as_const(reinterpret_cast<const uint32_t*>(a.batch.table + w.b * a.batch.table_stride));
-        int ahead = 0;                                            // page of this wave's keys of the tile after the next
-        auto ask = [&](int t) { ahead = (int)ids[min(t * KT + wave * KW, w.s.length - 1) >> a.pages.shift]; };
+        // page of this wave's keys of the tile after the next (by a vector load: a scalar one would be waited for with the first read of LDS)
+        const int* ids = a.batch.table + w.b * a.batch.table_stride;
+        int ahead = 0;
+        auto ask = [&](int t) { ahead = ids[min(t * KT + wave * KW, length - 1) >> a.pages.shift]; };
         u32x4 kreg[KL], vreg[KL];
         int kexp[KL], vexp[KL];
         auto fetch = [&](int t, int buf) {
-            const bool known = (unsigned)ahead < a.pages.pages;
+            const int number = scalar(ahead);
+            const bool known = (unsigned)number < a.pages.pages;
             wrong |= !known;
-            const int page = known ? ahead : 0, first = t * KT + wave * KW;
+            const int page = known ? number : 0, first = t * KT + wave * KW;
             const long long at = page * a.pages.page_stride + head_at;
             if constexpr (BYTES) {
                 const long long exp_at = ((long long)page * a.pages.kv_heads + u.kv_head) << a.pages.shift;
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
-                    const int key = first + i * KEYS + lane / PIECES, slot = min(key, w.s.length - 1) & mask;
+                    const int key = first + i * KEYS + lane / PIECES, slot = min(key, length - 1) & mask;
                     const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)(lane % PIECES) * VALUES;
                     kreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.k) + at + within);
                     vreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.v) + at + within);
@@ -408,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     vexp[i] = a.pages.v_exp[exp_at + slot];
                 }
             } else {
-                const int there = min(max(w.s.length - first, 0), KW), step = (int)a.pages.slot_stride * 2;
+                const int there = min(max(length - first, 0), KW), step = (int)a.pages.slot_stride * 2;
                 const long long from = (at + (long long)(there ? first & mask : 0) * a.pages.slot_stride) * 2;
                 const u32x4 kbuf = buffer_at(static_cast<const char*>(a.pages.k) + from, there * step), vbuf = buffer_at(static_cast<const char*>(a.pages.v) + from, there * step);
                 const uint32_t to = (uint32_t)scalar((int)(lds_at + buf * BUF + wave * KW * HD * 2));
@@ -431,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p) * 16) = lo;
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p + 1) * 16) = hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
-                    if (t * KT + key >= w.s.length) lo = hi = u32x4{0u, 0u, 0u, 0u};
+                    if (t * KT + key >= length) lo = hi = u32x4{0u, 0u, 0u, 0u};
                     u32x4* v = reinterpret_cast<u32x4*>(vd + key * HD * 2 + value_place(key, p) * 32);
                     v[0] = lo;
                     v[1] = hi;
@@ -470,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         wave_first = scalar(wave_first);
 
         __syncthreads();                                          // the unit before is done with LDS
-        if (tid == 0) wrong_somewhere = 0;
+        if (tid == 0) wrong_somewhere = 0, kept = w;
         if (first_tile < tiles) {
             fetch(first_tile, 0);
             if (first_tile + 1 < tiles) ask(first_tile + 1);
@@ -482,55 +531,87 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 #pragma unroll
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qx[f][s]));   // (here before the loop: waited for inside it, the next tile's loads are too)
 
-        for (int t = first_tile; t < tiles; ++t) {
-            const int buf = (t - first_tile) & 1;
+        // the next tile on its way, and in LDS; the tiles of which the wave's rows see nothing, which come last, are brought and no more
+        auto before = [&](int t) {
             if (t + 1 < tiles) {
-                fetch(t + 1, buf ^ 1);
+                fetch(t + 1, (t + 1 - first_tile) & 1);
                 if (t + 2 < tiles) ask(t + 2);
             }
-            const unsigned char* ks = lds + buf * BUF;
-            const unsigned char* vs = ks + KB;
-            if (t * KT <= wave_last) {                            // (a tile of which the wave's rows see nothing is skipped)
-                f32x4 sc[QF][NF];
-#pragma unroll
-                for (int i = 0; i < NF * KS; ++i) {
-                    const int s = HD == 64 ? i % KS : i / NF, n = HD == 64 ? i / KS : i % NF, key = n * 16 + r16;
-                    const u32x4 kx = *reinterpret_cast<const u32x4*>(ks + key * HD * 2 + key_place(key, s * 4 + g) * 16);
-#pragma unroll
-                    for (int f = 0; f < QF; ++f) sc[f][n] = matrix_step<false>(kx, qx[f][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[f][n]);
-                }
-                if (t * KT + KT - 1 > wave_first) {               // some row of the wave does not see all of the tile
-#pragma unroll
-                    for (int f = 0; f < QF; ++f) {
-                        const int seen = last[f] - t * KT - g * 4;
-#pragma unroll
-                        for (int n = 0; n < NF; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) sc[f][n][i] = n * 16 + i <= seen ? sc[f][n][i] : kNone;
-                    }
-                }
-                u32x4 px[QF][NF / 2];
-                softmax_step(sc, a.scale_log2, run, o, px);
-#pragma unroll
-                for (int s = 0; s < NF / 2; ++s)
-#pragma unroll
-                    for (int d = 0; d < DF; ++d) {
-                        const int key = s * 32 + g * 4 + (r16 >> 2);
-                        const unsigned char* from = vs + key * HD * 2 + value_place(key, d) * 32 + (r16 & 3) * 8;
-                        const uint2 x = column_read(from), y = column_read(from + 16 * HD * 2);   // (16 keys on: the same swizzle)
-                        const u32x4 vx{x.x, x.y, y.x, y.y};
-#pragma unroll
-                        for (int f = 0; f < QF; ++f) o[f][d] = matrix_step<false>(vx, px[f][s], o[f][d]);
-                    }
-            }
+        };
+        auto behind = [&](int t) {
             if (t + 1 < tiles) {
-                put(t + 1, buf ^ 1);                              // (read last before the barrier of the turn before)
+                put(t + 1, (t + 1 - first_tile) & 1);             // (read last before the barrier of the turn before)
                 __syncthreads();
             }
+        };
+        const int seen_tiles = min(tiles, wave_last / KT + (wave_last >= 0 ? 1 : 0));
+        int t = first_tile;
+        for (; t < seen_tiles; ++t) {
+            before(t);
+            const unsigned char* ks = lds + ((t - first_tile) & 1) * BUF;
+            const unsigned char* vs = ks + KB;
+            f32x4 sc[QF][NF];
+            // NF fragments of keys a step, the next ones read while these are multiplied.  (Left to the compiler all reads move to the front and
+            // fill the registers, until it copies the sums at every branch.)
+            u32x4 kx[2][NF];
+            auto keys = [&](int s, u32x4* to) {
+#pragma unroll
+                for (int n = 0; n < NF; ++n) to[n] = *reinterpret_cast<const u32x4*>(ks + (n * 16 + r16) * HD * 2 + key_place(r16, s * 4 + g) * 16);
+            };
+            keys(0, kx[0]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s + 1 < KS) keys(s + 1, kx[(s + 1) & 1]);
+#pragma unroll
+                for (int n = 0; n < NF; ++n)
+#pragma unroll
+                    for (int f = 0; f < QF; ++f) sc[f][n] = matrix_step<false>(kx[s & 1][n], qx[f][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[f][n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (t * KT + KT - 1 > wave_first) {               // some row of the wave does not see all of the tile
+#pragma unroll
+                for (int f = 0; f < QF; ++f) {
+                    const int seen = last[f] - t * KT - g * 4;
+#pragma unroll
+                    for (int n = 0; n < NF; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[f][n][i] = n * 16 + i <= seen ? sc[f][n][i] : kNone;
+                }
+            }
+            u32x4 px[QF][NF / 2];
+            softmax_step(sc, a.scale_log2, run, o, px);
+            constexpr int VG = 4, GROUPS = NF / 2 * DF / VG;  // values: VG fragments a step
+            u32x4 vx[2][VG];
+            auto values = [&](int i, u32x4* to) {
+#pragma unroll
+                for (int j = 0; j < VG; ++j) {
+                    const int key = i * VG / DF * 32 + g * 4 + (r16 >> 2), d = i * VG % DF + j;
+                    const unsigned char* from = vs + key * HD * 2 + value_place(g * 4 + (r16 >> 2), d) * 32 + (r16 & 3) * 8;
+                    const uint2 x = column_read(from), y = column_read(from + 16 * HD * 2);   // (16 keys on: the same swizzle)
+                    to[j] = u32x4{x.x, x.y, y.x, y.y};
+                }
+            };
+            values(0, vx[0]);
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                if (i + 1 < GROUPS) values(i + 1, vx[(i + 1) & 1]);
+#pragma unroll
+                for (int j = 0; j < VG; ++j)
+#pragma unroll
+                    for (int f = 0; f < QF; ++f) o[f][i * VG % DF + j] = matrix_step<false>(vx[i & 1][j], px[f][i * VG / DF], o[f][i * VG % DF + j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            behind(t);
+        }
+        for (; t < tiles; ++t) {
+            before(t);
+            behind(t);
         }
         if (wrong && lane == 0) wrong_somewhere = 1;
         __syncthreads();
         wrong = wrong_somewhere != 0;
+        w = scalar(kept);
+        u = unit_of<ROWS, HD>(a, w);
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const int r = wave * 16 * QF + f * 16 + r16;
@@ -569,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 // by columns).  The next tile is asked for as soon as this one's registers are free.  8-bit rows are loaded 16 values to a lane, and
 // the order of the values within a score is free: the queries are loaded to match.
 template <int HD, bool BYTES>
-__global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn a)
 {
     constexpr int ROWS = 16, KT = 32, KS = HD / 32, DF = HD / 16;
     constexpr int KL = BYTES ? HD / 64 : KS;                      // 16-byte pieces of a key that a lane loads
@@ -578,6 +659,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
     __shared__ __align__(16) unsigned char lds[4 * ROWS * LD * 4];                                              // >= 4 * KT * HD * 2
     __shared__ float tops[4][ROWS], sums[4][ROWS];
     __shared__ int wrong_somewhere;
+    __shared__ Walk kept;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
@@ -585,9 +667,11 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
     unsigned char* own = lds + wave * KT * HD * 2;
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
     for (;;) {
-        const Unit u = unit_of<ROWS, HD>(a, w);
+        Unit u = unit_of<ROWS, HD>(a, w);
+        if (tid == 0) kept = w;
         const int tiles = (u.end_key + KT - 1) / KT, first_tile = (u.first_key + KT - 1) / KT + wave;
         bool wrong = w.s.wrong;
+        const int length = w.s.length;
         const long long head_at = u.kv_head * a.pages.head_stride;
         const int* ids = a.batch.table + w.b * a.batch.table_stride;
         u32x4 kreg[2][KL], vreg[VL];
@@ -595,7 +679,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
         int ahead[2];                                             // pages of the next tile's keys
         auto ask = [&](int t) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) ahead[n] = (int)as_const(reinterpret_cast<const uint32_t*>(ids))[scalar(min(t * KT + n * 16, w.s.length - 1) >> a.pages.shift)];
+            for (int n = 0; n < 2; ++n) ahead[n] = (int)as_const(reinterpret_cast<const uint32_t*>(ids))[scalar(min(t * KT + n * 16, length - 1) >> a.pages.shift)];
         };
         auto fetch = [&](int t) {
             long long at[2], exp_at[2];
@@ -610,7 +694,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
             const int mask = (1 << a.pages.shift) - 1;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int slot = min(t * KT + n * 16 + r16, w.s.length - 1) & mask;
+                const int slot = min(t * KT + n * 16 + r16, length - 1) & mask;
                 const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)g * VALUES;
 #pragma unroll
                 for (int s = 0; s < KL; ++s) {
@@ -621,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
             }
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
-                const int n = i * VKEYS / 16, slot = min(t * KT + i * VKEYS + lane / PIECES, w.s.length - 1) & mask;
+                const int n = i * VKEYS / 16, slot = min(t * KT + i * VKEYS + lane / PIECES, length - 1) & mask;
                 const unsigned within = (unsigned)slot * (unsigned)a.pages.slot_stride + (unsigned)(lane % PIECES) * VALUES;
                 if constexpr (BYTES) {
                     vreg[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(a.pages.v) + at[n] + within);
@@ -652,12 +736,12 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
         const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
 
         for (int t = first_tile; t < tiles; t += 4) {
-            const bool ends = t * KT + KT > w.s.length;
+            const bool ends = t * KT + KT > length;
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
                 const int key = i * VKEYS + lane / PIECES, p = lane % PIECES;
                 // (a key past the end weighs 0, which would make NaN of a value that is not finite)
-                if (ends && t * KT + key >= w.s.length) vreg[i] = u32x4{0u, 0u, 0u, 0u};
+                if (ends && t * KT + key >= length) vreg[i] = u32x4{0u, 0u, 0u, 0u};
                 if constexpr (BYTES) {
                     u32x4 lo, hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
@@ -708,6 +792,8 @@ __global__ __launch_bounds__(256, 2) void tl_paged_few(PagedAttn a)
         const float sum = with_other_rows(run[0].sum, [](float v, float y) { return v + y; });
         if (tid == 0) wrong_somewhere = 0;
         __syncthreads();                                          // every wave is done with its values
+        w = scalar(kept);
+        u = unit_of<ROWS, HD>(a, w);
         float* mine = reinterpret_cast<float*>(lds) + (wave * ROWS + r16) * LD;
         if (x.there) {
 #pragma unroll
@@ -790,15 +876,28 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
     float4 o;
     float top, sum;
     auto start = [&] { o = make_float4(0.f, 0.f, 0.f, 0.f), top = kNone, sum = 0.f; };
-    auto add = [&](int i, int r) {
-        const float* piece = a.pieces + (((long long)(first + i) * 2 + (i == 0 ? 1 : 0)) * ROWS + r) * (HD + 4);
-        const float m = piece[HD], l = piece[HD + 1];
-        const float4 v = *reinterpret_cast<const float4*>(piece + lane * 4);
-        const float now = fmaxf(top, m), base = now == kNone ? 0.f : now * a.scale_log2;
-        const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -base));
-        o = make_float4(o.x * old + v.x * fresh, o.y * old + v.y * fresh, o.z * old + v.z * fresh, o.w * old + v.w * fresh);
-        sum = sum * old + l * fresh;
-        top = now;
+    // pieces i, i + step, ... of a row, four on their way at a time
+    auto add = [&](int i, int step, int r) {
+        for (; i < count; i += 4 * step) {
+            float m[4], l[4];
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int n = min(i + k * step, count - 1);
+                const float* piece = a.pieces + (((long long)(first + n) * 2 + (n == 0 ? 1 : 0)) * ROWS + r) * (HD + 4);
+                m[k] = piece[HD], l[k] = piece[HD + 1];
+                v[k] = *reinterpret_cast<const float4*>(piece + lane * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i + k * step >= count) break;
+                const float now = fmaxf(top, m[k]), base = now == kNone ? 0.f : now * a.scale_log2;
+                const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m[k], a.scale_log2, -base));
+                o = make_float4(o.x * old + v[k].x * fresh, o.y * old + v[k].y * fresh, o.z * old + v[k].z * fresh, o.w * old + v[k].w * fresh);
+                sum = sum * old + l[k] * fresh;
+                top = now;
+            }
+        }
     };
     auto finish = [&](const Row& x) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;          // (no key: 0)
@@ -810,7 +909,7 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
             const Row x = row_of(a, w, u, r);
             if (!x.there) continue;
             start();
-            for (int i = 0; i < count; ++i) add(i, r);
+            add(0, 1, r);
             finish(x);
         }
         return;
@@ -819,7 +918,7 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
         const Row x = row_of(a, w, u, r);
         if (!x.there) continue;                                   // (the same for all)
         start();
-        for (int i = own; i < count; i += AT_ONCE) add(i, r);
+        add(own, AT_ONCE, r);
         __syncthreads();                                          // the row before is done with LDS
         part[threadIdx.x] = o;
         if (lane == 0) tops[own] = top, sums[own] = sum;
@@ -842,21 +941,25 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
     }
 }
 
-// What a call takes: rows of a unit, workgroups at most, and the cost below which a part is not cut.
+// What a call takes: rows of a unit, workgroups at most, the cost of a unit beside its keys, the cost below which a part is not cut, and whether units
+// are not cut at all.
 struct Plan {
-    int rows, workgroups, fixed, least;
+    int rows, workgroups, fixed, least, uncut;
 };
 
 Plan plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows)
 {
-    const int group = heads / pages->kv_heads, workgroups = (int)ceil_div(2 * compute_units(), 8) * 8;
-    if (most_rows * group <= 16) return Plan{16, workgroups, 128, 128};
+    const int group = heads / pages->kv_heads, hd = pages->head_dim;
+    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;   // of a sequence, at most
+    auto workgroups = [](int each) { return (int)ceil_div(each * compute_units(), 8) * 8; };
+    // units of few keys are not cut, which saves the second launch
+    const int uncut = keys <= 1024;
+    if (most_rows * group <= 16) return Plan{16, workgroups(hd == 256 ? 1 : 2), 128, 128, uncut};
     // 128 rows to a workgroup read half as much from LDS for a product, 64 have twice as many units: from 2048 keys of 128 rows to a workgroup on, as
     // far as the host can tell (us with 128 / 64: 4096 rows over 4096, 32 heads on 8: 520 / 617; 723 rows of 8 sequences of up to 3500, 14
     // heads of 64 on 2: 57 / 43).
-    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;
-    const bool tall = pages->head_dim < 256 && most_rows * group >= 128 && tokens * heads / 128 * keys >= workgroups * 2048ll;
-    return Plan{tall ? 128 : 64, workgroups, 128, 512};
+    const bool tall = hd < 256 && most_rows * group >= 128 && tokens * heads / 128 * keys >= workgroups(2) * 2048ll;
+    return Plan{tall ? 128 : 64, workgroups(2), 128, 512, uncut};
 }
 
 int64_t workspace_of(const Plan& p, int hd)
@@ -872,24 +975,30 @@ int check_heads(int heads, const tl_pages* pages)
     return TL_OK;
 }
 
+template <int HD, int ROWS>
+void launch_join(const PagedAttn& a, const Plan& p, hipStream_t st)
+{
+    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(256), 0, st, a);
+}
+
 template <int HD, bool BYTES>
 void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
     const dim3 grid((unsigned)p.workgroups), block(256);
     if (p.rows == 16) {
         hipLaunchKernelGGL((tl_paged_few<HD, BYTES>), grid, block, 0, st, a);
-        hipLaunchKernelGGL((tl_paged_join<HD, 16>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
+        launch_join<HD, 16>(a, p, st);
         return;
     }
     if constexpr (HD < 256) {
         if (p.rows == 128) {
             hipLaunchKernelGGL((tl_paged_rows<HD, 2, BYTES>), grid, block, 0, st, a);
-            hipLaunchKernelGGL((tl_paged_join<HD, 128>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
+            launch_join<HD, 128>(a, p, st);
             return;
         }
     }
     hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES>), grid, block, 0, st, a);
-    hipLaunchKernelGGL((tl_paged_join<HD, 64>), dim3((unsigned)p.workgroups, 8), block, 0, st, a);
+    launch_join<HD, 64>(a, p, st);
 }
 
 }  // namespace
@@ -924,9 +1033,15 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
     a.tile_heads = std::min(a.group, p.rows);
     a.blocks = (int)ceil_div(a.group, a.tile_heads);
     a.tile_tokens = p.rows / a.tile_heads;
+    // the walk's products of costs stay below 2^53
+    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;
+    const int64_t units = (ceil_div(tokens, a.tile_tokens) + batch->seqs) * pages->kv_heads * a.blocks;
+    if (keys > (1 << 26) || units > (1ll << 42) / (keys + tokens + p.fixed + a.tile_tokens))
+        return fail(TL_ERR_SHAPE, "%lld rows over up to %lld keys are more than one call takes", (long long)tokens, (long long)keys);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.fixed = p.fixed;
     a.least = p.least;
+    a.uncut = p.uncut;
     a.shared = static_cast<Shared*>(workspace);
     a.pieces = reinterpret_cast<float*>(a.shared + p.workgroups);
     hipStream_t st = static_cast<hipStream_t>(stream);
