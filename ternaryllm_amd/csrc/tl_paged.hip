@@ -856,13 +856,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
 }
 
 // Joins the pieces of the units that were shared out: blockIdx.x is the workgroup in which one begins.  HD / 4 lanes take a row, four
-// values each.  Of a unit of a few pieces 1024 / HD rows are joined at a time; where they are many, as of a single long sequence, one row by as many
+// values each.  Of a unit of a few pieces 2048 / HD rows are joined at a time; where they are many, as of a single long sequence, one row by as many
 // groups of lanes, which share the pieces out.
 template <int HD, int ROWS>
-__global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
+__global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
 {
-    constexpr int LANES = HD / 4, AT_ONCE = 256 / LANES, FEW = 6;
-    __shared__ float4 part[256];
+    constexpr int LANES = HD / 4, AT_ONCE = 512 / LANES, FEW = ROWS > 16 ? 64 : 8, FLY = 8;
+    __shared__ float4 part[512];
     __shared__ float tops[AT_ONCE], sums[AT_ONCE];
     Shared sh = a.shared[blockIdx.x];
     sh.last = scalar(sh.last);
@@ -876,20 +876,20 @@ __global__ __launch_bounds__(256) void tl_paged_join(PagedAttn a)
     float4 o;
     float top, sum;
     auto start = [&] { o = make_float4(0.f, 0.f, 0.f, 0.f), top = kNone, sum = 0.f; };
-    // pieces i, i + step, ... of a row, four on their way at a time
+    // pieces i, i + step, ... of a row, several on their way at a time
     auto add = [&](int i, int step, int r) {
-        for (; i < count; i += 4 * step) {
-            float m[4], l[4];
-            float4 v[4];
+        for (; i < count; i += FLY * step) {
+            float m[FLY], l[FLY];
+            float4 v[FLY];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < FLY; ++k) {
                 const int n = min(i + k * step, count - 1);
                 const float* piece = a.pieces + (((long long)(first + n) * 2 + (n == 0 ? 1 : 0)) * ROWS + r) * (HD + 4);
                 m[k] = piece[HD], l[k] = piece[HD + 1];
                 v[k] = *reinterpret_cast<const float4*>(piece + lane * 4);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < FLY; ++k) {
                 if (i + k * step >= count) break;
                 const float now = fmaxf(top, m[k]), base = now == kNone ? 0.f : now * a.scale_log2;
                 const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m[k], a.scale_log2, -base));
@@ -978,7 +978,7 @@ int check_heads(int heads, const tl_pages* pages)
 template <int HD, int ROWS>
 void launch_join(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
-    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(256), 0, st, a);
+    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(512), 0, st, a);
 }
 
 template <int HD, bool BYTES>
