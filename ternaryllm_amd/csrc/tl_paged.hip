@@ -1022,7 +1022,7 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
     if (tokens == 0 || a.batch.seqs == 0) return TL_OK;
     if (!q || !out || !workspace) return fail(TL_ERR_ARG, "device pointer is null");
     if (most_rows < 0) return fail(TL_ERR_ARG, "most_rows is negative");
-    if (!(scale > 0.f) || scale > 3e38f) return fail(TL_ERR_ARG, "scale=%g is not a positive number", (double)scale);
+    if (!(scale > 0.f) || scale > 1e30f) return fail(TL_ERR_ARG, "scale=%g is not a positive number up to 1e30", (double)scale);
     if (!in_pieces(q, {q_token, q_head}, 2) || !in_pieces(out, {}, 2) || !in_pieces(workspace, {}, 1)) return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
     const Plan p = plan_of(tokens, heads, pages, batch, most_rows);
     if (workspace_bytes < workspace_of(p, pages->head_dim))

@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -186,14 +187,23 @@ int64_t step(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 
 
 bool absent(PyObject* o) { return o == Py_None; }
 
+// Whether a derivative is asked for, which Python refuses.
+bool differentiated(std::initializer_list<const at::Tensor*> tensors)
+{
+    if (!c10::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : tensors)
+        if (t->requires_grad()) return true;
+    return false;
+}
+
 // x [tokens, heads, head_dim] on `device`, of type `type`, its rows' last dimension in one piece; y where it goes (null: pages).
 bool head_rows(const at::Tensor& x, const at::Tensor* y, PyObject* norm, tl_head_rows* r)
 {
-    if (x.dim() != 3 || x.stride(2) != 1 || x.numel() == 0) return false;
+    if (x.dim() != 3 || x.stride(2) != 1 || x.numel() == 0 || differentiated({&x})) return false;
     const at::Tensor* w = nullptr;
     if (!absent(norm)) {
         w = plain(norm);
-        if (!w || w->dim() != 1 || w->size(0) != x.size(2) || w->scalar_type() != x.scalar_type() || w->device() != x.device() || !w->is_contiguous()) return false;
+        if (!w || w->dim() != 1 || w->size(0) != x.size(2) || w->scalar_type() != x.scalar_type() || w->device() != x.device() || !w->is_contiguous() || differentiated({w})) return false;
     }
     *r = tl_head_rows{x.data_ptr(), step(x, 0), step(x, 1), y ? y->data_ptr() : nullptr, y ? step(*y, 0) : 0, y ? step(*y, 1) : 0,
                       w ? w->data_ptr() : nullptr, (int32_t)x.size(1)};
@@ -385,7 +395,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
     tl_pages p;
     tl_page_batch b;
     int64_t most, need;
-    if (!q || q->dim() != 3 || q->numel() == 0 || q->stride(2) != 1 || q->scalar_type() != at::kHalf || !pages_and_batch(a[1], a[2], q->device(), &p, &b, &most) ||
+    if (!q || q->dim() != 3 || q->numel() == 0 || q->stride(2) != 1 || q->scalar_type() != at::kHalf || differentiated({q}) || !pages_and_batch(a[1], a[2], q->device(), &p, &b, &most) ||
         p.head_dim != q->size(2))
         Py_RETURN_NONE;
     const int64_t tokens = q->size(0), width = q->size(1) * q->size(2);

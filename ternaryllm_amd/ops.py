@@ -715,6 +715,11 @@ def _rotation(frequencies, positions, tokens, factor, interleaved, eps, like):
                          float(factor), float(eps))
 
 
+def _forward_only(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the operators of a paged cache have no backward pass: call them under torch.no_grad()")
+
+
 def _cuda(x, what):
     if x.device.type != "cuda":
         raise RuntimeError(f"{what} is on {x.device}: the kernels run on a GPU only")
@@ -729,6 +734,7 @@ def rope_heads(q, k, positions, frequencies, *, factor=1.0, interleaved=False, q
     both = _short().rope_heads(q, k, positions, frequencies, factor, interleaved, q_norm, k_norm, eps, q_out, k_out)
     if both is not None:
         return both
+    _forward_only(q, k, q_norm, k_norm)
     if k is not None and (k.dim() != 3 or k.shape[::2] != q.shape[::2] or k.dtype != q.dtype or k.device != q.device):
         raise ValueError("k must have q's tokens, head_dim, type and device")
     if frequencies is not None and positions is None:
@@ -749,13 +755,14 @@ def rope_heads(q, k, positions, frequencies, *, factor=1.0, interleaved=False, q
 def rope_to_pages(q, k, v, pages, batch, frequencies=None, positions=None, *, factor=1.0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6,
                   q_out=None):
     """rope_heads for the rows of a batch, the keys going into the pages of their sequences with the values v [tokens, kv_heads, head_dim] beside
-    them.  positions None: each row's index in its sequence.  q may be None.  Returns the rotated queries.  Pages of float8_e4m3fn: a row's
+    them (no two rows may have the same place).  positions None: each row's index in its sequence.  q may be None.  Returns the rotated queries.  Pages of float8_e4m3fn: a row's
     exponent is the least that keeps it within 448, its codes are rounded to the nearest; they saturate at the largest value that is a finite
     float16."""
     if q_out is None:
         rotated = _short().rope_to_pages(q, k, v, pages, batch, frequencies, positions, factor, interleaved, q_norm, k_norm, eps)
         if rotated is not None:
             return rotated
+    _forward_only(q, k, v, q_norm, k_norm)
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one type and device")
     if q is not None and (q.dim() != 3 or q.shape[::2] != k.shape[::2] or q.dtype != k.dtype or q.device != k.device):
@@ -810,6 +817,7 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
     y = _short().paged_attention(q, pages, batch, scale, out)
     if y is not None:
         return y
+    _forward_only(q)
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
     tokens, heads, hd = q.shape

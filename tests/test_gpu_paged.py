@@ -313,6 +313,119 @@ def test_no_sequences_and_no_rows():
     assert (out == 3).all()
 
 
+def test_a_peak_over_a_long_plain():
+    """One key above 60000 that are alike, each with 1.7e-5 of its weight, below fp16's normal range, and all of them together with as much."""
+    n = 60001
+    seqs = paged.Sequences([(1, n)], 256)
+    for kind in ("float16", "e4m3"):
+        pages = fresh_pages(seqs, 1, 64, kind, spoiled=False)
+        k = torch.zeros(pages.k.shape)
+        k[int(seqs.table[0, 100]), 0, 7, 0] = 11.0
+        v = torch.ones(pages.v.shape)
+        v[int(seqs.table[0, 100]), 0, 7] = 3.0
+        ke = None if kind == "float16" else torch.full(pages.k.shape[:3], 127, dtype=torch.uint8)
+        dtype = torch.float16 if kind == "float16" else torch.float8_e4m3fn
+        q = torch.zeros((1, 1, 64), dtype=torch.float16)
+        q[0, 0, 0] = 8.0                                          # a score of 11, and 0
+        got = ops.paged_attention(q.cuda(), on_gpu(ops.Pages(k.to(dtype), v.to(dtype), ke, ke)), seqs.batch(ops)).cpu().double()
+        weight = 1 / (1 + (n - 1) * math.exp(-11))
+        # the plain's probabilities are rounded to fp16's smallest step, 2^-24, in the sums above and below the line alike: 2^-25 of 1.67e-5 each
+        slack = 2.0 ** -25 / math.exp(-11) + 2.0 ** -10
+        assert (got - (3 * weight + 1 - weight)).abs().max() <= 3 * slack
+
+
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+@pytest.mark.parametrize("most", [1, 200])
+def test_pages_of_other_strides(kind, most):
+    """Slots before heads, and keys and values of a layer in one tensor."""
+    seqs = paged.Sequences([(2, 70), (1, 33), (3, 150)], 32)
+    pages = fresh_pages(seqs, 2, 128, kind)
+    q = random((seqs.tokens, 8, 128), 4).cuda()
+    want = ops.paged_attention(q, on_gpu(pages), seqs.batch(ops, most=most))
+    n, kv, page, hd = pages.k.shape
+    raw = torch.uint8 if kind == "e4m3" else torch.float16
+    both = torch.zeros((n, page, 2, kv, hd), dtype=raw, device="cuda")
+    views = [both[:, :, i].transpose(1, 2).view(pages.k.dtype) if kind == "e4m3" else both[:, :, i].transpose(1, 2) for i in range(2)]
+    for view, t in zip(views, (pages.k, pages.v)):
+        view.view(raw).copy_(t.view(raw).cuda())
+    other = ops.Pages(*views, *(None if t is None else t.cuda() for t in pages[2:]))
+    assert torch.equal(ops.paged_attention(q, other, seqs.batch(ops, most=most)), want)
+    k, v = random((seqs.tokens, 2, 128), 5).cuda(), random((seqs.tokens, 2, 128), 6).cuda()
+    plain = on_gpu(pages)
+    for p in (plain, other):
+        ops.rope_to_pages(None, k, v, p, seqs.batch(ops))
+    a, b = ops.read_pages(plain, seqs.batch(ops), seqs.tokens), ops.read_pages(other, seqs.batch(ops), seqs.tokens)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for view, t in zip(views, plain[:2]):
+        bits = torch.uint8 if kind == "e4m3" else torch.int16   # (what no sequence has is not a number)
+        assert torch.equal(view.view(bits), t.view(bits))
+
+
+@pytest.mark.parametrize("most", [1, 200])
+def test_pages_that_lie_far_apart(most):
+    """Offsets past 32 bits: pages of 5 GB."""
+    seqs = paged.Sequences([(1, 30), (2, 20)], 16, spare=0)
+    pages = fresh_pages(seqs, 2, 64, "float16")
+    step = (5 << 30) // 2
+    pool = torch.empty(4 * step, dtype=torch.float16, device="cuda")
+    far = ops.Pages(*(torch.as_strided(pool, pages.k.shape, (step, 16 * 64, 64, 1), i * 2 * 16 * 64) for i in range(2)))
+    for view, t in zip(far, pages[:2]):
+        view.copy_(t.cuda())
+    q = random((3, 4, 64), 4).cuda()
+    assert seqs.pages == 4 and torch.equal(ops.paged_attention(q, far, seqs.batch(ops, most=most)), ops.paged_attention(q, on_gpu(pages), seqs.batch(ops, most=most)))
+    k, v = random((3, 2, 64), 5).cuda(), random((3, 2, 64), 6).cuda()
+    ops.rope_to_pages(None, k, v, far, seqs.batch(ops))
+    back = ops.read_pages(far, seqs.batch(ops), 3)
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams do not share what they work in: each gives the bits that it gives alone."""
+    seqs = [paged.Sequences([(1, 3000 + 100 * i), (1, 500)], 64, seed=i) for i in range(2)]
+    pages = [on_gpu(fresh_pages(s, 2, 128, "float16", seed=i)) for i, s in enumerate(seqs)]
+    qs, batches = [random((2, 8, 128), i).cuda() for i in range(2)], [s.batch(ops) for s in seqs]
+    alone = [ops.paged_attention(q, p, b) for q, p, b in zip(qs, pages, batches)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.paged_attention(qs[i], pages[i], batches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, alone[i]) for g in got[i])
+
+
+def test_two_graphs_of_one_stream_replayed_on_two():
+    seqs = paged.Sequences([(1, 4000), (1, 700)], 64)
+    pages, batch = on_gpu(fresh_pages(seqs, 2, 128, "float16")), seqs.batch(ops)
+    qs = [random((2, 8, 128), i).cuda() for i in range(2)]
+    want = [ops.paged_attention(q, pages, batch) for q in qs]
+    graphs, outs = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.paged_attention(q, pages, batch))
+    streams = [torch.cuda.Stream() for _ in qs]
+    for turn in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), turn
+
+
+def test_the_same_bits_every_time():
+    both = [(1, (i * 997) % 4000 + 1) for i in range(40)]
+    seqs = paged.Sequences(both, 16)
+    pages, batch, q = on_gpu(fresh_pages(seqs, 2, 128, "float16")), seqs.batch(ops), random((40, 8, 128), 2).cuda()
+    first = ops.paged_attention(q, pages, batch)
+    assert all(torch.equal(ops.paged_attention(q, pages, batch), first) for _ in range(20))
+
+
 class _NoShortWay:
     def __getattr__(self, name):
         return lambda *args: None

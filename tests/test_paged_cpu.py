@@ -86,6 +86,18 @@ def test_heads_and_outputs_that_do_not_fit():
             pytest.fail(f"call {i} was taken")
 
 
+def test_no_backward_pass():
+    q, k, pages, batch = parts()
+    at, f = torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    w = torch.ones(64).half().requires_grad_()
+    for call in (lambda x: ops.rope_heads(x, k, at, f), lambda x: ops.rope_to_pages(None, x[:, :2], k, pages, batch), lambda x: ops.paged_attention(x, pages, batch),
+                 lambda x: ops.rope_heads(q, k, at, f, k_norm=w)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call(q.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+            call(q.clone().requires_grad_())
+
+
 def test_outputs_that_overlap_operands():
     at, f = torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
     rows = torch.zeros((5, 6, 64), dtype=torch.float16)
@@ -162,7 +174,7 @@ ARG, SHAPE, DTYPE, ALIGN, UNSUPPORTED, SIZE = -1, -2, -3, -4, -5, -8
     ("attend", {"dtype": 0}, UNSUPPORTED), ("attend", {"dtype": 2}, DTYPE), ("attend", {"heads": 3}, SHAPE), ("attend", {"heads": 0}, SHAPE),
     ("attend", {"pages__head_dim": 96, "pages__slot_stride": 96}, UNSUPPORTED), ("attend", {"out": None}, ARG), ("attend", {"workspace": None}, ARG),
     ("attend", {"workspace": 8}, ALIGN), ("attend", {"bytes": 100}, SIZE), ("attend", {"scale": 0.0}, ARG), ("attend", {"scale": -1.0}, ARG),
-    ("attend", {"scale": math.nan}, ARG), ("attend", {"scale": math.inf}, ARG), ("attend", {"most": -1}, ARG), ("attend", {"q_token": 100}, ALIGN),
+    ("attend", {"scale": math.nan}, ARG), ("attend", {"scale": 2e30}, ARG), ("attend", {"batch__table_pages": 1 << 23, "batch__table_stride": 1 << 23}, SHAPE), ("attend", {"scale": math.inf}, ARG), ("attend", {"most": -1}, ARG), ("attend", {"q_token": 100}, ALIGN),
     ("attend", {"out": (1 << 20) + 2}, ALIGN)])
 def test_the_library_refuses(call, changes, code):
     if code is None:                                # exponents beside fp16 pages: one alone is refused as well
