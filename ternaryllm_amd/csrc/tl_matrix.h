@@ -34,16 +34,6 @@ __device__ __forceinline__ f32x4 matrix_step(u32x4 w, u32x4 x, f32x4 acc)
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, x), acc, 0, 0, 0);
 }
 
-// f over the four lanes with the same number modulo 16, on the vector unit (16 x 512 of 16 heads took 48.4 us with shuffles, 47.6).
-template <typename F>
-__device__ __forceinline__ float with_other_rows(float v, F f)
-{
-    const auto near = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = f(__uint_as_float(near[0]), __uint_as_float(near[1]));
-    const auto far = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return f(__uint_as_float(far[0]), __uint_as_float(far[1]));
-}
-
 // 16 bytes per lane from `base` + offset into LDS at `lds` + 16 * lane.  (As assembly, because the compiler would wait for
 // all such loads before any read of LDS; here they are counted by hand.)
 #pragma clang diagnostic push

@@ -856,13 +856,16 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
 }
 
 // Joins the pieces of the units that were shared out: blockIdx.x is the workgroup in which one begins.  HD / 4 lanes take a row, four
-// values each.  Of a unit of a few pieces 2048 / HD rows are joined at a time; where they are many, as of a single long sequence, one row by as many
+// values each.  Of a unit of a few pieces as many rows as there are such groups of lanes are joined at a time; where they are many, as of a single long sequence, one row by as many
 // groups of lanes, which share the pieces out.
+template <int ROWS>
+constexpr int kJoinThreads = ROWS > 16 ? 512 : 256;
+
 template <int HD, int ROWS>
-__global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
+__global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
 {
-    constexpr int LANES = HD / 4, AT_ONCE = 512 / LANES, FEW = ROWS > 16 ? 64 : 8, FLY = 8;
-    __shared__ float4 part[512];
+    constexpr int THREADS = kJoinThreads<ROWS>, LANES = HD / 4, AT_ONCE = THREADS / LANES, FEW = ROWS > 16 ? 64 : 8;
+    __shared__ float4 part[THREADS];
     __shared__ float tops[AT_ONCE], sums[AT_ONCE];
     Shared sh = a.shared[blockIdx.x];
     sh.last = scalar(sh.last);
@@ -877,7 +880,8 @@ __global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
     float top, sum;
     auto start = [&] { o = make_float4(0.f, 0.f, 0.f, 0.f), top = kNone, sum = 0.f; };
     // pieces i, i + step, ... of a row, several on their way at a time
-    auto add = [&](int i, int step, int r) {
+    auto add = [&](auto fly, int i, int step, int r) {
+        constexpr int FLY = decltype(fly)::value;
         for (; i < count; i += FLY * step) {
             float m[FLY], l[FLY];
             float4 v[FLY];
@@ -888,6 +892,7 @@ __global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
                 m[k] = piece[HD], l[k] = piece[HD + 1];
                 v[k] = *reinterpret_cast<const float4*>(piece + lane * 4);
             }
+            if constexpr (FLY > 4) __builtin_amdgcn_sched_barrier(0);   // (or the compiler asks for them one after the other)
 #pragma unroll
             for (int k = 0; k < FLY; ++k) {
                 if (i + k * step >= count) break;
@@ -909,7 +914,7 @@ __global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
             const Row x = row_of(a, w, u, r);
             if (!x.there) continue;
             start();
-            add(0, 1, r);
+            add(std::integral_constant<int, 4>{}, 0, 1, r);
             finish(x);
         }
         return;
@@ -918,7 +923,8 @@ __global__ __launch_bounds__(512) void tl_paged_join(PagedAttn a)
         const Row x = row_of(a, w, u, r);
         if (!x.there) continue;                                   // (the same for all)
         start();
-        add(own, AT_ONCE, r);
+        if (ROWS > 16 || count <= 4 * AT_ONCE) add(std::integral_constant<int, 4>{}, own, AT_ONCE, r);
+        else add(std::integral_constant<int, (ROWS > 16 ? 4 : 8)>{}, own, AT_ONCE, r);
         __syncthreads();                                          // the row before is done with LDS
         part[threadIdx.x] = o;
         if (lane == 0) tops[own] = top, sums[own] = sum;
@@ -978,7 +984,7 @@ int check_heads(int heads, const tl_pages* pages)
 template <int HD, int ROWS>
 void launch_join(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
-    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(512), 0, st, a);
+    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(kJoinThreads<ROWS>), 0, st, a);
 }
 
 template <int HD, bool BYTES>

