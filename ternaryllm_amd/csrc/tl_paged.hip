@@ -299,6 +299,19 @@ __device__ __forceinline__ void sixteen_halves(u32x4 codes, float scale, u32x4* 
     }
 }
 
+// Eight fp16 values with those that are not finite made 0; whether there were any.  (A value that a row does not see weighs 0, which would make NaN of it.)
+__device__ __forceinline__ bool make_finite(u32x4* x)
+{
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t bad = (((*x)[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;   // the exponent's bits all set, in either half
+        (*x)[i] &= ~((bad >> 15) * 0xffffu);
+        any |= bad;
+    }
+    return any != 0;
+}
+
 // The running softmax of a row: its reference is a maximum that it has seen (in units of the scores), which probabilities are taken
 // against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, 8 in the exponent of 2: a
 // probability is then 256 at most, as exact in fp16 as one of 1, and the sums, which are fp32, hardly ever have to be scaled.
@@ -410,6 +423,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     __shared__ __align__(16) unsigned char lds[2 * BUF];
     __shared__ int wrong_somewhere;
     __shared__ Walk kept;
+    __shared__ int spoiled[2][KT];                                // keys of a buffer whose values were not finite
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
@@ -433,6 +447,11 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         const int first_tile = (u.first_key + KT - 1) / KT, tiles = (u.end_key + KT - 1) / KT;   // (a share may be empty)
         bool wrong = w.s.wrong;
         const int length = w.s.length;
+        // Tiles that some of the unit's rows see more of than others: values there that are not finite must not meet the weights of 0.  They are made 0
+        // in LDS, and the rows that do see their key are NaN.
+        const int all_see = length - w.s.n + u.first_token;       // the last key that every row sees
+        const bool rows_differ = min(a.tile_tokens, w.s.n - u.first_token) > 1;
+        auto mixed = [&](int t) { return rows_differ && t * KT + KT - 1 > all_see; };
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
         // page of this wave's keys of the tile after the next (by a vector load: a scalar one would be waited for with the first read of LDS)
@@ -471,6 +490,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             }
         };
         auto put = [&](int t, int buf) {                          // what fetch has asked for is in LDS
+            if (mixed(t) && lane < KW) spoiled[buf][wave * KW + lane] = 0;
             if constexpr (BYTES) {
                 unsigned char* kd = lds + buf * BUF;
                 unsigned char* vd = kd + KB;
@@ -483,12 +503,24 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p + 1) * 16) = hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
                     if (t * KT + key >= length) lo = hi = u32x4{0u, 0u, 0u, 0u};
+                    if (mixed(t)) {
+                        const bool low = make_finite(&lo), high = make_finite(&hi);
+                        if (low || high) spoiled[buf][key] = 1;
+                    }
                     u32x4* v = reinterpret_cast<u32x4*>(vd + key * HD * 2 + value_place(key, p) * 32);
                     v[0] = lo;
                     v[1] = hi;
                 }
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if (mixed(t)) {
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) {
+                        u32x4* at = reinterpret_cast<u32x4*>(lds + buf * BUF + KB + wave * KW * HD * 2 + i * 1024 + lane * 16);
+                        u32x4 x = *at;
+                        if (make_finite(&x)) *at = x, spoiled[buf][wave * KW + i * KEYS + lane / PIECES] = 1;
+                    }
+                }
             }
         };
         if (first_tile < tiles) ask(first_tile);
@@ -582,6 +614,16 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             }
             u32x4 px[QF][NF / 2];
             softmax_step(sc, a.scale_log2, run, o, px);
+            if (mixed(t)) {
+                const unsigned long long keys_spoiled = __builtin_amdgcn_ballot_w64(lane < KT && spoiled[(t - first_tile) & 1][lane & (KT - 1)] != 0);
+                if (keys_spoiled != 0) {
+#pragma unroll
+                    for (int f = 0; f < QF; ++f) {
+                        const int seen = last[f] - t * KT;
+                        if (seen >= 0 && (keys_spoiled & (~0ull >> (63 - min(seen, 63)))) != 0) run[f].sum = __builtin_nanf("");
+                    }
+                }
+            }
             constexpr int VG = 4, GROUPS = NF / 2 * DF / VG;  // values: VG fragments a step
             u32x4 vx[2][VG];
             auto values = [&](int i, u32x4* to) {
@@ -738,9 +780,16 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
+        const bool rows_differ = min(a.tile_tokens, w.s.n - u.first_token) > 1;
 
+        auto spoil = [&](unsigned long long lanes, int first) {   // lanes whose pieces of values were not finite, of keys from `first` on
+            for (int k = 0; lanes != 0 && k < VKEYS; ++k)
+                if ((lanes >> (k * PIECES) & (~0ull >> (64 - PIECES))) != 0 && first + k <= last) run[0].sum = __builtin_nanf("");
+        };
         for (int t = first_tile; t < tiles; t += 4) {
             const bool ends = t * KT + KT > length;
+            // a tile that some rows see more of than others: values that are not finite become 0, and the rows that see their key NaN
+            const bool mixed = rows_differ && t * KT + KT - 1 > all_see;
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
                 const int key = i * VKEYS + lane / PIECES, p = lane % PIECES;
@@ -749,10 +798,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                 if constexpr (BYTES) {
                     u32x4 lo, hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
+                    if (mixed) {
+                        const bool low = make_finite(&lo), high = make_finite(&hi);
+                        spoil(__builtin_amdgcn_ballot_w64(low || high), t * KT + i * VKEYS);
+                    }
                     u32x4* v = reinterpret_cast<u32x4*>(own + key * HD * 2 + value_place(key, p) * 32);
                     v[0] = lo;
                     v[1] = hi;
                 } else {
+                    if (mixed) spoil(__builtin_amdgcn_ballot_w64(make_finite(&vreg[i])), t * KT + i * VKEYS);
                     *reinterpret_cast<u32x4*>(own + key * HD * 2 + value_place(key, p >> 1) * 32 + (p & 1) * 16) = vreg[i];
                 }
             }

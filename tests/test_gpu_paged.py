@@ -301,6 +301,31 @@ def test_pages_and_lengths_that_are_none(most):
     assert torch.equal(got[:2], good[:2]) and torch.isnan(got[2:]).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("most", [1, 100])                        # 16 rows a workgroup, and 64
+def test_values_that_are_not_finite_among_the_new_tokens(hd, most):
+    """A key or a value that is not finite reaches the rows that see it and no others, of its sequence or of another."""
+    seqs = paged.Sequences([(100, 200), (3, 90)], 16)
+    for kind in ("float16", "e4m3"):
+        pages = fresh_pages(seqs, 1, hd, kind, spoiled=False)
+        held = [paged.values(*t) for t in zip(pages[:2], pages[2:])]
+        q = random((seqs.tokens, 2, hd), 3)
+        want = paged.attention(q, *held, seqs, 1 / math.sqrt(hd))
+        bound = attention_bound(q, *held, want, 200, 1 / math.sqrt(hd))
+        for which, token in ((0, 170), (1, 170), (1, 191), (1, 127), (1, 199), (1, 100), (0, 101)):
+            now = list(t if t is None else t.clone() for t in pages)
+            where = int(seqs.table[0, token // 16]), 0, token % 16, 5
+            if kind == "e4m3":
+                now[which].view(torch.uint8)[where] = 0x7f
+            else:
+                now[which][where] = math.nan if which == 0 else math.inf
+            got = ops.paged_attention(q.cuda(), on_gpu(ops.Pages(*now)), seqs.batch(ops, most=most)).cpu().view(seqs.tokens, 2, hd)
+            good = torch.ones(seqs.tokens, dtype=torch.bool)
+            good[token - 100:100] = False                         # row i is token 100 + i
+            assert ((got.double() - want).abs() <= bound)[good].all(), (kind, which, token)
+            assert not torch.isfinite(got[token - 100:100]).all(-1).any(), (kind, which, token)
+
+
 def test_no_sequences_and_no_rows():
     pages = ops.Pages(*(torch.zeros((2, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
     i32 = dict(dtype=torch.int32, device="cuda")
