@@ -451,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         // in LDS, and the rows that do see their key are NaN.
         const int all_see = length - w.s.n + u.first_token;       // the last key that every row sees
         const bool rows_differ = min(a.tile_tokens, w.s.n - u.first_token) > 1;
-        auto mixed = [&](int t) { return rows_differ && t * KT + KT - 1 > all_see; };
+        const int first_mixed = rows_differ ? max(all_see + 1, 0) / KT : INT_MAX;   // ... are the last
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
         // page of this wave's keys of the tile after the next (by a vector load: a scalar one would be waited for with the first read of LDS)
@@ -489,8 +489,9 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 }
             }
         };
-        auto put = [&](int t, int buf) {                          // what fetch has asked for is in LDS
-            if (mixed(t) && lane < KW) spoiled[buf][wave * KW + lane] = 0;
+        auto put = [&](auto may_mix, int t, int buf) {            // what fetch has asked for is in LDS
+            const bool mixed = decltype(may_mix)::value && t >= first_mixed;
+            if (mixed && lane < KW) spoiled[buf][wave * KW + lane] = 0;
             if constexpr (BYTES) {
                 unsigned char* kd = lds + buf * BUF;
                 unsigned char* vd = kd + KB;
@@ -503,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     *reinterpret_cast<u32x4*>(kd + key * HD * 2 + key_place(key, 2 * p + 1) * 16) = hi;
                     sixteen_halves(vreg[i], __uint_as_float((uint32_t)vexp[i] << 23), &lo, &hi);
                     if (t * KT + key >= length) lo = hi = u32x4{0u, 0u, 0u, 0u};
-                    if (mixed(t)) {
+                    if (mixed) {
                         const bool low = make_finite(&lo), high = make_finite(&hi);
                         if (low || high) spoiled[buf][key] = 1;
                     }
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 }
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                if (mixed(t)) {
+                if (mixed) {
 #pragma unroll
                     for (int i = 0; i < KL; ++i) {
                         u32x4* at = reinterpret_cast<u32x4*>(lds + buf * BUF + KB + wave * KW * HD * 2 + i * 1024 + lane * 16);
@@ -557,7 +558,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         if (first_tile < tiles) {
             fetch(first_tile, 0);
             if (first_tile + 1 < tiles) ask(first_tile + 1);
-            put(first_tile, 0);
+            put(std::true_type{}, first_tile, 0);
         }
         __syncthreads();
 #pragma unroll
@@ -572,15 +573,14 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 if (t + 2 < tiles) ask(t + 2);
             }
         };
-        auto behind = [&](int t) {
+        auto behind = [&](auto may_mix, int t) {
             if (t + 1 < tiles) {
-                put(t + 1, (t + 1 - first_tile) & 1);             // (read last before the barrier of the turn before)
+                put(may_mix, t + 1, (t + 1 - first_tile) & 1);             // (read last before the barrier of the turn before)
                 __syncthreads();
             }
         };
         const int seen_tiles = min(tiles, wave_last / KT + (wave_last >= 0 ? 1 : 0));
-        int t = first_tile;
-        for (; t < seen_tiles; ++t) {
+        auto work = [&](auto may_mix, int t) {
             before(t);
             const unsigned char* ks = lds + ((t - first_tile) & 1) * BUF;
             const unsigned char* vs = ks + KB;
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             }
             u32x4 px[QF][NF / 2];
             softmax_step(sc, a.scale_log2, run, o, px);
-            if (mixed(t)) {
+            if (decltype(may_mix)::value && t >= first_mixed) {
                 const unsigned long long keys_spoiled = __builtin_amdgcn_ballot_w64(lane < KT && spoiled[(t - first_tile) & 1][lane & (KT - 1)] != 0);
                 if (keys_spoiled != 0) {
 #pragma unroll
@@ -645,11 +645,14 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     for (int f = 0; f < QF; ++f) o[f][i * VG % DF + j] = matrix_step<false>(vx[i & 1][j], px[f][i * VG / DF], o[f][i * VG % DF + j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            behind(t);
-        }
+            behind(may_mix, t);
+        };
+        int t = first_tile;
+        for (; t < min(seen_tiles, first_mixed - 1); ++t) work(std::false_type{}, t);   // (nor is the next one mixed)
+        for (; t < seen_tiles; ++t) work(std::true_type{}, t);
         for (; t < tiles; ++t) {
             before(t);
-            behind(t);
+            behind(std::true_type{}, t);
         }
         if (wrong && lane == 0) wrong_somewhere = 1;
         __syncthreads();

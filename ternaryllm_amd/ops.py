@@ -812,7 +812,8 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
 def paged_attention(q, pages, batch, *, scale=None, out=None):
     """Causal attention of a batch's rows q [tokens, heads, head_dim] over everything their sequences have in the pages (their own keys and values
     among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
-    rows of no sequence are not written, a row that sees nothing is 0, rows of a sequence with a page that is none are NaN.  float16, head_dim 64,
+    rows of no sequence are not written, a row that sees nothing is 0, rows that would read a page that is none are NaN; what is not finite where a row
+    does not see it does not reach the row.  float16, head_dim 64,
     128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim)."""
     y = _short().paged_attention(q, pages, batch, scale, out)
     if y is not None:
