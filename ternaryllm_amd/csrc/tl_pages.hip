@@ -204,9 +204,11 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
         for (int i = tid; i < a.pairs; i += 256) {
             double turns = (double)position * a.freq[i] * 0.15915494309189535;   // 1 / (2 pi)
             turns -= rint(turns);
+            const float most = (float)turns, rest = (float)(turns - (double)most) * 6.2831853f;   // what the rounding to fp32 leaves, as an angle
             float s, c;
-            sincospif(2.0f * (float)turns, &s, &c);
-            reinterpret_cast<float2*>(&turn[(i & 7) >> 1][i >> 3])[i & 1] = make_float2(c * a.factor, s * a.factor);
+            sincospif(2.0f * most, &s, &c);
+            const float cosine = fmaf(-s, rest, c), sine = fmaf(c, rest, s);
+            reinterpret_cast<float2*>(&turn[(i & 7) >> 1][i >> 3])[i & 1] = make_float2(cosine * a.factor, sine * a.factor);
         }
         __syncthreads();
     }
@@ -231,7 +233,9 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) squares = fmaf(x.v[j], x.v[j], squares);
                 squares = over_lanes(squares, bits, [](float u, float v) { return u + v; });
-                const float inv = rsqrtf(fmaf(squares, part, a.eps));
+                // (a step of Newton's on the instruction's root: an error of all of a head's values alike turns more of its 8-bit codes than any other)
+                const float mean = fmaf(squares, part, a.eps), root = rsqrtf(mean);
+                const float inv = root < __builtin_huge_valf() ? fmaf(0.5f * root, fmaf(-mean * root, root, 1.0f), root) : root;
                 Eight w;
                 w.set(kind == 0 ? weight[0] : weight[1]);
                 if (there) {
