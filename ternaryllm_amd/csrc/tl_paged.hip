@@ -124,7 +124,8 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
             own += cost[i];
         }
         upto = own;
-        if (seqs - first > kSeqsOfThread) {
+        const bool one = seqs - first <= kSeqsOfThread;   // thread's
+        if (!one) {
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
                 const long long below = __shfl_up(upto, off, 64);
@@ -132,8 +133,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
             }
         }
         if (seqs > kPass) __syncthreads();       // the pass before is done with the sums
-        if (lane == 63) sums[wave] = upto;
-        if (tid == 0 && seqs - first <= kSeqsOfThread) sums[0] = upto;
+        if (one ? tid == 0 : lane == 63) sums[wave] = upto;   // (one writer each: of two, neither is the last)
         __syncthreads();
         pass = sums[0];
         if (seqs - first > 64 * kSeqsOfThread) {
