@@ -277,6 +277,14 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
+// Between what lanes of a wave put into LDS and what others of it read there, and between those reads and what is put there next.  (No instruction:
+// LDS takes a wave's requests in order, and this holds the compiler to that order, which it sees no reason for in a lane of its own.)
+__device__ __forceinline__ void wave_exchange()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Four 16-bit values of this lane's column from four rows of LDS: lanes 4 j + c of sixteen name row j, values 4 c .. 4 c + 3, and
 // lane i of the sixteen gets column i.
 __device__ __forceinline__ uint2 column_read(const unsigned char* p)
@@ -491,7 +499,10 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         };
         auto put = [&](auto may_mix, int t, int buf) {            // what fetch has asked for is in LDS
             const bool mixed = decltype(may_mix)::value && t >= first_mixed;
-            if (mixed && lane < KW) spoiled[buf][wave * KW + lane] = 0;
+            if (mixed) {
+                if (lane < KW) spoiled[buf][wave * KW + lane] = 0;
+                wave_exchange();
+            }
             if constexpr (BYTES) {
                 unsigned char* kd = lds + buf * BUF;
                 unsigned char* vd = kd + KB;
@@ -813,6 +824,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                     *reinterpret_cast<u32x4*>(own + key * HD * 2 + value_place(key, p >> 1) * 32 + (p & 1) * 16) = vreg[i];
                 }
             }
+            wave_exchange();
             f32x4 sc[1][2];
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -848,6 +860,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                 const uint2 lo = column_read(from), hi = column_read(from + 16 * HD * 2);   // (16 keys on: the same swizzle)
                 o[0][d] = matrix_step<false>(u32x4{lo.x, lo.y, hi.x, hi.y}, px[0][0], o[0][d]);
             }
+            wave_exchange();
         }
         // ---- the waves meet ----
         const float sum = with_other_rows(run[0].sum, [](float v, float y) { return v + y; });

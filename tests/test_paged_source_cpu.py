@@ -18,3 +18,18 @@ def body(name):
 def test_the_walks_sums_have_one_writer():
     """Two stores under conditions of different lanes are in no order: a thread makes one of them at most."""
     assert len(re.findall(r"\bsums\[\w+\] = ", body("begin_walk"))) == 1
+
+
+def test_values_cross_lanes_in_order():
+    """Single tokens: a wave's lanes write a tile's values into LDS, others of its lanes read them by columns, and the next tile is written.  Between each
+    two of these stands what orders them.  Likewise the marks of spoiled keys of a chunk's tile, cleared by some lanes and set by others."""
+    loop = body("tl_paged_few")
+    loop = loop[loop.index("for (int t = first_tile;"):loop.index("// ---- the waves meet")]
+    written, read = loop.rindex("reinterpret_cast<u32x4*>(own"), loop.index("column_read(")
+    assert "wave_exchange();" in loop[written:read] and "wave_exchange();" in loop[loop.rindex("column_read("):]
+    put = body("tl_paged_rows")
+    put = put[put.index("auto put = "):]
+    cleared = put.index("spoiled[buf][wave * KW + lane] = 0;")
+    assert "wave_exchange();" in put[cleared:put.index("] = 1;")]
+    exchange = body("wave_exchange")
+    assert '__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront")' in exchange and "__builtin_amdgcn_wave_barrier()" in exchange
