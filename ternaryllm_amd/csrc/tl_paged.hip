@@ -397,10 +397,11 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // (m0 is a register that the compiler reserves; named all the same, as this writes it)
 // 16 bytes per lane from a buffer's byte `offset` + `more` into LDS at `lds` + 16 * lane, zeros past the buffer's end.  (As assembly, because the
-// compiler would wait for all such loads before any read of LDS; here they are waited for by hand.)
+// compiler would wait for all such loads before any read of LDS; here they are waited for by hand.  The compiler does not see a load here either: the buffer's
+// description comes from the vector unit (v_readfirstlane), which a load may read five wait states later -- the move to m0 and the s_nop's four.)
 __device__ __forceinline__ void buffer_to_lds(uint32_t lds, u32x4 buffer, uint32_t offset, uint32_t more)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(offset), "s"(buffer), "s"(more) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(offset), "s"(buffer), "s"(more) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 

@@ -33,3 +33,25 @@ def test_values_cross_lanes_in_order():
     assert "wave_exchange();" in put[cleared:put.index("] = 1;")]
     exchange = body("wave_exchange")
     assert '__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront")' in exchange and "__builtin_amdgcn_wave_barrier()" in exchange
+
+
+def instructions(name):
+    """The instructions of the one asm statement of a function."""
+    statements = re.findall(r'asm volatile\(((?:\s*"(?:[^"\\]|\\.)*")+)', body(name))
+    assert len(statements) == 1
+    text = "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', statements[0]))
+    return [i.strip() for i in re.split(r"\\n|\\t", text) if i.strip() and not i.endswith(":")]
+
+
+def wait_states(lines):
+    """An instruction is one, s_nop n is n + 1."""
+    return sum(int(i.split()[1]) + 1 if i.startswith("s_nop") else 1 for i in lines)
+
+
+def test_loads_written_as_assembly_wait_for_their_scalars():
+    """A memory instruction may read a scalar register five wait states after a vector instruction wrote it, m0 one after a move."""
+    lines = instructions("buffer_to_lds")
+    load = next(i for i, line in enumerate(lines) if line.startswith("buffer_load"))
+    assert wait_states(lines[:load]) >= 5
+    moved = next(i for i, line in enumerate(lines) if "m0" in line)
+    assert wait_states(lines[moved + 1:load]) >= 1
