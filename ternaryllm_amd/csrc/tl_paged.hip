@@ -330,12 +330,13 @@ struct Running {
 constexpr Running kNothing{kNone, kNone, 0.f, 0.f};
 
 // Eight sums times `by` where `moves` says so.  (As assembly with a branch of its own: around a branch of the compiler's it keeps the sums in two
-// sets of registers and copies all of them from the one to the other at every tile.  The matrix products that made the sums are done: the scores
-// that moved the reference come from later ones.  Those that follow want two steps between a write and their read.)
+// sets of registers and copies all of them from the one to the other at every tile.  The compiler does not see what reads the sums here: a vector
+// instruction may 19 wait states after the longest matrix product that writes them, which are waited for where sums are scaled at all.  Products that
+// follow want two between a write and their read.)
 __device__ __forceinline__ void scale_if(int moves, float by, f32x4& x, f32x4& y)
 {
     float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-    asm volatile("s_cmp_eq_u32 %8, 0\n\ts_cbranch_scc1 .Lkeep%=\n\t"
+    asm volatile("s_cmp_eq_u32 %8, 0\n\ts_cbranch_scc1 .Lkeep%=\n\ts_nop 15\n\ts_nop 2\n\t"
                  "v_mul_f32 %0, %9, %0\n\tv_mul_f32 %1, %9, %1\n\tv_mul_f32 %2, %9, %2\n\tv_mul_f32 %3, %9, %3\n\t"
                  "v_mul_f32 %4, %9, %4\n\tv_mul_f32 %5, %9, %5\n\tv_mul_f32 %6, %9, %6\n\tv_mul_f32 %7, %9, %7\n.Lkeep%=:\n\ts_nop 1"
                  : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]) : "s"(moves), "v"(by) : "scc");

@@ -55,3 +55,12 @@ def test_loads_written_as_assembly_wait_for_their_scalars():
     assert wait_states(lines[:load]) >= 5
     moved = next(i for i, line in enumerate(lines) if "m0" in line)
     assert wait_states(lines[moved + 1:load]) >= 1
+
+
+def test_sums_scaled_in_assembly_wait_for_their_products():
+    """A vector instruction may read what a matrix product wrote 19 wait states after the longest of them, and a product what a vector instruction
+    wrote two after it."""
+    lines = instructions("scale_if")
+    branch = next(i for i, line in enumerate(lines) if line.startswith("s_cbranch"))
+    scaled = [i for i, line in enumerate(lines) if line.startswith("v_")]
+    assert wait_states(lines[branch + 1:scaled[0]]) >= 19 and wait_states(lines[scaled[-1] + 1:]) >= 2
