@@ -457,11 +457,10 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         const int first_tile = (u.first_key + KT - 1) / KT, tiles = (u.end_key + KT - 1) / KT;   // (a share may be empty)
         bool wrong = w.s.wrong;
         const int length = w.s.length;
-        // Tiles that some of the unit's rows see more of than others: values there that are not finite must not meet the weights of 0.  They are made 0
+        // Tiles with tokens that some of the unit's rows do not see: values there that are not finite must not meet the weights of 0.  They are made 0
         // in LDS, and the rows that do see their key are NaN.
         const int all_see = length - w.s.n + u.first_token;       // the last key that every row sees
-        const bool rows_differ = min(a.tile_tokens, w.s.n - u.first_token) > 1;
-        const int first_mixed = rows_differ ? max(all_see + 1, 0) / KT : INT_MAX;   // ... are the last
+        const int first_mixed = all_see < length - 1 ? max(all_see + 1, 0) / KT : INT_MAX;   // ... are the last
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
         // page of this wave's keys of the tile after the next (by a vector load: a scalar one would be waited for with the first read of LDS)
@@ -796,7 +795,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
-        const bool rows_differ = min(a.tile_tokens, w.s.n - u.first_token) > 1;
 
         auto spoil = [&](unsigned long long lanes, int first) {   // lanes whose pieces of values were not finite, of keys from `first` on
             for (int k = 0; lanes != 0 && k < VKEYS; ++k)
@@ -804,8 +802,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
         };
         for (int t = first_tile; t < tiles; t += 4) {
             const bool ends = t * KT + KT > length;
-            // a tile that some rows see more of than others: values that are not finite become 0, and the rows that see their key NaN
-            const bool mixed = rows_differ && t * KT + KT - 1 > all_see;
+            // a tile with tokens that some rows do not see: values that are not finite become 0, and the rows that see their key NaN
+            const bool mixed = all_see < length - 1 && t * KT + KT - 1 > all_see;
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
                 const int key = i * VKEYS + lane / PIECES, p = lane % PIECES;

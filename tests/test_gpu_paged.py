@@ -326,6 +326,32 @@ def test_values_that_are_not_finite_among_the_new_tokens(hd, most):
             assert not torch.isfinite(got[token - 100:100]).all(-1).any(), (kind, which, token)
 
 
+# so many query heads on a key head that a workgroup of 64, 128 or 16 rows has those of one token only
+@pytest.mark.parametrize("heads,hd,most,widest", [(40, 64, 20, None), (40, 128, 20, None), (33, 256, 20, None), (80, 64, 20, 65536), (80, 128, 20, 65536), (16, 128, 1, None), (11, 64, 0, None),
+                                                  (16, 256, 1, None)])
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+def test_later_tokens_that_are_not_finite_beside_rows_of_one_token(heads, hd, most, widest, kind):
+    """The chunk's later tokens share the last tile of an earlier row, and weigh nothing in it, whatever they hold."""
+    seqs = paged.Sequences([(20, 100), (7, 7)], 16, widest=None if widest is None else widest // 16)
+    pages = fresh_pages(seqs, 1, hd, kind, spoiled=False)
+    held = [paged.values(*t) for t in zip(pages[:2], pages[2:])]
+    q = random((seqs.tokens, heads, hd), 3)
+    want = paged.attention(q, *held, seqs, 1 / math.sqrt(hd))
+    bound = attention_bound(q, *held, want, 100, 1 / math.sqrt(hd))
+    for which, token in ((1, 90), (1, 99), (0, 85), (1, 97)):
+        now = list(t if t is None else t.clone() for t in pages)
+        where = int(seqs.table[0, token // 16]), 0, token % 16, 5
+        if kind == "e4m3":
+            now[which].view(torch.uint8)[where] = 0x7f
+        else:
+            now[which][where] = math.nan if which == 0 else math.inf
+        got = ops.paged_attention(q.cuda(), on_gpu(ops.Pages(*now)), seqs.batch(ops, most=most)).cpu().view(seqs.tokens, heads, hd)
+        good = torch.ones(seqs.tokens, dtype=torch.bool)
+        good[token - 80:20] = False                               # row i is token 80 + i
+        assert ((got.double() - want).abs() <= bound)[good].all(), (which, token)
+        assert not torch.isfinite(got[token - 80:20]).all(-1).any(), (which, token)
+
+
 def test_no_sequences_and_no_rows():
     pages = ops.Pages(*(torch.zeros((2, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
     i32 = dict(dtype=torch.int32, device="cuda")
