@@ -229,13 +229,26 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x.v[j] = 0.f;
             if (kind < 2 && (kind == 0 ? a.q.w : a.k.w)) {
-                float squares = 0.f;
+                auto mean_of_squares = [&](float eps) {
+                    float squares = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) squares = fmaf(x.v[j], x.v[j], squares);
-                squares = over_lanes(squares, bits, [](float u, float v) { return u + v; });
-                // (a step of Newton's on the instruction's root: an error of all of a head's values alike turns more of its 8-bit codes than any other)
-                const float mean = fmaf(squares, part, a.eps), root = rsqrtf(mean);
-                const float inv = root < __builtin_huge_valf() ? fmaf(0.5f * root, fmaf(-mean * root, root, 1.0f), root) : root;
+                    for (int j = 0; j < 8; ++j) squares = fmaf(x.v[j], x.v[j], squares);
+                    return fmaf(over_lanes(squares, bits, [](float u, float v) { return u + v; }), part, eps);
+                };
+                float mean = mean_of_squares(a.eps);
+                if constexpr (sizeof(T) == 4) {                 // heads whose squares leave the range of fp32: of x times a power of two, which cancels
+                    const bool large = !(mean < __builtin_huge_valf()), small = mean < 0x1p-100f;
+                    if (__builtin_amdgcn_ballot_w64(large || small) != 0) {
+                        const float by = large ? 0x1p-70f : small ? 0x1p100f : 1.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x.v[j] *= by;
+                        mean = mean_of_squares(a.eps * by * by);
+                    }
+                }
+                // (a step of Newton's on the instruction's root: an error of all of a head's values alike turns more of its 8-bit codes than any other; of 0 and
+                // infinity there is none)
+                const float root = rsqrtf(mean);
+                const float inv = root > 0.f && root < __builtin_huge_valf() ? fmaf(0.5f * root, fmaf(-mean * root, root, 1.0f), root) : root;
                 Eight w;
                 w.set(kind == 0 ? weight[0] : weight[1]);
                 if (there) {

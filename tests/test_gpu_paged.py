@@ -92,6 +92,38 @@ def test_rope_heads_keeps_what_is_not_finite_in_its_own_head():
     assert not bad.any()
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_norms_of_fp32_heads_of_any_magnitude(hd, eps):
+    """Squares that overflow or vanish in fp32 are no reason for a head of finite values not to be normalised.  Heads of every magnitude side by side in a wave."""
+    sizes = [3e37, 1e25, 2e18, 1.0, 1e-12, 1e-19, 1e-25, 1e-38]
+    x = random((3, len(sizes), hd), hd, torch.float32).clamp(-5, 5) * torch.tensor(sizes)[:, None]
+    w = 1 + 0.2 * random((hd,), 5, torch.float32)
+    f, at = frequencies(hd // 2), torch.tensor([0, 17, 900000])
+    want = paged.normed(x, w, eps)
+    bound = paged.rope_bound(want, paged.partners(want, hd // 2, False), 1.0, torch.float32, want)
+    got, _ = ops.rope_heads(x.cuda(), None, at.cuda(), f.cuda(), q_norm=w.cuda(), eps=eps)
+    assert ((got.cpu().double() - paged.rotated(want, at, f, False, 1.0)).abs() <= bound).all()
+    # and on the way into pages, of which they are the keys
+    seqs = paged.Sequences([(3, 3)], 16)
+    pages = on_gpu(fresh_pages(seqs, len(sizes), hd, "float16", spoiled=False))
+    ops.rope_to_pages(None, x.cuda(), torch.zeros_like(x).cuda(), pages, seqs.batch(ops), k_norm=w.cuda(), eps=eps)
+    keys = ops.read_pages(pages, seqs.batch(ops), 3)[0].cpu().double()
+    assert ((keys - want).abs() <= bound + 2.0 ** -11 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_norms_of_heads_with_an_infinity(dtype):
+    """Its root is infinite: what is finite beside it becomes 0, itself NaN."""
+    x = random((2, 3, 64), 3, dtype)
+    x[0, 1, 7], x[1, 2, 40] = math.inf, -math.inf
+    got = ops.rope_heads(x.cuda(), None, None, None, q_norm=torch.ones(64).to(dtype).cuda())[0].cpu()
+    want = paged.normed(x, torch.ones(64), 1e-6)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(got).sum()) == 2
+    for row in (got[0, 1], got[1, 2]):
+        assert (row[~torch.isnan(row)] == 0).all()
+
+
 # ---------------------------------------------------------------- into pages and back
 BATCHES = [
     ([(1, 1)], 16), ([(1, 17)], 16), ([(3, 3), (0, 5), (1, 40), (16, 16), (17, 33)], 16), ([(2, 130), (0, 0), (5, 64)], 64), ([(40, 40), (1, 257)], 256),
