@@ -458,13 +458,30 @@ class TernaryLlamaDecoder(nn.Module):
     @torch.no_grad()
     def extend(self, cache, chunks):
         """A pass over new tokens of sequences of any lengths: chunks = [(sequence of `cache`, LongTensor of its new tokens, one or more), ...].
-        Their keys and values go into the cache; returns the logits of each chunk's last token, [chunks, vocab]."""
-        if not chunks or any(t.dim() != 1 or t.numel() == 0 for _, t in chunks):
-            raise ValueError("every chunk is a sequence and a one-dimensional tensor of one or more new tokens")
+        Their keys and values go into the cache; returns the logits of each chunk's last token, [chunks, vocab].  Where it raises, the sequences
+        are as they were."""
+        if not chunks or any(t.dim() != 1 or t.numel() == 0 or t.dtype not in (torch.int64, torch.int32) for _, t in chunks):
+            raise ValueError("every chunk is a sequence and a one-dimensional integer tensor of one or more new tokens")
         if any(cache.length(s) + t.numel() > self.max_seq_len for s, t in chunks):
             raise ValueError("a sequence would be longer than max_seq_len")
+        self._check_paged()
+        c = self.config
+        if cache.layers < c.num_hidden_layers or (cache.kv_heads, cache.head_dim) != (c.num_attention_heads, c.head_dim):
+            raise ValueError("the cache's layers, heads or head_dim are not this decoder's")
+        tokens = torch.cat([t.to(self.embed_tokens.device) for _, t in chunks])
+        before = [(s, cache.length(s)) for s, _ in chunks]
         batch = cache.extend([(s, t.numel()) for s, t in chunks])
-        return self.extend_batch(cache, torch.cat([t for _, t in chunks]).to(self.embed_tokens.device), batch)
+        try:
+            return self.extend_batch(cache, tokens, batch)
+        except BaseException:
+            for s, length in reversed(before):       # (the last pages taken go back first: the next call gets the same)
+                cache.truncate(s, length)
+            raise
+
+    def _check_paged(self):
+        c = self.config
+        if self.dtype != torch.float16 or c.head_dim not in (64, 128, 256) or c.hidden_size != c.num_attention_heads * c.head_dim:
+            raise RuntimeError("sequences over pages need a float16 decoder with heads of 64, 128 or 256")
 
     @torch.no_grad()
     def extend_batch(self, cache, tokens, batch):
@@ -473,8 +490,7 @@ class TernaryLlamaDecoder(nn.Module):
         sequences.  Rows of no sequence are computed and mean nothing."""
         c = self.config
         nh, hd = c.num_attention_heads, c.head_dim
-        if self.dtype != torch.float16 or hd not in (64, 128, 256) or c.hidden_size != nh * hd:
-            raise RuntimeError("sequences over pages need a float16 decoder with heads of 64, 128 or 256")
+        self._check_paged()
         f = getattr(self, "_frequencies", None)
         if f is None or f.device != tokens.device:
             f = self._frequencies = rope_frequencies(hd, c.rope_theta, device=tokens.device)[0]

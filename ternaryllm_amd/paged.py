@@ -21,6 +21,7 @@ class PagedCache:
         if layers < 1 or pages < 1 or kv_heads < 1 or head_dim < 16 or head_dim % 16:
             raise ValueError("layers, pages and kv_heads must be positive, head_dim a multiple of 16")
         self.page_size, self.device = page_size, torch.device(device)
+        self.layers, self.kv_heads, self.head_dim = layers, kv_heads, head_dim
         shape = (layers, 2, pages, kv_heads, page_size, head_dim)
         self._rows = torch.zeros(shape, dtype=torch.float16 if dtype == torch.float16 else torch.uint8, device=device)
         self._exponents = None if dtype == torch.float16 else torch.zeros(shape[:-1], dtype=torch.uint8, device=device)
@@ -63,24 +64,29 @@ class PagedCache:
 
     def extend(self, chunks):
         """Makes room for new tokens, chunks = [(sequence, how many), ...], each sequence once, and returns the ops.PageBatch of a pass over
-        them.  Without pages enough nothing changes and RuntimeError is raised."""
+        them.  Without pages enough RuntimeError is raised; nothing changes where anything is."""
         numbers = [s for s, _ in chunks]
         if not chunks or len(set(numbers)) < len(numbers) or any(n < 0 for _, n in chunks) or any(s not in self._sequences for s in numbers):
             raise ValueError("chunks are of open sequences, each named once, and not negative")
         more = [-(-(self._sequences[s][1] + n) // self.page_size) - len(self._sequences[s][0]) for s, n in chunks]
         if sum(more) > len(self._free):
             raise RuntimeError(f"{sum(more)} pages needed, {len(self._free)} free")
+        after, left = {}, len(self._free)
         for (s, n), count in zip(chunks, more):
             held, length = self._sequences[s]
-            self._sequences[s] = (held + [self._free.pop() for _ in range(count)], length + n)
-        return self._batch(numbers, [n for _, n in chunks])
+            after[s] = (held + self._free[left - count:left][::-1], length + n)
+            left -= count
+        batch = self._batch(numbers, [n for _, n in chunks], after)
+        self._sequences.update(after)
+        del self._free[left:]
+        return batch
 
     def whole(self, sequences):
         """The ops.PageBatch whose rows are all tokens of these sequences (what ops.read_pages reads)."""
-        return self._batch(sequences, [self._sequences[s][1] for s in sequences])
+        return self._batch(sequences, [self._sequences[s][1] for s in sequences], self._sequences)
 
-    def _batch(self, numbers, rows):
-        held, lengths = zip(*(self._sequences[s] for s in numbers))
+    def _batch(self, numbers, rows, sequences):
+        held, lengths = zip(*(sequences[s] for s in numbers))
         columns = max(1, max(len(h) for h in held))
         starts = [0]
         for n in rows:

@@ -143,3 +143,25 @@ def test_norms_that_are_not_as_built_and_refusals(model, cuda):
     with pytest.raises(RuntimeError):
         model.extend(cache, [(a, text.repeat(4))])               # more pages than there are
     assert cache.length(a) == cache.length(b) == 30
+
+
+def test_a_pass_that_raises_can_be_made_again(model, cuda):
+    """A layer that raises, behind others that have written their pages: lengths and pages are as before it, and so are the logits of the next try."""
+    text, other = tokens_of(model, (60, 45), cuda)
+    cache = model.paged_cache(12, 16)
+    a, b = cache.open(), cache.open()
+    model.extend(cache, [(a, text[:20]), (b, other[:5])])
+    free = cache.free_pages
+    hook = model.layers[1].o_proj.register_forward_pre_hook(lambda *_: (_ for _ in ()).throw(RuntimeError("stopped")))
+    try:
+        with pytest.raises(RuntimeError, match="stopped"):
+            model.extend(cache, [(a, other[:30]), (b, text[:40])])
+    finally:
+        hook.remove()
+    assert (cache.length(a), cache.length(b), cache.free_pages) == (20, 5, free)
+    got = model.extend(cache, [(a, text[20:]), (b, other[5:])])
+    fresh = model.paged_cache(12, 16)
+    numbers = fresh.open(), fresh.open()
+    model.extend(fresh, [(numbers[0], text[:20]), (numbers[1], other[:5])])
+    want = model.extend(fresh, [(numbers[0], text[20:]), (numbers[1], other[5:])])
+    assert torch.equal(got, want)

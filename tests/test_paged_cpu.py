@@ -251,6 +251,51 @@ def test_sequences_hold_the_pages_that_they_need():
     assert cache.length(b) == 4
 
 
+def state_of(cache):
+    return list(cache._free), {s: (list(held), n) for s, (held, n) in cache._sequences.items()}
+
+
+def test_a_batch_that_cannot_be_made_takes_no_pages(monkeypatch):
+    from ternaryllm_amd import PagedCache
+    cache = PagedCache(1, 9, 2, 64, 16, device="cpu")
+    a, b = cache.open(), cache.open()
+    cache.extend([(a, 20), (b, 1)])
+    before = state_of(cache)
+
+    def none(*_):
+        raise RuntimeError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "PageBatch", none)
+        with pytest.raises(RuntimeError, match="no memory"):
+            cache.extend([(a, 20), (b, 40)])
+    assert state_of(cache) == before
+
+
+@pytest.mark.parametrize("shape,dtype,why", [((128, 4), torch.float16, RuntimeError), ((256, 4), torch.float32, RuntimeError), ((256, 4), torch.float16, None)])
+def test_a_pass_that_raises_leaves_the_sequences_as_they_were(shape, dtype, why):
+    """Refused before it begins -- heads of 32, a decoder of fp32 -- or raising on the way, as every pass does here, where there is no GPU."""
+    from ternaryllm_amd import PagedCache, TernaryConfig, TernaryLlamaDecoder
+    cfg = TernaryConfig(hidden_size=shape[0], intermediate_size=128, num_hidden_layers=2, num_attention_heads=shape[1], num_key_value_heads=shape[1], vocab_size=64,
+                        max_position_embeddings=200, sparsity=0.66)
+    model = TernaryLlamaDecoder(cfg, seed=5, device="cpu", dtype=dtype, pack_threads=2)
+    cache = PagedCache(2, 12, shape[1], cfg.head_dim, 16, device="cpu")
+    a, b, c = cache.open(), cache.open(), cache.open()
+    cache.extend([(a, 20), (b, 3), (c, 33)])
+    cache.close(c)
+    before, text = state_of(cache), torch.arange(40)
+    with pytest.raises(why or Exception):
+        model.extend(cache, [(b, text), (a, text[:13])])
+    assert state_of(cache) == before
+    for bad in (text.float(), text.bool(), text[None], text[:0], text.to(torch.uint8)):
+        with pytest.raises(ValueError):
+            model.extend(cache, [(a, text[:3]), (b, bad)])
+    with pytest.raises(ValueError if why is None else why):          # another decoder's cache
+        other = PagedCache(1, 12, shape[1], cfg.head_dim, 16, device="cpu")
+        model.extend(other, [(other.open(), text)])
+    assert state_of(cache) == before
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float8_e4m3fn])
 def test_layers_of_a_paged_cache(dtype):
     from ternaryllm_amd import PagedCache
