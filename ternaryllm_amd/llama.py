@@ -119,6 +119,8 @@ class TernaryLlamaDecoder(nn.Module):
         ang = torch.cat([ang, ang], dim=-1)
         self.register_buffer("rope_cos", ang.cos().to(dev, dtype), False)
         self.register_buffer("rope_sin", ang.sin().to(dev, dtype), False)
+        # of passes over pages (no buffer: float64 whatever the decoder is turned into)
+        self._frequencies = rope_frequencies(hd, config.rope_theta, device=dev)[0]
         self._cache = None
         self._graph = None
         # single-token steps use the library's rotary / cache / attention kernels; False keeps them on torch operators
@@ -150,6 +152,11 @@ class TernaryLlamaDecoder(nn.Module):
         # have no such kernel.
         self.piece_fold = 2
         self._layer_index = {id(layer): i for i, layer in enumerate(self.layers)}
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._frequencies = self._frequencies.to(self.embed_tokens.device)
+        return self
 
     # -- pieces ------------------------------------------------------------------------------
     @staticmethod
@@ -491,9 +498,7 @@ class TernaryLlamaDecoder(nn.Module):
         c = self.config
         nh, hd = c.num_attention_heads, c.head_dim
         self._check_paged()
-        f = getattr(self, "_frequencies", None)
-        if f is None or f.device != tokens.device:
-            f = self._frequencies = rope_frequencies(hd, c.rope_theta, device=tokens.device)[0]
+        f = self._frequencies
         fused = self._norms_as_built()
 
         def add_norm(x, y, norm):

@@ -165,3 +165,22 @@ def test_a_pass_that_raises_can_be_made_again(model, cuda):
     model.extend(fresh, [(numbers[0], text[:20]), (numbers[1], other[:5])])
     want = model.extend(fresh, [(numbers[0], text[20:]), (numbers[1], other[5:])])
     assert torch.equal(got, want)
+
+
+def test_the_first_pass_may_be_the_captured_one(cuda):
+    """Nothing of a pass is left to be made on the host at its first call, in a decoder made on the GPU or moved there."""
+    from ternaryllm_amd import TernaryConfig, TernaryLlamaDecoder
+    cfg = TernaryConfig(hidden_size=256, intermediate_size=512, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=2, vocab_size=128,
+                        max_position_embeddings=100, sparsity=0.66)
+    for model in (TernaryLlamaDecoder(cfg, seed=5, device=cuda, pack_threads=2), TernaryLlamaDecoder(cfg, seed=5, device="cpu", pack_threads=2).to(cuda)):
+        cache = model.paged_cache(10, 16)
+        text = torch.arange(6, device=cuda)
+        batch = cache.extend([(cache.open(), 4), (cache.open(), 2)])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = model.extend_batch(cache, text, batch)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            got = logits.clone()
+            assert torch.equal(model.extend_batch(cache, text, batch), got)
