@@ -187,12 +187,12 @@ int64_t step(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 
 
 bool absent(PyObject* o) { return o == Py_None; }
 
-// Whether a derivative is asked for, which Python refuses.
+// Whether a derivative is asked for, backward or forward, which Python refuses.
 bool differentiated(std::initializer_list<const at::Tensor*> tensors)
 {
-    if (!c10::GradMode::is_enabled()) return false;
+    const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const at::Tensor* t : tensors)
-        if (t->requires_grad()) return true;
+        if ((backward && t->requires_grad()) || (forward && t->_fw_grad(0).defined())) return true;
     return false;
 }
 
@@ -230,7 +230,7 @@ bool rotation(PyObject* frequencies, PyObject* positions, PyObject* factor, PyOb
     *r = tl_rotation{nullptr, nullptr, 0, 0, (float)f, (float)e};
     if (absent(frequencies)) return true;
     const at::Tensor* t = plain(frequencies);
-    if (!t || t->dim() != 1 || t->scalar_type() != at::kDouble || t->device() != like.device() || !t->is_contiguous()) return false;
+    if (!t || t->dim() != 1 || t->scalar_type() != at::kDouble || t->device() != like.device() || !t->is_contiguous() || differentiated({t})) return false;
     r->frequencies = static_cast<const double*>(t->data_ptr());
     r->pairs = (int32_t)t->numel();
     r->interleaved = pairs_side_by_side;
@@ -249,7 +249,7 @@ bool pages_and_batch(PyObject* pages, PyObject* batch, c10::Device device, tl_pa
     if (!PyTuple_Check(pages) || PyTuple_GET_SIZE(pages) != 4 || !PyTuple_Check(batch) || PyTuple_GET_SIZE(batch) != 4) return false;
     const at::Tensor *k = member(pages, 0), *v = member(pages, 1), *ke = member(pages, 2), *ve = member(pages, 3);
     if (!k || !v || k->dim() != 4 || k->numel() == 0 || k->sizes() != v->sizes() || k->strides() != v->strides() || k->stride(3) != 1 ||
-        k->scalar_type() != v->scalar_type() || k->device() != device || v->device() != device)
+        k->scalar_type() != v->scalar_type() || k->device() != device || v->device() != device || differentiated({k, v}))
         return false;
     const bool bytes = k->scalar_type() == at::kFloat8_e4m3fn;
     if (!bytes && k->scalar_type() != at::kHalf) return false;
@@ -407,7 +407,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
     const c10::DeviceGuard guard(q->device());
     const at::Tensor* given = absent(a[4]) ? nullptr : plain(a[4]);
     if (!absent(a[4]) && (!given || given->dim() != 2 || given->size(0) != tokens || given->size(1) != width || given->scalar_type() != at::kHalf ||
-                          given->device() != q->device() || !given->is_contiguous() || given->storage().data() == q->storage().data()))
+                          given->device() != q->device() || !given->is_contiguous() || differentiated({given}) || given->storage().data() == q->storage().data()))
         Py_RETURN_NONE;
     if (g_attention_workspace(tokens, (int)q->size(1), &p, &b, most, &need) != TL_OK) Py_RETURN_NONE;
     at::Tensor out = given ? *given : at::empty({tokens, width}, q->options().requires_grad(false));

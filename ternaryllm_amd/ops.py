@@ -8,6 +8,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .packing import PackedWeight
@@ -716,8 +717,9 @@ def _rotation(frequencies, positions, tokens, factor, interleaved, eps, like):
 
 
 def _forward_only(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the operators of a paged cache have no backward pass: call them under torch.no_grad()")
+    backward, forward = torch.is_grad_enabled(), torch._C._is_fwd_grad_enabled()
+    if any(t is not None and ((backward and t.requires_grad) or (forward and forward_ad.unpack_dual(t).tangent is not None)) for t in tensors):
+        raise RuntimeError("the operators of a paged cache have no backward pass and no tangents: call them under torch.no_grad(), with tensors that carry none")
 
 
 def _cuda(x, what):
@@ -734,7 +736,7 @@ def rope_heads(q, k, positions, frequencies, *, factor=1.0, interleaved=False, q
     both = _short().rope_heads(q, k, positions, frequencies, factor, interleaved, q_norm, k_norm, eps, q_out, k_out)
     if both is not None:
         return both
-    _forward_only(q, k, q_norm, k_norm)
+    _forward_only(q, k, frequencies, q_norm, k_norm, q_out, k_out)
     if k is not None and (k.dim() != 3 or k.shape[::2] != q.shape[::2] or k.dtype != q.dtype or k.device != q.device):
         raise ValueError("k must have q's tokens, head_dim, type and device")
     if frequencies is not None and positions is None:
@@ -762,7 +764,7 @@ def rope_to_pages(q, k, v, pages, batch, frequencies=None, positions=None, *, fa
         rotated = _short().rope_to_pages(q, k, v, pages, batch, frequencies, positions, factor, interleaved, q_norm, k_norm, eps)
         if rotated is not None:
             return rotated
-    _forward_only(q, k, v, q_norm, k_norm)
+    _forward_only(q, k, v, pages.k, pages.v, frequencies, q_norm, k_norm, q_out)
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one type and device")
     if q is not None and (q.dim() != 3 or q.shape[::2] != k.shape[::2] or q.dtype != k.dtype or q.device != k.device):
@@ -791,6 +793,7 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
         both = _short().read_pages(pages, batch, tokens, dtype is torch.float16)
         if both is not None:
             return both
+    _forward_only(pages.k, pages.v, k_out, v_out)
     if pages.k.dim() != 4:
         raise ValueError("pages must be [pages, kv_heads, page_size, head_dim]")
     device, (_, heads, _, hd) = pages.k.device, pages.k.shape
@@ -818,7 +821,7 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
     y = _short().paged_attention(q, pages, batch, scale, out)
     if y is not None:
         return y
-    _forward_only(q)
+    _forward_only(q, pages.k, pages.v, out)
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
     tokens, heads, hd = q.shape

@@ -538,3 +538,11 @@ def test_the_short_way_and_the_general_one(monkeypatch):
     monkeypatch.setattr(ops, "_short", _NoShortWay)
     general = all_of_them()
     assert len(short) == len(general) and all(torch.equal(a, b) for a, b in zip(short, general))
+
+
+def test_no_derivative_is_lost_on_the_short_way():
+    from tests.test_paged_cpu import check_no_derivative_is_lost, parts
+    q, k, pages, batch = parts()
+    to = lambda t: None if t is None else t.cuda()
+    check_no_derivative_is_lost(q.cuda(), k.cuda(), ops.Pages(*map(to, pages)), ops.PageBatch(*map(to, batch[:3]), 1), torch.zeros(3, dtype=torch.int64).cuda(),
+                                torch.ones(32, dtype=torch.float64).cuda(), torch.ones(64).half().cuda())

@@ -98,6 +98,35 @@ def test_no_backward_pass():
             call(q.clone().requires_grad_())
 
 
+def derived_calls(q, k, pages, batch, at, f, w):
+    """(operand, call of it) of every floating operand of every operator."""
+    return [(q, lambda x: ops.rope_heads(x, k, at, f)), (k, lambda x: ops.rope_heads(q, x, at, f)), (f, lambda x: ops.rope_heads(q, k, at, x)),
+            (w, lambda x: ops.rope_heads(q, k, at, f, q_norm=x)), (q, lambda x: ops.rope_heads(q, k, at, f, q_out=x)),
+            (q, lambda x: ops.rope_to_pages(x, k, k, pages, batch, f)), (k, lambda x: ops.rope_to_pages(q, x, k, pages, batch, f)),
+            (k, lambda x: ops.rope_to_pages(q, k, x, pages, batch, f)), (f, lambda x: ops.rope_to_pages(q, k, k, pages, batch, x)),
+            (pages.k, lambda x: ops.rope_to_pages(q, k, k, pages._replace(k=x), batch, f)), (pages.v, lambda x: ops.rope_to_pages(q, k, k, pages._replace(v=x), batch)),
+            (w, lambda x: ops.rope_to_pages(q, k, k, pages, batch, f, k_norm=x)), (pages.k, lambda x: ops.read_pages(pages._replace(k=x), batch, 3)),
+            (pages.v, lambda x: ops.read_pages(pages._replace(v=x), batch, 3)), (k, lambda x: ops.read_pages(pages, batch, 3, k_out=x, v_out=k)),
+            (q, lambda x: ops.paged_attention(x, pages, batch)), (pages.k, lambda x: ops.paged_attention(q, pages._replace(k=x), batch)),
+            (pages.v, lambda x: ops.paged_attention(q, pages._replace(v=x), batch)), (q, lambda x: ops.paged_attention(q, pages, batch, out=x.view(3, -1)))]
+
+
+def check_no_derivative_is_lost(q, k, pages, batch, at, f, w):
+    from torch.autograd import forward_ad
+    for i, (t, call) in enumerate(derived_calls(q, k, pages, batch, at, f, w)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call(t.detach().clone().requires_grad_())
+            pytest.fail(f"call {i} lost a gradient")
+        with torch.no_grad(), forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangents"):
+            call(forward_ad.make_dual(t.detach().clone(), torch.ones_like(t)))
+            pytest.fail(f"call {i} lost a tangent")
+
+
+def test_no_derivative_is_lost():
+    q, k, pages, batch = parts()
+    check_no_derivative_is_lost(q, k, pages, batch, torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64), torch.ones(64).half())
+
+
 def test_outputs_that_overlap_operands():
     at, f = torch.zeros(3, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
     rows = torch.zeros((5, 6, 64), dtype=torch.float16)
