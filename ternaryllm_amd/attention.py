@@ -42,7 +42,8 @@ def rope_frequencies(rotary_dim, theta, scaling=None, device=None):
       "llama3"   frequencies whose wave is longer than original_max_position_embeddings / low_freq_factor divided by factor, those shorter than
                  original_max_position_embeddings / high_freq_factor kept, between the two a mean weighted by the number of waves;
       "yarn"     divided by factor where fewer than beta_slow (1) waves fit the original length, kept from beta_fast (32) on, a ramp over the
-                 dimensions between (Peng et al. 2023), and attention_factor, 0.1 ln(factor) + 1, on cosines and sines."""
+                 dimensions between (Peng et al. 2023), whose ends are whole dimensions unless truncate is false; and attention_factor on cosines and
+                 sines, 0.1 ln(factor) + 1, or with mscale and mscale_all_dim (0.1 mscale ln(factor) + 1) / (0.1 mscale_all_dim ln(factor) + 1)."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim={rotary_dim} must be positive and even")
     scaling = scaling or {}
@@ -60,13 +61,19 @@ def rope_frequencies(rotary_dim, theta, scaling=None, device=None):
         def dimension(waves):   # the pair of which so many waves fit the original length
             return rotary_dim * math.log(scaling["original_max_position_embeddings"] / (2 * math.pi * waves)) / (2 * math.log(theta))
 
-        low = max(math.floor(dimension(scaling.get("beta_fast") or 32)), 0)
-        high = min(math.ceil(dimension(scaling.get("beta_slow") or 1)), rotary_dim - 1)
+        low, high = dimension(scaling.get("beta_fast") or 32), dimension(scaling.get("beta_slow") or 1)
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         kept = 1 - ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
         f = kept * f + (1 - kept) * f / scaling["factor"]
         factor = scaling.get("attention_factor")
         if factor is None:
-            factor = 0.1 * math.log(scaling["factor"]) + 1 if scaling["factor"] > 1 else 1.0
+            def grown(by):
+                return 0.1 * by * math.log(scaling["factor"]) + 1 if scaling["factor"] > 1 else 1.0
+
+            both = scaling.get("mscale"), scaling.get("mscale_all_dim")
+            factor = grown(both[0]) / grown(both[1]) if all(both) else grown(1.0)
     elif kind != "default":
         raise ValueError(f"rope_type {kind!r} is not known")
     return f.to(device), float(factor)

@@ -400,3 +400,32 @@ def test_rope_frequencies_refuses():
     for args in ((0, 1e4), (7, 1e4), (8, 1e4, {"rope_type": "no such"})):
         with pytest.raises(ValueError):
             rope_frequencies(*args)
+
+
+YARNS = [{"mscale": 1.0, "mscale_all_dim": 1.0}, {"mscale": 0.707, "mscale_all_dim": 1.2}, {"mscale": 0.5}, {"mscale_all_dim": 0.5}, {"mscale": 0.8, "mscale_all_dim": 0.0},
+         {"mscale": 0.8, "mscale_all_dim": 0.6, "attention_factor": 1.5}, {"truncate": False}, {"truncate": True}, {"truncate": False, "mscale": 0.7, "mscale_all_dim": 0.9}]
+
+
+@pytest.mark.parametrize("more", YARNS)
+@pytest.mark.parametrize("scale", [0.5, 1.0, 8.0])
+def test_yarn_takes_all_that_a_configuration_says(more, scale):
+    from ternaryllm_amd.attention import rope_frequencies
+    rotary, theta, length = 64, 10000.0, 4096
+    got, factor = rope_frequencies(rotary, theta, {"rope_type": "yarn", "factor": scale, "original_max_position_embeddings": length, **more})
+    log = math.log(scale) if scale > 1 else 0.0                   # (contexts that do not grow want no factor)
+    want = 0.1 * log + 1
+    if more.get("mscale") and more.get("mscale_all_dim"):
+        want = (0.1 * more["mscale"] * log + 1) / (0.1 * more["mscale_all_dim"] * log + 1)
+    assert abs(factor - more.get("attention_factor", want)) < 1e-15
+    edges = [rotary * math.log(length / (2 * math.pi * n)) / (2 * math.log(theta)) for n in (32, 1)]
+    if more.get("truncate", True):
+        edges = math.floor(edges[0]), math.ceil(edges[1])
+    for i in range(rotary // 2):
+        ramp = min(max((i - edges[0]) / (edges[1] - edges[0]), 0.0), 1.0)
+        f = theta ** (-2 * i / rotary)
+        assert abs(got[i].item() / (f / scale * ramp + f * (1 - ramp)) - 1) < 1e-12
+
+
+@pytest.mark.parametrize("more", YARNS)
+def test_yarn_is_that_of_transformers(more):
+    test_rope_frequencies_are_those_of_transformers({"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096, **more})
