@@ -23,9 +23,9 @@ struct Batch {
 };
 
 // Where a row of the batch belongs: its sequence (-1: none) and its index there (negative where the sequence is said to be
-// shorter than its rows).
+// shorter than its rows), and how long that is.
 struct Place {
-    int seq, index;
+    int seq, index, length;
 };
 
 // By a whole wave, for one row that is the same in all lanes: 64 starts are compared at a time.
@@ -40,11 +40,12 @@ __device__ __forceinline__ Place place_of(const Batch& b, int token)
         if (more < 64) break;
     }
     const int seq = below - 1;
-    if (seq < 0 || seq >= b.seqs) return Place{-1, 0};
-    return Place{seq, b.lengths[seq] - b.starts[seq + 1] + token};
+    if (seq < 0 || seq >= b.seqs) return Place{-1, 0, 0};
+    const int length = b.lengths[seq];
+    return Place{seq, length - b.starts[seq + 1] + token, length};
 }
 
-// Page and slot of a token of a sequence; page -1: the table has none that is a page.
+// Page and slot of a token of a sequence; page -1: the table has none that is a page, or does not hold the sequence.
 struct Slot {
     int page, slot;
 };
@@ -52,7 +53,7 @@ struct Slot {
 __device__ __forceinline__ Slot slot_of(const Pages& p, const Batch& b, const Place& at)
 {
     const int column = at.index >> p.shift;
-    if (at.seq < 0 || at.index < 0 || column >= b.table_pages) return Slot{-1, 0};
+    if (at.seq < 0 || at.index < 0 || column >= b.table_pages || at.length > b.table_pages << p.shift) return Slot{-1, 0};
     const int page = b.table[at.seq * b.table_stride + column];
     return Slot{(unsigned)page < p.pages ? page : -1, at.index & ((1 << p.shift) - 1)};
 }

@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
     Raw<T> weight[2];
     if (inside && a.q.w) weight[0] = raw_eight(static_cast<const T*>(a.q.w) + d);
     if (inside && a.k.w) weight[1] = raw_eight(static_cast<const T*>(a.k.w) + d);
-    Place at{0, 0};
+    Place at{0, 0, 0};
     Slot slot{-1, 0};
     if constexpr (W != kRows) {
         at = place_of(a.batch, token);

@@ -333,6 +333,28 @@ def test_pages_and_lengths_that_are_none(most):
     assert torch.equal(got[:2], good[:2]) and torch.isnan(got[2:]).all()
 
 
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+def test_a_length_that_the_table_does_not_hold_is_no_length(kind):
+    """Nothing of such a sequence is written or read, the rows whose pages the table does have neither; the others are as ever."""
+    seqs = paged.Sequences([(3, 40), (9, 60), (2, 2)], 16)
+    pages, batch = on_gpu(fresh_pages(seqs, 2, 64, kind, spoiled=False)), seqs.batch(ops)
+    k, v = random((seqs.tokens, 2, 64), 5).cuda(), random((seqs.tokens, 2, 64), 6).cuda()
+    good, want = ops.Pages(*(None if t is None else t.clone() for t in pages)), ops.Pages(*(None if t is None else t.clone() for t in pages))
+    ops.rope_to_pages(None, k, v, want, batch)
+    read = ops.read_pages(want, batch, seqs.tokens)
+    batch.lengths[1] = batch.table.shape[1] * 16 + 1              # its rows are tokens 56 to 64: the table ends at 63
+    ops.rope_to_pages(None, k, v, good, batch)
+    written = {number for _, b, _, number, _ in seqs.rows() if b != 1}
+    for now, then, done in zip(good, pages, want):
+        if now is not None:
+            for number in range(seqs.pages):
+                expected = done if number in written else then
+                assert torch.equal(now[number].view(torch.uint8), expected[number].view(torch.uint8)), number
+    back = ops.read_pages(want, batch, seqs.tokens)
+    for t, r in zip(back, read):
+        assert torch.isnan(t[3:12]).all() and torch.equal(t[:3], r[:3]) and torch.equal(t[12:], r[12:])
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("most", [1, 100])                        # 16 rows a workgroup, and 64
 def test_values_that_are_not_finite_among_the_new_tokens(hd, most):
