@@ -67,6 +67,15 @@ inline bool in_pieces(const void* p, std::initializer_list<int64_t> strides, int
     return true;
 }
 
+// Host: launches of at most 2^23 workgroups that make up `groups`, each told its first.  (A launch has fewer than 2^32 threads; of more, the excess over
+// 2^32 would run, without an error.)
+template <typename F>
+void in_launches(int64_t groups, F launch)
+{
+    constexpr int64_t kMost = 1 << 23;
+    for (int64_t first = 0; first < groups; first += kMost) launch((int)first, dim3((unsigned)std::min(groups - first, kMost)));
+}
+
 // Host: the caller's pages and batch as the kernels take them, or an error.
 int take_pages(const tl_pages* pages, const tl_page_batch* batch, int64_t tokens, Pages* p, Batch* b);
 

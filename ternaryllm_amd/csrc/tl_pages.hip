@@ -51,6 +51,7 @@ struct RopeHeads {
     const double* freq;
     const long long* positions;
     int hd, pairs, interleaved;
+    int first;                                  // row of this launch
     float factor, eps;
     Pages pages;
     Batch batch;
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(256) void tl_rope_heads_k(RopeHeads a, int bits)
     // the cosine and sine of pair i: float4 i / 8 of plane i % 8 / 2; a lane's eight values: half of them in each plane (lanes side by side hit all banks)
     __shared__ float4 turn[4][kHalf / 8];
     __shared__ float4 cross[2][256];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), token = (int)blockIdx.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), token = a.first + (int)blockIdx.x;
     const int p = lane & ((1 << bits) - 1), d = p * 8, each = 64 >> bits, sub = lane >> bits;   // each: heads of a wave at a time
     const bool inside = d < a.hd;
     const int gq = (a.q.heads + each - 1) / each, gk = gq + (a.k.heads + each - 1) / each, groups = gk + (a.v.heads + each - 1) / each;
@@ -334,6 +335,7 @@ struct ReadPages {
     Batch batch;
     void *k_out, *v_out;
     long long out_t, out_h;
+    int first;                                  // workgroup of this launch
 };
 
 // 2^bits lanes take a row of a token, a lane 16 bytes of it in the pages, a wave kReadTurns times as many rows as it has such lanes, all asked for at
@@ -345,7 +347,7 @@ template <typename T, bool BYTES>
 __global__ __launch_bounds__(256) void tl_read_pages_k(ReadPages a, int bits, int waves)
 {
     constexpr int VALUES = BYTES ? 16 : 8;
-    const int lane = (int)threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
+    const int lane = (int)threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane((a.first + (int)blockIdx.x) * 4 + ((int)threadIdx.x >> 6));
     const int token = id / waves, per_turn = 64 >> bits, rows = 2 * a.pages.kv_heads;
     if (token >= a.batch.tokens) return;
     const Place at = place_of(a.batch, token);
@@ -429,13 +431,16 @@ int take_rotation(const tl_rotation* r, int hd, int64_t tokens, bool batch, Rope
 }
 
 template <typename T>
-void launch_rope(const RopeHeads& a, Where where, int64_t tokens, hipStream_t st)
+void launch_rope(RopeHeads a, Where where, int64_t tokens, hipStream_t st)
 {
-    const dim3 grid((unsigned)tokens), block(256);
+    const dim3 block(256);
     const int bits = lane_bits(a.hd, 8);
-    if (where == kRows) hipLaunchKernelGGL((tl_rope_heads_k<T, kRows>), grid, block, 0, st, a, bits);
-    else if (where == kHalfPages) hipLaunchKernelGGL((tl_rope_heads_k<T, kHalfPages>), grid, block, 0, st, a, bits);
-    else hipLaunchKernelGGL((tl_rope_heads_k<T, kBytePages>), grid, block, 0, st, a, bits);
+    in_launches(tokens, [&](int first, dim3 grid) {
+        a.first = first;
+        if (where == kRows) hipLaunchKernelGGL((tl_rope_heads_k<T, kRows>), grid, block, 0, st, a, bits);
+        else if (where == kHalfPages) hipLaunchKernelGGL((tl_rope_heads_k<T, kHalfPages>), grid, block, 0, st, a, bits);
+        else hipLaunchKernelGGL((tl_rope_heads_k<T, kBytePages>), grid, block, 0, st, a, bits);
+    });
 }
 
 }  // namespace
@@ -491,9 +496,13 @@ extern "C" int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, 
     const int bits = lane_bits(a.pages.hd, bytes ? 16 : 8), waves = (int)ceil_div(2 * a.pages.kv_heads, kReadTurns * (64 >> bits));
     const int64_t groups = ceil_div(tokens * waves, 4);
     if (groups > INT32_MAX / 4) return fail(TL_ERR_SHAPE, "%lld rows of %d heads are more than one launch takes", (long long)tokens, a.pages.kv_heads);
-    const dim3 grid((unsigned)groups), block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, bits, waves); };
+    auto launch = [&](auto kernel) {
+        in_launches(groups, [&](int first, dim3 grid) {
+            a.first = first;
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, bits, waves);
+        });
+    };
     if (dtype == TL_F16) bytes ? launch(tl_read_pages_k<__half, true>) : launch(tl_read_pages_k<__half, false>);
     else bytes ? launch(tl_read_pages_k<float, true>) : launch(tl_read_pages_k<float, false>);
     return finish_launch();

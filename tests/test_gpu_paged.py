@@ -484,6 +484,29 @@ def test_pages_that_lie_far_apart(most):
     assert torch.equal(back[0], k) and torch.equal(back[1], v)
 
 
+def test_more_rows_than_one_launch_takes():
+    """A launch has fewer than 2^32 threads: 2^24 workgroups of 256."""
+    n = (1 << 24) + 5
+    q = torch.randn((n, 1, 16), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    f, at = frequencies(8).cuda(), torch.arange(n, device="cuda")
+    got, _ = ops.rope_heads(q, None, at, f)
+    edges = (0, 1, 1000, (1 << 23) - 3, (1 << 23) + 3, (1 << 24) - 2, n)
+    for a, b in zip(edges, edges[1:]):
+        assert torch.equal(ops.rope_heads(q[a:b], None, at[a:b], f)[0], got[a:b]), (a, b)
+    # into pages: one sequence, its pages in reverse order; and more rows out of them, of a sequence four times as long
+    count = -(-4 * n // 1024)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = ops.Pages(*(torch.zeros((count, 1, 1024, 16), dtype=torch.float16, device="cuda") for _ in range(2)))
+    batch = ops.PageBatch(torch.arange(count - 1, -1, -1, **i32)[None], torch.tensor([0, n], **i32), torch.tensor([n], **i32), n)
+    ops.rope_to_pages(None, q, q, pages, batch, f)
+    held = [t.flip(0).reshape(-1, 1, 16) for t in pages[:2]]
+    assert torch.equal(held[0][:n], got) and torch.equal(held[1][:n], q) and not held[0][n:].any() and not held[1][n:].any()
+    m = 4 * n
+    pages.v.copy_(torch.randn(pages.v.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(2), dtype=torch.float16))
+    k, v = ops.read_pages(pages, batch._replace(starts=torch.tensor([0, m], **i32), lengths=torch.tensor([m], **i32)), m)
+    assert torch.equal(k, held[0][:m]) and torch.equal(v, pages.v.flip(0).reshape(-1, 1, 16)[:m])
+
+
 def test_two_streams_at_once():
     """Calls on two streams do not share what they work in: each gives the bits that it gives alone."""
     seqs = [paged.Sequences([(1, 3000 + 100 * i), (1, 500)], 64, seed=i) for i in range(2)]
