@@ -327,6 +327,17 @@ struct Running {
     float top, limit, base, sum;                 // base: top as an exponent of 2 (0 while there is none); sum: of this lane's keys
 };
 
+// top as an exponent of 2 is rounded, and a score's difference from it is then off by as much, for all keys alike: that cancels in the quotient, but
+// but where sums with other references are joined; and from 2^30 on the rounding alone takes probabilities out of the range of any format.  From kFar on,
+// where it reaches 2^-12, top is taken from the scores themselves, before they are scaled.
+constexpr float kFar = 4096.0f;
+
+// The weight of sums taken against `top` among those against `now`, which is no less.  (Both -inf: there are none.)
+__device__ __forceinline__ float weight_of(float top, float now, float scale_log2)
+{
+    return __builtin_amdgcn_exp2f((top - (now == kNone ? 0.f : now)) * scale_log2);
+}
+
 constexpr Running kNothing{kNone, kNone, 0.f, 0.f};
 
 // Eight sums times `by` where `moves` says so.  (As assembly with a branch of its own: around a branch of the compiler's it keeps the sums in two
@@ -344,9 +355,10 @@ __device__ __forceinline__ void scale_if(int moves, float by, f32x4& x, f32x4& y
     y = f32x4{v[4], v[5], v[6], v[7]};
 }
 
-// Scores of QF rows and COUNT fragments of 16 keys in, probabilities out (as the operand of the product with the values).
+// Scores of QF rows and COUNT fragments of 16 keys in, probabilities out (as the operand of the product with the values).  far: whether some row of the
+// wave has a reference past kFar, 0 at the start.
 template <int QF, int COUNT, int DF>
-__device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale_log2, Running (&run)[QF], f32x4 (&o)[QF][DF], u32x4 (&px)[QF][COUNT / 2])
+__device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale_log2, Running (&run)[QF], int& far, f32x4 (&o)[QF][DF], u32x4 (&px)[QF][COUNT / 2])
 {
     float most[QF];
     bool past = false;
@@ -365,15 +377,31 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
     for (int f = 0; f < QF; ++f) shrink[f] = 1.0f;
     if (moves) {
         const float slack = 8.0f / scale_log2;
+        bool is_far = false;
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const float now = fmaxf(run[f].top, with_other_rows(most[f], [](float x, float y) { return fmaxf(x, y); }));
-            const float base = now == kNone ? 0.f : now * scale_log2;             // (nothing but -inf so far)
-            shrink[f] = __builtin_amdgcn_exp2f(fmaf(run[f].top, scale_log2, -base));
+            shrink[f] = weight_of(run[f].top, now, scale_log2);
             run[f].top = now;
-            run[f].limit = now + slack;
-            run[f].base = base;
+            run[f].base = now == kNone ? 0.f : now * scale_log2;                  // (nothing but -inf so far)
             run[f].sum *= shrink[f];
+            is_far |= fabsf(run[f].base) > kFar;
+        }
+        far |= scalar((int)__popcll(__builtin_amdgcn_ballot_w64(is_far)));
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+            run[f].limit = far || run[f].top == kNone ? run[f].top : run[f].top + slack;   // (far: of numbers so large the sum may be rounded up)
+            if (far) run[f].base = 0.f;
+        }
+    }
+    if (far) {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+            const float top = run[f].top == kNone ? 0.f : run[f].top;
+#pragma unroll
+            for (int n = 0; n < COUNT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[f][n][i] -= top;
         }
     }
 #pragma unroll
@@ -544,6 +572,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         int wave_last = -1, wave_first = INT_MAX;                 // ... any of the wave's, and all of them
         f32x4 o[QF][DF];
         Running run[QF];
+        int far = 0;
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const Row x = row_of(a, w, u, wave * 16 * QF + f * 16 + r16);
@@ -625,7 +654,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 }
             }
             u32x4 px[QF][NF / 2];
-            softmax_step(sc, a.scale_log2, run, o, px);
+            softmax_step(sc, a.scale_log2, run, far, o, px);
             if (decltype(may_mix)::value && t >= first_mixed) {
                 const unsigned long long keys_spoiled = __builtin_amdgcn_ballot_w64(lane < KT && spoiled[(t - first_tile) & 1][lane & (KT - 1)] != 0);
                 if (keys_spoiled != 0) {
@@ -792,6 +821,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
         }
         f32x4 o[1][DF];
         Running run[1] = {kNothing};
+        int far = 0;
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
@@ -852,7 +882,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                     for (int i = 0; i < 4; ++i) sc[0][n][i] = n * 16 + i <= seen ? sc[0][n][i] : kNone;
             }
             u32x4 px[1][1];
-            softmax_step(sc, a.scale_log2, run, o, px);
+            softmax_step(sc, a.scale_log2, run, far, o, px);
 #pragma unroll
             for (int d = 0; d < DF; ++d) {
                 const int key = g * 4 + (r16 >> 2);
@@ -884,14 +914,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                 float most = tops[0][r];
 #pragma unroll
                 for (int i = 1; i < 4; ++i) most = fmaxf(most, tops[i][r]);
-                const float base = most == kNone ? 0.f : most * a.scale_log2;
                 f32x4 v[EACH / 4];
 #pragma unroll
                 for (int j = 0; j < EACH / 4; ++j) v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 float all = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float weight = __builtin_amdgcn_exp2f(fmaf(tops[i][r], a.scale_log2, -base));
+                    const float weight = weight_of(tops[i][r], most, a.scale_log2);
                     all = fmaf(sums[i][r], weight, all);
                     const float* theirs = reinterpret_cast<const float*>(lds) + (i * ROWS + r) * LD + d;
 #pragma unroll
@@ -970,8 +999,8 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
 #pragma unroll
             for (int k = 0; k < FLY; ++k) {
                 if (i + k * step >= count) break;
-                const float now = fmaxf(top, m[k]), base = now == kNone ? 0.f : now * a.scale_log2;
-                const float old = __builtin_amdgcn_exp2f(fmaf(top, a.scale_log2, -base)), fresh = __builtin_amdgcn_exp2f(fmaf(m[k], a.scale_log2, -base));
+                const float now = fmaxf(top, m[k]);
+                const float old = weight_of(top, now, a.scale_log2), fresh = weight_of(m[k], now, a.scale_log2);
                 o = make_float4(o.x * old + v[k].x * fresh, o.y * old + v[k].y * fresh, o.z * old + v[k].z * fresh, o.w * old + v[k].w * fresh);
                 sum = sum * old + l[k] * fresh;
                 top = now;
@@ -1007,11 +1036,10 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
             float most = tops[0];
 #pragma unroll
             for (int i = 1; i < AT_ONCE; ++i) most = fmaxf(most, tops[i]);
-            const float base = most == kNone ? 0.f : most * a.scale_log2;
             start();
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
-                const float weight = __builtin_amdgcn_exp2f(fmaf(tops[i], a.scale_log2, -base));
+                const float weight = weight_of(tops[i], most, a.scale_log2);
                 const float4 v = part[i * LANES + lane];
                 o = make_float4(o.x + v.x * weight, o.y + v.y * weight, o.z + v.z * weight, o.w + v.w * weight);
                 sum += sums[i] * weight;

@@ -439,6 +439,60 @@ def test_a_peak_over_a_long_plain():
         assert (got - (3 * weight + 1 - weight)).abs().max() <= 3 * slack
 
 
+# 16, 64 and 128 rows to a workgroup, and one sequence cut into pieces
+LARGE_SCORES = [([(1, 90), (1, 33)], 4, 2, 128, None), ([(20, 90), (1, 33)], 4, 2, 64, None), ([(40, 130), (3, 3)], 16, 1, 128, 65536), ([(2, 7000)], 2, 1, 64, None),
+                ([(70, 4000)], 2, 1, 256, None)]
+
+
+@pytest.mark.parametrize("both,heads,kv,hd,widest", LARGE_SCORES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("kind", ["float16", "e4m3"])
+def test_scores_as_large_as_they_get(both, heads, kv, hd, widest, sign, kind):
+    """Finite queries and keys whose scores reach 2^31 and more.  Every score is one product, the two largest keys of three have the same, the third is below
+    by far more than a softmax sees: a row is the mean of the values of the two that it sees, up to its rounding and a few of fp32."""
+    seqs = paged.Sequences(both, 16, seed=2, widest=None if widest is None else widest // 16)
+    pages = fresh_pages(seqs, kv, hd, kind, seed=5, spoiled=False)
+    for c, scale in ((30000.0, 1.0), (57344.0, 1.0), (41000.0, 0.37), (33333.0, 2.5), (9000.0, 0.125), (60000.0, 1e6)):
+        keys = torch.zeros(pages.k.shape)
+        keys[..., 0] = sign * 57344.0
+        where = torch.arange(keys[..., 0].numel()).view(keys.shape[:3]) % 3 == 0   # (in the order of the pages: somewhere in each sequence)
+        keys[..., 0][where] = 53248.0 if sign == 1 else -61440.0
+        if kind == "e4m3":
+            now = pages._replace(k=(keys / 256).to(torch.float8_e4m3fn), k_exponents=torch.full(keys.shape[:3], 127 + 8, dtype=torch.uint8))
+        else:
+            now = pages._replace(k=keys.half())
+        q = torch.zeros((seqs.tokens, heads, hd), dtype=torch.float16)
+        q[..., 0] = c
+        got = ops.paged_attention(q.cuda(), on_gpu(now), seqs.batch(ops), scale=scale).cpu().double().view(q.shape)
+        held = [paged.values(*t) for t in zip(now[:2], now[2:])]
+        assert torch.equal(held[0], keys.double())
+        want = paged.attention(q, *held, seqs, scale)
+        assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -16 * held[1].abs().max()).all(), (c, scale)
+
+
+@pytest.mark.parametrize("both,heads,kv,hd,widest", LARGE_SCORES)
+@pytest.mark.parametrize("height", [2.0 ** 10, 2.0 ** 11, 3000.0, 2.0 ** 12, -2.0 ** 12, 2.0 ** 14, 2.0 ** 17, -2.0 ** 17])
+def test_small_differences_of_large_scores(both, heads, kv, hd, widest, height):
+    """Scores of `height` and up to 10 more, in steps of a half that fp32 holds exactly, growing along the sequence.  Beside the bound of any scores, references
+    below 4096 are rounded by 2^-12 as exponents of 2, once in each of two sums that meet."""
+    seqs = paged.Sequences(both, 16, seed=2, widest=None if widest is None else widest // 16)
+    pages = fresh_pages(seqs, kv, hd, "float16", seed=5, spoiled=False)
+    k = torch.zeros(pages.k.shape)
+    k[..., 0] = height / 16
+    for b, (_, length) in enumerate(both):
+        for j in range(length):
+            k[int(seqs.table[b, j // 16]), :, j % 16, 1] = 0.5 * (20 * j // length)
+    q = torch.zeros((seqs.tokens, heads, hd), dtype=torch.float16)
+    q[..., 0], q[..., 1] = 16.0, 1.0
+    now = pages._replace(k=k.half())
+    assert torch.equal(now.k.float(), k)
+    got = ops.paged_attention(q.cuda(), on_gpu(now), seqs.batch(ops), scale=1.0).cpu().double().view(q.shape)
+    want = paged.attention(q, now.k.double(), now.v.double(), seqs, 1.0)
+    zero = torch.zeros((1, 1))
+    bound = attention_bound(zero, zero, now.v.double(), want, max(length for _, length in both), 1.0)   # (of scores that are exact)
+    assert ((got - want).abs() <= bound + 2 * 2.0 ** -12 * now.v.double().abs().max()).all()
+
+
 @pytest.mark.parametrize("kind", ["float16", "e4m3"])
 @pytest.mark.parametrize("most", [1, 200])
 def test_pages_of_other_strides(kind, most):
