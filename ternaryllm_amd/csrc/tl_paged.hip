@@ -324,7 +324,7 @@ __device__ __forceinline__ bool make_finite(u32x4* x)
 // against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, 8 in the exponent of 2: a
 // probability is then 256 at most, as exact in fp16 as one of 1, and the sums, which are fp32, hardly ever have to be scaled.
 struct Running {
-    float top, limit, base, sum;                 // base: top as an exponent of 2 (0 while there is none); sum: of this lane's keys
+    float top, limit, base, sum;                 // base: of probabilities, an exponent of 2 (0 while there is no top); sum: of this lane's keys
 };
 
 // top as an exponent of 2 is rounded, and a score's difference from it is then off by as much, for all keys alike: that cancels in the quotient, but
@@ -356,8 +356,9 @@ __device__ __forceinline__ void scale_if(int moves, float by, f32x4& x, f32x4& y
 }
 
 // Scores of QF rows and COUNT fragments of 16 keys in, probabilities out (as the operand of the product with the values).  far: whether some row of the
-// wave has a reference past kFar, 0 at the start.
-template <int QF, int COUNT, int DF>
+// wave has a reference past kFar, 0 at the start.  MAY_BE: also at the start of this step; else that is looked at where a reference moves only (a branch
+// of its own at every tile cost 4.5 % of a chunk's time).
+template <bool MAY_BE, int QF, int COUNT, int DF>
 __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale_log2, Running (&run)[QF], int& far, f32x4 (&o)[QF][DF], u32x4 (&px)[QF][COUNT / 2])
 {
     float most[QF];
@@ -371,6 +372,16 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
             for (int i = 0; i < 4; ++i) most[f] = fmaxf(most[f], sc[f][n][i]);
         past |= most[f] > run[f].limit;
     }
+    auto from_top = [&] {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+            const float top = run[f].top == kNone ? 0.f : run[f].top;
+#pragma unroll
+            for (int n = 0; n < COUNT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[f][n][i] -= top;
+        }
+    };
     const int moves = scalar((int)__popcll(__builtin_amdgcn_ballot_w64(past)));
     float shrink[QF];
 #pragma unroll
@@ -383,27 +394,24 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
             const float now = fmaxf(run[f].top, with_other_rows(most[f], [](float x, float y) { return fmaxf(x, y); }));
             shrink[f] = weight_of(run[f].top, now, scale_log2);
             run[f].top = now;
-            run[f].base = now == kNone ? 0.f : now * scale_log2;                  // (nothing but -inf so far)
+            const float base = now == kNone ? 0.f : now * scale_log2;             // (nothing but -inf so far)
+            run[f].base = base;
             run[f].sum *= shrink[f];
-            is_far |= fabsf(run[f].base) > kFar;
+            is_far |= fabsf(base) > kFar;
         }
         far |= scalar((int)__popcll(__builtin_amdgcn_ballot_w64(is_far)));
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             run[f].limit = far || run[f].top == kNone ? run[f].top : run[f].top + slack;   // (far: of numbers so large the sum may be rounded up)
-            if (far) run[f].base = 0.f;
+        }
+        if (far) {
+#pragma unroll
+            for (int f = 0; f < QF; ++f) run[f].base = 0.f;
+            if constexpr (!MAY_BE) from_top();
         }
     }
-    if (far) {
-#pragma unroll
-        for (int f = 0; f < QF; ++f) {
-            const float top = run[f].top == kNone ? 0.f : run[f].top;
-#pragma unroll
-            for (int n = 0; n < COUNT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[f][n][i] -= top;
-        }
-    }
+    if constexpr (MAY_BE)
+        if (far) from_top();
 #pragma unroll
     for (int f = 0; f < QF; ++f)
 #pragma unroll
@@ -654,7 +662,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                 }
             }
             u32x4 px[QF][NF / 2];
-            softmax_step(sc, a.scale_log2, run, far, o, px);
+            softmax_step<decltype(may_mix)::value>(sc, a.scale_log2, run, far, o, px);
             if (decltype(may_mix)::value && t >= first_mixed) {
                 const unsigned long long keys_spoiled = __builtin_amdgcn_ballot_w64(lane < KT && spoiled[(t - first_tile) & 1][lane & (KT - 1)] != 0);
                 if (keys_spoiled != 0) {
@@ -689,7 +697,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             behind(may_mix, t);
         };
         int t = first_tile;
-        for (; t < min(seen_tiles, first_mixed - 1); ++t) work(std::false_type{}, t);   // (nor is the next one mixed)
+        for (; t < min(seen_tiles, first_mixed - 1) && !far; ++t) work(std::false_type{}, t);   // (nor is the next one mixed)
         for (; t < seen_tiles; ++t) work(std::true_type{}, t);
         for (; t < tiles; ++t) {
             before(t);
@@ -882,7 +890,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                     for (int i = 0; i < 4; ++i) sc[0][n][i] = n * 16 + i <= seen ? sc[0][n][i] : kNone;
             }
             u32x4 px[1][1];
-            softmax_step(sc, a.scale_log2, run, far, o, px);
+            softmax_step<true>(sc, a.scale_log2, run, far, o, px);
 #pragma unroll
             for (int d = 0; d < DF; ++d) {
                 const int key = g * 4 + (r16 >> 2);
