@@ -321,8 +321,12 @@ __device__ __forceinline__ bool make_finite(u32x4* x)
 }
 
 // The running softmax of a row: its reference is a maximum that it has seen (in units of the scores), which probabilities are taken
-// against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, 8 in the exponent of 2: a
-// probability is then 256 at most, as exact in fp16 as one of 1, and the sums, which are fp32, hardly ever have to be scaled.
+// against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, kSlack in the exponent of 2, and the
+// sums, which are fp32, hardly ever have to be scaled.  The reference's own probability is 2^kAbove, so that the largest is 2^15, the last power of two that fp16
+// has.  Then its lower end rounds off 2^-32 of the largest a key at most, less than fp32 sums do (2^-29, where each addition brings 32 keys that are alike).
+// (From 1 on, it was 2^-25: all of what lies 17.4 below the largest score, 0.4 % of a row over 131072 such keys.)
+constexpr float kSlack = 8.0f, kAbove = 7.0f;
+
 struct Running {
     float top, limit, base, sum;                 // base: of probabilities, an exponent of 2 (0 while there is no top); sum: of this lane's keys
 };
@@ -387,7 +391,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
 #pragma unroll
     for (int f = 0; f < QF; ++f) shrink[f] = 1.0f;
     if (moves) {
-        const float slack = 8.0f / scale_log2;
+        const float slack = kSlack / scale_log2;
         bool is_far = false;
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
@@ -395,7 +399,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
             shrink[f] = weight_of(run[f].top, now, scale_log2);
             run[f].top = now;
             const float base = now == kNone ? 0.f : now * scale_log2;             // (nothing but -inf so far)
-            run[f].base = base;
+            run[f].base = base - kAbove;
             run[f].sum *= shrink[f];
             is_far |= fabsf(base) > kFar;
         }
@@ -406,7 +410,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
         }
         if (far) {
 #pragma unroll
-            for (int f = 0; f < QF; ++f) run[f].base = 0.f;
+            for (int f = 0; f < QF; ++f) run[f].base = -kAbove;
             if constexpr (!MAY_BE) from_top();
         }
     }
@@ -417,7 +421,8 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
 #pragma unroll
         for (int d = 0; d < DF; d += 2) scale_if(moves, shrink[f], o[f][d], o[f][d + 1]);
 #pragma unroll
-    for (int f = 0; f < QF; ++f)
+    for (int f = 0; f < QF; ++f) {
+        float sum = 0.f;                                          // of this step's keys, as many as a lane has: a sum of all keys has few additions
 #pragma unroll
         for (int n = 0; n < COUNT; ++n)
 #pragma unroll
@@ -426,9 +431,11 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[QF][COUNT], float scale
 #pragma unroll
                 for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(sc[f][n][2 * i + j], scale_log2, -run[f].base));
                 const half2v two = __builtin_convertvector(e, half2v);
-                run[f].sum = __builtin_amdgcn_fdot2(two, half2v{(_Float16)1.0f, (_Float16)1.0f}, run[f].sum, false);
+                sum = __builtin_amdgcn_fdot2(two, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
                 px[f][n >> 1][(n & 1) * 2 + i] = __builtin_bit_cast(uint32_t, two);
             }
+        run[f].sum += sum;
+    }
 }
 
 #pragma clang diagnostic push

@@ -439,6 +439,33 @@ def test_a_peak_over_a_long_plain():
         assert (got - (3 * weight + 1 - weight)).abs().max() <= 3 * slack
 
 
+@pytest.mark.parametrize("depth", [14.0, 17.5, 18.5])
+@pytest.mark.parametrize("rows,most,hd,widest", [(1, 1, 64, None), (3, 40, 64, None), (2, 40, 256, None), (3, 140, 64, 1 << 22)])   # of 16, 64 and 128 rows a workgroup
+def test_a_plain_far_below_its_peaks_keeps_its_weight(rows, most, hd, widest, depth):
+    """Four keys `depth` above 2^20 others that are alike, over which one workgroup goes alone (of so many sequences that each has one; all have the same pages).
+    fp16's lower end takes 2^-25 a key where the largest probability is 2^7 at least, of a row that weighs that or more.  The sums are fp32 and lose by additions of
+    little to much, half a step (2^-24) each: a lane's sum takes 8 keys at a time of its sixteenth of them all (16 rows), or 16 of its quarter; sums of values take 32
+    a time, of which the instruction may cut off a whole step (2^-23), of a quarter of the keys or of all.  Twice each, as values reach 2.  Beside it the
+    result's rounding."""
+    n, page, seqs = 1 << 20, 1024, 520
+    k, v = (torch.zeros((n // page, 1, page, hd), dtype=torch.float16, device="cuda") for _ in range(2))
+    v.fill_(1.0)
+    k[0, 0, 5:128:32, 0], v[0, 0, 5:128:32] = depth, -2.0         # (every wave has one)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.arange(n // page, **i32)[None].repeat(seqs, 1)
+    if widest is not None:
+        table = torch.cat([table, torch.zeros((seqs, (widest - n) // page), **i32)], 1)
+    batch = ops.PageBatch(table, rows * torch.arange(seqs + 1, **i32), torch.full((seqs,), n, **i32), most)
+    q = torch.zeros((rows * seqs, 1, hd), dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0                                               # scores of `depth`, and 0
+    got = ops.paged_attention(q, ops.Pages(k, v), batch, scale=0.125).cpu().double().view(seqs, rows, hd)
+    plain = (n - rows + 1 - 4 + torch.arange(rows, dtype=torch.float64)) * math.exp(-depth)
+    want = ((plain - 8.0) / (plain + 4.0))[None, :, None]
+    sums = n / 16 / 8 * 2.0 ** -24 + n / 4 / 32 * 2.0 ** -23 if most == 1 else n / 4 / 16 * 2.0 ** -24 + n / 32 * 2.0 ** -23
+    slack = 3 * n * 2.0 ** -32 + 2 * sums + 2.0 ** -11 * want.abs() + 2.0 ** -16
+    assert ((got - want).abs() <= slack).all(), (got[0, :, 0], want[0, :, 0])
+
+
 # 16, 64 and 128 rows to a workgroup, and one sequence cut into pieces
 LARGE_SCORES = [([(1, 90), (1, 33)], 4, 2, 128, None), ([(20, 90), (1, 33)], 4, 2, 64, None), ([(40, 130), (3, 3)], 16, 1, 128, 65536), ([(2, 7000)], 2, 1, 64, None),
                 ([(70, 4000)], 2, 1, 256, None)]
