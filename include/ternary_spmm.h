@@ -606,7 +606,8 @@ int tl_spmm_gated(const tl_layout_header* header, const void* blob_dev,
 /* The pages of one layer's keys and values.  Slot `s` of page `p` holds a token: key head h's head_dim values lie side by side at element
  * p * page_stride + h * head_stride + s * slot_stride of k, and the values' at that of v.
  *   dtype      TL_F16, or TL_E4M3: a value is code * 2^(exponent - 127), the codes finite numbers of sign, 4 bits of exponent (bias 7) and 3 of
- *              fraction, the exponents one byte to a row, [pages][kv_heads][page_size] (NULL for TL_F16)
+ *              fraction, the exponents one byte to a row, [pages][kv_heads][page_size] (NULL for TL_F16).  As fp16, which the attention takes them
+ *              as, values are exact where their code's last bit is 2^-24 or more (exponents from -15 on), else rounded to that, and infinite past 65504
  *   page_size  a power of two, 16 to 1024;  strides in elements, addresses and strides whole 16-byte pieces */
 typedef struct tl_pages {
     void *k, *v;

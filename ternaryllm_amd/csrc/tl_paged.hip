@@ -464,7 +464,8 @@ __device__ __forceinline__ u32x4 buffer_at(const void* base, int bytes)
 // pairs swizzled so that the eight keys of a read do); one barrier a tile.  A wave brings a quarter of a tile's keys, which share a page.
 // fp16 rows go from memory into LDS by themselves, from lane offsets that do not change: a tile costs a wave a page number and two
 // buffer descriptions, and what lies past the sequence's end, outside the buffer, is zero (a key there weighs 0, which would make NaN of a value
-// that is not finite).  8-bit rows pass through registers, where they become fp16, exactly.
+// that is not finite).  8-bit rows pass through registers, where they become fp16: exactly for
+// exponents from -15 on, of smaller ones rounded to its 2^-24.
 // Measured, 4096 rows over 4096 keys, 32 heads on 8 of 128: 402 us and 15 of the join, 980 TFLOP/s; the matrix cores are busy for 49 % of it, the vector
 // unit for 33 % and 18 % (exponentials) beside them.  64 rows: 545.  8-bit pages: 490.  Heads of 64: 288.
 template <int HD, int QF, bool BYTES>

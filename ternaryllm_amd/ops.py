@@ -786,8 +786,8 @@ def rope_to_pages(q, k, v, pages, batch, frequencies=None, positions=None, *, fa
 
 
 def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=None):
-    """The keys and values of a batch's `tokens` rows out of the pages, [tokens, kv_heads, head_dim] each, float16 (which every 8-bit row fits
-    exactly) or float32: new tensors (rows of no sequence are not written there either), or k_out and v_out of the same strides.  A row whose
+    """The keys and values of a batch's `tokens` rows out of the pages, [tokens, kv_heads, head_dim] each, float16 (rows of 8 bits fit
+    exactly from an exponent of -15 on, smaller ones are rounded to its 2^-24) or float32: new tensors (rows of no sequence are not written there either), or k_out and v_out of the same strides.  A row whose
     page is none is NaN."""
     if k_out is None and v_out is None and (dtype is torch.float16 or dtype is torch.float32):
         both = _short().read_pages(pages, batch, tokens, dtype is torch.float16)
@@ -817,7 +817,8 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
     among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
     rows of no sequence are not written, a row that sees nothing is 0, rows that would read a page that is none are NaN; what is not finite where a row
     does not see it does not reach the row.  float16, head_dim 64,
-    128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim)."""
+    128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim).  Rows of 8 bits are taken as the float16 values that read_pages
+    gives."""
     y = _short().paged_attention(q, pages, batch, scale, out)
     if y is not None:
         return y

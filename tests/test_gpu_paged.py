@@ -380,6 +380,31 @@ def test_values_that_are_not_finite_among_the_new_tokens(hd, most):
             assert not torch.isfinite(got[token - 100:100]).all(-1).any(), (kind, which, token)
 
 
+@pytest.mark.parametrize("both,heads,kv,hd", [([(1, 300), (1, 33)], 4, 2, 128), ([(20, 90), (3, 3)], 2, 1, 64), ([(20, 90)], 1, 1, 256)])
+@pytest.mark.parametrize("low,high", [(-32, -16), (-24, -10), (-15, -15)])
+def test_bytes_of_small_exponents(both, heads, kv, hd, low, high):
+    """fp16 holds values of exponents under -15 to half of its 2^-24: so does what is read back in it, so do the attention's keys and values.  fp32 holds all."""
+    seqs = paged.Sequences(both, 16, seed=4)
+    pages = fresh_pages(seqs, kv, hd, "e4m3", seed=2, spoiled=False)
+    ke, ve = (torch.randint(127 + low, 128 + high, pages.k.shape[:3], generator=torch.Generator().manual_seed(i), dtype=torch.uint8) for i in range(2))
+    pages = pages._replace(k_exponents=ke, v_exponents=ve)
+    k, v = paged.values(pages.k, ke), paged.values(pages.v, ve)
+    device = on_gpu(pages)
+    whole = paged.Sequences([(n, n) for _, n in both], 16, seed=4)
+    assert torch.equal(whole.table, seqs.table)
+    for dtype in (torch.float16, torch.float32):
+        for t, held in zip(ops.read_pages(device, whole.batch(ops), whole.tokens, dtype), (k, v)):
+            want = torch.cat([whole.held(b, held) for b in range(len(both))])
+            assert torch.equal(t.cpu(), want.to(dtype)) and (dtype == torch.float16 or torch.equal(t.cpu().double(), want))
+    q = (2.0 ** -high * random((seqs.tokens, heads, hd), 9).float()).clamp(-60000, 60000).half()      # scores that tell keys apart
+    scale = 1 / math.sqrt(hd) / 100
+    got = ops.paged_attention(q.cuda(), device, seqs.batch(ops), scale=scale).cpu().double().view(q.shape)
+    want = paged.attention(q, k, v, seqs, scale)
+    bound = attention_bound(q, k, v, want, max(n for _, n in both), scale)
+    bound = bound + 2.0 ** -25 + 2 * scale * 2.0 ** -25 * q.double().abs().sum(-1).max() * v.abs().max()   # of a value, and of a score's keys, twice
+    assert ((got - want).abs() <= bound).all()
+
+
 # so many query heads on a key head that a workgroup of 64, 128 or 16 rows has those of one token only
 @pytest.mark.parametrize("heads,hd,most,widest", [(40, 64, 20, None), (40, 128, 20, None), (33, 256, 20, None), (80, 64, 20, 65536), (80, 128, 20, 65536), (16, 128, 1, None), (11, 64, 0, None),
                                                   (16, 256, 1, None)])
