@@ -17,7 +17,7 @@ int take_pages(const tl_pages* g, const tl_page_batch* c, int64_t tokens, Pages*
     if (g->page_size < 16 || g->page_size > 1024 || (g->page_size & (g->page_size - 1))) return fail(TL_ERR_SHAPE, "page_size=%d is not a power of two from 16 to 1024", g->page_size);
     if (g->pages <= 0 || g->pages > INT32_MAX || g->kv_heads <= 0 || g->kv_heads > (1 << 16)) return fail(TL_ERR_SHAPE, "pages and kv_heads must be positive");
     if (g->head_dim <= 0 || g->head_dim % 16 || g->head_dim > 512) return fail(TL_ERR_SHAPE, "head_dim=%d is not a multiple of 16 up to 512", g->head_dim);
-    if (g->slot_stride < g->head_dim || g->head_stride <= 0 || g->page_stride <= 0 || g->slot_stride * g->page_size > (1 << 30))
+    if (g->slot_stride < g->head_dim || g->head_stride <= 0 || g->page_stride <= 0 || g->slot_stride > (1 << 30) / g->page_size)
         return fail(TL_ERR_SHAPE, "strides of the pages must be positive, and a head's slots within 2^30 elements");
     if (c->seqs < 0 || c->table_pages < 0 || c->table_stride < c->table_pages || (int64_t)c->table_pages * g->page_size > INT32_MAX)
         return fail(TL_ERR_SHAPE, "the page table has %d x %d pages, rows %lld apart", c->seqs, c->table_pages, (long long)c->table_stride);
@@ -410,7 +410,7 @@ int take_rows(const tl_head_rows* r, int64_t es, int64_t tokens, bool out, Rows*
     if (!in_pieces(r->x, {r->x_token, r->x_head}, es) || (out && !in_pieces(r->y, {r->y_token, r->y_head}, es)) || !in_pieces(r->norm_weight, {}, es))
         return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
     const int64_t reach = std::max(r->x_head, out ? r->y_head : 0);
-    if (r->x_head < 0 || (out && r->y_head < 0) || reach * r->heads > INT32_MAX) return fail(TL_ERR_SHAPE, "a token's heads must lie within 2^31 elements, in order");
+    if (r->x_head < 0 || (out && r->y_head < 0) || reach > INT32_MAX / r->heads) return fail(TL_ERR_SHAPE, "a token's heads must lie within 2^31 elements, in order");
     *to = Rows{r->x, r->x_token, r->x_head, r->y, r->y_token, r->y_head, r->norm_weight, r->heads};
     return TL_OK;
 }

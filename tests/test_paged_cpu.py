@@ -214,6 +214,13 @@ def test_the_library_refuses(call, changes, code):
     assert _lib.lib().tl_last_error()
 
 
+@pytest.mark.parametrize("call,changes", [
+    ("read", {"pages__slot_stride": 1 << 60}), ("to_pages", {"pages__slot_stride": (1 << 60) + 64}), ("attend", {"pages__slot_stride": 1 << 60}),
+    ("heads", {"q__x_head": 1 << 62}), ("heads", {"k__y_head": 1 << 63 - 1}), ("to_pages", {"v__x_head": 1 << 63 - 1}), ("to_pages", {"q__y_head": (1 << 62) + 64})])
+def test_strides_whose_products_leave_64_bits(call, changes):
+    assert getattr(Raw(**changes), call)() == SHAPE
+
+
 @pytest.mark.parametrize("call", ["heads", "to_pages", "read", "attend"])
 def test_no_rows_need_no_addresses(call):
     raw = Raw(tokens=0, q__x=None, q__y=None, k__x=None, k__y=None, v__x=None, rotation__positions=None, k_out=None, out=None, workspace=None)
