@@ -686,6 +686,22 @@ def _overlap(x, y):
     return not (xs == ys >= max(xr, yr) and xr <= (y0 - x0) % xs <= xs - yr)
 
 
+def _alike_overlap(x, y):
+    """The same for tensors of one shape and one set of strides, whatever these are."""
+    tokens, heads, hd = x.shape
+    token, head = _steps(x, (0, 1))
+    apart, left = divmod(abs(y.data_ptr() - x.data_ptr()), x.element_size())
+    apart += left > 0
+    if x.numel() == 0 or apart >= (tokens - 1) * token + (heads - 1) * head + hd:
+        return False
+    for h in range(1 - heads, heads):                             # rows whose heads are h apart: by how many tokens do they have to be?
+        rest = apart - h * head
+        near = min(max(rest // token, 1 - tokens), tokens - 1) if token else 0
+        if min(abs(rest - t * token) for t in (near, min(near + 1, tokens - 1))) < hd:
+            return True
+    return False
+
+
 def _same_place(x, y):
     return x.data_ptr() == y.data_ptr() and x.shape == y.shape and _steps(x, (0, 1)) == _steps(y, (0, 1))
 
@@ -805,6 +821,8 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
     for t in (k_out, v_out):
         if t.shape != (tokens, heads, hd) or t.device != device or t.stride(2) != 1 or t.dtype != k_out.dtype or _steps(t, (0, 1)) != _steps(k_out, (0, 1)):
             raise ValueError("k_out and v_out must be [tokens, kv_heads, head_dim] of one type, of the same strides, on the pages' device")
+    if _alike_overlap(k_out, v_out):
+        raise ValueError("k_out and v_out must lie apart from each other")
     code = _code(k_out.dtype, "the output")
     _cuda(pages.k, "pages")
     with torch.cuda.device(device):

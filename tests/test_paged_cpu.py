@@ -143,6 +143,32 @@ def test_outputs_that_overlap_operands():
             ops.rope_heads(q, k, at, f, **outs)
 
 
+def test_rows_read_back_lie_apart():
+    _, _, pages, batch = parts()
+    both = torch.zeros((6, 4, 64), dtype=torch.float16)
+    for k, v in ((both[:3, :2], both[:3, :2]), (both[:3, :2], both[1:4, :2]), (both[:3, :2], both[:3, 1:3])):
+        with pytest.raises(ValueError):
+            ops.read_pages(pages, batch, 3, k_out=k, v_out=v)
+    for k, v in ((both[:3, :2], both[3:, :2]), (both[:3, :2], both[:3, 2:])):
+        with pytest.raises(RuntimeError):                         # taken, up to the GPU that is not there
+            ops.read_pages(pages, batch, 3, k_out=k, v_out=v)
+
+
+def test_rows_alike_overlap():
+    """Against the places themselves, over layouts of every order."""
+    pool = torch.arange(4000)
+    taken = set()
+    for token, head, offsets in ((64, 16, (0, 16, 48, 64, 8, 130)), (16, 64, (0, 16, 64, 48, 24)), (32, 80, (0, 16, 8, 96)), (16, 96, (0, 32, 48, 112)), (96, 32, (0, 16, 64, 80, 1))):
+        for tokens, heads in ((3, 2), (1, 4), (4, 1), (2, 5), (1, 1)):
+            x = pool.as_strided((tokens, heads, 16), (token, head, 1))
+            for offset in offsets:
+                y = pool.as_strided((tokens, heads, 16), (token, head, 1), offset)
+                real = bool(set(x.flatten().tolist()) & set(y.flatten().tolist()))
+                assert ops._alike_overlap(x, y) == ops._alike_overlap(y, x) == real, (token, head, tokens, heads, offset)
+                taken.add(real)
+    assert taken == {True, False}
+
+
 class Raw:
     """The library's structures over addresses that are never followed: every call here is refused before a launch."""
 
