@@ -667,9 +667,9 @@ int tl_read_pages(const tl_pages* pages, const tl_page_batch* batch, int64_t tok
 
 /* Causal softmax attention of a batch's rows over everything their sequences have in the pages (TernaryLLM/TernaryAttn.py:100-113 with the
  * causal mask): row i of sequence b's n sees its tokens 0 .. lengths[b] - n + i; a row that sees none gives 0.  What is not finite where a row
- * does not see it does not reach the row; where it does, values of the chunk's own tokens may make all of it NaN.  fp16 queries, head_dim 64, 128
- * or 256, scores, softmax and sums in fp32, probabilities rounded to fp16 for the product with the values.  Query head h reads key head
- * h / (heads / kv_heads).
+ * does not see it does not reach the row; where it does, values of the chunk's own tokens may make all of it NaN.  (A page number that is none may make
+ * NaN of rows of its sequence that do not see it.)  fp16 queries, head_dim 64, 128 or 256, scores, softmax and sums in fp32, probabilities rounded to
+ * fp16 for the product with the values.  Query head h reads key head h / (heads / kv_heads).
  *   q          element (t, h, 0) at t * q_token + h * q_head
  *   most_rows  the most rows that a sequence has: it chooses the kernel, nothing else
  *   out        [tokens][heads * head_dim]

@@ -466,8 +466,8 @@ __device__ __forceinline__ u32x4 buffer_at(const void* base, int bytes)
 // buffer descriptions, and what lies past the sequence's end, outside the buffer, is zero (a key there weighs 0, which would make NaN of a value
 // that is not finite).  8-bit rows pass through registers, where they become fp16: exactly for
 // exponents from -15 on, of smaller ones rounded to its 2^-24.
-// Measured, 4096 rows over 4096 keys, 32 heads on 8 of 128: 402 us and 15 of the join, 980 TFLOP/s; the matrix cores are busy for 49 % of it, the vector
-// unit for 33 % and 18 % (exponentials) beside them.  64 rows: 545.  8-bit pages: 490.  Heads of 64: 288.
+// Measured with the join (15 us), 4096 rows over 4096 keys, 32 heads on 8 of 128: 402 us, 1025 TFLOP/s (425 on other cards); the matrix cores are busy for
+// 48 % of it, the vector unit for 31 % and 18 % (exponentials) beside them.  64 rows: 526.  8-bit pages: 472 (64 rows: 665).  Heads of 64: 291, of 256: 1107.
 template <int HD, int QF, bool BYTES>
 __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 {
@@ -753,8 +753,8 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 // before: a wave's keys go from memory straight into the registers that its products want, its values through LDS of its own (to be read
 // by columns).  The next tile is asked for as soon as this one's registers are free.  8-bit rows are loaded 16 values to a lane, and
 // the order of the values within a score is free: the queries are loaded to match.
-// Measured, with the join: 32 sequences of 4096, 32 heads on 8 of 128: 103 us, 5.2 TB/s (8-bit pages 60, 4.5); heads of 256, whose registers allow one
-// workgroup a compute unit, 109 for the same bytes (241 while they spilled).
+// Measured, with the join: 32 sequences of 4096, 32 heads on 8 of 128: 102 us, 5.3 TB/s (8-bit pages 58, 4.7); heads of 256, whose registers allow one
+// workgroup a compute unit, 104 for the same bytes (241 while they spilled).
 template <int HD, bool BYTES>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn a)
 {
@@ -1076,13 +1076,14 @@ Plan plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_bat
     const int group = heads / pages->kv_heads, hd = pages->head_dim;
     const int64_t keys = (int64_t)batch->table_pages * pages->page_size;   // of a sequence, at most
     auto workgroups = [](int each) { return (int)ceil_div(each * compute_units(), 8) * 8; };
-    // units of few keys are not cut, which saves the second launch (us uncut / cut: one sequence of 600, 32 heads, 13.1 / 15.2; 256 of up to 200, 32
-    // heads on 8, 23.7 / 30.4)
+    // units of few keys are not cut, which saves the second launch (us uncut / cut: one sequence of 600, 32 heads, 12.7 / 15.7; 8 of 300, 32 heads on 8,
+    // 10.9 / 15.4; 256 of up to 200 25.3 / 31.6; 64 of 1000 51.3 / 53.4).  At the edge a few units alone would be quicker cut: one sequence of 1000, 32 heads,
+    // 17.1 / 15.4; 8 heads on one 16.1 / 12.0, of 600 12.7 / 12.2.  (The lengths are on the device: the table's width is what the host knows.)
     const int uncut = keys <= 1024;
     if (most_rows * group <= 16) return Plan{16, workgroups(hd == 256 ? 1 : 2), 128, 128, uncut};
     // 128 rows to a workgroup read half as much from LDS for a product, 64 have twice as many units: from 2048 keys of 128 rows to a workgroup on, as
-    // far as the host can tell (us with 128 / 64: 4096 rows over 4096, 32 heads on 8: 417 / 545; 723 rows of 8 sequences of up to 3500, 14
-    // heads of 64 on 2: 38 / 36; 64 rows over 32768, 32 heads on 8: 104 / 94).
+    // far as the host can tell (us with 128 / 64: 4096 rows over 4096, 32 heads on 8: 402 / 526; 723 rows of 8 sequences of up to 3500, 14
+    // heads of 64 on 2: 37 / 34; 64 rows over 32768, 32 heads on 8: 92 / 78).
     const bool tall = hd < 256 && most_rows * group >= 128 && tokens * heads / 128 * keys >= workgroups(2) * 2048ll;
     return Plan{tall ? 128 : 64, workgroups(2), 128, 512, uncut};
 }

@@ -833,7 +833,7 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
 def paged_attention(q, pages, batch, *, scale=None, out=None):
     """Causal attention of a batch's rows q [tokens, heads, head_dim] over everything their sequences have in the pages (their own keys and values
     among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
-    rows of no sequence are not written, a row that sees nothing is 0, rows that would read a page that is none are NaN; what is not finite where a row
+    rows of no sequence are not written, a row that sees nothing is 0, rows that would read a page that is none are NaN (others of their sequence may be); what is not finite where a row
     does not see it does not reach the row.  float16, head_dim 64,
     128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim).  Rows of 8 bits are taken as the float16 values that read_pages
     gives."""
