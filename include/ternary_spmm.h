@@ -679,6 +679,47 @@ int tl_paged_attention_workspace(int64_t tokens, int heads, const tl_pages* page
 int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
                        const tl_page_batch* batch, int64_t most_rows, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ======================================================================== */
+/* What a head's rows are worth: losses over a large vocabulary, the logits not kept. */
+/* ======================================================================== */
+
+/* What is wanted of every row's distribution softmax(z / temperature), z = (x * W) * scale: either an entry for each row (cross entropy; temperature 1), or
+ * a teacher's, as tl_teacher_entries leaves them. */
+typedef struct tl_loss_target {
+    const int64_t* targets;  /* [M], or NULL.  A row of `ignore` counts for nothing: loss and gradient 0; any other that is no column makes them NaN */
+    int64_t ignore;
+    const int32_t* entries;  /* [M][top], or NULL */
+    const float *shares, *known;
+    int32_t top;
+    float temperature;
+} tl_loss_target;
+
+/* A teacher's top logits as the losses take them: probabilities t = softmax(logits / temperature) over the `top` (1 to 1024) entries of a row, ids
+ * [M][ids_ld] naming columns of the head.  An entry of logit -inf is none, whatever its id; a repeated id's probabilities add up; a row of -inf alone
+ * has no teacher (loss and gradient 0); a row with a logit that is NaN or +inf, or with an id that is no column, is NaN.
+ *   entries, shares [M][top], known [M]: the columns that are named (-1: none), each once, their probabilities, and sum t log t */
+int tl_teacher_entries(const int64_t* ids, int64_t ids_ld, const void* logits, int dtype, int64_t logits_ld, int64_t M, int top, int columns,
+                       float temperature, int32_t* entries, float* shares, float* known, void* stream);
+
+/* A weight's codes transposed, for the product dz * W^T of a backward pass: made on the device, once for a weight, from a blob with codes. */
+int tl_back_codes_size(const tl_layout_header* header, int64_t* bytes);
+int tl_back_codes_make(const tl_layout_header* header, const void* blob_dev, void* back, void* stream);
+
+/* loss[m] = temperature^2 * sum_v t_v (log t_v - log softmax(z_m / temperature)_v): cross entropy where t is one entry.  x is [M][ldx] of x_dtype, row-major.
+ *   lse        [M + 1] float: what the backward pass wants of the forward one
+ *   workspace  device, 256-byte aligned, of tl_head_loss_workspace bytes at least; calls that share it must not overlap
+ * A row of x that is not finite, or whose logits are not, has loss NaN and does not reach other rows' (it does reach dscale).  The reference has no
+ * counterpart: it runs a model's forward pass alone (TernaryLLM/TernaryLlama.py:69-75). */
+int tl_head_loss_workspace(const tl_layout_header* header, int64_t M, int x_dtype, const tl_loss_target* target, int backward, int64_t* bytes);
+int tl_head_loss(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, int64_t M, const void* scale, int scale_dtype,
+                 const tl_loss_target* target, float* loss, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The gradients of sum_m grad[m] * loss[m]: dx [M][dx_ld] of x_dtype, dscale [N] of scale_dtype; either may be NULL (dx: back too).  dz is rounded to
+ * x_dtype for the product with W^T, which is summed in fp32. */
+int tl_head_loss_backward(const tl_layout_header* header, const void* blob_dev, const void* back, const void* x, int x_dtype, int64_t ldx, int64_t M,
+                          const void* scale, int scale_dtype, const tl_loss_target* target, const float* lse, const float* grad, void* dx, int64_t dx_ld,
+                          void* dscale, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,6 +58,12 @@ class Rotation(ctypes.Structure):
                 ("factor", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
+class LossTarget(ctypes.Structure):
+    """Mirror of tl_loss_target."""
+    _fields_ = [("targets", ctypes.c_void_p), ("ignore", ctypes.c_int64), ("entries", ctypes.c_void_p), ("shares", ctypes.c_void_p),
+                ("known", ctypes.c_void_p), ("top", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
 class LayoutHeader(ctypes.Structure):
     """Mirror of tl_layout_header (256 bytes)."""
     _fields_ = [
@@ -78,7 +84,7 @@ assert ctypes.sizeof(LayoutHeader) == 256
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HDRP = ctypes.POINTER(LayoutHeader)
-_PAGESP, _BATCHP, _ROWSP, _ROTP = (ctypes.POINTER(t) for t in (Pages, PageBatch, HeadRows, Rotation))
+_PAGESP, _BATCHP, _ROWSP, _ROTP, _TARGETP = (ctypes.POINTER(t) for t in (Pages, PageBatch, HeadRows, Rotation, LossTarget))
 _VP = ctypes.c_void_p
 _INT = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -142,6 +148,12 @@ SIGNATURES = {
     "tl_read_pages": (_INT, [_PAGESP, _BATCHP, _I64, _INT, _VP, _VP, _I64, _I64, _VP]),
     "tl_paged_attention_workspace": (_INT, [_I64, _INT, _PAGESP, _BATCHP, _I64, _I64P]),
     "tl_paged_attention": (_INT, [_VP, _I64, _I64, _INT, _I64, _INT, _PAGESP, _BATCHP, _I64, ctypes.c_float, _VP, _VP, _I64, _VP]),
+    "tl_teacher_entries": (_INT, [_VP, _I64, _VP, _INT, _I64, _I64, _INT, _INT, ctypes.c_float, _VP, _VP, _VP, _VP]),
+    "tl_back_codes_size": (_INT, [_HDRP, _I64P]),
+    "tl_back_codes_make": (_INT, [_HDRP, _VP, _VP, _VP]),
+    "tl_head_loss_workspace": (_INT, [_HDRP, _I64, _INT, _TARGETP, _INT, _I64P]),
+    "tl_head_loss": (_INT, [_HDRP, _VP, _VP, _INT, _I64, _I64, _VP, _INT, _TARGETP, _VP, _VP, _VP, _I64, _VP]),
+    "tl_head_loss_backward": (_INT, [_HDRP, _VP, _VP, _VP, _INT, _I64, _I64, _VP, _INT, _TARGETP, _VP, _VP, _VP, _I64, _VP, _VP, _I64, _VP]),
 }
 
 _lib = None

@@ -10,7 +10,7 @@ ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libternary_spmm.so")
 BINDING_PATH = os.path.join(PKG_DIR, "_tl_torch.so")
 SOURCES = ["tl_pack.cpp", "tl_layout.cpp", "tl_kernels.hip", "tl_small_m.hip", "tl_matrix.hip", "tl_few.hip", "tl_decode.hip", "tl_prefill.hip",
-           "tl_pages.hip", "tl_paged.hip"]
+           "tl_pages.hip", "tl_paged.hip", "tl_loss.hip"]
 
 
 def hipcc():

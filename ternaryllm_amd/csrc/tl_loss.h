@@ -1,0 +1,60 @@
+// What the kernels of a head's losses share: their arguments, and what a row's gradient is multiplied by.
+#pragma once
+#include "tl_device.h"
+
+namespace tl {
+
+constexpr int kPieceColumns = 16384;  // columns of the head to a piece of its transposed codes (whole units of them)
+constexpr int kMostTop = 1024;        // entries of a teacher's row
+
+struct TeacherArgs {
+    const int64_t* ids;               // [M][ids_ld]
+    const void* logits;               // [M][logits_ld]
+    long long ids_ld, logits_ld;
+    int f16, top, N;
+    float cool;                       // 1 / temperature
+    int* entry;                       // [M][top]
+    float *share, *known;             // [M][top], [M]
+};
+
+struct LossArgs {
+    const void* scale;                // [N] or null
+    int scale_f16;
+    int M, N, K, top;
+    int first;                        // row of the call that the launch begins with
+    float heat, cool;                 // the temperature, and 1 / it
+    const int64_t* targets;           // [M], or null: the teacher's entries
+    long long ignore;
+    const int* entry;                 // [M][top], -1: none
+    const float *share, *known;
+    float *loss, *lse;                // [M], [M + 1]: what the backward pass keeps, and the largest column scale
+    const float* raw;                 // [rows][raw_ld]: products without scales
+    long long raw_ld;
+    const float* grad;                // [M], of the losses
+    void* P;                          // [rows][raw_ld], x's type
+    float* ds;                        // [N] or null
+    void* dx;                         // [M][dx_ld], x's type
+    long long dx_ld;
+};
+
+// The power of two that fp16 probabilities are raised by, times their columns' scales, so that the largest is 2^15 at most and those that are lost, below
+// 2^-25, are 2^-40 of it: without it, and with the scales of a head of 4096 rows, all probabilities below 2^-19 would lose bits.
+__device__ __forceinline__ float raise_of(float largest_scale)
+{
+    if (!(largest_scale < __builtin_huge_valf())) return __builtin_nanf("");
+    return largest_scale > 0.f ? ldexpf(1.f, min(max(14 - ilogbf(largest_scale), -100), 100)) : 1.f;
+}
+
+// Whether a row has a gradient of its own: not, it counts for nothing (-inf), or its loss is NaN.
+__device__ __forceinline__ bool lse_counts(float lse) { return fabsf(lse) < __builtin_huge_valf(); }
+
+// What the product of a row's P is multiplied by: 0 for a row that counts for nothing, NaN where its loss is.
+__device__ __forceinline__ float row_factor(const LossArgs& a, int row, bool f16)
+{
+    const float lse = a.lse[row];
+    if (lse == -__builtin_huge_valf()) return 0.f;
+    if (lse != lse) return lse;
+    return a.grad[row] * a.heat / (f16 ? raise_of(a.lse[a.M]) : 1.f);
+}
+
+}  // namespace tl

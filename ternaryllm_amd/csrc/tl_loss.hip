@@ -1,0 +1,552 @@
+// What a ternary head's rows are worth: softmax cross entropy, and the divergence from a teacher whose top logits are known, with their gradients.
+//
+//   z_v = s_v / T * sum_k x_k W_kv,  lse = log sum_v exp z_v,  loss = T^2 (sum_i t_i log t_i + sum_i t_i (lse - z_i)),
+//   dz_v = T (exp(z_v - lse) - t_v) times the gradient of the row's loss,  dx_k = sum_v dz_v s_v W_kv,  ds_v = sum over rows of dz_v * (sum_k x_k W_kv),
+//
+// t: the teacher's probabilities of the vocabulary's entries that it names, which add up to 1; of cross entropy, one entry of 1 and T = 1.
+// The logits are not kept: the backward pass multiplies again.
+#include "tl_loss.h"
+
+using namespace tl;
+
+namespace {
+
+constexpr int kFewColumns = 128;                 // of a workgroup of tl_loss_few_grad
+constexpr int kRowThreads = 1024;                // of a workgroup that takes a row
+constexpr float kNone = -__builtin_huge_valf();
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+
+// A maximum and the sum of exponentials against it, joined with another pair.  (Nothing yet: -inf and 0.)
+__device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2)
+{
+    const float now = fmaxf(top, top2), base = now == kNone ? 0.f : now;
+    sum = sum * __expf(top - base) + sum2 * __expf(top2 - base);
+    top = now;
+}
+
+// The same over a workgroup of WAVES waves; the result in all threads.
+template <int WAVES>
+__device__ __forceinline__ void join_all(float& top, float& sum)
+{
+    __shared__ float tops[WAVES], sums[WAVES];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) join(top, sum, __shfl_xor(top, off, 64), __shfl_xor(sum, off, 64));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, sums[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    top = kNone, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) join(top, sum, tops[i], sums[i]);
+    __syncthreads();
+}
+
+template <int WAVES, typename F>
+__device__ __forceinline__ float fold_all(float v, F f)
+{
+    __shared__ float parts[WAVES];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = f(v, __shfl_xor(v, off, 64));
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = parts[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) v = f(v, parts[i]);
+    __syncthreads();
+    return v;
+}
+
+// The teacher of a row: what a row's ids and logits stand for.  A wave takes a row.  Repeated ids add up, in the place of the first of them; an entry of
+// probability 0 and those added elsewhere get id -1.  known: sum t log t; +inf: the row has no teacher; NaN: one of its entries is none.
+__global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
+{
+    __shared__ int ids[kMostTop];
+    __shared__ float shares[kMostTop];
+    const int lane = (int)threadIdx.x;
+    const long long row = blockIdx.x;
+    const int64_t* from = a.ids + row * a.ids_ld;
+    auto logit = [&](int i) { return (a.f16 ? __half2float(static_cast<const __half*>(a.logits)[row * a.logits_ld + i]) : static_cast<const float*>(a.logits)[row * a.logits_ld + i]) * a.cool; };
+    float top = kNone;
+    bool wrong = false;
+    for (int i = lane; i < a.top; i += 64) {
+        const float v = logit(i);
+        wrong |= v != v;
+        top = fmaxf(top, v);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const bool none = top == kNone;
+    float sum = 0.f;
+    for (int i = lane; i < a.top; i += 64) {
+        const float e = none ? 0.f : expf(logit(i) - top);
+        const long long id = from[i];
+        const bool outside = id < 0 || id >= a.N;
+        wrong |= e > 0.f && outside;
+        ids[i] = e > 0.f && !outside ? (int)id : -1;
+        shares[i] = e;
+        sum += e;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    wrong = __builtin_amdgcn_ballot_w64(wrong) != 0 || !(fabsf(top) < __builtin_huge_valf() || none);
+    __syncthreads();
+    float known = 0.f;
+    for (int i = lane; i < a.top; i += 64) {
+        int id = ids[i];
+        float share = 0.f;
+        for (int j = 0; j < a.top; ++j)
+            if (id >= 0 && ids[j] == id) {
+                if (j < i) id = -1;              // (added where it stands first)
+                share += shares[j];
+            }
+        share = id < 0 ? 0.f : share / sum;
+        a.entry[row * a.top + i] = wrong ? -1 : id;
+        a.share[row * a.top + i] = share;
+        known += share > 0.f ? share * logf(share) : 0.f;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) known += __shfl_xor(known, off, 64);
+    if (lane == 0) a.known[row] = wrong ? __builtin_nanf("") : none ? __builtin_huge_valf() : known;
+}
+
+// A row's loss from its lse and its entries' logits (z(entry), each asked for by one thread of the workgroup), and what the backward pass wants of it: lse,
+// NaN where the loss is, -inf for a row that counts for nothing.
+template <int WAVES, typename Z>
+__device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, float sum, Z z)
+{
+    const int tid = (int)threadIdx.x;
+    const float lse = finite(top) ? top + logf(sum) : __builtin_nanf("");
+    if (a.targets) {
+        if (tid != 0) return;
+        const long long target = a.targets[row];
+        const bool counts = target != a.ignore, there = target >= 0 && target < a.N;
+        const float loss = !counts ? 0.f : there ? lse - z((int)target, 0) : __builtin_nanf("");
+        a.loss[row] = loss;
+        a.lse[row] = !counts ? kNone : there ? lse : __builtin_nanf("");
+        return;
+    }
+    float gap = 0.f;
+    for (int i = tid; i < a.top; i += WAVES * 64) {
+        const int id = a.entry[(long long)row * a.top + i];
+        if (id >= 0) gap = fmaf(a.share[(long long)row * a.top + i], lse - z(id, i), gap);
+    }
+    gap = fold_all<WAVES>(gap, [](float x, float y) { return x + y; });
+    if (tid != 0) return;
+    const float known = a.known[row];
+    const bool none = known == __builtin_huge_valf();
+    a.loss[row] = none ? 0.f : a.heat * a.heat * (known + gap);
+    a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
+}
+
+// The largest column scale, by one workgroup, where lse ends: what the gradients' fp16 probabilities are raised by goes by it.
+template <int WAVES>
+__device__ __forceinline__ void put_largest_scale(const LossArgs& a)
+{
+    float most = a.scale ? 0.f : 1.f;
+    bool wrong = false;
+    if (a.scale)
+        for (int n = (int)threadIdx.x; n < a.N; n += WAVES * 64) {
+            const float s = fabsf(load_scale(a.scale, a.scale_f16, n));
+            wrong |= !finite(s);
+            most = fmaxf(most, s);
+        }
+    most = fold_all<WAVES>(wrong ? __builtin_huge_valf() : most, [](float x, float y) { return fmaxf(x, y); });
+    if (threadIdx.x == 0) a.lse[a.M] = most;
+}
+
+// Few rows: their logits are in the workspace, without scales.  A workgroup takes a row, one more the scales.  Bound by latency.
+__global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
+{
+    constexpr int WAVES = kRowThreads / 64, U = 8;
+    const int row = a.first + (int)blockIdx.x, tid = (int)threadIdx.x;
+    if (row == a.M) {
+        put_largest_scale<WAVES>(a);
+        return;
+    }
+    const float* raw = a.raw + (long long)blockIdx.x * a.raw_ld;
+    auto z = [&](int n) { return raw[n] * load_scale(a.scale, a.scale_f16, n) * a.cool; };
+    float top = kNone, sum = 0.f;
+    bool wrong = false;
+    for (int first = tid; first < a.N; first += kRowThreads * U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = first + u * kRowThreads < a.N ? z(first + u * kRowThreads) : kNone;
+        float most = v[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u) most = fmaxf(most, v[u]), wrong |= v[u] != v[u];
+        float part = 0.f;
+        const float base = most == kNone ? 0.f : most;
+#pragma unroll
+        for (int u = 0; u < U; ++u) part += __expf(v[u] - base);
+        join(top, sum, most, part);
+    }
+    // (a maximum passes over what is not a number; +inf does not count as a maximum either)
+    if (wrong) top = __builtin_huge_valf();
+    join_all<WAVES>(top, sum);
+    put_loss<WAVES>(a, row, top, sum, [&](int n, int) { return z(n); });
+}
+
+// Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after the other.
+template <typename T>
+__global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a, int rows)
+{
+    __shared__ float wanted[kSmallMaxM][kFewColumns];
+    const int tid = (int)threadIdx.x, first = (int)blockIdx.x * kFewColumns, n = first + tid;
+    for (int m = 0; m < rows; ++m) wanted[m][tid] = 0.f;
+    __syncthreads();
+    if (a.targets) {
+        if (tid < rows) {
+            const long long target = a.targets[a.first + tid] - first;
+            if (target >= 0 && target < kFewColumns) wanted[tid][target] = 1.f;
+        }
+    } else {
+        for (int i = tid; i < rows * a.top; i += kFewColumns) {
+            const long long at = (long long)a.first * a.top + i;
+            const int entry = a.entry[at];
+            const unsigned c = (unsigned)(entry - first);
+            if (entry >= 0 && c < kFewColumns) wanted[i / a.top][c] = a.share[at];   // (an entry stands once in a row)
+        }
+    }
+    __syncthreads();
+    if (n >= a.raw_ld) return;
+    const bool there = n < a.N;
+    const float s = there ? load_scale(a.scale, a.scale_f16, n) : 0.f, up = sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f;
+    float ds = 0.f;
+    constexpr int U = 8;
+    for (int m0 = 0; m0 < rows; m0 += U) {
+        float raw[U], lse[U], grad[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int m = min(m0 + u, rows - 1);
+            raw[u] = there ? a.raw[(long long)m * a.raw_ld + n] : 0.f;
+            lse[u] = a.lse[a.first + m];
+            grad[u] = a.grad[a.first + m];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (m0 + u >= rows) break;
+            const bool counts = finite(lse[u]);
+            const float dz = counts && there ? __expf(raw[u] * s * a.cool - lse[u]) - wanted[m0 + u][tid] : 0.f;
+            static_cast<T*>(a.P)[(long long)(m0 + u) * a.raw_ld + n] = (T)settled(dz * s * up);
+            ds += counts ? dz * raw[u] * grad[u] : lse[u] == kNone ? 0.f : __builtin_nanf("");
+        }
+    }
+    if (a.ds && there) {
+        ds *= a.heat;
+        a.ds[n] = a.first > 0 ? a.ds[n] + ds : ds;
+    }
+}
+
+// dx = what a row is multiplied by times the product of P, a sum of those of the vocabulary's pieces.
+template <typename T>
+__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int rows, int pieces)
+{
+    const int m = (int)blockIdx.y, k = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (k >= a.K) return;
+    const float factor = row_factor(a, a.first + m, sizeof(T) == 2);
+    float sum = 0.f;
+    for (int i = 0; i < pieces; ++i) sum += from[((long long)i * rows + m) * a.K + k];
+    static_cast<T*>(a.dx)[(long long)(a.first + m) * a.dx_ld + k] = (T)settled(lse_counts(a.lse[a.first + m]) ? sum * factor : factor);
+}
+
+__global__ __launch_bounds__(256) void tl_loss_scale_out(const float* ds, void* out, int f16, int N)
+{
+    const int n = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (n < N) store_out(out, f16, n, ds[n]);
+}
+
+// The codes of a weight [K][N], transposed: for pieces of kPieceColumns columns, one after the other, the codes of a weight of as many rows and K columns.
+// Once for a weight; a thread makes a dword (16 weights).
+__global__ __launch_bounds__(256) void tl_back_codes(const uint32_t* codes, int K, int N, int planes, uint32_t* out, long long dwords)
+{
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= dwords) return;
+    const int blocks = (K + 15) / 16, units_in = (K + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS;
+    const long long whole = (long long)blocks * planes * (kPieceColumns / TL_CODE_UNIT_ROWS) * (TL_CODE_UNIT_BYTES / 4);   // dwords of a piece
+    const int piece = (int)(at / whole), first = piece * kPieceColumns;
+    const int units = (min(N - first, kPieceColumns) + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS;
+    const long long in = at - piece * whole;
+    const int d = (int)(in & 3), lane = (int)(in >> 2 & 63);
+    const long long unit = in >> 8;
+    const int u = (int)(unit % units), plane = (int)(unit / units % planes), block = (int)(unit / units / planes);
+    const int k = block * 16 + (lane & 15);
+    uint32_t word = 0;
+    if (k < K) {
+        const int r = k % TL_CODE_UNIT_ROWS;
+        const int shift = 14 - 2 * (4 * (r >> 5 & 1) + (r >> 1 & 3)) + 16 * (r & 1);
+        for (int i = 0; i < 16; ++i) {
+            const int h = i >> 3, p = i >> 1 & 3, j = i & 1;
+            const int v = first + u * TL_CODE_UNIT_ROWS + 64 * d + 32 * h + 8 * (lane >> 4) + 2 * p + j;
+            if (v >= N) continue;
+            const long long from = (((long long)(v / 16) * planes + plane) * units_in + k / TL_CODE_UNIT_ROWS) * (TL_CODE_UNIT_BYTES / 4) +
+                                   ((r >> 3 & 3) * 16 + v % 16) * 4 + (r >> 6);
+            word |= (codes[from] >> shift & 3u) << (14 - 2 * (4 * h + p) + 16 * j);
+        }
+    }
+    out[at] = word;
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+// ---------------------------------------------------------------------------
+int64_t back_units(const tl_layout_header* h)
+{
+    int64_t units = 0;
+    for (int64_t n = 0; n < (int64_t)h->columns; n += kPieceColumns) units += ceil_div(std::min<int64_t>(h->columns - n, kPieceColumns), TL_CODE_UNIT_ROWS);
+    return units * ceil_div(h->inners, 16) * h->code_planes;
+}
+
+int check_weight(const tl_layout_header* h, const void* blob)
+{
+    if (int rc = check_header(h)) return rc;
+    if (!blob || reinterpret_cast<uintptr_t>(blob) % 256) return fail(TL_ERR_ALIGN, "the blob must be on the device, 256-byte aligned");
+    if (!h->off_codes) return fail(TL_ERR_UNSUPPORTED, "a weight without codes has no loss: pack it anew");
+    return TL_OK;
+}
+
+int check_target(const tl_loss_target* t)
+{
+    if (!t) return fail(TL_ERR_ARG, "null pointer");
+    if (!(t->temperature > 0.f) || t->temperature > 1e6f) return fail(TL_ERR_ARG, "temperature=%g is not a positive number up to 1e6", (double)t->temperature);
+    if ((t->targets != nullptr) == (t->entries != nullptr)) return fail(TL_ERR_ARG, "either targets or a teacher's entries");
+    if (t->targets && t->temperature != 1.f) return fail(TL_ERR_ARG, "cross entropy has no temperature");
+    if (t->entries && (t->top < 1 || t->top > kMostTop)) return fail(TL_ERR_ARG, "%d entries of a teacher (1 to %d)", t->top, kMostTop);
+    if (t->entries && (!t->shares || !t->known)) return fail(TL_ERR_ARG, "entries, shares and known come together");
+    return TL_OK;
+}
+
+int check_rows(const void* x, int x_dtype, int64_t ldx, int64_t M, const tl_layout_header* h, const void* scale, int scale_dtype)
+{
+    if (int rc = check_dtype(x_dtype, "x")) return rc;
+    if (int rc = check_dtype(scale_dtype, "scale")) return rc;
+    if (M < 0 || M > (1 << 24)) return fail(TL_ERR_SHAPE, "%lld rows (0 to 2^24)", (long long)M);
+    if (M == 0) return TL_OK;
+    if (!x) return fail(TL_ERR_ARG, "device pointer is null");
+    if (ldx < (int64_t)h->inners || ldx > (1 << 24)) return fail(TL_ERR_SHAPE, "ldx=%lld is none for rows of %u", (long long)ldx, h->inners);
+    if (reinterpret_cast<uintptr_t>(x) % (x_dtype == TL_F16 ? 2 : 4) || reinterpret_cast<uintptr_t>(scale) % (scale_dtype == TL_F16 ? 2 : 4))
+        return fail(TL_ERR_ALIGN, "x and scale must be aligned to their type");
+    return TL_OK;
+}
+
+LossArgs loss_args(const tl_layout_header* h, int64_t M, const void* scale, int scale_dtype, const tl_loss_target* t)
+{
+    LossArgs a{};
+    a.M = (int)M, a.N = (int)h->columns, a.K = (int)h->inners;
+    a.scale = scale, a.scale_f16 = scale_dtype == TL_F16;
+    a.targets = t->targets, a.ignore = t->ignore;
+    a.entry = t->entries, a.share = t->shares, a.known = t->known, a.top = t->entries ? t->top : 1;
+    a.heat = t->temperature, a.cool = 1.0f / t->temperature;
+    return a;
+}
+
+// The parts of a workspace, each a whole number of 256 bytes.
+struct Parts {
+    char* base;
+    int64_t used = 0;
+    void* take(int64_t bytes)
+    {
+        void* p = base ? base + used : nullptr;
+        used += round_up(bytes, 256);
+        return p;
+    }
+};
+
+struct FewParts {
+    float* raw;          // [rows][ld]
+    void* product;       // workspace of the product of the logits
+    void* P;             // backward: [rows][ld]
+    float* sums;         // [pieces][rows][K]
+    float* ds;           // [N]
+};
+
+int64_t few_rows(int64_t M) { return std::min<int64_t>(M, kSmallMaxM); }
+
+FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, bool backward, int64_t product_bytes)
+{
+    const int64_t rows = few_rows(M), ld = round_up(h->columns, 64);
+    FewParts f{};
+    f.raw = static_cast<float*>(p.take(rows * ld * 4));
+    f.product = p.take(product_bytes);
+    if (backward) {
+        f.P = p.take(rows * ld * (x_dtype == TL_F16 ? 2 : 4));
+        f.sums = static_cast<float*>(p.take(ceil_div(h->columns, kPieceColumns) * rows * h->inners * 4));
+        f.ds = static_cast<float*>(p.take((int64_t)h->columns * 4));
+    }
+    return f;
+}
+
+int product_workspace(const tl_layout_header* h, int64_t M, int x_dtype, int64_t* bytes)
+{
+    *bytes = 0;
+    for (int64_t rows : {few_rows(M), M % kSmallMaxM}) {
+        int64_t need = 0;
+        if (rows)
+            if (int rc = tl_spmm_workspace(h, rows, x_dtype, TL_X_ROW_MAJOR, &need)) return rc;
+        *bytes = std::max(*bytes, need);
+    }
+    return TL_OK;
+}
+
+// The products of P's rows with the pieces of the transposed weight.
+int back_product(const tl_layout_header* h, const void* back, const LossArgs& a, int x_dtype, int rows, float* sums, hipStream_t st)
+{
+    KernelArgs k;
+    std::memset(&k, 0, sizeof(k));
+    const int es = x_dtype == TL_F16 ? 2 : 4;
+    const unsigned char* codes = static_cast<const unsigned char*>(back);
+    k.N = (int)h->inners, k.NB = (int)ceil_div(h->inners, 16), k.M = rows;
+    k.planes = (int)h->code_planes;
+    k.x_f16 = x_dtype == TL_F16, k.one = 1.0f;
+    k.tile_rows = 1;                             // (T = 0: there is no index stream to walk, and P's sums are finite)
+    k.ldx = a.raw_ld, k.ldy = h->inners;
+    for (int64_t n = 0; n < (int64_t)h->columns; n += kPieceColumns) {
+        const int64_t wide = std::min<int64_t>(h->columns - n, kPieceColumns);
+        k.X = static_cast<const char*>(a.P) + n * es;
+        k.Y = sums + n / kPieceColumns * rows * (int64_t)h->inners;
+        k.K = (int)round_up(wide, 8);            // (P is padded with zeros, the codes too)
+        k.units = (int)ceil_div(wide, TL_CODE_UNIT_ROWS);
+        k.c0 = Codes{codes, k.planes};
+        if (int rc = launch_matrix_few(k, x_dtype, false, st)) return rc;
+        codes += (int64_t)k.NB * k.planes * k.units * TL_CODE_UNIT_BYTES;
+    }
+    return TL_OK;
+}
+
+}  // namespace
+
+extern "C" int tl_teacher_entries(const int64_t* ids, int64_t ids_ld, const void* logits, int dtype, int64_t logits_ld, int64_t M, int top, int columns,
+                                  float temperature, int32_t* entries, float* shares, float* known, void* stream)
+{
+    if (int rc = check_dtype(dtype, "logits")) return rc;
+    if (M < 0 || M > (1 << 24) || columns < 1) return fail(TL_ERR_SHAPE, "%lld rows over %d columns", (long long)M, columns);
+    if (top < 1 || top > kMostTop) return fail(TL_ERR_ARG, "%d entries of a teacher (1 to %d)", top, kMostTop);
+    if (!(temperature > 0.f) || temperature > 1e6f) return fail(TL_ERR_ARG, "temperature=%g is not a positive number up to 1e6", (double)temperature);
+    if (M == 0) return TL_OK;
+    if (!ids || !logits || !entries || !shares || !known) return fail(TL_ERR_ARG, "device pointer is null");
+    if (ids_ld < top || logits_ld < top) return fail(TL_ERR_SHAPE, "rows of ids or logits are shorter than %d", top);
+    TeacherArgs a{ids, logits, ids_ld, logits_ld, dtype == TL_F16, top, columns, 1.0f / temperature, entries, shares, known};
+    hipLaunchKernelGGL(tl_teacher, dim3((unsigned)M), dim3(64), 0, static_cast<hipStream_t>(stream), a);
+    return finish_launch();
+}
+
+extern "C" int tl_back_codes_size(const tl_layout_header* header, int64_t* bytes)
+{
+    if (int rc = check_header(header)) return rc;
+    if (!bytes) return fail(TL_ERR_ARG, "null pointer");
+    if (!header->off_codes) return fail(TL_ERR_UNSUPPORTED, "a weight without codes cannot be transposed: pack it anew");
+    *bytes = back_units(header) * TL_CODE_UNIT_BYTES;
+    return TL_OK;
+}
+
+extern "C" int tl_back_codes_make(const tl_layout_header* header, const void* blob_dev, void* back, void* stream)
+{
+    if (int rc = check_weight(header, blob_dev)) return rc;
+    if (!back || reinterpret_cast<uintptr_t>(back) % 16) return fail(TL_ERR_ALIGN, "the transposed codes must be on the device, 16-byte aligned");
+    const int64_t dwords = back_units(header) * (TL_CODE_UNIT_BYTES / 4);
+    if (dwords > (int64_t)INT32_MAX * 256) return fail(TL_ERR_SHAPE, "a weight of %u x %u is too large", header->inners, header->columns);
+    hipLaunchKernelGGL(tl_back_codes, dim3((unsigned)ceil_div(dwords, 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       reinterpret_cast<const uint32_t*>(static_cast<const char*>(blob_dev) + header->off_codes), (int)header->inners, (int)header->columns,
+                       (int)header->code_planes, static_cast<uint32_t*>(back), (long long)dwords);
+    return finish_launch();
+}
+
+extern "C" int tl_head_loss_workspace(const tl_layout_header* header, int64_t M, int x_dtype, const tl_loss_target* target, int backward, int64_t* bytes)
+{
+    if (int rc = check_header(header)) return rc;
+    if (int rc = check_dtype(x_dtype, "x")) return rc;
+    if (int rc = check_target(target)) return rc;
+    if (!bytes || M < 0 || M > (1 << 24)) return fail(TL_ERR_ARG, "a pointer is null, or %lld rows (0 to 2^24)", (long long)M);
+    int64_t product = 0;
+    if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
+    Parts p{nullptr};
+    few_parts(p, header, M, x_dtype, backward != 0, product);
+    *bytes = p.used;
+    return TL_OK;
+}
+
+namespace {
+
+int check_call(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, int64_t M, const void* scale, int scale_dtype,
+               const tl_loss_target* target, bool backward, const void* workspace, int64_t workspace_bytes)
+{
+    if (int rc = check_weight(header, blob_dev)) return rc;
+    if (int rc = check_target(target)) return rc;
+    if (int rc = check_rows(x, x_dtype, ldx, M, header, scale, scale_dtype)) return rc;
+    int64_t need = 0;
+    if (int rc = tl_head_loss_workspace(header, M, x_dtype, target, backward, &need)) return rc;
+    if (M > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)) return fail(TL_ERR_ALIGN, "the workspace must be on the device, 256-byte aligned");
+    if (workspace_bytes < need) return fail(TL_ERR_SIZE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    return TL_OK;
+}
+
+// The logits of rows a.first .. without scales.
+int raw_product(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, const LossArgs& a, int rows, const FewParts& f,
+                int64_t product_bytes, void* stream)
+{
+    const char* from = static_cast<const char*>(x) + (int64_t)a.first * ldx * (x_dtype == TL_F16 ? 2 : 4);
+    return tl_spmm(header, blob_dev, from, x_dtype, TL_X_ROW_MAJOR, ldx, rows, f.raw, TL_F32, a.raw_ld, nullptr, TL_F32, product_bytes ? f.product : nullptr,
+                   product_bytes, stream);
+}
+
+}  // namespace
+
+extern "C" int tl_head_loss(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, int64_t M, const void* scale,
+                            int scale_dtype, const tl_loss_target* target, float* loss, float* lse, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    if (int rc = check_call(header, blob_dev, x, x_dtype, ldx, M, scale, scale_dtype, target, false, workspace, workspace_bytes)) return rc;
+    if (M == 0) return TL_OK;
+    if (!loss || !lse) return fail(TL_ERR_ARG, "device pointer is null");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    LossArgs a = loss_args(header, M, scale, scale_dtype, target);
+    a.loss = loss, a.lse = lse;
+    int64_t product = 0;
+    if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
+    Parts p{static_cast<char*>(workspace)};
+    const FewParts f = few_parts(p, header, M, x_dtype, false, product);
+    a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
+    for (int64_t m = 0; m < M; m += kSmallMaxM) {
+        const int rows = (int)std::min<int64_t>(M - m, kSmallMaxM);
+        a.first = (int)m;
+        if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, rows, f, product, stream)) return rc;
+        hipLaunchKernelGGL(tl_loss_few, dim3((unsigned)(rows + (m + rows == M))), dim3(kRowThreads), 0, st, a);
+    }
+    return finish_launch();
+}
+
+extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void* blob_dev, const void* back, const void* x, int x_dtype, int64_t ldx, int64_t M,
+                                     const void* scale, int scale_dtype, const tl_loss_target* target, const float* lse, const float* grad, void* dx,
+                                     int64_t dx_ld, void* dscale, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    if (int rc = check_call(header, blob_dev, x, x_dtype, ldx, M, scale, scale_dtype, target, true, workspace, workspace_bytes)) return rc;
+    if (dx && (!back || reinterpret_cast<uintptr_t>(back) % 16)) return fail(TL_ERR_ALIGN, "the transposed codes must be on the device, 16-byte aligned");
+    if (dx && dx_ld < (int64_t)header->inners) return fail(TL_ERR_SHAPE, "dx_ld=%lld is none for rows of %u", (long long)dx_ld, header->inners);
+    if (dscale && !scale) return fail(TL_ERR_ARG, "a gradient of scales that there are none of");
+    if (M == 0) return TL_OK;
+    if (!lse || !grad) return fail(TL_ERR_ARG, "device pointer is null");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    LossArgs a = loss_args(header, M, scale, scale_dtype, target);
+    int64_t product = 0;
+    if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
+    Parts p{static_cast<char*>(workspace)};
+    const FewParts f = few_parts(p, header, M, x_dtype, true, product);
+    a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
+    a.lse = const_cast<float*>(lse), a.grad = grad;
+    a.P = f.P, a.dx = dx, a.dx_ld = dx_ld;
+    a.ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : f.ds;
+    const unsigned groups = (unsigned)ceil_div(a.raw_ld, kFewColumns);
+    const int pieces = (int)ceil_div(header->columns, kPieceColumns);
+    for (int64_t m = 0; m < M; m += kSmallMaxM) {
+        const int rows = (int)std::min<int64_t>(M - m, kSmallMaxM);
+        a.first = (int)m;
+        if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, rows, f, product, stream)) return rc;
+        if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_few_grad<_Float16>, dim3(groups), dim3(kFewColumns), 0, st, a, rows);
+        else hipLaunchKernelGGL(tl_loss_few_grad<float>, dim3(groups), dim3(kFewColumns), 0, st, a, rows);
+        if (!dx) continue;
+        if (int rc = back_product(header, back, a, x_dtype, rows, f.sums, st)) return rc;
+        const dim3 grid((unsigned)ceil_div(header->inners, 256), (unsigned)rows);
+        if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, f.sums, rows, pieces);
+        else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, f.sums, rows, pieces);
+    }
+    if (dscale && scale_dtype == TL_F16)
+        hipLaunchKernelGGL(tl_loss_scale_out, dim3((unsigned)ceil_div(header->columns, 256)), dim3(256), 0, st, f.ds, dscale, 1, a.N);
+    return finish_launch();
+}
