@@ -679,6 +679,23 @@ int tl_paged_attention_workspace(int64_t tokens, int heads, const tl_pages* page
 int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
                        const tl_page_batch* batch, int64_t most_rows, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Groups of a batch's sequences that begin with the same tokens, in the same pages: group g is the sequences groups[g] .. groups[g + 1] - 1, and each of
+ * them has its first shared[b] tokens in common with the others (the same number in all of a group, 0 in sequences of no group).  They are read once for
+ * all of the group's rows, from the pages of its first sequence; so each of its sequences has to have them in front of its rows. */
+typedef struct tl_page_prefix {
+    const int32_t* groups;   /* [count + 1], not falling */
+    const int32_t* shared;   /* [seqs] */
+    int32_t count;
+} tl_page_prefix;
+
+/* tl_paged_attention for such a batch: the same rows, of the same keys.  Where the device finds that a group's numbers differ, or that they are more than
+ * the tokens in front of a sequence's rows, or negative, rows may be NaN.  Whether the shared keys are read apart is chosen by sizes. */
+int tl_paged_attention_shared_workspace(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, const tl_page_prefix* prefix,
+                                        int64_t most_rows, int64_t* bytes);
+int tl_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
+                              const tl_page_batch* batch, const tl_page_prefix* prefix, int64_t most_rows, float scale, void* out, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
 /* ======================================================================== */
 /* What a head's rows are worth: losses over a large vocabulary, the logits not kept. */
 /* ======================================================================== */

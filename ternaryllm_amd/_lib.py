@@ -58,6 +58,11 @@ class Rotation(ctypes.Structure):
                 ("factor", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
+class PagePrefix(ctypes.Structure):
+    """Mirror of tl_page_prefix."""
+    _fields_ = [("groups", ctypes.c_void_p), ("shared", ctypes.c_void_p), ("count", ctypes.c_int32)]
+
+
 class LossTarget(ctypes.Structure):
     """Mirror of tl_loss_target."""
     _fields_ = [("targets", ctypes.c_void_p), ("ignore", ctypes.c_int64), ("entries", ctypes.c_void_p), ("shares", ctypes.c_void_p),
@@ -84,7 +89,7 @@ assert ctypes.sizeof(LayoutHeader) == 256
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HDRP = ctypes.POINTER(LayoutHeader)
-_PAGESP, _BATCHP, _ROWSP, _ROTP, _TARGETP = (ctypes.POINTER(t) for t in (Pages, PageBatch, HeadRows, Rotation, LossTarget))
+_PAGESP, _BATCHP, _ROWSP, _ROTP, _TARGETP, _PREFIXP = (ctypes.POINTER(t) for t in (Pages, PageBatch, HeadRows, Rotation, LossTarget, PagePrefix))
 _VP = ctypes.c_void_p
 _INT = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -148,6 +153,8 @@ SIGNATURES = {
     "tl_read_pages": (_INT, [_PAGESP, _BATCHP, _I64, _INT, _VP, _VP, _I64, _I64, _VP]),
     "tl_paged_attention_workspace": (_INT, [_I64, _INT, _PAGESP, _BATCHP, _I64, _I64P]),
     "tl_paged_attention": (_INT, [_VP, _I64, _I64, _INT, _I64, _INT, _PAGESP, _BATCHP, _I64, ctypes.c_float, _VP, _VP, _I64, _VP]),
+    "tl_paged_attention_shared_workspace": (_INT, [_I64, _INT, _PAGESP, _BATCHP, _PREFIXP, _I64, _I64P]),
+    "tl_paged_attention_shared": (_INT, [_VP, _I64, _I64, _INT, _I64, _INT, _PAGESP, _BATCHP, _PREFIXP, _I64, ctypes.c_float, _VP, _VP, _I64, _VP]),
     "tl_teacher_entries": (_INT, [_VP, _I64, _VP, _INT, _I64, _I64, _INT, _INT, ctypes.c_float, _VP, _VP, _VP, _VP]),
     "tl_back_codes_size": (_INT, [_HDRP, _I64P]),
     "tl_back_codes_make": (_INT, [_HDRP, _VP, _VP, _VP]),

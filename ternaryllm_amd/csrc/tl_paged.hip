@@ -21,6 +21,10 @@ constexpr int kRound = 64;                       // keys: units are cut at multi
 constexpr int kSeqsOfThread = 4;                 // of a pass over the lengths
 constexpr float kNone = -__builtin_huge_valf();
 
+// Which keys a launch's units have: those that each sequence sees; those that a group of sequences begins with, seen by all of the group's rows; those
+// that a sequence sees behind its group's.  Units of the last two leave pieces whatever they are, which a launch of its own joins.
+enum Keys { kCausal, kPrefix, kOwn };
+
 // The unit that begins in a workgroup and goes on behind it: last is the workgroup that ends it, -1: none does.
 struct Shared {
     int seq, head, tile, last;
@@ -40,6 +44,13 @@ struct PagedAttn {
     int uncut;                                   // units go to one workgroup whole
     float* pieces;                               // [workgroups][2][rows][head_dim + 4]
     Shared* shared;                              // [workgroups]
+    // groups of sequences that begin alike (kPrefix, kOwn)
+    const int *groups, *begin;                   // [group_count + 1] sequences; [seqs] tokens that a sequence shares
+    int group_count;
+    float* firsts;                               // [tokens][heads][head_dim + 4]: of every row the piece of the workgroup in which its unit begins; pieces then
+                                                 // are [workgroups][rows][head_dim + 4], of units that began before
+    int2* ends;                                  // of every unit the workgroups in which it begins and ends
+    int workgroups, rows;                        // of the launch, of a unit
 };
 
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -53,11 +64,35 @@ struct Seq {
     int start, n, length, tiles;
     int before;                                  // its keys that every row sees, 0 at least
     bool wrong;                                  // the table does not hold its length
+    int skip;                                    // kOwn: its first key, a multiple of kRound
 };
 
+// Tokens shared, as many as whole rounds of keys: the rest is every sequence's own.
+__device__ __forceinline__ int whole_rounds(int tokens) { return max(tokens, 0) / kRound * kRound; }
+
+// The first sequence of a group, and the one behind its last.
+__device__ __forceinline__ int2 group_of(const PagedAttn& a, int g)
+{
+    const int first = min(max(a.groups[g], 0), a.batch.seqs);
+    return make_int2(first, min(max(a.groups[g + 1], first), a.batch.seqs));
+}
+
+template <Keys SET = kCausal>
 __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
 {
     Seq s;
+    s.skip = 0;
+    if constexpr (SET == kPrefix) {             // all of a group's rows; the keys are its first sequence's
+        const int2 g = group_of(a, b);
+        const int length = g.x < g.y ? a.begin[g.x] : 0, room = a.batch.table_pages << a.pages.shift;
+        s.start = a.batch.starts[g.x];
+        s.n = s.start >= 0 ? max(min(a.batch.starts[g.y], a.batch.tokens) - s.start, 0) : 0;
+        s.wrong = length > room;
+        s.length = whole_rounds(min(length, room));
+        s.tiles = s.length > 0 ? (s.n + a.tile_tokens - 1) / a.tile_tokens : 0;
+        s.before = s.length;
+        return s;
+    }
     s.start = a.batch.starts[b];
     const int end = min(a.batch.starts[b + 1], a.batch.tokens);
     s.n = s.start >= 0 ? max(end - s.start, 0) : 0;
@@ -66,13 +101,19 @@ __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
     s.length = min(max(length, 0), room);
     s.tiles = (s.n + a.tile_tokens - 1) / a.tile_tokens;
     s.before = max(s.length - s.n, 0);
+    if constexpr (SET == kOwn) {
+        const int begin = a.begin[b];            // (tokens in front of its rows, all of them)
+        s.wrong |= begin < 0 || begin > s.before;
+        s.skip = whole_rounds(min(begin, s.before));
+        s.before -= s.skip;
+    }
     return s;
 }
 
 // The same for a sequence that all lanes look at.
 __device__ __forceinline__ Seq scalar(Seq s)
 {
-    return Seq{scalar(s.start), scalar(s.n), scalar(s.length), scalar(s.tiles), scalar(s.before), scalar((int)s.wrong) != 0};
+    return Seq{scalar(s.start), scalar(s.n), scalar(s.length), scalar(s.tiles), scalar(s.before), scalar((int)s.wrong) != 0, scalar(s.skip)};
 }
 
 // Cost of a key head's first `tiles` units: unit i costs fixed + before + (i + 1) * tile_tokens.
@@ -96,9 +137,11 @@ __device__ __forceinline__ long long unit_cost(const PagedAttn& a, const Walk& w
 // integers takes several times as long).
 __device__ __forceinline__ long long share_of(long long a, long long b, long long c) { return (long long)((double)(a * b) / (double)c); }
 
+template <Keys SET>
 __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long cost);
 
 // By a whole workgroup of 256 threads.  False where it has no part.
+template <Keys SET>
 __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
 {
     __shared__ long long sums[4];
@@ -107,7 +150,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     __shared__ Seq found;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr int kPass = 256 * kSeqsOfThread;
-    const int seqs = a.batch.seqs, heads = a.pages.kv_heads * a.blocks;
+    const int seqs = SET == kPrefix ? a.group_count : a.batch.seqs, heads = a.pages.kv_heads * a.blocks;
     Seq s[kSeqsOfThread];
     long long cost[kSeqsOfThread], upto = 0, total = 0, pass = 0;
     // this thread's sequences from `first` on, what they cost, and the sum of all before and of its own
@@ -118,7 +161,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
             const int b = first + tid * kSeqsOfThread + i;
             cost[i] = 0;
             if (b < seqs) {
-                s[i] = sequence(a, b);
+                s[i] = sequence<SET>(a, b);
                 cost[i] = tiles_cost(a, s[i].before, s[i].tiles) * heads;
             }
             own += cost[i];
@@ -153,7 +196,7 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     const int eighth = (w.wgs + 7) / 8, inside = (int)blockIdx.x / 8;
     w.wg = inside < eighth ? ((int)blockIdx.x & 7) * eighth + inside : (int)blockIdx.x;
     if (w.wg >= w.wgs) {
-        if (tid == 0) a.shared[w.wg].last = -1;
+        if (SET == kCausal && tid == 0) a.shared[w.wg].last = -1;
         return false;
     }
     w.total = total;
@@ -188,10 +231,11 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     w.tile = low;
     w.at += tiles_cost(a, w.s.before, low);
     // units that are not cut belong to the part in which they begin
-    return !(a.uncut && w.at < w.from) || next_unit(a, w, unit_cost(a, w));
+    return !(a.uncut && w.at < w.from) || next_unit<SET>(a, w, unit_cost(a, w));
 }
 
 // On to the next unit; false behind the last of the part.
+template <Keys SET>
 __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long cost)
 {
     w.at += cost;
@@ -201,8 +245,8 @@ __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long
     if (++w.head < a.pages.kv_heads * a.blocks) return true;
     w.head = 0;
     do {
-        if (++w.b >= a.batch.seqs) return false;
-        w.s = scalar(sequence(a, w.b));
+        if (++w.b >= (SET == kPrefix ? a.group_count : a.batch.seqs)) return false;
+        w.s = scalar(sequence<SET>(a, w.b));
     } while (w.s.tiles == 0);
     return true;
 }
@@ -222,7 +266,7 @@ struct Unit {
     float* piece;
 };
 
-template <int ROWS, int HD>
+template <int ROWS, int HD, Keys SET = kCausal>
 __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
 {
     Unit u;
@@ -230,29 +274,47 @@ __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
     u.first_token = w.tile * a.tile_tokens;
     u.kv_head = w.head / a.blocks;
     u.first_head = (w.head - u.kv_head * a.blocks) * a.tile_heads;
-    const int seen = max(w.s.length - w.s.n + min(u.first_token + a.tile_tokens, w.s.n), 0);   // by its last row
+    const int skip = SET == kOwn ? w.s.skip : 0;
+    const int seen = SET == kPrefix ? w.s.length : max(w.s.length - w.s.n + min(u.first_token + a.tile_tokens, w.s.n) - skip, 0);   // by its last row
     u.begins = a.uncut || w.at >= w.from;
     const bool ends = a.uncut || w.at + u.cost <= w.to;
     u.whole = u.begins && ends;
     // (its keys in proportion to its cost)
     auto cut = [&](long long at) { return min((int)(share_of(at - w.at, seen, u.cost) + kRound - 1) / kRound * kRound, seen); };
-    u.first_key = u.begins ? 0 : cut(w.from);
-    u.end_key = ends ? seen : cut(w.to);
-    u.piece = a.pieces + ((long long)w.wg * 2 + (u.begins ? 1 : 0)) * ROWS * (HD + 4);
+    u.first_key = skip + (u.begins ? 0 : cut(w.from));
+    u.end_key = skip + (ends ? seen : cut(w.to));
+    if constexpr (SET == kCausal) u.piece = a.pieces + ((long long)w.wg * 2 + (u.begins ? 1 : 0)) * ROWS * (HD + 4);
+    else u.piece = a.pieces + (long long)w.wg * ROWS * (HD + 4);
     return u;
+}
+
+// Where a unit of kPrefix or kOwn stands among all: tiles are counted from the row that a sequence begins with, so that those of different ones are apart.
+__device__ __forceinline__ long long unit_at(const PagedAttn& a, int b, int start, int tile, int head)
+{
+    return ((long long)(start / a.tile_tokens) + b + tile) * (a.pages.kv_heads * a.blocks) + head;
+}
+
+// The workgroup in which what ends at `end` of the list does: the last whose part begins before.
+__device__ __forceinline__ int ends_in(const Walk& w, long long end)
+{
+    int last = (int)share_of(end, w.wgs, w.total);                // or one beside it
+    while (last + 1 < w.wgs && share_of(w.total, last + 1, w.wgs) < end) ++last;
+    while (share_of(w.total, last, w.wgs) >= end) --last;
+    return last;
 }
 
 // By one thread, once it has the last unit of its part: what the second launch has to join.
 __device__ __forceinline__ void tell_shared(const PagedAttn& a, const Walk& w, const Unit& u)
 {
     Shared s{w.b, w.head, w.tile, -1};
-    if (u.begins && !u.whole) {
-        const long long end = w.at + u.cost;
-        s.last = (int)share_of(end, w.wgs, w.total);              // or one beside it: the last whose part begins before the unit's end
-        while (s.last + 1 < w.wgs && share_of(w.total, s.last + 1, w.wgs) < end) ++s.last;
-        while (share_of(w.total, s.last, w.wgs) >= end) --s.last;
-    }
+    if (u.begins && !u.whole) s.last = ends_in(w, w.at + u.cost);
     a.shared[w.wg] = s;
+}
+
+// The same of every unit of kPrefix or kOwn, by one thread of the workgroup in which it begins.
+__device__ __forceinline__ void tell_ends(const PagedAttn& a, const Walk& w, const Unit& u)
+{
+    if (u.begins) a.ends[unit_at(a, w.b, w.s.start, w.tile, w.head)] = make_int2(w.wg, u.whole ? w.wg : ends_in(w, w.at + u.cost));
 }
 
 __device__ __forceinline__ bool last_unit(const Walk& w, const Unit& u) { return w.at + u.cost >= w.to; }
@@ -271,6 +333,25 @@ __device__ __forceinline__ Row row_of(const PagedAttn& a, const Walk& w, const U
     x.there = t < a.tile_tokens && x.token < w.s.n && u.first_head + h < a.group;
     x.head = u.kv_head * a.group + u.first_head + h;
     return x;
+}
+
+// The last key that a row sees, and the last that all rows of a unit do.
+template <Keys SET>
+__device__ __forceinline__ int last_key(const Seq& s, int token) { return SET == kPrefix ? s.length - 1 : s.length - s.n + token; }
+
+// Where the pages of a sequence's (a group's) keys stand in the table.
+template <Keys SET>
+__device__ __forceinline__ const int* page_ids(const PagedAttn& a, int b)
+{
+    return a.batch.table + (SET == kPrefix ? scalar(group_of(a, b).x) : b) * a.batch.table_stride;
+}
+
+// Where a row's piece goes.
+template <Keys SET, int HD>
+__device__ __forceinline__ float* piece_of(const PagedAttn& a, const Walk& w, const Unit& u, const Row& x, int r)
+{
+    if (SET != kCausal && u.begins) return a.firsts + ((long long)(w.s.start + x.token) * a.heads + x.head) * (HD + 4);
+    return u.piece + r * (HD + 4);
 }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
@@ -468,7 +549,7 @@ __device__ __forceinline__ u32x4 buffer_at(const void* base, int bytes)
 // exponents from -15 on, of smaller ones rounded to its 2^-24.
 // Measured with the join (15 us), 4096 rows over 4096 keys, 32 heads on 8 of 128: 402 us, 1025 TFLOP/s (425 on other cards); the matrix cores are busy for
 // 48 % of it, the vector unit for 31 % and 18 % (exponentials) beside them.  64 rows: 526.  8-bit pages: 472 (64 rows: 665).  Heads of 64: 291, of 256: 1107.
-template <int HD, int QF, bool BYTES>
+template <int HD, int QF, bool BYTES, Keys SET>
 __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 {
     constexpr int ROWS = 64 * QF, KT = HD == 256 ? 32 : 64, NF = KT / 16, KS = HD / 32, DF = HD / 16;
@@ -481,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
-    if (!begin_walk(a, w)) return;
+    if (!begin_walk<SET>(a, w)) return;
     auto key_place = [](int key, int p) { return HD == 64 ? p ^ ((key >> 1) & 7) : p ^ (key & 15); };
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
     const int mask = (1 << a.pages.shift) - 1;
@@ -497,18 +578,18 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
     }
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;             // (the low half of such an address is the offset in LDS)
     for (;;) {
-        Unit u = unit_of<ROWS, HD>(a, w);
+        Unit u = unit_of<ROWS, HD, SET>(a, w);
         const int first_tile = (u.first_key + KT - 1) / KT, tiles = (u.end_key + KT - 1) / KT;   // (a share may be empty)
         bool wrong = w.s.wrong;
         const int length = w.s.length;
         // Tiles with tokens that some of the unit's rows do not see: values there that are not finite must not meet the weights of 0.  They are made 0
         // in LDS, and the rows that do see their key are NaN.
-        const int all_see = length - w.s.n + u.first_token;       // the last key that every row sees
+        const int all_see = last_key<SET>(w.s, u.first_token);   // the last key that every row sees
         const int first_mixed = all_see < length - 1 ? max(all_see + 1, 0) / KT : INT_MAX;   // ... are the last
         // ---- tiles on their way ----
         const long long head_at = u.kv_head * a.pages.head_stride;
         // page of this wave's keys of the tile after the next (by a vector load: a scalar one would be waited for with the first read of LDS)
-        const int* ids = a.batch.table + w.b * a.batch.table_stride;
+        const int* ids = page_ids<SET>(a, w.b);
         int ahead = 0;
         auto ask = [&](int t) { ahead = ids[min(t * KT + wave * KW, length - 1) >> a.pages.shift]; };
         u32x4 kreg[KL], vreg[KL];
@@ -592,7 +673,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const Row x = row_of(a, w, u, wave * 16 * QF + f * 16 + r16);
-            last[f] = x.there ? w.s.length - w.s.n + x.token : -1;
+            last[f] = x.there ? last_key<SET>(w.s, x.token) : -1;
             const __half* row = a.q + (long long)(w.s.start + x.token) * a.q_t + x.head * a.q_h + g * 8;
 #pragma unroll
             for (int s = 0; s < KS; ++s) qx[f][s] = x.there ? *reinterpret_cast<const u32x4*>(row + s * 32) : u32x4{0u, 0u, 0u, 0u};
@@ -715,7 +796,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
         __syncthreads();
         wrong = wrong_somewhere != 0;
         w = scalar(kept);
-        u = unit_of<ROWS, HD>(a, w);
+        u = unit_of<ROWS, HD, SET>(a, w);
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
             const int r = wave * 16 * QF + f * 16 + r16;
@@ -723,7 +804,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
             float all = with_other_rows(run[f].sum, [](float v, float y) { return v + y; });
             if (wrong) all = __builtin_nanf("");
             if (!x.there) continue;
-            if (u.whole) {
+            if (SET == kCausal && u.whole) {
                 const float inv = all == 0.f ? 0.f : 1.0f / all;  // (no key: 0)
                 __half* row = a.out + ((long long)(w.s.start + x.token) * a.heads + x.head) * HD + g * 4;
 #pragma unroll
@@ -734,17 +815,18 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
                     *reinterpret_cast<uint2*>(row + d * 16) = *reinterpret_cast<const uint2*>(h);
                 }
             } else {
-                float* row = u.piece + r * (HD + 4);
+                float* row = piece_of<SET, HD>(a, w, u, x, r);
 #pragma unroll
                 for (int d = 0; d < DF; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + g * 4) = o[f][d];
                 if (g == 0) row[HD] = run[f].top, row[HD + 1] = all;
             }
         }
+        if (SET != kCausal && tid == 0) tell_ends(a, w, u);
         if (last_unit(w, u)) {
-            if (tid == 0) tell_shared(a, w, u);
+            if (SET == kCausal && tid == 0) tell_shared(a, w, u);
             return;
         }
-        if (!next_unit(a, w, u.cost)) return;
+        if (!next_unit<SET>(a, w, u.cost)) return;
     }
 }
 
@@ -755,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 // the order of the values within a score is free: the queries are loaded to match.
 // Measured, with the join: 32 sequences of 4096, 32 heads on 8 of 128: 102 us, 5.3 TB/s (8-bit pages 58, 4.7); heads of 256, whose registers allow one
 // workgroup a compute unit, 104 for the same bytes (241 while they spilled).
-template <int HD, bool BYTES>
+template <int HD, bool BYTES, Keys SET>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn a)
 {
     constexpr int ROWS = 16, KT = 32, KS = HD / 32, DF = HD / 16;
@@ -769,17 +851,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
-    if (!begin_walk(a, w)) return;
+    if (!begin_walk<SET>(a, w)) return;
     unsigned char* own = lds + wave * KT * HD * 2;
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
     for (;;) {
-        Unit u = unit_of<ROWS, HD>(a, w);
+        Unit u = unit_of<ROWS, HD, SET>(a, w);
         if (tid == 0) kept = w;
         const int tiles = (u.end_key + KT - 1) / KT, first_tile = (u.first_key + KT - 1) / KT + wave;
         bool wrong = w.s.wrong;
         const int length = w.s.length;
         const long long head_at = u.kv_head * a.pages.head_stride;
-        const int* ids = a.batch.table + w.b * a.batch.table_stride;
+        const int* ids = page_ids<SET>(a, w.b);
         u32x4 kreg[2][KL], vreg[VL];
         int kexp[2], vexp[VL];
         int ahead[2];                                             // pages of the next tile's keys
@@ -827,7 +909,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
             if (first_tile + 4 < tiles) ask(first_tile + 4);
         }
         const Row x = row_of(a, w, u, r16);
-        const int last = x.there ? w.s.length - w.s.n + x.token : -1;
+        const int last = x.there ? last_key<SET>(w.s, x.token) : -1;
         u32x4 qx[KS];
         const __half* row = a.q + (long long)(w.s.start + x.token) * a.q_t + x.head * a.q_h;
 #pragma unroll
@@ -840,7 +922,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
         int far = 0;
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int all_see = w.s.length - w.s.n + u.first_token;   // the last key that every row sees
+        const int all_see = last_key<SET>(w.s, u.first_token);   // the last key that every row sees
 
         auto spoil = [&](unsigned long long lanes, int first) {   // lanes whose pieces of values were not finite, of keys from `first` on
             for (int k = 0; lanes != 0 && k < VKEYS; ++k)
@@ -913,7 +995,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
         if (tid == 0) wrong_somewhere = 0;
         __syncthreads();                                          // every wave is done with its values
         w = scalar(kept);
-        u = unit_of<ROWS, HD>(a, w);
+        u = unit_of<ROWS, HD, SET>(a, w);
         float* mine = reinterpret_cast<float*>(lds) + (wave * ROWS + r16) * LD;
         if (x.there) {
 #pragma unroll
@@ -947,7 +1029,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                     }
                 }
                 if (wrong_somewhere) all = __builtin_nanf("");
-                if (u.whole) {
+                if (SET == kCausal && u.whole) {
                     const float inv = all == 0.f ? 0.f : 1.0f / all;   // (no key: 0)
                     __half* to = a.out + ((long long)(w.s.start + y.token) * a.heads + y.head) * HD + d;
 #pragma unroll
@@ -958,18 +1040,19 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
                         *reinterpret_cast<uint2*>(to + j * 64) = *reinterpret_cast<const uint2*>(h);
                     }
                 } else {
-                    float* to = u.piece + r * LD;
+                    float* to = piece_of<SET, HD>(a, w, u, y, r);
 #pragma unroll
                     for (int j = 0; j < EACH / 4; ++j) *reinterpret_cast<f32x4*>(to + d + j * 64) = v[j];
                     if (d == 0) to[HD] = most, to[HD + 1] = all;
                 }
             }
         }
+        if (SET != kCausal && tid == 0) tell_ends(a, w, u);
         if (last_unit(w, u)) {
-            if (tid == 0) tell_shared(a, w, u);
+            if (SET == kCausal && tid == 0) tell_shared(a, w, u);
             return;
         }
-        if (!next_unit(a, w, u.cost)) return;
+        if (!next_unit<SET>(a, w, u.cost)) return;
         __syncthreads();                                          // the unit is done with LDS
     }
 }
@@ -1065,6 +1148,99 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
     }
 }
 
+// Joins the pieces of a row's keys that its group shares and of its own: a workgroup to a row of a query head, HD / 4 lanes to a piece, four values each.
+// Bound by latency: the row's place, its units' workgroups, the pieces, one after the other.
+template <int HD>
+__global__ __launch_bounds__(256) void tl_paged_merge(PagedAttn a, PagedAttn b)
+{
+    constexpr int LANES = HD / 4, AT_ONCE = 256 / LANES, FLY = 4;
+    __shared__ float4 part[256];
+    __shared__ float tops[AT_ONCE], sums[AT_ONCE];
+    const int token = (int)(blockIdx.x / (unsigned)a.heads), head = (int)(blockIdx.x % (unsigned)a.heads);
+    const int lane = (int)threadIdx.x % LANES, own = (int)threadIdx.x / LANES;
+    const Place at = place_of(a.batch, token);
+    if (at.seq < 0) return;
+    // its group, if there is one; the pieces of that unit, and of the sequence's own
+    int below = 0;
+    for (int first = 0; first <= a.group_count; first += 64) {
+        const int i = first + (int)(threadIdx.x & 63u);
+        const int more = __popcll(__builtin_amdgcn_ballot_w64(i <= a.group_count && a.groups[min(i, a.group_count)] <= at.seq));
+        below += more;
+        if (more < 64) break;
+    }
+    const int g = below - 1, begin = a.begin[at.seq];
+    const bool grouped = g >= 0 && g < a.group_count;
+    bool wrong = grouped ? begin != a.begin[group_of(a, g).x] : begin != 0;
+    struct Pieces {
+        const float *first, *more;               // (more: of the workgroup behind the first)
+        long long step;
+        int count;
+    };
+    auto pieces = [&](const PagedAttn& p, int which, const Seq& s) {
+        Pieces y{};
+        const int t = token - s.start, of_group = head % p.group, block = of_group / p.tile_heads;
+        if (t < 0 || t >= s.n || s.tiles == 0) return y;
+        const int r = t % p.tile_tokens * p.tile_heads + of_group % p.tile_heads, rows = p.rows;
+        const int2 ends = p.ends[unit_at(p, which, s.start, t / p.tile_tokens, head / p.group * p.blocks + block)];
+        const int from = min(max(ends.x, 0), p.workgroups - 1), to = min(max(ends.y, from), p.workgroups - 1);
+        y.first = p.firsts + ((long long)token * p.heads + head) * (HD + 4);
+        y.step = (long long)rows * (HD + 4);
+        y.more = p.pieces + (from + 1) * y.step + r * (HD + 4);
+        y.count = to - from + 1;
+        return y;
+    };
+    Pieces front{};
+    if (grouped) {
+        const Seq s = sequence<kPrefix>(a, g);
+        front = pieces(a, g, s);
+    }
+    const Pieces behind = pieces(b, at.seq, sequence<kOwn>(b, at.seq));
+    const int count = front.count + behind.count;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = kNone, sum = 0.f;
+    for (int i = own; i < count; i += FLY * AT_ONCE) {
+        float m[FLY], l[FLY];
+        float4 v[FLY];
+#pragma unroll
+        for (int k = 0; k < FLY; ++k) {
+            const int n = min(i + k * AT_ONCE, count - 1);
+            const Pieces& p = n < front.count ? front : behind;
+            const int j = n < front.count ? n : n - front.count;
+            const float* piece = j == 0 ? p.first : p.more + (j - 1) * p.step;
+            m[k] = piece[HD], l[k] = piece[HD + 1];
+            v[k] = *reinterpret_cast<const float4*>(piece + lane * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < FLY; ++k) {
+            if (i + k * AT_ONCE >= count) break;
+            const float now = fmaxf(top, m[k]);
+            const float old = weight_of(top, now, a.scale_log2), fresh = weight_of(m[k], now, a.scale_log2);
+            o = make_float4(o.x * old + v[k].x * fresh, o.y * old + v[k].y * fresh, o.z * old + v[k].z * fresh, o.w * old + v[k].w * fresh);
+            sum = sum * old + l[k] * fresh;
+            top = now;
+        }
+    }
+    part[threadIdx.x] = o;
+    if (lane == 0) tops[own] = top, sums[own] = sum;
+    __syncthreads();
+    if (own != 0) return;
+    float most = tops[0];
+#pragma unroll
+    for (int i = 1; i < AT_ONCE; ++i) most = fmaxf(most, tops[i]);
+    o = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+        const float weight = weight_of(tops[i], most, a.scale_log2);
+        const float4 v = part[i * LANES + lane];
+        o = make_float4(o.x + v.x * weight, o.y + v.y * weight, o.z + v.z * weight, o.w + v.w * weight);
+        sum += sums[i] * weight;
+    }
+    if (wrong) sum = __builtin_nanf("");
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;              // (no key: 0)
+    const __half h[4] = {__float2half(o.x * inv), __float2half(o.y * inv), __float2half(o.z * inv), __float2half(o.w * inv)};
+    *reinterpret_cast<uint2*>(a.out + ((long long)token * a.heads + head) * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
+}
+
 // What a call takes: rows of a unit, workgroups at most, the cost of a unit beside its keys, the cost below which a part is not cut, and whether units
 // are not cut at all.
 struct Plan {
@@ -1107,24 +1283,72 @@ void launch_join(const PagedAttn& a, const Plan& p, hipStream_t st)
     if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(kJoinThreads<ROWS>), 0, st, a);
 }
 
-template <int HD, bool BYTES>
-void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
+template <int HD, bool BYTES, Keys SET>
+void launch_units(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
     const dim3 grid((unsigned)p.workgroups), block(256);
     if (p.rows == 16) {
-        hipLaunchKernelGGL((tl_paged_few<HD, BYTES>), grid, block, 0, st, a);
-        launch_join<HD, 16>(a, p, st);
+        hipLaunchKernelGGL((tl_paged_few<HD, BYTES, SET>), grid, block, 0, st, a);
         return;
     }
-    if constexpr (HD < 256) {
+    if constexpr (HD < 256 && SET != kOwn) {
         if (p.rows == 128) {
-            hipLaunchKernelGGL((tl_paged_rows<HD, 2, BYTES>), grid, block, 0, st, a);
-            launch_join<HD, 128>(a, p, st);
+            hipLaunchKernelGGL((tl_paged_rows<HD, 2, BYTES, SET>), grid, block, 0, st, a);
             return;
         }
     }
-    hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES>), grid, block, 0, st, a);
-    launch_join<HD, 64>(a, p, st);
+    hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES, SET>), grid, block, 0, st, a);
+}
+
+template <int HD, bool BYTES>
+void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
+{
+    launch_units<HD, BYTES, kCausal>(a, p, st);
+    if (p.rows == 16) launch_join<HD, 16>(a, p, st);
+    else if (p.rows == 128) launch_join<HD, 128>(a, p, st);
+    else launch_join<HD, 64>(a, p, st);
+}
+
+template <int HD, bool BYTES>
+void launch_shared(const PagedAttn& a, const Plan& pa, const PagedAttn& b, const Plan& pb, hipStream_t st)
+{
+    launch_units<HD, BYTES, kPrefix>(a, pa, st);
+    launch_units<HD, BYTES, kOwn>(b, pb, st);
+    hipLaunchKernelGGL(tl_paged_merge<HD>, dim3((unsigned)a.batch.tokens * (unsigned)a.heads), dim3(256), 0, st, a, b);
+}
+
+// The launches of groups that begin alike: the shared keys' and the sequences' own.
+struct SharedPlan {
+    Plan prefix, own;
+    bool apart;                                  // the shared keys in a launch of their own; not, the call is one without groups
+};
+
+SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows, int64_t groups)
+{
+    const int group = heads / pages->kv_heads, hd = pages->head_dim;
+    auto workgroups = [](int each) { return (int)ceil_div(each * compute_units(), 8) * 8; };
+    auto plan = [&](int rows) { return Plan{rows, workgroups(rows == 16 && hd == 256 ? 1 : 2), 128, rows == 16 ? 128 : 512, 0}; };
+    SharedPlan p;
+    const int64_t together = groups > 0 ? ceil_div(tokens, groups) * group : 0;   // rows of a group and a key head, on average
+    p.prefix = plan(together <= 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
+    p.own = plan(most_rows * group <= 16 ? 16 : 64);
+    p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23);
+    return p;
+}
+
+int64_t units_of(const Plan& p, int64_t tokens, int heads, const tl_pages* pages, int64_t sequences)
+{
+    const int group = heads / pages->kv_heads, tile_heads = std::min(group, p.rows), blocks = (int)ceil_div(group, tile_heads);
+    return (tokens / (p.rows / tile_heads) + sequences + 1) * pages->kv_heads * blocks;
+}
+
+// Parts of a shared call's workspace: bytes, from the start of one launch's.
+int64_t shared_part(const Plan& p, int64_t tokens, int heads, const tl_pages* pages, int64_t sequences, int64_t* pieces, int64_t* ends)
+{
+    const int64_t row = (pages->head_dim + 4) * (int64_t)sizeof(float);
+    *pieces = round_up(tokens * heads * row, 256);
+    *ends = *pieces + round_up((int64_t)p.workgroups * p.rows * row, 256);
+    return *ends + round_up(units_of(p, tokens, heads, pages, sequences) * (int64_t)sizeof(int2), 256);
 }
 
 }  // namespace
@@ -1136,6 +1360,28 @@ extern "C" int tl_paged_attention_workspace(int64_t tokens, int heads, const tl_
     *bytes = workspace_of(plan_of(tokens, heads, pages, batch, most_rows), pages->head_dim);
     return TL_OK;
 }
+
+namespace {
+
+// The checked arguments of a call, and what they make of a plan; the walk's products of costs stay below 2^53.
+int set_plan(PagedAttn* a, const Plan& p, const tl_page_batch* batch, const tl_pages* pages, int64_t tokens)
+{
+    a->tile_heads = std::min(a->group, p.rows);
+    a->blocks = (int)ceil_div(a->group, a->tile_heads);
+    a->tile_tokens = p.rows / a->tile_heads;
+    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;
+    const int64_t units = (ceil_div(tokens, a->tile_tokens) + batch->seqs + a->group_count) * pages->kv_heads * a->blocks;
+    if (keys > (1 << 26) || units > (1ll << 42) / (keys + tokens + p.fixed + a->tile_tokens))
+        return fail(TL_ERR_SHAPE, "%lld rows over up to %lld keys are more than one call takes", (long long)tokens, (long long)keys);
+    a->fixed = p.fixed;
+    a->least = p.least;
+    a->uncut = p.uncut;
+    a->workgroups = p.workgroups;
+    a->rows = p.rows;
+    return TL_OK;
+}
+
+}  // namespace
 
 extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
                                   const tl_page_batch* batch, int64_t most_rows, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream)
@@ -1156,18 +1402,8 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
     a.q = static_cast<const __half*>(q), a.q_t = q_token, a.q_h = q_head;
     a.out = static_cast<__half*>(out);
     a.heads = heads, a.group = heads / pages->kv_heads;
-    a.tile_heads = std::min(a.group, p.rows);
-    a.blocks = (int)ceil_div(a.group, a.tile_heads);
-    a.tile_tokens = p.rows / a.tile_heads;
-    // the walk's products of costs stay below 2^53
-    const int64_t keys = (int64_t)batch->table_pages * pages->page_size;
-    const int64_t units = (ceil_div(tokens, a.tile_tokens) + batch->seqs) * pages->kv_heads * a.blocks;
-    if (keys > (1 << 26) || units > (1ll << 42) / (keys + tokens + p.fixed + a.tile_tokens))
-        return fail(TL_ERR_SHAPE, "%lld rows over up to %lld keys are more than one call takes", (long long)tokens, (long long)keys);
+    if (int rc = set_plan(&a, p, batch, pages, tokens)) return rc;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.fixed = p.fixed;
-    a.least = p.least;
-    a.uncut = p.uncut;
     a.shared = static_cast<Shared*>(workspace);
     a.pieces = reinterpret_cast<float*>(a.shared + p.workgroups);
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -1176,6 +1412,65 @@ extern "C" int tl_paged_attention(const void* q, int64_t q_token, int64_t q_head
         case 64: bytes ? launch_attention<64, true>(a, p, st) : launch_attention<64, false>(a, p, st); break;
         case 128: bytes ? launch_attention<128, true>(a, p, st) : launch_attention<128, false>(a, p, st); break;
         default: bytes ? launch_attention<256, true>(a, p, st) : launch_attention<256, false>(a, p, st);
+    }
+    return finish_launch();
+}
+
+extern "C" int tl_paged_attention_shared_workspace(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, const tl_page_prefix* prefix,
+                                                   int64_t most_rows, int64_t* bytes)
+{
+    if (int rc = tl_paged_attention_workspace(tokens, heads, pages, batch, most_rows, bytes)) return rc;
+    if (!prefix || prefix->count < 0) return fail(TL_ERR_ARG, "the groups are null or fewer than none");
+    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix->count);
+    if (!p.apart) return TL_OK;
+    int64_t pieces, ends;
+    *bytes = shared_part(p.prefix, tokens, heads, pages, prefix->count, &pieces, &ends) + shared_part(p.own, tokens, heads, pages, batch->seqs, &pieces, &ends);
+    return TL_OK;
+}
+
+extern "C" int tl_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,
+                                         const tl_page_batch* batch, const tl_page_prefix* prefix, int64_t most_rows, float scale, void* out,
+                                         void* workspace, int64_t workspace_bytes, void* stream)
+{
+    if (int rc = check_dtype(dtype, "q")) return rc;
+    if (dtype != TL_F16) return fail(TL_ERR_UNSUPPORTED, "fp16 queries only");
+    PagedAttn a{};
+    if (int rc = check_heads(heads, pages)) return rc;
+    if (int rc = take_pages(pages, batch, tokens, &a.pages, &a.batch)) return rc;
+    if (!prefix || prefix->count < 0 || prefix->count > (1 << 24)) return fail(TL_ERR_ARG, "the groups are null, fewer than none or more than 2^24");
+    if (prefix->count > 0 && (!prefix->groups || (a.batch.seqs > 0 && !prefix->shared))) return fail(TL_ERR_ARG, "device pointer is null");
+    if (tokens == 0 || a.batch.seqs == 0) return TL_OK;
+    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix->count);
+    if (!p.apart) return tl_paged_attention(q, q_token, q_head, dtype, tokens, heads, pages, batch, most_rows, scale, out, workspace, workspace_bytes, stream);
+    if (!q || !out || !workspace) return fail(TL_ERR_ARG, "device pointer is null");
+    if (most_rows < 0) return fail(TL_ERR_ARG, "most_rows is negative");
+    if (!(scale > 0.f) || scale > 1e30f) return fail(TL_ERR_ARG, "scale=%g is not a positive number up to 1e30", (double)scale);
+    if (!in_pieces(q, {q_token, q_head}, 2) || !in_pieces(out, {}, 2) || !in_pieces(workspace, {}, 1)) return fail(TL_ERR_ALIGN, "addresses and strides must be whole 16-byte pieces");
+    int64_t pieces, ends, pieces_own, ends_own;
+    const int64_t first = shared_part(p.prefix, tokens, heads, pages, prefix->count, &pieces, &ends);
+    const int64_t need = first + shared_part(p.own, tokens, heads, pages, batch->seqs, &pieces_own, &ends_own);
+    if (workspace_bytes < need) return fail(TL_ERR_SIZE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    a.q = static_cast<const __half*>(q), a.q_t = q_token, a.q_h = q_head;
+    a.out = static_cast<__half*>(out);
+    a.heads = heads, a.group = heads / pages->kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.groups = prefix->groups, a.begin = prefix->shared, a.group_count = prefix->count;
+    PagedAttn b = a;
+    if (int rc = set_plan(&a, p.prefix, batch, pages, tokens)) return rc;
+    if (int rc = set_plan(&b, p.own, batch, pages, tokens)) return rc;
+    auto place = [](PagedAttn* to, char* at, int64_t pieces_at, int64_t ends_at) {
+        to->firsts = reinterpret_cast<float*>(at);
+        to->pieces = reinterpret_cast<float*>(at + pieces_at);
+        to->ends = reinterpret_cast<int2*>(at + ends_at);
+    };
+    place(&a, static_cast<char*>(workspace), pieces, ends);
+    place(&b, static_cast<char*>(workspace) + first, pieces_own, ends_own);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool bytes = pages->dtype == TL_E4M3;
+    switch (pages->head_dim) {
+        case 64: bytes ? launch_shared<64, true>(a, p.prefix, b, p.own, st) : launch_shared<64, false>(a, p.prefix, b, p.own, st); break;
+        case 128: bytes ? launch_shared<128, true>(a, p.prefix, b, p.own, st) : launch_shared<128, false>(a, p.prefix, b, p.own, st); break;
+        default: bytes ? launch_shared<256, true>(a, p.prefix, b, p.own, st) : launch_shared<256, false>(a, p.prefix, b, p.own, st);
     }
     return finish_launch();
 }

@@ -642,6 +642,14 @@ class PageBatch(NamedTuple):
     most_rows: int
 
 
+class PagePrefix(NamedTuple):
+    """Sequences of a batch that begin with the same tokens, in the same pages.  Group g is the batch's sequences groups[g] .. groups[g + 1] - 1; each of
+    them shares its first shared[b] tokens with the others: the same number in all of a group, 0 in sequences of no group, and no more than a sequence
+    has in front of its rows.  Both int32 on the device: groups [groups + 1], shared [seqs]."""
+    groups: torch.Tensor
+    shared: torch.Tensor
+
+
 _PAGE_CODE = {torch.float16: _lib.TL_F16, torch.float8_e4m3fn: _lib.TL_E4M3}
 
 
@@ -672,6 +680,17 @@ def _page_args(pages, batch, device):
                    k.shape[2], k.shape[1], k.shape[3], _PAGE_CODE[k.dtype])
     return p, _lib.PageBatch(batch.table.data_ptr() or None, batch.starts.data_ptr(), batch.lengths.data_ptr() or None,
                              batch.table.stride(0) if seqs > 1 else columns, columns, seqs)
+
+
+def _prefix_args(prefix, batch, device):
+    for t, what in ((prefix.groups, "groups"), (prefix.shared, "shared")):
+        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous int32 tensor of one dimension")
+        if t.device != device:
+            raise RuntimeError(f"{what} is on {t.device}, the rows on {device}")
+    if prefix.groups.numel() < 1 or prefix.shared.numel() != batch.table.shape[0]:
+        raise ValueError("groups has one entry more than there are groups, shared one for each sequence")
+    return _lib.PagePrefix(prefix.groups.data_ptr(), prefix.shared.data_ptr() or None, prefix.groups.numel() - 1)
 
 
 def _overlap(x, y):
@@ -830,16 +849,18 @@ def read_pages(pages, batch, tokens, dtype=torch.float16, *, k_out=None, v_out=N
     return k_out, v_out
 
 
-def paged_attention(q, pages, batch, *, scale=None, out=None):
+def paged_attention(q, pages, batch, *, scale=None, out=None, prefix=None):
     """Causal attention of a batch's rows q [tokens, heads, head_dim] over everything their sequences have in the pages (their own keys and values
     among it: rope_to_pages first): a sequence's row i of n sees its tokens up to lengths - n + i.  Returns [tokens, heads * head_dim] (or `out`);
     rows of no sequence are not written, a row that sees nothing is 0, rows that would read a page that is none are NaN (others of their sequence may be); what is not finite where a row
     does not see it does not reach the row.  float16, head_dim 64,
     128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim).  Rows of 8 bits are taken as the float16 values that read_pages
-    gives."""
-    y = _short().paged_attention(q, pages, batch, scale, out)
-    if y is not None:
-        return y
+    gives.  prefix: a PagePrefix, whose shared tokens are read once for all rows of their group: the same results, up to the rounding of sums (rows of which it
+    does not hold may be NaN)."""
+    if prefix is None:
+        y = _short().paged_attention(q, pages, batch, scale, out)
+        if y is not None:
+            return y
     _forward_only(q, pages.k, pages.v, out)
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
@@ -854,15 +875,17 @@ def paged_attention(q, pages, batch, *, scale=None, out=None):
         raise ValueError("out must be a contiguous [tokens, heads * head_dim] tensor of q's type and device")
     elif _overlap(q, out.view(tokens, heads, hd)):
         raise ValueError("out must lie apart from q")
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    groups = () if prefix is None else (_prefix_args(prefix, batch, q.device),)
     _cuda(q, "q")
-    need = ctypes.c_int64(0)
+    need, L = ctypes.c_int64(0), _lib.lib()
+    size, call = (L.tl_paged_attention_shared_workspace, L.tl_paged_attention_shared) if groups else (L.tl_paged_attention_workspace, L.tl_paged_attention)
     with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().tl_paged_attention_workspace(tokens, heads, p, b, batch.most_rows, ctypes.byref(need)))
+        _lib.check(size(tokens, heads, p, b, *groups, batch.most_rows, ctypes.byref(need)))
         # (of the call's own: kept for the next, it would be shared by graphs that were captured on one stream and are replayed on several)
         ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        _lib.check(_lib.lib().tl_paged_attention(q.data_ptr(), *_steps(q, (0, 1)), code, tokens, heads, p, b, batch.most_rows,
-                                                 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                 _stream_ptr(q.device)))
+        _lib.check(call(q.data_ptr(), *_steps(q, (0, 1)), code, tokens, heads, p, b, *groups, batch.most_rows, scale, out.data_ptr(), ws.data_ptr(),
+                        ws.numel(), _stream_ptr(q.device)))
     return out
 
 
