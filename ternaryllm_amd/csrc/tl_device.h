@@ -39,6 +39,27 @@ struct Codes {
     int planes;                  // ternary matrices that they hold
 };
 
+// What the products of a head's losses (tl_matrix.hip) do with their sums; arrays of rows begin with the launch's first.
+struct LossRows {
+    const int64_t* targets;      // [M], or null: the teacher's entries
+    const int* entry;            // [M][top], -1: none
+    const float* share;
+    int top;
+    unsigned top_magic;          // ceil(2^32 / top)
+    int first;                   // the weight's first column among all of the head's
+    float cool, heat;            // 1 / temperature, and it
+    float2* parts;               // logits: [M][parts of the columns]: maximum, sum of exponentials against it
+    float* gaps;                 // ... [M][parts]: sum of t z
+    float* picks;                // ... [M]: the target's logit
+    const float *lse, *grad;     // gradients: [M]
+    const float* largest;        // ... the largest column scale
+    int padded;                  // ... columns of P, the last ones 0
+    float* ds;                   // ... null, or [row parts][ds_ld]
+    long long ds_ld;
+    const float* sums;           // product of P: null, or the sums of the pieces before, [M][ldy of theirs = N]
+    int last;                    // ... the last piece: times what the row is multiplied by
+};
+
 struct KernelArgs {
     WeightPtrs w0;
     WeightPtrs w1;  // second weight set of the fused gate/up kernel
@@ -88,6 +109,7 @@ struct KernelArgs {
     long long image_plane;    // ... and, for fp32 activations in three bf16 parts, between parts
     int call_rows;            // of the whole call, of which a launch may have a part (M)
     int vector_out;           // whole pieces of 16 bytes of an output row may be stored (from 8-byte boundaries)
+    LossRows loss;
 };
 
 // rsqrt(mean square + eps) of the rows behind a chained product.  Called by the first 64 threads of a workgroup (one
@@ -227,6 +249,16 @@ enum MatrixTile { kShared32x32, kShared32x64, kShared64x64, kSmall, kWide, kHalv
 MatrixTile matrix_tile(int64_t rows, int64_t columns, int64_t depth, bool f32, bool two, int64_t units);
 // Whether rows of more than 48 are read where they lie, which products with chained steps need.
 bool matrix_reads_rows(const KernelArgs& a, int x_dtype);
+
+// The products of a head's losses, of more than 48 rows: logits whose maxima and sums are kept; gradients of them, P, in x's type, and of the scales;
+// the product of P with a piece of the transposed weight.
+enum LossProduct { kLossLogits, kLossGradients, kLossBack };
+// The image that such products read: none where rows are read where they lie (bytes 0).  a.image, a.image_ld and a.image_plane are set.
+int64_t loss_image_bytes(int64_t K, int64_t rows, int x_dtype);
+int make_loss_image(KernelArgs* a, int x_dtype, void* image, hipStream_t st);
+// Columns that one of parts and gaps has, or rows that one of ds has.
+int loss_part(const KernelArgs& a, int x_dtype, LossProduct what);
+int launch_loss(KernelArgs a, int x_dtype, LossProduct what, hipStream_t st);
 
 // tl_few.hip
 // Up to 48 rows, any layout, blobs with codes; gated and chained steps for fp16 rows.  Two weights: silu(w0 product) * w1 product.

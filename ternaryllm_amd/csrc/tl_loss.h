@@ -49,12 +49,11 @@ __device__ __forceinline__ float raise_of(float largest_scale)
 __device__ __forceinline__ bool lse_counts(float lse) { return fabsf(lse) < __builtin_huge_valf(); }
 
 // What the product of a row's P is multiplied by: 0 for a row that counts for nothing, NaN where its loss is.
-__device__ __forceinline__ float row_factor(const LossArgs& a, int row, bool f16)
+__device__ __forceinline__ float row_factor(float lse, float grad, float heat, float raised)
 {
-    const float lse = a.lse[row];
     if (lse == -__builtin_huge_valf()) return 0.f;
     if (lse != lse) return lse;
-    return a.grad[row] * a.heat / (f16 ? raise_of(a.lse[a.M]) : 1.f);
+    return grad * heat / raised;
 }
 
 }  // namespace tl

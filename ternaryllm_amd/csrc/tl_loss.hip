@@ -108,13 +108,24 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
     if (lane == 0) a.known[row] = wrong ? __builtin_nanf("") : none ? __builtin_huge_valf() : known;
 }
 
+__device__ __forceinline__ float lse_of(float top, float sum) { return finite(top) ? top + logf(sum) : __builtin_nanf(""); }
+
+// A row's divergence from sum t (lse - z), by one thread.
+__device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float lse, float gap)
+{
+    const float known = a.known[row];
+    const bool none = known == __builtin_huge_valf();
+    a.loss[row] = none ? 0.f : a.heat * a.heat * (known + gap);
+    a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
+}
+
 // A row's loss from its lse and its entries' logits (z(entry), each asked for by one thread of the workgroup), and what the backward pass wants of it: lse,
 // NaN where the loss is, -inf for a row that counts for nothing.
 template <int WAVES, typename Z>
 __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, float sum, Z z)
 {
     const int tid = (int)threadIdx.x;
-    const float lse = finite(top) ? top + logf(sum) : __builtin_nanf("");
+    const float lse = lse_of(top, sum);
     if (a.targets) {
         if (tid != 0) return;
         const long long target = a.targets[row];
@@ -130,11 +141,7 @@ __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, 
         if (id >= 0) gap = fmaf(a.share[(long long)row * a.top + i], lse - z(id, i), gap);
     }
     gap = fold_all<WAVES>(gap, [](float x, float y) { return x + y; });
-    if (tid != 0) return;
-    const float known = a.known[row];
-    const bool none = known == __builtin_huge_valf();
-    a.loss[row] = none ? 0.f : a.heat * a.heat * (known + gap);
-    a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
+    if (tid == 0) put_divergence(a, row, lse, gap);
 }
 
 // The largest column scale, by one workgroup, where lse ends: what the gradients' fp16 probabilities are raised by goes by it.
@@ -157,7 +164,7 @@ __device__ __forceinline__ void put_largest_scale(const LossArgs& a)
 __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
 {
     constexpr int WAVES = kRowThreads / 64, U = 8;
-    const int row = a.first + (int)blockIdx.x, tid = (int)threadIdx.x;
+    const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
     if (row == a.M) {
         put_largest_scale<WAVES>(a);
         return;
@@ -185,25 +192,57 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
     put_loss<WAVES>(a, row, top, sum, [&](int n, int) { return z(n); });
 }
 
+// Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted.  A workgroup takes a row, one more the scales.
+__global__ __launch_bounds__(256) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
+{
+    const int row = a.first + (int)blockIdx.x;
+    if (row == a.M) {
+        put_largest_scale<4>(a);
+        return;
+    }
+    const float2* own = parts + (long long)blockIdx.x * count;
+    float top = kNone, sum = 0.f;
+    for (int i = (int)threadIdx.x; i < count; i += 256) join(top, sum, own[i].x, own[i].y);
+    join_all<4>(top, sum);
+    if (a.targets) {
+        put_loss<4>(a, row, top, sum, [&](int, int) { return picks[blockIdx.x]; });
+        return;
+    }
+    float gap = 0.f;
+    for (int i = (int)threadIdx.x; i < count; i += 256) gap += gaps[(long long)blockIdx.x * count + i];
+    gap = fold_all<4>(gap, [](float x, float y) { return x + y; });
+    if (threadIdx.x == 0) put_divergence(a, row, lse_of(top, sum), lse_of(top, sum) - gap);
+}
+
+// ds from its parts, rows one after the other; what rows of the call before have left in it is added to.
+__global__ __launch_bounds__(256) void tl_loss_ds(float* ds, const float* parts, int count, long long ld, int N, float heat, int more)
+{
+    const int n = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (n >= N) return;
+    float sum = 0.f;
+    for (int i = 0; i < count; ++i) sum += parts[i * ld + n];
+    ds[n] = more ? fmaf(sum, heat, ds[n]) : sum * heat;
+}
+
 // Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after the other.
 template <typename T>
-__global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a, int rows)
+__global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
 {
+    const int rows = a.M;
     __shared__ float wanted[kSmallMaxM][kFewColumns];
     const int tid = (int)threadIdx.x, first = (int)blockIdx.x * kFewColumns, n = first + tid;
     for (int m = 0; m < rows; ++m) wanted[m][tid] = 0.f;
     __syncthreads();
     if (a.targets) {
         if (tid < rows) {
-            const long long target = a.targets[a.first + tid] - first;
+            const long long target = a.targets[tid] - first;
             if (target >= 0 && target < kFewColumns) wanted[tid][target] = 1.f;
         }
     } else {
         for (int i = tid; i < rows * a.top; i += kFewColumns) {
-            const long long at = (long long)a.first * a.top + i;
-            const int entry = a.entry[at];
+            const int entry = a.entry[i];
             const unsigned c = (unsigned)(entry - first);
-            if (entry >= 0 && c < kFewColumns) wanted[i / a.top][c] = a.share[at];   // (an entry stands once in a row)
+            if (entry >= 0 && c < kFewColumns) wanted[i / a.top][c] = a.share[i];   // (an entry stands once in a row)
         }
     }
     __syncthreads();
@@ -218,8 +257,8 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a, int 
         for (int u = 0; u < U; ++u) {
             const int m = min(m0 + u, rows - 1);
             raw[u] = there ? a.raw[(long long)m * a.raw_ld + n] : 0.f;
-            lse[u] = a.lse[a.first + m];
-            grad[u] = a.grad[a.first + m];
+            lse[u] = a.lse[m];
+            grad[u] = a.grad[m];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -230,22 +269,19 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a, int 
             ds += counts ? dz * raw[u] * grad[u] : lse[u] == kNone ? 0.f : __builtin_nanf("");
         }
     }
-    if (a.ds && there) {
-        ds *= a.heat;
-        a.ds[n] = a.first > 0 ? a.ds[n] + ds : ds;
-    }
+    if (a.ds && there) a.ds[n] = ds * a.heat;
 }
 
 // dx = what a row is multiplied by times the product of P, a sum of those of the vocabulary's pieces.
 template <typename T>
-__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int rows, int pieces)
+__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int pieces)
 {
     const int m = (int)blockIdx.y, k = (int)(blockIdx.x * 256 + threadIdx.x);
     if (k >= a.K) return;
-    const float factor = row_factor(a, a.first + m, sizeof(T) == 2);
+    const float factor = row_factor(a.lse[m], a.grad[m], a.heat, sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f);
     float sum = 0.f;
-    for (int i = 0; i < pieces; ++i) sum += from[((long long)i * rows + m) * a.K + k];
-    static_cast<T*>(a.dx)[(long long)(a.first + m) * a.dx_ld + k] = (T)settled(lse_counts(a.lse[a.first + m]) ? sum * factor : factor);
+    for (int i = 0; i < pieces; ++i) sum += from[((long long)i * a.M + m) * a.K + k];
+    static_cast<T*>(a.dx)[m * a.dx_ld + k] = (T)settled(lse_counts(a.lse[m]) ? sum * factor : factor);
 }
 
 __global__ __launch_bounds__(256) void tl_loss_scale_out(const float* ds, void* out, int f16, int N)
@@ -358,11 +394,9 @@ struct FewParts {
     float* ds;           // [N]
 };
 
-int64_t few_rows(int64_t M) { return std::min<int64_t>(M, kSmallMaxM); }
-
 FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, bool backward, int64_t product_bytes)
 {
-    const int64_t rows = few_rows(M), ld = round_up(h->columns, 64);
+    const int64_t rows = M, ld = round_up(h->columns, 64);
     FewParts f{};
     f.raw = static_cast<float*>(p.take(rows * ld * 4));
     f.product = p.take(product_bytes);
@@ -377,13 +411,7 @@ FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, 
 int product_workspace(const tl_layout_header* h, int64_t M, int x_dtype, int64_t* bytes)
 {
     *bytes = 0;
-    for (int64_t rows : {few_rows(M), M % kSmallMaxM}) {
-        int64_t need = 0;
-        if (rows)
-            if (int rc = tl_spmm_workspace(h, rows, x_dtype, TL_X_ROW_MAJOR, &need)) return rc;
-        *bytes = std::max(*bytes, need);
-    }
-    return TL_OK;
+    return M ? tl_spmm_workspace(h, M, x_dtype, TL_X_ROW_MAJOR, bytes) : TL_OK;
 }
 
 // The products of P's rows with the pieces of the transposed weight.
@@ -407,6 +435,128 @@ int back_product(const tl_layout_header* h, const void* back, const LossArgs& a,
         k.c0 = Codes{codes, k.planes};
         if (int rc = launch_matrix_few(k, x_dtype, false, st)) return rc;
         codes += (int64_t)k.NB * k.planes * k.units * TL_CODE_UNIT_BYTES;
+    }
+    return TL_OK;
+}
+
+// Many rows: so many at a time, and what the workspace holds for them.
+constexpr int64_t kForwardRows = 16384;
+constexpr int64_t kGradientBytes = 128 << 20;    // of P, and of its image
+
+int64_t piece_columns(const tl_layout_header* h) { return std::min<int64_t>(h->columns, kPieceColumns); }
+
+int64_t backward_rows(const tl_layout_header* h, int64_t M, int x_dtype)
+{
+    const int64_t rows = kGradientBytes / (round_up(piece_columns(h), 64) * (x_dtype == TL_F16 ? 2 : 4 + 6));
+    return std::min(M, std::min(kForwardRows, std::max<int64_t>(rows / 128 * 128, 128)));
+}
+
+struct ManyParts {
+    int64_t rows;
+    void* image;         // of the rows of x
+    float2* parts;       // forward: [rows][columns / 64 or 32]
+    float *gaps, *picks;
+    void *P, *P_image;   // backward: [rows][piece]
+    float *sums, *ds_parts, *ds;
+};
+
+ManyParts many_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, bool backward)
+{
+    const int64_t N = h->columns, K = h->inners, piece = round_up(piece_columns(h), 64);
+    ManyParts f{};
+    f.rows = backward ? backward_rows(h, M, x_dtype) : std::min(M, kForwardRows);
+    f.image = p.take(loss_image_bytes(K, f.rows, x_dtype));
+    if (!backward) {
+        const int64_t count = f.rows * ceil_div(N, x_dtype == TL_F16 ? 64 : 32);
+        f.parts = static_cast<float2*>(p.take(count * 8));
+        f.gaps = static_cast<float*>(p.take(count * 4));
+        f.picks = static_cast<float*>(p.take(f.rows * 4));
+        return f;
+    }
+    f.P = p.take(f.rows * piece * (x_dtype == TL_F16 ? 2 : 4));
+    f.P_image = x_dtype == TL_F16 ? nullptr : p.take(loss_image_bytes(piece, f.rows, x_dtype));
+    f.sums = N > kPieceColumns ? static_cast<float*>(p.take(f.rows * K * 4)) : nullptr;
+    f.ds_parts = static_cast<float*>(p.take(ceil_div(f.rows, 32) * piece * 4));
+    f.ds = static_cast<float*>(p.take(N * 4));
+    return f;
+}
+
+KernelArgs rows_product(const tl_layout_header* h, const void* blob, const void* x, int x_dtype, int64_t ldx, int64_t first, int rows, const LossArgs& a)
+{
+    KernelArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.w0 = weight_ptrs(h, blob, a.scale);
+    k.X = static_cast<const char*>(x) + first * ldx * (x_dtype == TL_F16 ? 2 : 4);
+    k.ldx = ldx;
+    k.M = k.call_rows = rows, k.N = a.N, k.K = a.K, k.T = (int)h->n_tiles, k.tile_rows = (int)h->tile_rows;
+    k.NB = (int)h->n_blocks, k.c0 = weight_codes(h, blob), k.units = (int)h->code_units, k.planes = k.c0.planes;
+    k.x_f16 = x_dtype == TL_F16, k.scale_f16 = a.scale_f16;
+    k.one = 1.0f;
+    LossRows& l = k.loss;
+    l.targets = a.targets ? a.targets + first : nullptr;
+    l.entry = a.entry ? a.entry + first * a.top : nullptr;
+    l.share = a.share ? a.share + first * a.top : nullptr;
+    l.top = a.top;
+    l.top_magic = a.top > 1 ? (unsigned)((((uint64_t)1 << 32) + a.top - 1) / a.top) : 0;
+    l.cool = a.cool, l.heat = a.heat;
+    return k;
+}
+
+int many_forward(const tl_layout_header* h, const void* blob, const void* x, int x_dtype, int64_t ldx, LossArgs a, const ManyParts& f, hipStream_t st)
+{
+    for (int64_t m = 0; m < a.M; m += f.rows) {
+        const int rows = (int)std::min<int64_t>(a.M - m, f.rows);
+        KernelArgs k = rows_product(h, blob, x, x_dtype, ldx, m, rows, a);
+        if (int rc = make_loss_image(&k, x_dtype, f.image, st)) return rc;
+        k.loss.parts = f.parts, k.loss.gaps = f.gaps, k.loss.picks = f.picks;
+        if (int rc = launch_loss(k, x_dtype, kLossLogits, st)) return rc;
+        a.first = (int)m;
+        hipLaunchKernelGGL(tl_loss_join, dim3((unsigned)(rows + (m + rows == a.M))), dim3(256), 0, st, a, f.parts, f.gaps, f.picks,
+                           (int)ceil_div(a.N, loss_part(k, x_dtype, kLossLogits)));
+    }
+    return TL_OK;
+}
+
+int many_backward(const tl_layout_header* h, const void* blob, const void* back, const void* x, int x_dtype, int64_t ldx, const LossArgs& a, const ManyParts& f,
+                  hipStream_t st)
+{
+    const int es = x_dtype == TL_F16 ? 2 : 4, planes = (int)h->code_planes;
+    const int64_t blocks = ceil_div(a.K, 16);
+    for (int64_t m = 0; m < a.M; m += f.rows) {
+        const int rows = (int)std::min<int64_t>(a.M - m, f.rows);
+        KernelArgs k = rows_product(h, blob, x, x_dtype, ldx, m, rows, a);
+        if (int rc = make_loss_image(&k, x_dtype, f.image, st)) return rc;
+        k.loss.lse = a.lse + m, k.loss.grad = a.grad + m, k.loss.largest = x_dtype == TL_F16 ? a.lse + a.M : nullptr;
+        const unsigned char* codes = static_cast<const unsigned char*>(back);
+        for (int64_t n = 0; n < a.N; n += kPieceColumns) {
+            const int64_t wide = std::min<int64_t>(a.N - n, kPieceColumns), units = ceil_div(wide, TL_CODE_UNIT_ROWS), padded = round_up(wide, 8);
+            KernelArgs some = k;
+            some.N = (int)wide, some.NB = (int)ceil_div(wide, 16);
+            some.c0.base += n / 16 * planes * k.units * TL_CODE_UNIT_BYTES;
+            if (a.scale) some.w0.scale = static_cast<const char*>(a.scale) + n * (a.scale_f16 ? 2 : 4);
+            some.Y = f.P, some.y_f16 = k.x_f16, some.ldy = round_up(wide, 64);
+            some.loss.first = (int)n, some.loss.padded = (int)padded;
+            some.loss.ds = a.ds ? f.ds_parts : nullptr, some.loss.ds_ld = some.ldy;
+            if (int rc = launch_loss(some, x_dtype, kLossGradients, st)) return rc;
+            if (a.ds)
+                hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 256)), dim3(256), 0, st, a.ds + n, f.ds_parts,
+                                   (int)ceil_div(rows, loss_part(some, x_dtype, kLossGradients)), some.loss.ds_ld, (int)wide, a.heat, (int)(m > 0));
+            if (!a.dx) continue;
+            const bool last = n + wide == a.N;
+            KernelArgs b;
+            std::memset(&b, 0, sizeof(b));
+            b.X = f.P, b.ldx = some.ldy;
+            b.M = b.call_rows = rows, b.N = a.K, b.K = (int)padded, b.NB = (int)blocks;
+            b.c0 = Codes{codes, planes}, b.units = (int)units, b.planes = planes;
+            b.x_f16 = k.x_f16, b.one = 1.0f, b.tile_rows = 1;
+            if (int rc = make_loss_image(&b, x_dtype, f.P_image, st)) return rc;
+            b.loss = k.loss;
+            b.loss.sums = n > 0 ? f.sums : nullptr, b.loss.last = last;
+            b.Y = last ? static_cast<char*>(a.dx) + m * a.dx_ld * es : static_cast<void*>(f.sums);
+            b.y_f16 = last && k.x_f16, b.ldy = last ? a.dx_ld : a.K;
+            if (int rc = launch_loss(b, x_dtype, kLossBack, st)) return rc;
+            codes += blocks * planes * units * TL_CODE_UNIT_BYTES;
+        }
     }
     return TL_OK;
 }
@@ -455,10 +605,14 @@ extern "C" int tl_head_loss_workspace(const tl_layout_header* header, int64_t M,
     if (int rc = check_dtype(x_dtype, "x")) return rc;
     if (int rc = check_target(target)) return rc;
     if (!bytes || M < 0 || M > (1 << 24)) return fail(TL_ERR_ARG, "a pointer is null, or %lld rows (0 to 2^24)", (long long)M);
-    int64_t product = 0;
-    if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
     Parts p{nullptr};
-    few_parts(p, header, M, x_dtype, backward != 0, product);
+    if (M > kSmallMaxM) {
+        many_parts(p, header, M, x_dtype, backward != 0);
+    } else {
+        int64_t product = 0;
+        if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
+        few_parts(p, header, M, x_dtype, backward != 0, product);
+    }
     *bytes = p.used;
     return TL_OK;
 }
@@ -478,12 +632,11 @@ int check_call(const tl_layout_header* header, const void* blob_dev, const void*
     return TL_OK;
 }
 
-// The logits of rows a.first .. without scales.
-int raw_product(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, const LossArgs& a, int rows, const FewParts& f,
+// The logits of few rows, without scales.
+int raw_product(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, const LossArgs& a, const FewParts& f,
                 int64_t product_bytes, void* stream)
 {
-    const char* from = static_cast<const char*>(x) + (int64_t)a.first * ldx * (x_dtype == TL_F16 ? 2 : 4);
-    return tl_spmm(header, blob_dev, from, x_dtype, TL_X_ROW_MAJOR, ldx, rows, f.raw, TL_F32, a.raw_ld, nullptr, TL_F32, product_bytes ? f.product : nullptr,
+    return tl_spmm(header, blob_dev, x, x_dtype, TL_X_ROW_MAJOR, ldx, a.M, f.raw, TL_F32, a.raw_ld, nullptr, TL_F32, product_bytes ? f.product : nullptr,
                    product_bytes, stream);
 }
 
@@ -498,17 +651,17 @@ extern "C" int tl_head_loss(const tl_layout_header* header, const void* blob_dev
     hipStream_t st = static_cast<hipStream_t>(stream);
     LossArgs a = loss_args(header, M, scale, scale_dtype, target);
     a.loss = loss, a.lse = lse;
+    Parts p{static_cast<char*>(workspace)};
+    if (M > kSmallMaxM) {
+        if (int rc = many_forward(header, blob_dev, x, x_dtype, ldx, a, many_parts(p, header, M, x_dtype, false), st)) return rc;
+        return finish_launch();
+    }
     int64_t product = 0;
     if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
-    Parts p{static_cast<char*>(workspace)};
     const FewParts f = few_parts(p, header, M, x_dtype, false, product);
     a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
-    for (int64_t m = 0; m < M; m += kSmallMaxM) {
-        const int rows = (int)std::min<int64_t>(M - m, kSmallMaxM);
-        a.first = (int)m;
-        if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, rows, f, product, stream)) return rc;
-        hipLaunchKernelGGL(tl_loss_few, dim3((unsigned)(rows + (m + rows == M))), dim3(kRowThreads), 0, st, a);
-    }
+    if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, f, product, stream)) return rc;
+    hipLaunchKernelGGL(tl_loss_few, dim3((unsigned)M + 1), dim3(kRowThreads), 0, st, a);
     return finish_launch();
 }
 
@@ -524,29 +677,35 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
     if (!lse || !grad) return fail(TL_ERR_ARG, "device pointer is null");
     hipStream_t st = static_cast<hipStream_t>(stream);
     LossArgs a = loss_args(header, M, scale, scale_dtype, target);
-    int64_t product = 0;
-    if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
-    Parts p{static_cast<char*>(workspace)};
-    const FewParts f = few_parts(p, header, M, x_dtype, true, product);
-    a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
     a.lse = const_cast<float*>(lse), a.grad = grad;
-    a.P = f.P, a.dx = dx, a.dx_ld = dx_ld;
-    a.ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : f.ds;
-    const unsigned groups = (unsigned)ceil_div(a.raw_ld, kFewColumns);
-    const int pieces = (int)ceil_div(header->columns, kPieceColumns);
-    for (int64_t m = 0; m < M; m += kSmallMaxM) {
-        const int rows = (int)std::min<int64_t>(M - m, kSmallMaxM);
-        a.first = (int)m;
-        if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, rows, f, product, stream)) return rc;
-        if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_few_grad<_Float16>, dim3(groups), dim3(kFewColumns), 0, st, a, rows);
-        else hipLaunchKernelGGL(tl_loss_few_grad<float>, dim3(groups), dim3(kFewColumns), 0, st, a, rows);
-        if (!dx) continue;
-        if (int rc = back_product(header, back, a, x_dtype, rows, f.sums, st)) return rc;
-        const dim3 grid((unsigned)ceil_div(header->inners, 256), (unsigned)rows);
-        if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, f.sums, rows, pieces);
-        else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, f.sums, rows, pieces);
+    a.dx = dx, a.dx_ld = dx_ld;
+    Parts p{static_cast<char*>(workspace)};
+    float* ds = nullptr;                         // where the scales' gradient is summed up
+    auto sum_ds = [&](float* own) { a.ds = ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : own; };
+    if (M > kSmallMaxM) {
+        const ManyParts f = many_parts(p, header, M, x_dtype, true);
+        sum_ds(f.ds);
+        if (int rc = many_backward(header, blob_dev, back, x, x_dtype, ldx, a, f, st)) return rc;
+    } else {
+        int64_t product = 0;
+        if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
+        const FewParts f = few_parts(p, header, M, x_dtype, true, product);
+        sum_ds(f.ds);
+        a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
+        a.P = f.P;
+        const dim3 groups((unsigned)ceil_div(a.raw_ld, kFewColumns));
+        const int rows = (int)M, pieces = (int)ceil_div(header->columns, kPieceColumns);
+        if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, f, product, stream)) return rc;
+        if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_few_grad<_Float16>, groups, dim3(kFewColumns), 0, st, a);
+        else hipLaunchKernelGGL(tl_loss_few_grad<float>, groups, dim3(kFewColumns), 0, st, a);
+        if (dx) {
+            if (int rc = back_product(header, back, a, x_dtype, rows, f.sums, st)) return rc;
+            const dim3 grid((unsigned)ceil_div(header->inners, 256), (unsigned)rows);
+            if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, f.sums, pieces);
+            else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, f.sums, pieces);
+        }
     }
     if (dscale && scale_dtype == TL_F16)
-        hipLaunchKernelGGL(tl_loss_scale_out, dim3((unsigned)ceil_div(header->columns, 256)), dim3(256), 0, st, f.ds, dscale, 1, a.N);
+        hipLaunchKernelGGL(tl_loss_scale_out, dim3((unsigned)ceil_div(header->columns, 256)), dim3(256), 0, st, ds, dscale, 1, a.N);
     return finish_launch();
 }

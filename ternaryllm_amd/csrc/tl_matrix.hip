@@ -6,7 +6,9 @@
 // registers, where they serve all of its activation rows.  tl_x_image makes the row-major, padded copy of activations that
 // come in another layout, and the three bf16 parts of fp32 ones.  tl_walk_rows multiplies from the index stream, for blobs
 // without codes and K-major rows without a workspace.
+#include "tl_loss.h"
 #include "tl_matrix.h"
+#include "tl_rope.h"
 
 using namespace tl;
 
@@ -95,7 +97,8 @@ __device__ __forceinline__ void read_scales(const void* scale, int is_f16, int n
     else read(float{});
 }
 
-enum { kPlain = 0, kPairs = 1, kTwoWeights = 2, kSteps = 3 };   // (kSteps: with what a decoder layer does around a product)
+enum { kPlain = 0, kPairs = 1, kTwoWeights = 2, kSteps = 3,     // (kSteps: with what a decoder layer does around a product)
+       kLogits = 4, kGradients = 5, kBack = 6 };                  // of a head's losses
 
 // The product of one output: from the index stream where the matrix cores' sum is not finite.
 __device__ __forceinline__ float exact_output(const KernelArgs& a, const WeightPtrs& w, int m, int n) { return walk_column(w, a.T, a.tile_rows, n, callers_x(a, m)); }
@@ -141,6 +144,178 @@ __device__ __forceinline__ float put_steps(const KernelArgs& a, int row, int n, 
         store_piece<COUNT>(image, row, n, a.N, v);
     }
     return sum;
+}
+
+// Between what lanes of a wave put into LDS and what others of it read there, and before it is written over.  (No instruction: LDS takes a wave's requests
+// in order; it holds the compiler to that order.)
+__device__ __forceinline__ void lanes_meet()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kTeacherRows = 32;                                  // of a wave's, whose teacher's shares stand in LDS at a time
+constexpr int teacher_ld(int columns) { return columns + 4; }
+
+// The last steps of a head's losses (put_out's arguments; own: LDS of the wave's own, kTeacherRows * teacher_ld floats of it, once every wave of the
+// workgroup is done with its buffers).  A row's logits lie with four lanes; a wave leaves their maximum and sum for its columns.  Its teacher's entries are
+// few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.
+template <int CF, int FW, int F, int G, int MODE>
+__device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0, unsigned char* own)
+{
+    constexpr int C = 4 * CF, GROUPS = FW / CF, COLUMNS = 16 * FW, LD = teacher_ld(COLUMNS);
+    static_assert(F == FW && G % 2 == 0);
+    const LossRows& l = a.loss;
+    const int lane = (int)threadIdx.x & 63, q = lane >> 4, r16 = lane & 15;
+    const int first_n = lane_n0 - q * C, first_m = lane_m0 - r16;
+    if constexpr (MODE == kBack) {
+        const float raised = l.largest ? raise_of(*l.largest) : 1.f;
+#pragma unroll
+        for (int m = 0; m < G; ++m) {
+            const int row = lane_m0 + m * 16;
+            if (row >= a.M) continue;
+            const float lse = l.last ? l.lse[row] : 0.f, factor = l.last ? row_factor(lse, l.grad[row], l.heat, raised) : 0.5f;
+            const bool counts = lse_counts(lse);
+#pragma unroll
+            for (int group = 0; group < GROUPS; ++group) {
+                const int n = lane_n0 + group * 4 * C;
+                if (n >= a.N) continue;
+                float v[C], before[C];
+                const float* sums = l.sums ? l.sums + (long long)row * a.N + n : nullptr;
+                if (sums && n + C <= a.N) __builtin_memcpy(before, sums, sizeof(before));
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    if (!sums) before[i] = 0.f;
+                    else if (n + C > a.N) before[i] = n + i < a.N ? sums[i] : 0.f;
+                    v[i] = fmaf(acc[group * CF + i / 4][m][i % 4], 0.5f, before[i]);   // (the products are with +-2)
+                    if (l.last) v[i] = counts ? v[i] * factor : factor;
+                }
+                store_piece<C>(a, row, n, a.N, v);
+            }
+        }
+        return;
+    }
+    float s[GROUPS][C];
+#pragma unroll
+    for (int group = 0; group < GROUPS; ++group) read_scales(a.w0.scale, a.scale_f16, lane_n0 + group * 4 * C, a.N, 1.0f, s[group]);
+    float* wanted = reinterpret_cast<float*>(own);
+    auto find_wanted = [&](int row0) {                            // what is wanted of kTeacherRows rows from row0 on, in the wave's columns
+        lanes_meet();
+        for (int i = lane; i < kTeacherRows * LD / 4; i += 64) reinterpret_cast<f32x4*>(wanted)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        lanes_meet();
+        const int count = min(kTeacherRows, a.M - row0) * l.top;
+        const long long from = (long long)row0 * l.top;
+        constexpr int U = 16;
+        for (int j0 = lane; j0 < count; j0 += 64 * U) {
+            int c[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) c[u] = j0 + u * 64 < count ? l.entry[from + j0 + u * 64] : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (c[u] < 0 || (unsigned)(c[u] - l.first - first_n) >= (unsigned)COLUMNS) continue;
+                const int j = j0 + u * 64, r = l.top > 1 ? (int)__umulhi((unsigned)j, l.top_magic) : j;   // (j / top, of fewer than 2^16)
+                wanted[r * LD + c[u] - l.first - first_n] = l.share[from + j];
+            }
+        }
+        lanes_meet();
+    };
+    if (!l.targets) __syncthreads();
+    const float up = MODE == kGradients && a.x_f16 ? raise_of(*l.largest) : 1.f;
+    float ds[GROUPS][C];
+#pragma unroll
+    for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+        for (int i = 0; i < C; ++i) ds[group][i] = 0.f;
+    KernelArgs to = a;
+    to.N = l.padded;
+#pragma unroll
+    for (int m = 0; m < G; ++m) {
+        const int row = lane_m0 + m * 16;
+        if (!l.targets && m % 2 == 0) {
+            if (first_m + m * 16 >= a.M) break;                   // (the same for all lanes)
+            find_wanted(first_m + m * 16);
+        }
+        const long long target = l.targets && row < a.M ? l.targets[row] - l.first : -1;
+        float t[GROUPS][C];
+#pragma unroll
+        for (int group = 0; group < GROUPS; ++group) {
+            const int n = lane_n0 + group * 4 * C;
+            if (l.targets) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) t[group][i] = target == n + i ? 1.f : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < C / 4; ++i) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(wanted + (m % 2 * 16 + r16) * LD + n - first_n + 4 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[group][4 * i + e] = x[e];
+                }
+            }
+        }
+        if constexpr (MODE == kLogits) {
+            float z[GROUPS][C], top = -__builtin_huge_valf(), sum = 0.f, gap = 0.f;
+            bool wrong = false;
+#pragma unroll
+            for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    float& v = z[group][i];
+                    v = 0.5f * acc[group * CF + i / 4][m][i % 4] * s[group][i] * l.cool;
+                    if (lane_n0 + group * 4 * C + i >= a.N) v = -__builtin_huge_valf();
+                    wrong |= v != v;
+                    top = fmaxf(top, v);
+                    if (t[group][i] > 0.f) gap = fmaf(t[group][i], v, gap);
+                }
+            // (a maximum passes over what is not a number: +inf, which is none either, stands for it)
+            top = with_other_rows(wrong ? __builtin_huge_valf() : top, [](float x, float y) { return fmaxf(x, y); });
+            const float base = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+            for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+                for (int i = 0; i < C; ++i) sum += __expf(z[group][i] - base);
+            sum = with_other_rows(sum, [](float x, float y) { return x + y; });
+            const int part = first_n / COLUMNS, parts = (a.N + COLUMNS - 1) / COLUMNS;
+            if (l.targets) {
+                const long long c = target - first_n;
+                if (row < a.M && c >= 0 && c < COLUMNS && (c / C & 3) == q) l.picks[row] = gap;
+            } else {
+                gap = with_other_rows(gap, [](float x, float y) { return x + y; });
+                if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap;
+            }
+            if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top, sum);
+        } else {
+            if (row >= a.M) continue;
+            const float lse = l.lse[row], grad = l.grad[row];
+            const bool counts = lse_counts(lse);
+#pragma unroll
+            for (int group = 0; group < GROUPS; ++group) {
+                const int n = lane_n0 + group * 4 * C;
+                float p[C];
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    const float raw = 0.5f * acc[group * CF + i / 4][m][i % 4];
+                    const float dz = counts && n + i < a.N ? __expf(raw * s[group][i] * l.cool - lse) - t[group][i] : 0.f;
+                    p[i] = dz * s[group][i] * up;
+                    ds[group][i] += counts ? dz * raw * grad : lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
+                }
+                if (n < l.padded) store_piece<C>(to, row, n, l.padded, p);
+            }
+        }
+    }
+    if constexpr (MODE == kGradients) {
+        if (!l.ds) return;
+        float* out = l.ds + first_m / (16 * G) * l.ds_ld;
+#pragma unroll
+        for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                float v = ds[group][i];
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) v += __shfl_xor(v, off, 64);
+                const int n = lane_n0 + group * 4 * C + i;
+                if (r16 == 0 && n < a.N && first_m < a.M) out[n] = v;
+            }
+    }
 }
 
 // A lane's sums of G rows on their way out: C = 4 * CF neighbouring columns of each row from each CF fragments, of one weight or of
@@ -465,6 +640,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArg
     }
 
     // ---- out ----
+    unsigned char* teacher = all_lds + wg_wave * (kTeacherRows * teacher_ld(FN * 32) * 4);
     constexpr int WAVE_N = MODE == kTwoWeights ? FN * 16 : FN * 32;   // output columns of a wave
     if constexpr (SHARED && WK > 1) {
         // A wave and the other group's wave of the same outputs give each other half of their sums, by rows, through LDS (all of the
@@ -501,7 +677,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArg
                     for (int e = 0; e < 4; ++e) v[f][g][e] += high[e];
                 }
             }
-        put_out<CF, FW, F, HALF, MODE>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
+        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, HALF, MODE>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
+        else put_out<CF, FW, F, HALF, MODE>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
     } else if constexpr (WK > 1) {
         // every wave has sums of the whole tile, of its own rows of K: they meet in LDS (a wave's in its own part, which it is
         // done with), and each goes on with 16 rows, or, where those are fewer than waves, with a group of their columns.  fp32
@@ -548,7 +725,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArg
 #pragma unroll
                 for (int m = 0; m < G; ++m) add_low(acc[f][m], low[f][m]);
         }
-        put_out<CF, FW, F, G, MODE>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
+        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, G, MODE>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
+        else put_out<CF, FW, F, G, MODE>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
     }
 }
 
@@ -956,4 +1134,67 @@ int tl::launch_matrix_rows(KernelArgs a, int x_dtype, void* workspace, int64_t w
         if (int rc = x_dtype == TL_F16 ? launch_parts<1>(some, two_weights, st) : launch_parts<3>(some, two_weights, st)) return rc;
     }
     return TL_OK;
+}
+
+int64_t tl::loss_image_bytes(int64_t K, int64_t rows, int x_dtype) { return rows * image_row_bytes(K, x_dtype); }
+
+int tl::make_loss_image(KernelArgs* a, int x_dtype, void* image, hipStream_t st)
+{
+    const bool direct = matrix_reads_rows(*a, x_dtype);
+    a->x_sm = a->ldx, a->x_sk = 1;
+    a->image_ld = direct ? a->ldx : round_up(a->K, 8);
+    if (a->image_ld > kMostLd) return fail(TL_ERR_ARG, "rows of %lld activations are too long for one call", (long long)a->image_ld);
+    a->image = direct ? a->X : image;
+    a->image_plane = a->image_ld * a->M;
+    if (!direct) make_image(*a, x_dtype, static_cast<unsigned short*>(image), st);
+    return TL_OK;
+}
+
+namespace {
+
+// The tiles of a head's losses: of those of any product (matrix_tile) the ones for many, and one for few, in whose place others are up to a few us quicker.
+MatrixTile loss_tile(const KernelArgs& a, bool f32)
+{
+    const MatrixTile tile = matrix_tile(a.call_rows, a.N, (int64_t)a.planes * a.units, f32, false, compute_units());
+    if (tile == kTall || tile == kFlat) return tile;
+    return tile == kGroups ? kFlat : f32 ? kWide : kHalves;
+}
+
+template <int PARTS, int MODE>
+int launch_loss_mode(const KernelArgs& a, hipStream_t st)
+{
+    switch (loss_tile(a, PARTS > 1)) {
+    case kWide:
+        if constexpr (PARTS > 1) return launch_tile<PARTS, 1, 4, 1, 2, 1, MODE>(a, st);
+        break;
+    case kHalves:
+        if constexpr (PARTS == 1) return launch_tile<PARTS, 1, 2, 2, 2, 2, MODE>(a, st);
+        break;
+    case kTall:
+        if constexpr (PARTS == 1) return launch_tile<PARTS, 1, 4, 1, 4, 2, MODE>(a, st);
+        break;
+    default: return launch_tile<PARTS, 1, 4, 1, 2, 2, MODE>(a, st);
+    }
+    return fail(TL_ERR_UNSUPPORTED, "no such tile");
+}
+
+template <int PARTS>
+int launch_loss_parts(const KernelArgs& a, LossProduct what, hipStream_t st)
+{
+    return what == kLossLogits ? launch_loss_mode<PARTS, kLogits>(a, st) : what == kLossGradients ? launch_loss_mode<PARTS, kGradients>(a, st) : launch_loss_mode<PARTS, kBack>(a, st);
+}
+
+}  // namespace
+
+int tl::loss_part(const KernelArgs& a, int x_dtype, LossProduct what)
+{
+    const MatrixTile tile = loss_tile(a, x_dtype != TL_F16);
+    if (what == kLossLogits) return tile == kWide ? 32 : 64;
+    return tile == kTall ? 128 : tile == kHalves ? 32 : 64;
+}
+
+int tl::launch_loss(KernelArgs a, int x_dtype, LossProduct what, hipStream_t st)
+{
+    a.vector_out = a.ldy % (a.y_f16 ? 4 : 2) == 0 && reinterpret_cast<uintptr_t>(a.Y) % 8 == 0;
+    return x_dtype == TL_F16 ? launch_loss_parts<1>(a, what, st) : launch_loss_parts<3>(a, what, st);
 }
