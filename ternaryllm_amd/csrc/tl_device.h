@@ -54,10 +54,13 @@ struct LossRows {
     const float *lse, *grad;     // gradients: [M]
     const float* largest;        // ... the largest column scale
     int padded;                  // ... columns of P, the last ones 0
+    long long plane;             // ... of fp32 rows: between the parts of P
     float* ds;                   // ... null, or [row parts][ds_ld]
     long long ds_ld;
     const float* sums;           // product of P: null, or the sums of the pieces before, [M][ldy of theirs = N]
     int last;                    // ... the last piece: times what the row is multiplied by
+    int unit0, units;            // ... units of K that the launch multiplies, planes one after the other
+    int splits;                  // ... shared out among workgroups: each its own [M][ldy] of Y
 };
 
 struct KernelArgs {
@@ -259,6 +262,8 @@ int make_loss_image(KernelArgs* a, int x_dtype, void* image, hipStream_t st);
 // Columns that one of parts and gaps has, or rows that one of ds has.
 int loss_part(const KernelArgs& a, int x_dtype, LossProduct what);
 int launch_loss(KernelArgs a, int x_dtype, LossProduct what, hipStream_t st);
+// Into how many parts the product of P of `units` units of K is split.
+int loss_splits(const KernelArgs& a, int x_dtype, int units);
 
 // tl_few.hip
 // Up to 48 rows, any layout, blobs with codes; gated and chained steps for fp16 rows.  Two weights: silu(w0 product) * w1 product.

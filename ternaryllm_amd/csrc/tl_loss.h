@@ -4,7 +4,7 @@
 
 namespace tl {
 
-constexpr int kPieceColumns = 16384;  // columns of the head to a piece of its transposed codes (whole units of them)
+constexpr int kPieceColumns = 16384;  // columns of P at a time, of many rows (whole units of the transposed codes)
 constexpr int kMostTop = 1024;        // entries of a teacher's row
 
 struct TeacherArgs {

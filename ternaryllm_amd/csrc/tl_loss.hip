@@ -12,7 +12,7 @@ using namespace tl;
 namespace {
 
 constexpr int kFewColumns = 128;                 // of a workgroup of tl_loss_few_grad
-constexpr int kRowThreads = 1024;                // of a workgroup that takes a row
+constexpr int kRowThreads = 1024, kJoinThreads = 256;   // of a workgroup that takes a row of logits, of what is left of them
 constexpr float kNone = -__builtin_huge_valf();
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
@@ -144,18 +144,31 @@ __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, 
     if (tid == 0) put_divergence(a, row, lse, gap);
 }
 
+// f(a column's scale), for scales of the call's kind.  (Loads that each ask for the kind are on their way one after the other: they took 30 us of a launch.)
+template <typename F>
+__device__ __forceinline__ void with_scales(const LossArgs& a, F f)
+{
+    if (!a.scale) f([](int) { return 1.0f; });
+    else if (a.scale_f16) f([p = static_cast<const _Float16*>(a.scale)](int n) { return (float)p[n]; });
+    else f([p = static_cast<const float*>(a.scale)](int n) { return p[n]; });
+}
+
 // The largest column scale, by one workgroup, where lse ends: what the gradients' fp16 probabilities are raised by goes by it.
 template <int WAVES>
 __device__ __forceinline__ void put_largest_scale(const LossArgs& a)
 {
+    constexpr int U = 16, THREADS = WAVES * 64;
     float most = a.scale ? 0.f : 1.f;
     bool wrong = false;
-    if (a.scale)
-        for (int n = (int)threadIdx.x; n < a.N; n += WAVES * 64) {
-            const float s = fabsf(load_scale(a.scale, a.scale_f16, n));
-            wrong |= !finite(s);
-            most = fmaxf(most, s);
+    with_scales(a, [&](auto scale) {
+        for (int first = (int)threadIdx.x; first < a.N; first += THREADS * U) {
+            float s[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] = scale(min(first + u * THREADS, a.N - 1));
+#pragma unroll
+            for (int u = 0; u < U; ++u) wrong |= !finite(s[u]), most = fmaxf(most, fabsf(s[u]));
         }
+    });
     most = fold_all<WAVES>(wrong ? __builtin_huge_valf() : most, [](float x, float y) { return fmaxf(x, y); });
     if (threadIdx.x == 0) a.lse[a.M] = most;
 }
@@ -173,19 +186,26 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
     auto z = [&](int n) { return raw[n] * load_scale(a.scale, a.scale_f16, n) * a.cool; };
     float top = kNone, sum = 0.f;
     bool wrong = false;
-    for (int first = tid; first < a.N; first += kRowThreads * U) {
-        float v[U];
+    with_scales(a, [&](auto scale) {
+        for (int first = tid; first < a.N; first += kRowThreads * U) {
+            float v[U], s[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = first + u * kRowThreads < a.N ? z(first + u * kRowThreads) : kNone;
-        float most = v[0];
+            for (int u = 0; u < U; ++u) {
+                const int n = min(first + u * kRowThreads, a.N - 1);
+                v[u] = raw[n], s[u] = scale(n);
+            }
+            float most = kNone, part = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) most = fmaxf(most, v[u]), wrong |= v[u] != v[u];
-        float part = 0.f;
-        const float base = most == kNone ? 0.f : most;
+            for (int u = 0; u < U; ++u) {
+                v[u] = first + u * kRowThreads < a.N ? v[u] * s[u] * a.cool : kNone;
+                most = fmaxf(most, v[u]), wrong |= v[u] != v[u];
+            }
+            const float base = most == kNone ? 0.f : most;
 #pragma unroll
-        for (int u = 0; u < U; ++u) part += __expf(v[u] - base);
-        join(top, sum, most, part);
-    }
+            for (int u = 0; u < U; ++u) part += __expf(v[u] - base);
+            join(top, sum, most, part);
+        }
+    });
     // (a maximum passes over what is not a number; +inf does not count as a maximum either)
     if (wrong) top = __builtin_huge_valf();
     join_all<WAVES>(top, sum);
@@ -193,11 +213,11 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
 }
 
 // Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted.  A workgroup takes a row, one more the scales.
-__global__ __launch_bounds__(256) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
+__global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
 {
     const int row = a.first + (int)blockIdx.x;
     if (row == a.M) {
-        put_largest_scale<4>(a);
+        put_largest_scale<kJoinThreads / 64>(a);
         return;
     }
     const float2* own = parts + (long long)blockIdx.x * count;
@@ -214,14 +234,26 @@ __global__ __launch_bounds__(256) void tl_loss_join(LossArgs a, const float2* pa
     if (threadIdx.x == 0) put_divergence(a, row, lse_of(top, sum), lse_of(top, sum) - gap);
 }
 
-// ds from its parts, rows one after the other; what rows of the call before have left in it is added to.
+// ds from its parts, rows one after the other; what rows of the call before have left in it is added to.  64 columns to a workgroup, whose waves share the
+// parts out.
 __global__ __launch_bounds__(256) void tl_loss_ds(float* ds, const float* parts, int count, long long ld, int N, float heat, int more)
 {
-    const int n = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (n >= N) return;
+    __shared__ float sums[4][64];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, n = (int)blockIdx.x * 64 + lane;
+    constexpr int U = 8;
     float sum = 0.f;
-    for (int i = 0; i < count; ++i) sum += parts[i * ld + n];
-    ds[n] = more ? fmaf(sum, heat, ds[n]) : sum * heat;
+    for (int first = wave; first < count; first += 4 * U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = first + 4 * u < count && n < N ? parts[(first + 4 * u) * ld + n] : 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum += v[u];
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || n >= N) return;
+    sum = (sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]) * heat;
+    ds[n] = more ? ds[n] + sum : sum;
 }
 
 // Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after the other.
@@ -272,16 +304,31 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
     if (a.ds && there) a.ds[n] = ds * a.heat;
 }
 
-// dx = what a row is multiplied by times the product of P, a sum of those of the vocabulary's pieces.
+// dx = what a row is multiplied by times the product of P, the sum of `parts` of them.  A thread takes four values of a row.
 template <typename T>
-__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int pieces)
+__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int rows, int parts)
 {
-    const int m = (int)blockIdx.y, k = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (k >= a.K) return;
-    const float factor = row_factor(a.lse[m], a.grad[m], a.heat, sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f);
-    float sum = 0.f;
-    for (int i = 0; i < pieces; ++i) sum += from[((long long)i * a.M + m) * a.K + k];
-    static_cast<T*>(a.dx)[m * a.dx_ld + k] = (T)settled(lse_counts(a.lse[m]) ? sum * factor : factor);
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int pieces = (a.K + 3) / 4, m = (int)(at / pieces), k = (int)(at % pieces) * 4;
+    if (m >= rows) return;
+    const int row = a.first + m;
+    const float factor = row_factor(a.lse[row], a.grad[row], a.heat, sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f);
+    const bool counts = lse_counts(a.lse[row]);
+    float sum[4] = {};
+    T* to = static_cast<T*>(a.dx) + row * a.dx_ld + k;
+    if (a.K % 4 == 0) {
+        for (int i = 0; i < parts; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(from + ((long long)i * rows + m) * a.K + k);
+            sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+        }
+    } else {
+        for (int i = 0; i < parts; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += k + e < a.K ? from[((long long)i * rows + m) * a.K + k + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (k + e < a.K) to[e] = (T)settled(counts ? sum[e] * factor : factor);
 }
 
 __global__ __launch_bounds__(256) void tl_loss_scale_out(const float* ds, void* out, int f16, int N)
@@ -290,19 +337,14 @@ __global__ __launch_bounds__(256) void tl_loss_scale_out(const float* ds, void* 
     if (n < N) store_out(out, f16, n, ds[n]);
 }
 
-// The codes of a weight [K][N], transposed: for pieces of kPieceColumns columns, one after the other, the codes of a weight of as many rows and K columns.
-// Once for a weight; a thread makes a dword (16 weights).
+// The codes of a weight [K][N], transposed: those of a weight of N rows and K columns.  Once for a weight; a thread makes a dword (16 weights).
 __global__ __launch_bounds__(256) void tl_back_codes(const uint32_t* codes, int K, int N, int planes, uint32_t* out, long long dwords)
 {
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
     if (at >= dwords) return;
-    const int blocks = (K + 15) / 16, units_in = (K + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS;
-    const long long whole = (long long)blocks * planes * (kPieceColumns / TL_CODE_UNIT_ROWS) * (TL_CODE_UNIT_BYTES / 4);   // dwords of a piece
-    const int piece = (int)(at / whole), first = piece * kPieceColumns;
-    const int units = (min(N - first, kPieceColumns) + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS;
-    const long long in = at - piece * whole;
-    const int d = (int)(in & 3), lane = (int)(in >> 2 & 63);
-    const long long unit = in >> 8;
+    const int units_in = (K + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS, units = (N + TL_CODE_UNIT_ROWS - 1) / TL_CODE_UNIT_ROWS;
+    const int d = (int)(at & 3), lane = (int)(at >> 2 & 63);
+    const long long unit = at >> 8;
     const int u = (int)(unit % units), plane = (int)(unit / units % planes), block = (int)(unit / units / planes);
     const int k = block * 16 + (lane & 15);
     uint32_t word = 0;
@@ -311,7 +353,7 @@ __global__ __launch_bounds__(256) void tl_back_codes(const uint32_t* codes, int 
         const int shift = 14 - 2 * (4 * (r >> 5 & 1) + (r >> 1 & 3)) + 16 * (r & 1);
         for (int i = 0; i < 16; ++i) {
             const int h = i >> 3, p = i >> 1 & 3, j = i & 1;
-            const int v = first + u * TL_CODE_UNIT_ROWS + 64 * d + 32 * h + 8 * (lane >> 4) + 2 * p + j;
+            const int v = u * TL_CODE_UNIT_ROWS + 64 * d + 32 * h + 8 * (lane >> 4) + 2 * p + j;
             if (v >= N) continue;
             const long long from = (((long long)(v / 16) * planes + plane) * units_in + k / TL_CODE_UNIT_ROWS) * (TL_CODE_UNIT_BYTES / 4) +
                                    ((r >> 3 & 3) * 16 + v % 16) * 4 + (r >> 6);
@@ -324,12 +366,7 @@ __global__ __launch_bounds__(256) void tl_back_codes(const uint32_t* codes, int 
 // ---------------------------------------------------------------------------
 // Host.
 // ---------------------------------------------------------------------------
-int64_t back_units(const tl_layout_header* h)
-{
-    int64_t units = 0;
-    for (int64_t n = 0; n < (int64_t)h->columns; n += kPieceColumns) units += ceil_div(std::min<int64_t>(h->columns - n, kPieceColumns), TL_CODE_UNIT_ROWS);
-    return units * ceil_div(h->inners, 16) * h->code_planes;
-}
+int64_t back_units(const tl_layout_header* h) { return ceil_div(h->columns, TL_CODE_UNIT_ROWS) * ceil_div(h->inners, 16) * h->code_planes; }
 
 int check_weight(const tl_layout_header* h, const void* blob)
 {
@@ -390,7 +427,7 @@ struct FewParts {
     float* raw;          // [rows][ld]
     void* product;       // workspace of the product of the logits
     void* P;             // backward: [rows][ld]
-    float* sums;         // [pieces][rows][K]
+    float* sums;         // [rows][K]
     float* ds;           // [N]
 };
 
@@ -402,7 +439,7 @@ FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, 
     f.product = p.take(product_bytes);
     if (backward) {
         f.P = p.take(rows * ld * (x_dtype == TL_F16 ? 2 : 4));
-        f.sums = static_cast<float*>(p.take(ceil_div(h->columns, kPieceColumns) * rows * h->inners * 4));
+        f.sums = static_cast<float*>(p.take(rows * h->inners * 4));
         f.ds = static_cast<float*>(p.take((int64_t)h->columns * 4));
     }
     return f;
@@ -414,41 +451,45 @@ int product_workspace(const tl_layout_header* h, int64_t M, int x_dtype, int64_t
     return M ? tl_spmm_workspace(h, M, x_dtype, TL_X_ROW_MAJOR, bytes) : TL_OK;
 }
 
-// The products of P's rows with the pieces of the transposed weight.
-int back_product(const tl_layout_header* h, const void* back, const LossArgs& a, int x_dtype, int rows, float* sums, hipStream_t st)
+void rows_out(const LossArgs& a, int x_dtype, const float* sums, int rows, int parts, hipStream_t st)
+{
+    const dim3 grid((unsigned)ceil_div((int64_t)ceil_div(a.K, 4) * rows, 256));
+    if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, sums, rows, parts);
+    else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, sums, rows, parts);
+}
+
+// The product of few rows of P with the transposed weight.
+int back_product(const tl_layout_header* h, const void* back, const LossArgs& a, int x_dtype, float* sums, hipStream_t st)
 {
     KernelArgs k;
     std::memset(&k, 0, sizeof(k));
-    const int es = x_dtype == TL_F16 ? 2 : 4;
-    const unsigned char* codes = static_cast<const unsigned char*>(back);
-    k.N = (int)h->inners, k.NB = (int)ceil_div(h->inners, 16), k.M = rows;
-    k.planes = (int)h->code_planes;
+    k.X = a.P, k.ldx = a.raw_ld;
+    k.Y = sums, k.ldy = a.K;
+    k.M = a.M, k.N = a.K, k.NB = (int)ceil_div(a.K, 16);
+    k.K = (int)round_up(a.N, 8);                 // (P is padded with zeros, the codes too)
+    k.planes = (int)h->code_planes, k.units = (int)ceil_div(a.N, TL_CODE_UNIT_ROWS);
+    k.c0 = Codes{static_cast<const unsigned char*>(back), k.planes};
     k.x_f16 = x_dtype == TL_F16, k.one = 1.0f;
     k.tile_rows = 1;                             // (T = 0: there is no index stream to walk, and P's sums are finite)
-    k.ldx = a.raw_ld, k.ldy = h->inners;
-    for (int64_t n = 0; n < (int64_t)h->columns; n += kPieceColumns) {
-        const int64_t wide = std::min<int64_t>(h->columns - n, kPieceColumns);
-        k.X = static_cast<const char*>(a.P) + n * es;
-        k.Y = sums + n / kPieceColumns * rows * (int64_t)h->inners;
-        k.K = (int)round_up(wide, 8);            // (P is padded with zeros, the codes too)
-        k.units = (int)ceil_div(wide, TL_CODE_UNIT_ROWS);
-        k.c0 = Codes{codes, k.planes};
-        if (int rc = launch_matrix_few(k, x_dtype, false, st)) return rc;
-        codes += (int64_t)k.NB * k.planes * k.units * TL_CODE_UNIT_BYTES;
-    }
-    return TL_OK;
+    return launch_matrix_few(k, x_dtype, false, st);
 }
 
 // Many rows: so many at a time, and what the workspace holds for them.
 constexpr int64_t kForwardRows = 16384;
 constexpr int64_t kGradientBytes = 128 << 20;    // of P, and of its image
 
-int64_t piece_columns(const tl_layout_header* h) { return std::min<int64_t>(h->columns, kPieceColumns); }
+// Rows and columns of P at a time.  All columns where all rows of them fit; else pieces of the vocabulary, and as many rows as fit of those.  (Of a weight whose
+// rows repeat all columns in any case: its planes of codes are walked one after the other.)
+struct PieceOfP {
+    int64_t rows, columns;
+};
 
-int64_t backward_rows(const tl_layout_header* h, int64_t M, int x_dtype)
+PieceOfP piece_of_p(const tl_layout_header* h, int64_t M, int x_dtype)
 {
-    const int64_t rows = kGradientBytes / (round_up(piece_columns(h), 64) * (x_dtype == TL_F16 ? 2 : 4 + 6));
-    return std::min(M, std::min(kForwardRows, std::max<int64_t>(rows / 128 * 128, 128)));
+    const int64_t each = x_dtype == TL_F16 ? 2 : 6, all = round_up(h->columns, 64);
+    const bool whole = h->code_planes > 1 || all <= kPieceColumns || std::min(M, kForwardRows) * all * each <= kGradientBytes;
+    const int64_t columns = whole ? all : kPieceColumns;
+    return PieceOfP{std::min(M, std::min(kForwardRows, std::max<int64_t>(kGradientBytes / (columns * each) / 128 * 128, 128))), columns};
 }
 
 struct ManyParts {
@@ -456,15 +497,30 @@ struct ManyParts {
     void* image;         // of the rows of x
     float2* parts;       // forward: [rows][columns / 64 or 32]
     float *gaps, *picks;
-    void *P, *P_image;   // backward: [rows][piece]
-    float *sums, *ds_parts, *ds;
+    int64_t columns;     // backward: of P
+    int splits;          // workgroups that share out the columns of P for an output of their product
+    void* P;             // [rows][columns]; of fp32 rows in three bf16 parts
+    float *sums;         // [pieces * splits][rows][K], or, of one split, [rows][K]; null: neither
+    float *ds_parts, *ds;
 };
+
+KernelArgs back_args(const tl_layout_header* h, int x_dtype, int rows)
+{
+    KernelArgs b;
+    std::memset(&b, 0, sizeof(b));
+    b.M = b.call_rows = rows, b.N = (int)h->inners, b.NB = (int)ceil_div(h->inners, 16);
+    b.planes = (int)h->code_planes, b.units = (int)ceil_div(h->columns, TL_CODE_UNIT_ROWS);
+    b.x_f16 = x_dtype == TL_F16, b.one = 1.0f, b.tile_rows = 1;
+    return b;
+}
+
 
 ManyParts many_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, bool backward)
 {
-    const int64_t N = h->columns, K = h->inners, piece = round_up(piece_columns(h), 64);
+    const int64_t N = h->columns, K = h->inners;
+    const PieceOfP piece = piece_of_p(h, M, x_dtype);
     ManyParts f{};
-    f.rows = backward ? backward_rows(h, M, x_dtype) : std::min(M, kForwardRows);
+    f.rows = backward ? piece.rows : std::min(M, kForwardRows);
     f.image = p.take(loss_image_bytes(K, f.rows, x_dtype));
     if (!backward) {
         const int64_t count = f.rows * ceil_div(N, x_dtype == TL_F16 ? 64 : 32);
@@ -473,10 +529,12 @@ ManyParts many_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype
         f.picks = static_cast<float*>(p.take(f.rows * 4));
         return f;
     }
-    f.P = p.take(f.rows * piece * (x_dtype == TL_F16 ? 2 : 4));
-    f.P_image = x_dtype == TL_F16 ? nullptr : p.take(loss_image_bytes(piece, f.rows, x_dtype));
-    f.sums = N > kPieceColumns ? static_cast<float*>(p.take(f.rows * K * 4)) : nullptr;
-    f.ds_parts = static_cast<float*>(p.take(ceil_div(f.rows, 32) * piece * 4));
+    f.columns = piece.columns;
+    f.splits = loss_splits(back_args(h, x_dtype, (int)f.rows), x_dtype, (int)ceil_div(std::min(f.columns, N), TL_CODE_UNIT_ROWS));
+    const int64_t pieces = ceil_div(N, f.columns);
+    f.P = p.take(f.rows * f.columns * (x_dtype == TL_F16 ? 2 : 6));
+    f.sums = pieces * f.splits > 1 ? static_cast<float*>(p.take((f.splits > 1 ? pieces * f.splits : 1) * f.rows * K * 4)) : nullptr;
+    f.ds_parts = static_cast<float*>(p.take(ceil_div(f.rows, 32) * f.columns * 4));
     f.ds = static_cast<float*>(p.take(N * 4));
     return f;
 }
@@ -511,7 +569,7 @@ int many_forward(const tl_layout_header* h, const void* blob, const void* x, int
         k.loss.parts = f.parts, k.loss.gaps = f.gaps, k.loss.picks = f.picks;
         if (int rc = launch_loss(k, x_dtype, kLossLogits, st)) return rc;
         a.first = (int)m;
-        hipLaunchKernelGGL(tl_loss_join, dim3((unsigned)(rows + (m + rows == a.M))), dim3(256), 0, st, a, f.parts, f.gaps, f.picks,
+        hipLaunchKernelGGL(tl_loss_join, dim3((unsigned)(rows + (m + rows == a.M))), dim3(kJoinThreads), 0, st, a, f.parts, f.gaps, f.picks,
                            (int)ceil_div(a.N, loss_part(k, x_dtype, kLossLogits)));
     }
     return TL_OK;
@@ -520,42 +578,44 @@ int many_forward(const tl_layout_header* h, const void* blob, const void* x, int
 int many_backward(const tl_layout_header* h, const void* blob, const void* back, const void* x, int x_dtype, int64_t ldx, const LossArgs& a, const ManyParts& f,
                   hipStream_t st)
 {
-    const int es = x_dtype == TL_F16 ? 2 : 4, planes = (int)h->code_planes;
-    const int64_t blocks = ceil_div(a.K, 16);
+    const int es = x_dtype == TL_F16 ? 2 : 4, planes = (int)h->code_planes, pieces = (int)ceil_div(a.N, f.columns);
     for (int64_t m = 0; m < a.M; m += f.rows) {
         const int rows = (int)std::min<int64_t>(a.M - m, f.rows);
         KernelArgs k = rows_product(h, blob, x, x_dtype, ldx, m, rows, a);
         if (int rc = make_loss_image(&k, x_dtype, f.image, st)) return rc;
         k.loss.lse = a.lse + m, k.loss.grad = a.grad + m, k.loss.largest = x_dtype == TL_F16 ? a.lse + a.M : nullptr;
-        const unsigned char* codes = static_cast<const unsigned char*>(back);
-        for (int64_t n = 0; n < a.N; n += kPieceColumns) {
-            const int64_t wide = std::min<int64_t>(a.N - n, kPieceColumns), units = ceil_div(wide, TL_CODE_UNIT_ROWS), padded = round_up(wide, 8);
+        KernelArgs b = back_args(h, x_dtype, rows);
+        b.c0 = Codes{static_cast<const unsigned char*>(back), planes};
+        b.loss = k.loss;
+        b.loss.splits = f.splits;
+        for (int piece = 0; piece < pieces; ++piece) {
+            const int64_t n = piece * f.columns, wide = std::min<int64_t>(a.N - n, f.columns), padded = round_up(wide, 8);
             KernelArgs some = k;
             some.N = (int)wide, some.NB = (int)ceil_div(wide, 16);
             some.c0.base += n / 16 * planes * k.units * TL_CODE_UNIT_BYTES;
             if (a.scale) some.w0.scale = static_cast<const char*>(a.scale) + n * (a.scale_f16 ? 2 : 4);
-            some.Y = f.P, some.y_f16 = k.x_f16, some.ldy = round_up(wide, 64);
-            some.loss.first = (int)n, some.loss.padded = (int)padded;
-            some.loss.ds = a.ds ? f.ds_parts : nullptr, some.loss.ds_ld = some.ldy;
+            some.Y = f.P, some.y_f16 = 1, some.ldy = f.columns;
+            some.loss.first = (int)n, some.loss.padded = (int)padded, some.loss.plane = f.rows * f.columns;
+            some.loss.ds = a.ds ? f.ds_parts : nullptr, some.loss.ds_ld = f.columns;
             if (int rc = launch_loss(some, x_dtype, kLossGradients, st)) return rc;
             if (a.ds)
-                hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 256)), dim3(256), 0, st, a.ds + n, f.ds_parts,
+                hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 64)), dim3(256), 0, st, a.ds + n, f.ds_parts,
                                    (int)ceil_div(rows, loss_part(some, x_dtype, kLossGradients)), some.loss.ds_ld, (int)wide, a.heat, (int)(m > 0));
             if (!a.dx) continue;
-            const bool last = n + wide == a.N;
-            KernelArgs b;
-            std::memset(&b, 0, sizeof(b));
-            b.X = f.P, b.ldx = some.ldy;
-            b.M = b.call_rows = rows, b.N = a.K, b.K = (int)padded, b.NB = (int)blocks;
-            b.c0 = Codes{codes, planes}, b.units = (int)units, b.planes = planes;
-            b.x_f16 = k.x_f16, b.one = 1.0f, b.tile_rows = 1;
-            if (int rc = make_loss_image(&b, x_dtype, f.P_image, st)) return rc;
-            b.loss = k.loss;
-            b.loss.sums = n > 0 ? f.sums : nullptr, b.loss.last = last;
-            b.Y = last ? static_cast<char*>(a.dx) + m * a.dx_ld * es : static_cast<void*>(f.sums);
+            // (rows of P begin with column n, those of the transposed weight with column 0: pointers meet where they would be)
+            b.K = (int)(n + padded);
+            b.image = static_cast<const char*>(f.P) - n * 2, b.image_ld = f.columns, b.image_plane = some.loss.plane;
+            b.loss.unit0 = (int)(n / TL_CODE_UNIT_ROWS), b.loss.units = planes > 1 ? planes * b.units : (int)ceil_div(wide, TL_CODE_UNIT_ROWS);
+            const bool last = f.splits == 1 && piece + 1 == pieces;
+            b.loss.sums = f.splits == 1 && piece > 0 ? f.sums : nullptr, b.loss.last = last;
+            b.Y = last ? static_cast<char*>(a.dx) + m * a.dx_ld * es : reinterpret_cast<char*>(f.sums + (int64_t)(f.splits == 1 ? 0 : piece * f.splits) * rows * a.K);
             b.y_f16 = last && k.x_f16, b.ldy = last ? a.dx_ld : a.K;
             if (int rc = launch_loss(b, x_dtype, kLossBack, st)) return rc;
-            codes += blocks * planes * units * TL_CODE_UNIT_BYTES;
+        }
+        if (a.dx && f.splits > 1) {
+            LossArgs some = a;
+            some.first = (int)m;
+            rows_out(some, x_dtype, f.sums, rows, pieces * f.splits, st);
         }
     }
     return TL_OK;
@@ -694,15 +754,12 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
         a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
         a.P = f.P;
         const dim3 groups((unsigned)ceil_div(a.raw_ld, kFewColumns));
-        const int rows = (int)M, pieces = (int)ceil_div(header->columns, kPieceColumns);
         if (int rc = raw_product(header, blob_dev, x, x_dtype, ldx, a, f, product, stream)) return rc;
         if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_few_grad<_Float16>, groups, dim3(kFewColumns), 0, st, a);
         else hipLaunchKernelGGL(tl_loss_few_grad<float>, groups, dim3(kFewColumns), 0, st, a);
         if (dx) {
-            if (int rc = back_product(header, back, a, x_dtype, rows, f.sums, st)) return rc;
-            const dim3 grid((unsigned)ceil_div(header->inners, 256), (unsigned)rows);
-            if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, f.sums, pieces);
-            else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, f.sums, pieces);
+            if (int rc = back_product(header, back, a, x_dtype, f.sums, st)) return rc;
+            rows_out(a, x_dtype, f.sums, a.M, 1, st);
         }
     }
     if (dscale && scale_dtype == TL_F16)

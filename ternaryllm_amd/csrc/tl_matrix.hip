@@ -157,6 +157,23 @@ __device__ __forceinline__ void lanes_meet()
 constexpr int kTeacherRows = 32;                                  // of a wave's, whose teacher's shares stand in LDS at a time
 constexpr int teacher_ld(int columns) { return columns + 4; }
 
+// COUNT neighbouring values of row m from column n on, of which whole pieces of eight are there, in the three bf16 parts of an image.
+template <int COUNT>
+__device__ __forceinline__ void store_parts(const KernelArgs& a, int m, int n, const float* v)
+{
+    static_assert(COUNT % 4 == 0);
+    unsigned short* to = static_cast<unsigned short*>(a.Y) + (long long)m * a.ldy + n;
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 4) {
+        uint32_t part[4][3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split3(v[i + e], &part[e][0], &part[e][1], &part[e][2]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            *reinterpret_cast<uint2*>(to + p * a.loss.plane + i) = make_uint2((part[0][p] >> 16) | part[1][p], (part[2][p] >> 16) | part[3][p]);
+    }
+}
+
 // The last steps of a head's losses (put_out's arguments; own: LDS of the wave's own, kTeacherRows * teacher_ld floats of it, once every wave of the
 // workgroup is done with its buffers).  A row's logits lie with four lanes; a wave leaves their maximum and sum for its columns.  Its teacher's entries are
 // few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.
@@ -170,6 +187,8 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
     const int first_n = lane_n0 - q * C, first_m = lane_m0 - r16;
     if constexpr (MODE == kBack) {
         const float raised = l.largest ? raise_of(*l.largest) : 1.f;
+        KernelArgs to = a;                                        // (of several parts each has its own)
+        if (l.splits > 1) to.Y = static_cast<float*>(a.Y) + (long long)blockIdx.y * a.M * a.ldy;
 #pragma unroll
         for (int m = 0; m < G; ++m) {
             const int row = lane_m0 + m * 16;
@@ -190,7 +209,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                     v[i] = fmaf(acc[group * CF + i / 4][m][i % 4], 0.5f, before[i]);   // (the products are with +-2)
                     if (l.last) v[i] = counts ? v[i] * factor : factor;
                 }
-                store_piece<C>(a, row, n, a.N, v);
+                store_piece<C>(to, row, n, a.N, v);
             }
         }
         return;
@@ -298,7 +317,9 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                     p[i] = dz * s[group][i] * up;
                     ds[group][i] += counts ? dz * raw * grad : lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
                 }
-                if (n < l.padded) store_piece<C>(to, row, n, l.padded, p);
+                if (n >= l.padded) continue;
+                if (a.x_f16) store_piece<C>(to, row, n, l.padded, p);
+                else store_parts<C>(to, row, n, p);
             }
         }
     }
@@ -481,7 +502,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArg
     const int stages_k = (a.K + kStageRows - 1) / kStageRows;     // stages of K that hold anything
     const int all_units = a.planes * a.units;
     // this wave's units, and its turns: the last stage of the only plane may end a unit early
-    const int unit0 = all_units * wk / WK, units = all_units * (wk + 1) / WK - unit0;
+    int part0 = 0, part_units = all_units;                        // (kBack: a workgroup has a part of K)
+    if constexpr (MODE == kBack) {
+        part0 = a.loss.unit0 + a.loss.units * (int)blockIdx.y / (int)gridDim.y;
+        part_units = a.loss.unit0 + a.loss.units * ((int)blockIdx.y + 1) / (int)gridDim.y - part0;
+    }
+    const int unit0 = part0 + part_units * wk / WK, units = part0 + part_units * (wk + 1) / WK - unit0;
     const int all_stages = a.planes == 1 ? stages_k : all_units * kUnitStages;
     auto turns_of = [&](int first, int count) { return PARTS * (min((first + count) * kUnitStages, all_stages) - first * kUnitStages); };
     const int total = turns_of(unit0, units);
@@ -635,7 +661,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArg
     if constexpr (SHARED && WK > 1) {
         int most = 0;
 #pragma unroll
-        for (int o = 0; o < WK; ++o) most = max(most, turns_of(all_units * o / WK, all_units * (o + 1) / WK - all_units * o / WK));
+        for (int o = 0; o < WK; ++o) most = max(most, turns_of(part0 + part_units * o / WK, part_units * (o + 1) / WK - part_units * o / WK));
         for (int i = max(total, 1); i < most; ++i) __builtin_amdgcn_s_barrier();
     }
 
@@ -967,7 +993,7 @@ int launch_tile(const KernelArgs& a, hipStream_t st)
     static LdsLimit raised;
     if (int rc = raised.raise(kernel, lds)) return rc;
     const int64_t tiles = ceil_div(a.M, TM) * ceil_div(a.N, OUT_TN);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(WM * WN * WK * 64), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, MODE == kBack ? (unsigned)a.loss.splits : 1u), dim3(WM * WN * WK * 64), lds, st, a);
     return TL_OK;
 }
 
@@ -1191,6 +1217,16 @@ int tl::loss_part(const KernelArgs& a, int x_dtype, LossProduct what)
     const MatrixTile tile = loss_tile(a, x_dtype != TL_F16);
     if (what == kLossLogits) return tile == kWide ? 32 : 64;
     return tile == kTall ? 128 : tile == kHalves ? 32 : 64;
+}
+
+// A product of fewer tiles than the device holds two to a unit is split along K, into parts of four units at least, eight at most (whose sums are another
+// pass over the result in fp32 each).
+int tl::loss_splits(const KernelArgs& a, int x_dtype, int units)
+{
+    const MatrixTile tile = loss_tile(a, x_dtype != TL_F16);
+    const int64_t height = tile == kTall ? 128 : 64, width = tile == kHalves || tile == kWide ? 128 : 256;
+    const int64_t tiles = ceil_div(a.M, height) * ceil_div(a.N, width);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * compute_units() / tiles, a.planes * (int64_t)units / 4), 8));
 }
 
 int tl::launch_loss(KernelArgs a, int x_dtype, LossProduct what, hipStream_t st)
