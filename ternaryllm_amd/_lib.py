@@ -196,10 +196,12 @@ def binding(workspaces):
         except ImportError as e:
             raise RuntimeError("ternaryllm_amd/_tl_torch.so is missing or does not load: build it with `python -m ternaryllm_amd.build`. "
                                "There is no fallback path.") from e
-        address = [ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
-                   for name in ("tl_spmm", "tl_spmm_workspace", "tl_mlp_gate_up", "tl_mlp_gate_up_few", "tl_rope_heads", "tl_rope_to_pages",
-                                "tl_read_pages", "tl_paged_attention_workspace", "tl_paged_attention")]
-        _tl_torch.init(*address, workspaces)
+        address = tuple(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
+                        for name in ("tl_spmm", "tl_spmm_workspace", "tl_mlp_gate_up", "tl_mlp_gate_up_few", "tl_rope_heads", "tl_rope_to_pages",
+                                     "tl_read_pages", "tl_paged_attention_workspace", "tl_paged_attention", "tl_paged_attention_shared_workspace",
+                                     "tl_paged_attention_shared", "tl_teacher_entries", "tl_head_loss_workspace", "tl_head_loss", "tl_head_loss_backward",
+                                     "tl_last_error"))
+        _tl_torch.init(address, workspaces)
         _binding = _tl_torch
     return _binding
 

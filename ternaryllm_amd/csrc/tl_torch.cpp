@@ -12,9 +12,14 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <cmath>
+#include <mutex>
 
 #include "ternary_spmm.h"
 
@@ -30,6 +35,13 @@ decltype(&tl_rope_to_pages) g_rope_to_pages;
 decltype(&tl_read_pages) g_read_pages;
 decltype(&tl_paged_attention_workspace) g_attention_workspace;
 decltype(&tl_paged_attention) g_attention;
+decltype(&tl_paged_attention_shared_workspace) g_shared_workspace;
+decltype(&tl_paged_attention_shared) g_shared;
+decltype(&tl_teacher_entries) g_teacher;
+decltype(&tl_head_loss_workspace) g_loss_workspace;
+decltype(&tl_head_loss) g_loss;
+decltype(&tl_head_loss_backward) g_loss_backward;
+decltype(&tl_last_error) g_last_error;
 PyObject* g_workspaces;  // {(device index, stream): uint8 tensor}: the scratch of ops
 
 int type_code(const at::Tensor& t)
@@ -383,12 +395,24 @@ PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t count)
     END_HANDLE_TH_ERRORS
 }
 
-// paged_attention(q, pages, batch, scale or None, out or None) -> out or None
+// Groups of the batch's sequences that begin alike; false where they are none of a plain call.
+bool prefix_of(PyObject* prefix, const tl_page_batch& b, c10::Device device, tl_page_prefix* p)
+{
+    if (!PyTuple_Check(prefix) || PyTuple_GET_SIZE(prefix) != 2) return false;
+    const at::Tensor *groups = member(prefix, 0), *shared = member(prefix, 1);
+    for (const at::Tensor* t : {groups, shared})
+        if (!t || t->scalar_type() != at::kInt || t->device() != device || t->numel() == 0 || t->dim() != 1 || !t->is_contiguous()) return false;
+    if (shared->numel() != b.seqs || groups->numel() > INT32_MAX) return false;
+    *p = tl_page_prefix{static_cast<const int32_t*>(groups->data_ptr()), static_cast<const int32_t*>(shared->data_ptr()), (int32_t)(groups->numel() - 1)};
+    return true;
+}
+
+// paged_attention(q, pages, batch, scale or None, out or None, prefix or None) -> out or None
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
 {
     HANDLE_TH_ERRORS
-    if (count != 5) {
-        PyErr_SetString(PyExc_TypeError, "paged_attention takes five arguments");
+    if (count != 6) {
+        PyErr_SetString(PyExc_TypeError, "paged_attention takes six arguments");
         return nullptr;
     }
     const at::Tensor* q = plain(a[0]);
@@ -409,30 +433,207 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count)
     if (!absent(a[4]) && (!given || given->dim() != 2 || given->size(0) != tokens || given->size(1) != width || given->scalar_type() != at::kHalf ||
                           given->device() != q->device() || !given->is_contiguous() || differentiated({given}) || given->storage().data() == q->storage().data()))
         Py_RETURN_NONE;
-    if (g_attention_workspace(tokens, (int)q->size(1), &p, &b, most, &need) != TL_OK) Py_RETURN_NONE;
+    tl_page_prefix prefix;
+    const bool grouped = !absent(a[5]);
+    if (grouped && !prefix_of(a[5], b, q->device(), &prefix)) Py_RETURN_NONE;
+    if ((grouped ? g_shared_workspace(tokens, (int)q->size(1), &p, &b, &prefix, most, &need)
+                 : g_attention_workspace(tokens, (int)q->size(1), &p, &b, most, &need)) != TL_OK)
+        Py_RETURN_NONE;
     at::Tensor out = given ? *given : at::empty({tokens, width}, q->options().requires_grad(false));
     at::Tensor ws = at::empty({need}, q->options().dtype(at::kByte).requires_grad(false));
     void* stream = current_stream(q->device());
     int rc;
     {
         const pybind11::gil_scoped_release no_gil;
-        rc = g_attention(q->data_ptr(), step(*q, 0), step(*q, 1), TL_F16, tokens, (int)q->size(1), &p, &b, most, (float)scale, out.data_ptr(), ws.data_ptr(), need,
-                         stream);
+        if (grouped) {
+            rc = g_shared(q->data_ptr(), step(*q, 0), step(*q, 1), TL_F16, tokens, (int)q->size(1), &p, &b, &prefix, most, (float)scale, out.data_ptr(),
+                          ws.data_ptr(), need, stream);
+        } else {
+            rc = g_attention(q->data_ptr(), step(*q, 0), step(*q, 1), TL_F16, tokens, (int)q->size(1), &p, &b, most, (float)scale, out.data_ptr(), ws.data_ptr(),
+                             need, stream);
+        }
     }
     if (rc != TL_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
 
+// ---- a head's losses.  Forty rows' loss and gradients took the host 184 us through an autograd function of Python's, for 100 us of kernels.
+
+// What is wanted of the rows: targets, or a teacher's entries (and what those were made into).
+struct Wanted {
+    at::Tensor targets, entries, shares, known;
+    int64_t ignore = 0;
+    float temperature = 1.f;
+    tl_loss_target call() const
+    {
+        if (targets.defined()) return tl_loss_target{static_cast<const int64_t*>(targets.data_ptr()), ignore, nullptr, nullptr, nullptr, 1, 1.f};
+        return tl_loss_target{nullptr, 0, static_cast<const int32_t*>(entries.data_ptr()), static_cast<const float*>(shares.data_ptr()),
+                              static_cast<const float*>(known.data_ptr()), (int32_t)entries.size(1), temperature};
+    }
+};
+
+int64_t row_step(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : std::max<int64_t>(x.size(1), 1); }
+
+at::Tensor bytes_on(const at::Tensor& like, int64_t bytes) { return at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false)); }
+
+// The backward pass of a loss, once.
+struct HeadLossBackward : torch::autograd::Node {
+    tl_layout_header header;
+    at::Tensor blob, codes, lse;
+    Wanted wanted;                         // (its targets are `targets`, whose later changes are noticed)
+    torch::autograd::SavedVariable x_, scale_, targets_;
+    bool has_scale, has_targets;
+    std::mutex mutex_;
+
+    std::string name() const override { return "HeadLossBackward"; }
+
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data(), scale_.reset_data(), targets_.reset_data();
+        lse.reset();
+        wanted = Wanted();
+    }
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list out(2);
+        if (!grads[0].defined()) return out;
+        const at::Tensor x = x_.unpack(), scale = has_scale ? scale_.unpack() : at::Tensor();   // (raises if they were changed or are gone)
+        Wanted w = wanted;
+        if (has_targets) w.targets = targets_.unpack();
+        at::Tensor dx, ds;
+        {
+            const at::AutoGradMode no_grad(false);
+            const c10::DeviceGuard guard(x.device());
+            const at::Tensor grad = grads[0].detach().to(at::kFloat).contiguous();
+            if (task_should_compute_output(0)) dx = at::empty(x.sizes(), x.options().requires_grad(false));
+            if (has_scale && task_should_compute_output(1)) ds = at::empty(scale.sizes(), scale.options().requires_grad(false));
+            const tl_loss_target target = w.call();
+            const int type = type_code(x);
+            int64_t need = 0;
+            TORCH_CHECK(g_loss_workspace(&header, x.size(0), type, &target, 1, &need) == TL_OK, g_last_error());
+            const at::Tensor ws = bytes_on(x, need);
+            TORCH_CHECK(g_loss_backward(&header, blob.data_ptr(), codes.defined() ? codes.data_ptr() : nullptr, x.data_ptr(), type, row_step(x), x.size(0),
+                                        has_scale ? scale.data_ptr() : nullptr, has_scale ? type_code(scale) : TL_F32, &target,
+                                        static_cast<const float*>(lse.data_ptr()), static_cast<const float*>(grad.data_ptr()),
+                                        dx.defined() ? dx.data_ptr() : nullptr, x.size(1), ds.defined() ? ds.data_ptr() : nullptr, ws.data_ptr(), need,
+                                        current_stream(x.device())) == TL_OK,
+                        g_last_error());
+        }
+        if (c10::GradMode::is_enabled()) {     // (a graph of the gradients is asked for: they have none, which whoever follows it is told)
+            const auto once = std::make_shared<torch::autograd::DelayedError>("the losses of a head are differentiable once", 2);
+            auto ends = (*once)({dx, ds});
+            dx = ends[0], ds = ends[1];
+        }
+        out[0] = dx, out[1] = ds;
+        return out;
+    }
+};
+
+// head_loss(header address, blob, transposed codes or None, x, scale or None, targets or None, ignore, ids or None, logits or None, temperature)
+// -> losses, None for a call that is not a plain one, or the library's status
+PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t count)
+{
+    HANDLE_TH_ERRORS
+    if (count != 10) {
+        PyErr_SetString(PyExc_TypeError, "head_loss takes ten arguments");
+        return nullptr;
+    }
+    const tl_layout_header* header = header_at(a[0]);
+    const at::Tensor *blob = plain(a[1]), *codes = absent(a[2]) ? nullptr : plain(a[2]), *x = plain(a[3]), *scale;
+    const double temperature = PyFloat_AsDouble(a[9]);
+    const long long ignore = PyLong_AsLongLong(a[6]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (!header || !blob || !x || (!absent(a[2]) && (!codes || codes->device() != blob->device())) || x->device() != blob->device() || type_code(*x) < 0 ||
+        x->dim() != 2 || x->size(0) == 0 || x->size(1) != header->inners || (x->size(1) > 1 && x->stride(1) != 1) || row_step(*x) < x->size(1) ||
+        !scale_fits(a[4], &scale, header->columns, x->device()) || (scale && scale->dim() != 1))
+        Py_RETURN_NONE;
+    const int64_t rows = x->size(0);
+    const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    const bool by_x = backward && x->requires_grad(), by_scale = backward && scale && scale->requires_grad();
+    if ((by_x && !codes) || (forward && (x->_fw_grad(0).defined() || (scale && scale->_fw_grad(0).defined())))) Py_RETURN_NONE;
+    Wanted wanted;
+    const at::Tensor *ids = nullptr, *logits = nullptr;
+    if (!absent(a[5])) {
+        const at::Tensor* t = plain(a[5]);
+        if (!t || t->dim() != 1 || t->size(0) != rows || t->scalar_type() != at::kLong || t->device() != x->device() || !t->is_contiguous()) Py_RETURN_NONE;
+        wanted.targets = *t;
+        wanted.ignore = ignore;
+    } else {
+        ids = plain(a[7]), logits = plain(a[8]);
+        if (!ids || !logits || ids->dim() != 2 || ids->size(0) != rows || ids->size(1) == 0 || logits->sizes() != ids->sizes() || ids->scalar_type() != at::kLong ||
+            type_code(*logits) < 0 || ids->device() != x->device() || logits->device() != x->device() || differentiated({logits}))
+            Py_RETURN_NONE;
+        for (const at::Tensor* t : {ids, logits})
+            if ((t->size(1) > 1 && t->stride(1) != 1) || row_step(*t) < t->size(1)) Py_RETURN_NONE;
+    }
+    const c10::DeviceGuard guard(x->device());
+    void* stream = current_stream(x->device());
+    const auto floats = x->options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor loss = at::empty({rows}, floats), lse = at::empty({rows + 1}, floats);
+    const int type = type_code(*x);
+    int rc = TL_OK;
+    if (ids) {
+        wanted.entries = at::empty(ids->sizes(), floats.dtype(at::kInt));
+        wanted.shares = at::empty(ids->sizes(), floats);
+        wanted.known = at::empty({rows}, floats);
+        wanted.temperature = (float)temperature;
+        rc = g_teacher(static_cast<const int64_t*>(ids->data_ptr()), row_step(*ids), logits->data_ptr(), type_code(*logits), row_step(*logits), rows,
+                       (int)ids->size(1), (int)header->columns, (float)temperature, static_cast<int32_t*>(wanted.entries.data_ptr()),
+                       static_cast<float*>(wanted.shares.data_ptr()), static_cast<float*>(wanted.known.data_ptr()), stream);
+    }
+    if (rc == TL_OK) {
+        const tl_loss_target target = wanted.call();
+        int64_t need = 0;
+        rc = g_loss_workspace(header, rows, type, &target, 0, &need);
+        if (rc == TL_OK) {
+            const at::Tensor ws = bytes_on(*x, need);
+            const pybind11::gil_scoped_release no_gil;
+            rc = g_loss(header, blob->data_ptr(), x->data_ptr(), type, row_step(*x), rows, scale ? scale->data_ptr() : nullptr, scale ? type_code(*scale) : TL_F32,
+                        &target, static_cast<float*>(loss.data_ptr()), static_cast<float*>(lse.data_ptr()), ws.data_ptr(), need, stream);
+        }
+    }
+    if (rc != TL_OK) return PyLong_FromLong(rc);
+    if (by_x || by_scale) {
+        const std::shared_ptr<HeadLossBackward> node(new HeadLossBackward(), torch::autograd::deleteNode);
+        node->header = *header;
+        node->blob = *blob, node->lse = lse;
+        if (codes) node->codes = *codes;
+        node->x_ = torch::autograd::SavedVariable(*x, false);
+        node->has_scale = scale != nullptr;
+        if (scale) node->scale_ = torch::autograd::SavedVariable(*scale, false);
+        node->has_targets = wanted.targets.defined();
+        if (node->has_targets) node->targets_ = torch::autograd::SavedVariable(wanted.targets, false);
+        node->wanted = wanted;
+        node->wanted.targets.reset();
+        node->set_next_edges(torch::autograd::collect_next_edges(*x, scale ? *scale : at::Tensor()));
+        torch::autograd::set_history(loss, node);
+    }
+    return THPVariable_Wrap(std::move(loss));
+    END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the library's entry points in the order of g_*, the scratch dict)
 PyObject* init(PyObject*, PyObject* args)
 {
-    PyObject *at[9], *dict;
-    if (!PyArg_ParseTuple(args, "OOOOOOOOOO!", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8], &PyDict_Type, &dict)) return nullptr;
-    int i = 0;
-    auto take = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(PyLong_AsVoidPtr(at[i++])); };
+    PyObject *addresses, *dict;
+    constexpr Py_ssize_t kEntries = 16;
+    if (!PyArg_ParseTuple(args, "O!O!", &PyTuple_Type, &addresses, &PyDict_Type, &dict)) return nullptr;
+    if (PyTuple_GET_SIZE(addresses) != kEntries) {
+        PyErr_SetString(PyExc_TypeError, "init takes the address of each entry point");
+        return nullptr;
+    }
+    Py_ssize_t i = 0;
+    auto take = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, i++))); };
     take(g_spmm), take(g_workspace), take(g_gate_up), take(g_gate_up_few);
     take(g_rope_heads), take(g_rope_to_pages), take(g_read_pages), take(g_attention_workspace), take(g_attention);
+    take(g_shared_workspace), take(g_shared), take(g_teacher), take(g_loss_workspace), take(g_loss), take(g_loss_backward), take(g_last_error);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(dict);
     g_workspaces = dict;
@@ -447,6 +648,7 @@ PyMethodDef g_methods[] = {
     {"rope_to_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope_to_pages)), METH_FASTCALL, "the same into pages, or None"},
     {"read_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(read_pages)), METH_FASTCALL, "rows out of pages, or None"},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, "attention over pages, or None"},
+    {"head_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(head_loss)), METH_FASTCALL, "what a head's rows are worth, None, or a status"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tl_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -857,10 +857,9 @@ def paged_attention(q, pages, batch, *, scale=None, out=None, prefix=None):
     128 or 256, kv_heads a divisor of heads; scale: of the scores, 1 / sqrt(head_dim).  Rows of 8 bits are taken as the float16 values that read_pages
     gives.  prefix: a PagePrefix, whose shared tokens are read once for all rows of their group: the same results, up to the rounding of sums (rows of which it
     does not hold may be NaN)."""
-    if prefix is None:
-        y = _short().paged_attention(q, pages, batch, scale, out)
-        if y is not None:
-            return y
+    y = _short().paged_attention(q, pages, batch, scale, out, prefix)
+    if y is not None:
+        return y
     _forward_only(q, pages.k, pages.v, out)
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with unit last stride")
@@ -1123,73 +1122,17 @@ class BackWeight:
             _lib.check(_lib.lib().tl_back_codes_make(ctypes.byref(weight.header), weight.blob.data_ptr(), self.codes.data_ptr(), _stream_ptr(weight.device)))
 
 
-class _Wanted(NamedTuple):
-    """What is wanted of the rows' distributions: targets, or a teacher's entries, their shares and what is known of them (tl_teacher_entries)."""
-    targets: Optional[torch.Tensor]
-    ignore: int
-    entries: Optional[torch.Tensor]
-    shares: Optional[torch.Tensor]
-    known: Optional[torch.Tensor]
-    temperature: float
-
-    def call(self):
-        if self.targets is not None:
-            return _lib.LossTarget(self.targets.data_ptr(), self.ignore, None, None, None, 1, 1.0)
-        return _lib.LossTarget(None, 0, self.entries.data_ptr(), self.shares.data_ptr(), self.known.data_ptr(), self.entries.shape[1], self.temperature)
+def _loss(weight, x, scale, back, targets, ignore, ids, logits, temperature):
+    return _short().head_loss(ctypes.addressof(weight.header), weight.blob, None if back is None else back.codes, x, scale, targets, ignore, ids, logits, temperature)
 
 
-def _loss_workspace(header, rows, code, target, backward, device):
-    need = ctypes.c_int64(0)
-    _lib.check(_lib.lib().tl_head_loss_workspace(ctypes.byref(header), rows, code, target, int(backward), ctypes.byref(need)))
-    # (of the call's own, as paged_attention's)
-    return torch.empty(need.value, dtype=torch.uint8, device=device)
-
-
-class _HeadLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, scale, weight, back, wanted):
-        rows, code = x.shape[0], _code(x.dtype, "x")
-        loss = torch.empty(rows, dtype=torch.float32, device=x.device)
-        lse = torch.empty(rows + 1, dtype=torch.float32, device=x.device)
-        ctx.save_for_backward(x, scale, lse, *wanted[:1], *wanted[2:5])
-        ctx.weight, ctx.back, ctx.ignore, ctx.temperature = weight, back, wanted.ignore, wanted.temperature
-        if rows == 0:
-            return loss
-        target = wanted.call()
-        with torch.cuda.device(x.device):
-            ws = _loss_workspace(weight.header, rows, code, target, False, x.device)
-            _lib.check(_lib.lib().tl_head_loss(ctypes.byref(weight.header), weight.blob.data_ptr(), x.data_ptr(), code, _row_step(x), rows,
-                                               None if scale is None else scale.data_ptr(), _lib.TL_F32 if scale is None else _code(scale.dtype, "scale"),
-                                               target, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream_ptr(x.device)))
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, scale, lse, targets, entries, shares, known = ctx.saved_tensors
-        weight, back = ctx.weight, ctx.back
-        rows, code = x.shape[0], _code(x.dtype, "x")
-        if rows == 0:
-            return (*(torch.zeros_like(t) if needed else None for t, needed in zip((x, scale), ctx.needs_input_grad)), None, None, None)
-        target = _Wanted(targets, ctx.ignore, entries, shares, known, ctx.temperature).call()
-        grad = grad.to(torch.float32).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
-        ds = torch.empty_like(scale) if ctx.needs_input_grad[1] else None
-        with torch.cuda.device(x.device):
-            ws = _loss_workspace(weight.header, rows, code, target, True, x.device)
-            _lib.check(_lib.lib().tl_head_loss_backward(
-                ctypes.byref(weight.header), weight.blob.data_ptr(), None if back is None else back.codes.data_ptr(), x.data_ptr(), code, _row_step(x), rows,
-                None if scale is None else scale.data_ptr(), _lib.TL_F32 if scale is None else _code(scale.dtype, "scale"), target, lse.data_ptr(),
-                grad.data_ptr(), None if dx is None else dx.data_ptr(), x.shape[1], None if ds is None else ds.data_ptr(), ws.data_ptr(), ws.numel(),
-                _stream_ptr(x.device)))
-        return dx, ds, None, None, None
-
-
-def _row_step(x):
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+def _rows_in_pieces(t):
+    """A [rows, n] tensor as it is, or its copy where its rows are not in one piece each, one behind the other."""
+    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
 def _loss_operands(weight, x, scale, back):
+    """What a loss refuses of its operands."""
     if x.dim() != 2 or x.shape[1] != weight.inners:
         raise ValueError(f"x must be [rows, {weight.inners}]")
     _code(x.dtype, "x")
@@ -1200,12 +1143,19 @@ def _loss_operands(weight, x, scale, back):
         raise ValueError("scale must have one dimension")
     if back is not None and (back.blob.data_ptr() != weight.blob.data_ptr() or back.header.checksum != weight.header.checksum):
         raise ValueError("back is the BackWeight of another weight")
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, scale)):
+        raise RuntimeError("a head's losses have no forward-mode tangents")
     if back is None and torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("the gradient of x needs back=BackWeight(weight)")
-    _cuda(x, "x")
-    if (x.stride(1) != 1 and x.shape[1] > 1) or _row_step(x) < x.shape[1]:
-        x = x.contiguous()
-    return x
+
+
+def _loss_result(y):
+    """What the binding has made of checked operands: the losses, or the library's status."""
+    if y is None:
+        raise ValueError("operands of a loss must be ordinary tensors")
+    if isinstance(y, int):
+        _lib.check(y)
+    return y
 
 
 def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
@@ -1213,10 +1163,17 @@ def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
     [rows]; a row whose target is `ignore` has loss and gradient 0, one whose target is no column NaN.  x and scale [N]: float16 or float32.
     Differentiable once by x, with back = BackWeight(weight), and by scale; logits, sums and what is kept are fp32, x's gradient takes the
     distribution's in x's type.  A row that is not finite has loss NaN (and makes the scales' gradient NaN), which no other row has of it."""
-    x = _loss_operands(weight, x, scale, back)
+    if back is None or back.blob is weight.blob:
+        y = _loss(weight, x, scale, back, targets, ignore, None, None, 1.0)
+        if torch.is_tensor(y):
+            return y
+    _loss_operands(weight, x, scale, back)
     if targets.shape != x.shape[:1] or targets.dtype != torch.int64 or targets.device != x.device:
         raise ValueError("targets must be an int64 tensor of one target to a row, on x's device")
-    return _HeadLoss.apply(x, scale, weight, back, _Wanted(targets.contiguous(), int(ignore), None, None, None, 1.0))
+    _cuda(x, "x")
+    if x.shape[0] == 0:
+        return (x.sum(1) * 0.0 if scale is None else x.sum(1) * scale.sum()).to(torch.float32)
+    return _loss_result(_loss(weight, _rows_in_pieces(x), scale, back, targets.contiguous(), int(ignore), None, None, 1.0))
 
 
 def distillation(weight, x, ids, logits, scale=None, *, temperature=1.0, back=None):
@@ -1225,19 +1182,22 @@ def distillation(weight, x, ids, logits, scale=None, *, temperature=1.0, back=No
     to 1024; its probabilities are softmax(logits / temperature) over them.  A logit of -inf names nothing, whatever its id; a repeated id's probabilities
     add up; a row of -inf alone has loss and gradient 0; one with NaN, +inf or an id that is no column is NaN.  Differentiable as cross_entropy is,
     by the student alone."""
-    x = _loss_operands(weight, x, scale, back)
+    if back is None or back.blob is weight.blob:
+        y = _loss(weight, x, scale, back, None, 0, ids, logits, temperature)
+        if torch.is_tensor(y):
+            return y
+    _loss_operands(weight, x, scale, back)
     for t, kind in ((ids, torch.int64), (logits, logits.dtype)):
         if t.dim() != 2 or t.shape != ids.shape or t.shape[0] != x.shape[0] or t.dtype != kind or t.device != x.device:
             raise ValueError("ids (int64) and logits must be [rows, top] on x's device")
-    if logits.requires_grad and torch.is_grad_enabled():
+    _code(logits.dtype, "logits")
+    if (logits.requires_grad and torch.is_grad_enabled()) or (torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(logits).tangent is not None):
         raise RuntimeError("a teacher's logits have no gradient here: detach them")
-    code, (rows, top), heat = _code(logits.dtype, "logits"), ids.shape, float(temperature)
-    if not 0.0 < heat <= 1e6:
+    if not 0.0 < float(temperature) <= 1e6:
         raise ValueError(f"temperature={temperature} is not a positive number up to 1e6")
-    ids, logits = (t if t.stride(1) == 1 and _row_step(t) >= top else t.contiguous() for t in (ids, logits))
-    entries, shares = (torch.empty((rows, top), dtype=t, device=x.device) for t in (torch.int32, torch.float32))
-    known = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().tl_teacher_entries(ids.data_ptr(), _row_step(ids), logits.data_ptr(), code, _row_step(logits), rows, top, weight.columns, heat,
-                                                 entries.data_ptr(), shares.data_ptr(), known.data_ptr(), _stream_ptr(x.device)))
-    return _HeadLoss.apply(x, scale, weight, back, _Wanted(None, 0, entries, shares, known, heat))
+    if not 1 <= ids.shape[1] <= 1024:
+        raise ValueError(f"a teacher has 1 to 1024 entries to a row, not {ids.shape[1]}")
+    _cuda(x, "x")
+    if x.shape[0] == 0:
+        return (x.sum(1) * 0.0 if scale is None else x.sum(1) * scale.sum()).to(torch.float32)
+    return _loss_result(_loss(weight, _rows_in_pieces(x), scale, back, None, 0, _rows_in_pieces(ids), _rows_in_pieces(logits), float(temperature)))
