@@ -523,10 +523,12 @@ struct HeadLossBackward : torch::autograd::Node {
                                         current_stream(x.device())) == TL_OK,
                         g_last_error());
         }
-        if (c10::GradMode::is_enabled()) {     // (a graph of the gradients is asked for: they have none, which whoever follows it is told)
-            const auto once = std::make_shared<torch::autograd::DelayedError>("the losses of a head are differentiable once", 2);
-            auto ends = (*once)({dx, ds});
-            dx = ends[0], ds = ends[1];
+        if (c10::GradMode::is_enabled()) {     // (a graph of the gradients is asked for: they have none, which whoever follows it to an operand is told)
+            const std::shared_ptr<torch::autograd::Node> once(
+                new torch::autograd::Error("the losses of a head are differentiable once", torch::autograd::collect_next_edges(x, scale, grads[0])),
+                torch::autograd::deleteNode);
+            for (at::Tensor* d : {&dx, &ds})
+                if (d->defined()) torch::autograd::set_history(*d, once);
         }
         out[0] = dx, out[1] = ds;
         return out;

@@ -110,6 +110,7 @@ class TernaryLinear(nn.Module):
     `reference_buffers` (also build the reference's merged arrays; they are not used by forward).
     """
     __constants__ = ["in_features", "out_features"]
+    _back = None                                 # the ops.BackWeight of the packed weight, once a gradient has asked for it
 
     def __init__(self, in_features, out_features, sparsity=0.8, uniform=False, uniform_blk_size=512, padding=False,
                  padding_size=4, bias=True, device=None, dtype=torch.int32, *, weight=None, scale=None, generator=None,
@@ -253,6 +254,30 @@ class TernaryLinear(nn.Module):
                 return ops.spmm(w, input, scale, x_layout=1)
             return ops.spmm_kmajor_batch(w, input, scale)
         raise ValueError(f"input of shape {tuple(input.shape)} does not match in_features={K}")
+
+    def _rated(self, input, wanted, rate):
+        """rate(weight, rows, rows of every tensor of `wanted`, BackWeight or None) for input [.., K]: [..]."""
+        if input.shape[-1:] != (self.in_features,):
+            raise ValueError(f"input of shape {tuple(input.shape)} does not match in_features={self.in_features}")
+        if any(t.shape[:input.dim() - 1] != input.shape[:-1] for t in wanted):
+            raise ValueError("targets, ids and logits go with the input's rows")
+        w, back = self.device_weight(), None
+        if torch.is_grad_enabled() and input.requires_grad:
+            back = self._back
+            if back is None or back.blob is not w.blob:
+                back = self._back = ops.BackWeight(w)
+        lead, rows = input.dim() - 1, input.shape[:-1].numel()
+        return rate(w, input.reshape(rows, self.in_features), [t.reshape(rows, *t.shape[lead:]) for t in wanted], back).view(input.shape[:-1])
+
+    def cross_entropy(self, input, targets, *, ignore=-100):
+        """-log softmax(self(input))[targets] for input [.., K] and int64 targets [..], float32 [..], without the [.., N] that forward would give: for a
+        module that is a model's head (`ops.cross_entropy`).  Differentiable by the input, and by w_scale where it asks for that."""
+        return self._rated(input, (targets,), lambda w, x, t, back: ops.cross_entropy(w, x, t[0], self.w_scale, ignore=ignore, back=back))
+
+    def distillation(self, input, ids, logits, *, temperature=1.0):
+        """How far softmax(self(input) / temperature) is from that of a teacher whose top logits [.., top] of columns ids [.., top] are known, times the
+        temperature's square, float32 [..] (`ops.distillation`)."""
+        return self._rated(input, (ids, logits), lambda w, x, t, back: ops.distillation(w, x, *t, self.w_scale, temperature=temperature, back=back))
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, nnz={self._packed_nnz}"

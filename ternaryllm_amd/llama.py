@@ -466,7 +466,40 @@ class TernaryLlamaDecoder(nn.Module):
     def extend(self, cache, chunks):
         """A pass over new tokens of sequences of any lengths: chunks = [(sequence of `cache`, LongTensor of its new tokens, one or more), ...].
         Their keys and values go into the cache; returns the logits of each chunk's last token, [chunks, vocab].  Where it raises, the sequences
-        are as they were."""
+        are as they were.  Sequences that were forked from one (`cache.fork`) and stand side by side have the keys that they share read once."""
+        return self._extend(cache, chunks, lambda tokens, batch, prefix: self.extend_batch(cache, tokens, batch, prefix))
+
+    @torch.no_grad()
+    def score(self, cache, chunks):
+        """extend, but what the pass says of the chunks' own tokens: for each chunk the log-probabilities (float32) of its tokens from the second on, each given
+        all before it.  (To rate what follows a prompt, leave the prompt's last token out of the sequence that is forked, and begin each chunk with it.)"""
+        rows, first = [], 0
+        for _, t in chunks:
+            rows += range(first, first + t.numel() - 1)
+            first += t.numel()
+
+        def rate(tokens, batch, prefix):
+            at = torch.tensor(rows, dtype=torch.long).to(tokens.device)
+            h = self._extend_rows(cache, tokens, batch, prefix).index_select(0, at)
+            return -self.lm_head.cross_entropy(h, tokens.long().index_select(0, at + 1))
+
+        return self._extend(cache, chunks, rate).split([t.numel() - 1 for _, t in chunks])
+
+    @torch.no_grad()
+    def divergence(self, cache, chunks, teacher, temperature=1.0):
+        """extend, but how far the distribution behind every token of the chunks is from a teacher's (float32, `TernaryLinear.distillation`): teacher = for each
+        chunk the ids and the logits [tokens, top] of the teacher's likeliest next tokens, the same number for all."""
+        if len(teacher) != len(chunks) or any(ids.shape[:1] != t.shape or logits.shape != ids.shape for (_, t), (ids, logits) in zip(chunks, teacher)):
+            raise ValueError("a teacher has ids and logits [tokens, top] for every chunk")
+
+        def rate(tokens, batch, prefix):
+            ids, logits = (torch.cat([pair[i].to(tokens.device) for pair in teacher]) for i in (0, 1))
+            return self.lm_head.distillation(self._extend_rows(cache, tokens, batch, prefix), ids, logits, temperature=temperature)
+
+        return self._extend(cache, chunks, rate).split([t.numel() for _, t in chunks])
+
+    def _extend(self, cache, chunks, work):
+        """work(tokens, batch, prefix) of a pass over chunks, which go into the cache unless it raises."""
         if not chunks or any(t.dim() != 1 or t.numel() == 0 or t.dtype not in (torch.int64, torch.int32) for _, t in chunks):
             raise ValueError("every chunk is a sequence and a one-dimensional integer tensor of one or more new tokens")
         if any(cache.length(s) + t.numel() > self.max_seq_len for s, t in chunks):
@@ -479,7 +512,7 @@ class TernaryLlamaDecoder(nn.Module):
         before = [(s, cache.length(s)) for s, _ in chunks]
         batch = cache.extend([(s, t.numel()) for s, t in chunks])
         try:
-            return self.extend_batch(cache, tokens, batch)
+            return work(tokens, batch, cache.prefix([(s, t.numel()) for s, t in chunks]))
         except BaseException:
             for s, length in reversed(before):       # (the last pages taken go back first: the next call gets the same)
                 cache.truncate(s, length)
@@ -491,10 +524,16 @@ class TernaryLlamaDecoder(nn.Module):
             raise RuntimeError("sequences over pages need a float16 decoder with heads of 64, 128 or 256")
 
     @torch.no_grad()
-    def extend_batch(self, cache, tokens, batch):
-        """extend for an ops.PageBatch that the caller keeps (cache.extend makes one): tokens [rows].  No part of it is done on the host, so it
-        can be captured in a graph; the batch's tensors may then hold other sequences and lengths at every replay, for as many rows and
-        sequences.  Rows of no sequence are computed and mean nothing."""
+    def extend_batch(self, cache, tokens, batch, prefix=None):
+        """extend for an ops.PageBatch that the caller keeps (cache.extend makes one, cache.prefix an ops.PagePrefix): tokens [rows].  No part of it is done
+        on the host, so it can be captured in a graph; the batch's and the prefix's tensors may then hold other sequences and lengths at every replay, for as
+        many rows, sequences and groups.  Rows of no sequence are computed and mean nothing."""
+        h = self._extend_rows(cache, tokens, batch, prefix)
+        last = (batch.starts[1:].long() - 1).clamp(min=0)
+        return self.lm_head(h.index_select(0, last))
+
+    def _extend_rows(self, cache, tokens, batch, prefix):
+        """The rows [rows, hidden] that the head multiplies."""
         c = self.config
         nh, hd = c.num_attention_heads, c.head_dim
         self._check_paged()
@@ -515,12 +554,11 @@ class TernaryLlamaDecoder(nn.Module):
             q, k, v = layer.qkv_proj(h).view(-1, 3, nh, hd).unbind(1)
             pages = cache.layer(li)
             q = ops.rope_to_pages(q, k, v, pages, batch, f)
-            ops.paged_attention(q, pages, batch, out=a)
+            ops.paged_attention(q, pages, batch, out=a, prefix=prefix)
             x, h = add_norm(x, layer.o_proj(a), layer.post_attention_layernorm)
             y = self._mlp(layer, h)
             x, h = add_norm(x, y, self.layers[li + 1].input_layernorm if li + 1 < len(self.layers) else self.norm)
-        last = (batch.starts[1:].long() - 1).clamp(min=0)
-        return self.lm_head(h.index_select(0, last))
+        return h
 
     @torch.no_grad()
     def adopt(self, cache, sequences):
