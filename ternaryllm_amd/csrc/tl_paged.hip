@@ -64,7 +64,6 @@ struct Seq {
     int start, n, length, tiles;
     int before;                                  // its keys that every row sees, 0 at least
     bool wrong;                                  // the table does not hold its length
-    int skip;                                    // kOwn: its first key, a multiple of kRound
 };
 
 // Tokens shared, as many as whole rounds of keys: the rest is every sequence's own.
@@ -81,7 +80,6 @@ template <Keys SET = kCausal>
 __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
 {
     Seq s;
-    s.skip = 0;
     if constexpr (SET == kPrefix) {             // all of a group's rows; the keys are its first sequence's
         const int2 g = group_of(a, b);
         const int length = g.x < g.y ? a.begin[g.x] : 0, room = a.batch.table_pages << a.pages.shift;
@@ -104,8 +102,7 @@ __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
     if constexpr (SET == kOwn) {
         const int begin = a.begin[b];            // (tokens in front of its rows, all of them)
         s.wrong |= begin < 0 || begin > s.before;
-        s.skip = whole_rounds(min(begin, s.before));
-        s.before -= s.skip;
+        s.before -= whole_rounds(min(begin, s.before));
     }
     return s;
 }
@@ -113,7 +110,7 @@ __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b)
 // The same for a sequence that all lanes look at.
 __device__ __forceinline__ Seq scalar(Seq s)
 {
-    return Seq{scalar(s.start), scalar(s.n), scalar(s.length), scalar(s.tiles), scalar(s.before), scalar((int)s.wrong) != 0, scalar(s.skip)};
+    return Seq{scalar(s.start), scalar(s.n), scalar(s.length), scalar(s.tiles), scalar(s.before), scalar((int)s.wrong) != 0};
 }
 
 // Cost of a key head's first `tiles` units: unit i costs fixed + before + (i + 1) * tile_tokens.
@@ -140,9 +137,9 @@ __device__ __forceinline__ long long share_of(long long a, long long b, long lon
 template <Keys SET>
 __device__ __forceinline__ bool next_unit(const PagedAttn& a, Walk& w, long long cost);
 
-// By a whole workgroup of 256 threads.  False where it has no part.
+// By a whole workgroup of 256 threads, number `block` of `blocks` that walk the list.  False where it has no part.
 template <Keys SET>
-__device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
+__device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w, int block, int blocks)
 {
     __shared__ long long sums[4];
     __shared__ long long found_at;
@@ -192,9 +189,9 @@ __device__ __forceinline__ bool begin_walk(const PagedAttn& a, Walk& w)
     total = scalar(total);
     // as many parts as there are workgroups, but none of less than `least`; neighbours of the list stay in one part of the chip, whose
     // cache they share
-    w.wgs = (int)min(share_of(total + a.least - 1, 1, a.least), (long long)gridDim.x);
-    const int eighth = (w.wgs + 7) / 8, inside = (int)blockIdx.x / 8;
-    w.wg = inside < eighth ? ((int)blockIdx.x & 7) * eighth + inside : (int)blockIdx.x;
+    w.wgs = (int)min(share_of(total + a.least - 1, 1, a.least), (long long)blocks);
+    const int eighth = (w.wgs + 7) / 8, inside = block / 8;
+    w.wg = inside < eighth ? (block & 7) * eighth + inside : block;
     if (w.wg >= w.wgs) {
         if (SET == kCausal && tid == 0) a.shared[w.wg].last = -1;
         return false;
@@ -274,7 +271,7 @@ __device__ __forceinline__ Unit unit_of(const PagedAttn& a, const Walk& w)
     u.first_token = w.tile * a.tile_tokens;
     u.kv_head = w.head / a.blocks;
     u.first_head = (w.head - u.kv_head * a.blocks) * a.tile_heads;
-    const int skip = SET == kOwn ? w.s.skip : 0;
+    const int skip = SET == kOwn ? max(w.s.length - w.s.n, 0) - w.s.before : 0;   // (what is not counted among the keys that every row sees)
     const int seen = SET == kPrefix ? w.s.length : max(w.s.length - w.s.n + min(u.first_token + a.tile_tokens, w.s.n) - skip, 0);   // by its last row
     u.begins = a.uncut || w.at >= w.from;
     const bool ends = a.uncut || w.at + u.cost <= w.to;
@@ -400,6 +397,12 @@ __device__ __forceinline__ bool make_finite(u32x4* x)
     }
     return any != 0;
 }
+
+// Bytes of LDS that a workgroup's tiles take, of many rows and of few; heads of 64 have tiles half as large.
+template <int HD>
+constexpr int kRowsLdsOf = HD == 64 ? 32768 : 65536;
+template <int HD>
+constexpr int kFewLds = 4 * 16 * (HD + 4) * 4;
 
 // The running softmax of a row: its reference is a maximum that it has seen (in units of the scores), which probabilities are taken
 // against; limit is how far a score may lie above it.  The reference moves only where a score passes the limit, kSlack in the exponent of 2, and the
@@ -550,19 +553,19 @@ __device__ __forceinline__ u32x4 buffer_at(const void* base, int bytes)
 // Measured with the join (15 us), 4096 rows over 4096 keys, 32 heads on 8 of 128: 402 us, 1025 TFLOP/s (425 on other cards); the matrix cores are busy for
 // 48 % of it, the vector unit for 31 % and 18 % (exponentials) beside them.  64 rows: 526.  8-bit pages: 472 (64 rows: 665).  Heads of 64: 291, of 256: 1107.
 template <int HD, int QF, bool BYTES, Keys SET>
-__global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
+__device__ __forceinline__ void tl_paged_rows(const PagedAttn& a, int block, int blocks, unsigned char* lds)
 {
     constexpr int ROWS = 64 * QF, KT = HD == 256 ? 32 : 64, NF = KT / 16, KS = HD / 32, DF = HD / 16;
     constexpr int KB = KT * HD * 2, BUF = 2 * KB, KW = KT / 4;    // KW: keys that a wave brings
     constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, KL = KW * PIECES / 64, KEYS = 64 / PIECES;   // of a load
-    __shared__ __align__(16) unsigned char lds[2 * BUF];
+    static_assert(2 * BUF == kRowsLdsOf<HD>);
     __shared__ int wrong_somewhere;
     __shared__ Walk kept;
     __shared__ int spoiled[2][KT];                                // keys of a buffer whose values were not finite
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
-    if (!begin_walk<SET>(a, w)) return;
+    if (!begin_walk<SET>(a, w, block, blocks)) return;
     auto key_place = [](int key, int p) { return HD == 64 ? p ^ ((key >> 1) & 7) : p ^ (key & 15); };
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
     const int mask = (1 << a.pages.shift) - 1;
@@ -838,20 +841,20 @@ __global__ __launch_bounds__(256, 2) void tl_paged_rows(PagedAttn a)
 // Measured, with the join: 32 sequences of 4096, 32 heads on 8 of 128: 102 us, 5.3 TB/s (8-bit pages 58, 4.7); heads of 256, whose registers allow one
 // workgroup a compute unit, 104 for the same bytes (241 while they spilled).
 template <int HD, bool BYTES, Keys SET>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn a)
+__device__ __forceinline__ void tl_paged_few(const PagedAttn& a, int block, int blocks, unsigned char* lds)
 {
     constexpr int ROWS = 16, KT = 32, KS = HD / 32, DF = HD / 16;
     constexpr int KL = BYTES ? HD / 64 : KS;                      // 16-byte pieces of a key that a lane loads
     constexpr int VALUES = BYTES ? 16 : 8, PIECES = HD / VALUES, VL = KT * PIECES / 64, VKEYS = 64 / PIECES;   // keys of one load of values
     constexpr int LD = HD + 4;
-    __shared__ __align__(16) unsigned char lds[4 * ROWS * LD * 4];                                              // >= 4 * KT * HD * 2
+    static_assert(4 * ROWS * LD * 4 == kFewLds<HD> && kFewLds<HD> >= 4 * KT * HD * 2);
     __shared__ float tops[4][ROWS], sums[4][ROWS];
     __shared__ int wrong_somewhere;
     __shared__ Walk kept;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     Walk w;
-    if (!begin_walk<SET>(a, w)) return;
+    if (!begin_walk<SET>(a, w, block, blocks)) return;
     unsigned char* own = lds + wave * KT * HD * 2;
     auto value_place = [](int key, int pair) { return HD == 64 ? pair ^ ((key >> 1) & 3) : pair ^ (key & 7); };
     for (;;) {
@@ -1057,6 +1060,37 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tl_paged_few(PagedAttn
     }
 }
 
+// The walks as kernels, rows of a unit 16, 64 or 128.
+template <int HD, int ROWS, bool BYTES, Keys SET>
+__global__ __launch_bounds__(256, HD == 256 && ROWS == 16 ? 1 : 2) void tl_paged_units(PagedAttn a)
+{
+    if constexpr (ROWS == 16) {
+        __shared__ __align__(16) unsigned char lds[kFewLds<HD>];
+        tl_paged_few<HD, BYTES, SET>(a, (int)blockIdx.x, (int)gridDim.x, lds);
+    } else {
+        __shared__ __align__(16) unsigned char lds[kRowsLdsOf<HD>];
+        tl_paged_rows<HD, ROWS / 64, BYTES, SET>(a, (int)blockIdx.x, (int)gridDim.x, lds);
+    }
+}
+
+// The keys that groups share and the sequences' own, side by side in one launch: a.workgroups workgroups have parts of the first list, those behind them of the
+// second, which fill the chip up as the first ones end.  (One after the other, us: 4 rows over 512 keys, 32 heads, 11.0 + 10.1; 64 over 8192, 32 heads on 8,
+// 31.5 + 16.4.)
+template <int HD, int ROWS, int OWN_ROWS, bool BYTES>
+__global__ __launch_bounds__(256, 2) void tl_paged_both(PagedAttn a, PagedAttn b)
+{
+    constexpr int kRows = ROWS > 16 || OWN_ROWS > 16 ? kRowsLdsOf<HD> : 0;
+    __shared__ __align__(16) unsigned char lds[kRows > kFewLds<HD> ? kRows : kFewLds<HD>];
+    const int block = (int)blockIdx.x;
+    if (block < a.workgroups) {
+        if constexpr (ROWS == 16) tl_paged_few<HD, BYTES, kPrefix>(a, block, a.workgroups, lds);
+        else tl_paged_rows<HD, ROWS / 64, BYTES, kPrefix>(a, block, a.workgroups, lds);
+    } else {
+        if constexpr (OWN_ROWS == 16) tl_paged_few<HD, BYTES, kOwn>(b, block - a.workgroups, b.workgroups, lds);
+        else tl_paged_rows<HD, OWN_ROWS / 64, BYTES, kOwn>(b, block - a.workgroups, b.workgroups, lds);
+    }
+}
+
 // Joins the pieces of the units that were shared out: blockIdx.x is the workgroup in which one begins.  HD / 4 lanes take a row, four
 // values each.  Of a unit of a few pieces as many rows as there are such groups of lanes are joined at a time; where they are many, as of a single long sequence, one row by as many
 // groups of lanes, which share the pieces out.
@@ -1148,97 +1182,102 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
     }
 }
 
-// Joins the pieces of a row's keys that its group shares and of its own: a workgroup to a row of a query head, HD / 4 lanes to a piece, four values each.
-// Bound by latency: the row's place, its units' workgroups, the pieces, one after the other.
-template <int HD>
+// Where the pieces of a row's unit lie: of the workgroup in which it begins, and of those behind.
+struct Pieces {
+    const float *first, *more;
+    long long step;
+    int count;
+};
+
+__device__ __forceinline__ Pieces pieces_of(const PagedAttn& p, int which, const Seq& s, int token, int head)
+{
+    Pieces y{};
+    const int t = token - s.start, of_group = head % p.group, block = of_group / p.tile_heads;
+    if (t < 0 || t >= s.n || s.tiles == 0) return y;
+    const int r = t % p.tile_tokens * p.tile_heads + of_group % p.tile_heads;
+    const int2 ends = p.ends[unit_at(p, which, s.start, t / p.tile_tokens, head / p.group * p.blocks + block)];
+    const int from = min(max(ends.x, 0), p.workgroups - 1), to = min(max(ends.y, from), p.workgroups - 1);
+    y.first = p.firsts + ((long long)token * p.heads + head) * (p.pages.hd + 4);
+    y.step = (long long)p.rows * (p.pages.hd + 4);
+    y.more = p.pieces + (from + 1) * y.step + r * (p.pages.hd + 4);
+    y.count = to - from + 1;
+    return y;
+}
+
+// Joins the pieces of a row's keys that its group shares and of its own: WAVES waves to a row of a query head, HD / 4 lanes to a piece, four values each.  Bound
+// by latency: the row's place, its units' workgroups, the pieces, one after the other.
+template <int HD, int WAVES>
 __global__ __launch_bounds__(256) void tl_paged_merge(PagedAttn a, PagedAttn b)
 {
-    constexpr int LANES = HD / 4, AT_ONCE = 256 / LANES, FLY = 4;
-    __shared__ float4 part[256];
+    constexpr int LANES = HD / 4, AT_ONCE = WAVES * 64 / LANES, FLY = 4;
+    __shared__ float4 part[WAVES == 1 ? 1 : 256];
     __shared__ float tops[AT_ONCE], sums[AT_ONCE];
-    const int token = (int)(blockIdx.x / (unsigned)a.heads), head = (int)(blockIdx.x % (unsigned)a.heads);
-    const int lane = (int)threadIdx.x % LANES, own = (int)threadIdx.x / LANES;
+    const int tid = WAVES == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
+    const long long row = scalar((int)(WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x));
+    if (row >= (long long)a.batch.tokens * a.heads) return;
+    const int token = (int)(row / a.heads), head = (int)(row - (long long)token * a.heads);
+    const int lane = tid % LANES, own = tid / LANES;
     const Place at = place_of(a.batch, token);
-    if (at.seq < 0) return;
+    const int seq = scalar(at.seq);
+    if (seq < 0) return;
     // its group, if there is one; the pieces of that unit, and of the sequence's own
     int below = 0;
     for (int first = 0; first <= a.group_count; first += 64) {
         const int i = first + (int)(threadIdx.x & 63u);
-        const int more = __popcll(__builtin_amdgcn_ballot_w64(i <= a.group_count && a.groups[min(i, a.group_count)] <= at.seq));
+        const int more = __popcll(__builtin_amdgcn_ballot_w64(i <= a.group_count && a.groups[min(i, a.group_count)] <= seq));
         below += more;
         if (more < 64) break;
     }
-    const int g = below - 1, begin = a.begin[at.seq];
+    const int g = below - 1, begin = a.begin[seq];
     const bool grouped = g >= 0 && g < a.group_count;
-    bool wrong = grouped ? begin != a.begin[group_of(a, g).x] : begin != 0;
-    struct Pieces {
-        const float *first, *more;               // (more: of the workgroup behind the first)
-        long long step;
-        int count;
-    };
-    auto pieces = [&](const PagedAttn& p, int which, const Seq& s) {
-        Pieces y{};
-        const int t = token - s.start, of_group = head % p.group, block = of_group / p.tile_heads;
-        if (t < 0 || t >= s.n || s.tiles == 0) return y;
-        const int r = t % p.tile_tokens * p.tile_heads + of_group % p.tile_heads, rows = p.rows;
-        const int2 ends = p.ends[unit_at(p, which, s.start, t / p.tile_tokens, head / p.group * p.blocks + block)];
-        const int from = min(max(ends.x, 0), p.workgroups - 1), to = min(max(ends.y, from), p.workgroups - 1);
-        y.first = p.firsts + ((long long)token * p.heads + head) * (HD + 4);
-        y.step = (long long)rows * (HD + 4);
-        y.more = p.pieces + (from + 1) * y.step + r * (HD + 4);
-        y.count = to - from + 1;
-        return y;
-    };
+    const bool wrong = grouped ? begin != a.begin[group_of(a, g).x] : begin != 0;
     Pieces front{};
-    if (grouped) {
-        const Seq s = sequence<kPrefix>(a, g);
-        front = pieces(a, g, s);
-    }
-    const Pieces behind = pieces(b, at.seq, sequence<kOwn>(b, at.seq));
+    if (grouped) front = pieces_of(a, g, sequence<kPrefix>(a, g), token, head);
+    const Pieces behind = pieces_of(b, seq, sequence<kOwn>(b, seq), token, head);
     const int count = front.count + behind.count;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = kNone, sum = 0.f;
+    auto add = [&](float m, float l, const float4& v) {
+        const float now = fmaxf(top, m), old = weight_of(top, now, a.scale_log2), fresh = weight_of(m, now, a.scale_log2);
+        o = make_float4(o.x * old + v.x * fresh, o.y * old + v.y * fresh, o.z * old + v.z * fresh, o.w * old + v.w * fresh);
+        sum = sum * old + l * fresh;
+        top = now;
+    };
     for (int i = own; i < count; i += FLY * AT_ONCE) {
         float m[FLY], l[FLY];
         float4 v[FLY];
 #pragma unroll
         for (int k = 0; k < FLY; ++k) {
             const int n = min(i + k * AT_ONCE, count - 1);
-            const Pieces& p = n < front.count ? front : behind;
-            const int j = n < front.count ? n : n - front.count;
-            const float* piece = j == 0 ? p.first : p.more + (j - 1) * p.step;
+            const bool ahead = n < front.count;
+            const int j = ahead ? n : n - front.count;
+            const float* more = (ahead ? front.more : behind.more) + (j - 1) * (ahead ? front.step : behind.step);
+            const float* piece = j == 0 ? (ahead ? front.first : behind.first) : more;
             m[k] = piece[HD], l[k] = piece[HD + 1];
             v[k] = *reinterpret_cast<const float4*>(piece + lane * 4);
         }
 #pragma unroll
-        for (int k = 0; k < FLY; ++k) {
-            if (i + k * AT_ONCE >= count) break;
-            const float now = fmaxf(top, m[k]);
-            const float old = weight_of(top, now, a.scale_log2), fresh = weight_of(m[k], now, a.scale_log2);
-            o = make_float4(o.x * old + v[k].x * fresh, o.y * old + v[k].y * fresh, o.z * old + v[k].z * fresh, o.w * old + v[k].w * fresh);
-            sum = sum * old + l[k] * fresh;
-            top = now;
-        }
+        for (int k = 0; k < FLY; ++k)
+            if (i + k * AT_ONCE < count) add(m[k], l[k], v[k]);
     }
-    part[threadIdx.x] = o;
-    if (lane == 0) tops[own] = top, sums[own] = sum;
-    __syncthreads();
+    if constexpr (WAVES == 1) {
+#pragma unroll
+        for (int off = LANES; off < 64; off <<= 1)
+            add(__shfl_xor(top, off, 64), __shfl_xor(sum, off, 64),
+                make_float4(__shfl_xor(o.x, off, 64), __shfl_xor(o.y, off, 64), __shfl_xor(o.z, off, 64), __shfl_xor(o.w, off, 64)));
+    } else {
+        part[threadIdx.x] = o;
+        if (lane == 0) tops[own] = top, sums[own] = sum;
+        __syncthreads();
+        if (own != 0) return;
+#pragma unroll
+        for (int i = 1; i < AT_ONCE; ++i) add(tops[i], sums[i], part[i * LANES + lane]);
+    }
     if (own != 0) return;
-    float most = tops[0];
-#pragma unroll
-    for (int i = 1; i < AT_ONCE; ++i) most = fmaxf(most, tops[i]);
-    o = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-        const float weight = weight_of(tops[i], most, a.scale_log2);
-        const float4 v = part[i * LANES + lane];
-        o = make_float4(o.x + v.x * weight, o.y + v.y * weight, o.z + v.z * weight, o.w + v.w * weight);
-        sum += sums[i] * weight;
-    }
     if (wrong) sum = __builtin_nanf("");
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;              // (no key: 0)
     const __half h[4] = {__float2half(o.x * inv), __float2half(o.y * inv), __float2half(o.z * inv), __float2half(o.w * inv)};
-    *reinterpret_cast<uint2*>(a.out + ((long long)token * a.heads + head) * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
+    *reinterpret_cast<uint2*>(a.out + row * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
 }
 
 // What a call takes: rows of a unit, workgroups at most, the cost of a unit beside its keys, the cost below which a part is not cut, and whether units
@@ -1288,16 +1327,16 @@ void launch_units(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
     const dim3 grid((unsigned)p.workgroups), block(256);
     if (p.rows == 16) {
-        hipLaunchKernelGGL((tl_paged_few<HD, BYTES, SET>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((tl_paged_units<HD, 16, BYTES, SET>), grid, block, 0, st, a);
         return;
     }
-    if constexpr (HD < 256 && SET != kOwn) {
+    if constexpr (HD < 256) {
         if (p.rows == 128) {
-            hipLaunchKernelGGL((tl_paged_rows<HD, 2, BYTES, SET>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((tl_paged_units<HD, 128, BYTES, SET>), grid, block, 0, st, a);
             return;
         }
     }
-    hipLaunchKernelGGL((tl_paged_rows<HD, 1, BYTES, SET>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((tl_paged_units<HD, 64, BYTES, SET>), grid, block, 0, st, a);
 }
 
 template <int HD, bool BYTES>
@@ -1309,12 +1348,27 @@ void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
     else launch_join<HD, 64>(a, p, st);
 }
 
+constexpr int64_t kRowsOfFourWaves = 1024;
+
 template <int HD, bool BYTES>
 void launch_shared(const PagedAttn& a, const Plan& pa, const PagedAttn& b, const Plan& pb, hipStream_t st)
 {
-    launch_units<HD, BYTES, kPrefix>(a, pa, st);
-    launch_units<HD, BYTES, kOwn>(b, pb, st);
-    hipLaunchKernelGGL(tl_paged_merge<HD>, dim3((unsigned)a.batch.tokens * (unsigned)a.heads), dim3(256), 0, st, a, b);
+    const dim3 grid((unsigned)(pa.workgroups + pb.workgroups)), block(256);
+    if constexpr (HD == 256) {                   // (few rows of such heads have a compute unit's registers to themselves)
+        launch_units<HD, BYTES, kPrefix>(a, pa, st);
+        launch_units<HD, BYTES, kOwn>(b, pb, st);
+    } else if (pb.rows == 16) {
+        if (pa.rows == 16) hipLaunchKernelGGL((tl_paged_both<HD, 16, 16, BYTES>), grid, block, 0, st, a, b);
+        else if (pa.rows == 64) hipLaunchKernelGGL((tl_paged_both<HD, 64, 16, BYTES>), grid, block, 0, st, a, b);
+        else hipLaunchKernelGGL((tl_paged_both<HD, 128, 16, BYTES>), grid, block, 0, st, a, b);
+    } else {
+        if (pa.rows == 64) hipLaunchKernelGGL((tl_paged_both<HD, 64, 64, BYTES>), grid, block, 0, st, a, b);
+        else hipLaunchKernelGGL((tl_paged_both<HD, 128, 64, BYTES>), grid, block, 0, st, a, b);
+    }
+    // a wave to a row, or, of so few rows that many workgroups share each one's keys, four
+    const int64_t rows = (int64_t)a.batch.tokens * a.heads;
+    if (rows > kRowsOfFourWaves) hipLaunchKernelGGL((tl_paged_merge<HD, 1>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a, b);
+    else hipLaunchKernelGGL((tl_paged_merge<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, b);
 }
 
 // The launches of groups that begin alike: the shared keys' and the sequences' own.
@@ -1330,8 +1384,8 @@ SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, cons
     auto plan = [&](int rows) { return Plan{rows, workgroups(rows == 16 && hd == 256 ? 1 : 2), 128, rows == 16 ? 128 : 512, 0}; };
     SharedPlan p;
     const int64_t together = groups > 0 ? ceil_div(tokens, groups) * group : 0;   // rows of a group and a key head, on average
-    p.prefix = plan(together <= 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
     p.own = plan(most_rows * group <= 16 ? 16 : 64);
+    p.prefix = plan(together <= 16 && p.own.rows == 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
     p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23);
     return p;
 }
