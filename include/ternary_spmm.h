@@ -686,10 +686,12 @@ typedef struct tl_page_prefix {
     const int32_t* groups;   /* [count + 1], not falling */
     const int32_t* shared;   /* [seqs] */
     int32_t count;
+    int32_t most_shared;     /* the most tokens that a group shares, as far as the host knows, or a negative number: it chooses how they are read, nothing else */
 } tl_page_prefix;
 
 /* tl_paged_attention for such a batch: the same rows, of the same keys.  Where the device finds that a group's numbers differ, or that they are more than
- * the tokens in front of a sequence's rows, or negative, rows may be NaN.  Whether the shared keys are read apart is chosen by sizes. */
+ * the tokens in front of a sequence's rows, or negative, rows may be NaN.  Whether the shared keys are read apart is chosen by sizes; where they are not, the
+ * call is tl_paged_attention's. */
 int tl_paged_attention_shared_workspace(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, const tl_page_prefix* prefix,
                                         int64_t most_rows, int64_t* bytes);
 int tl_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const tl_pages* pages,

@@ -60,7 +60,7 @@ class Rotation(ctypes.Structure):
 
 class PagePrefix(ctypes.Structure):
     """Mirror of tl_page_prefix."""
-    _fields_ = [("groups", ctypes.c_void_p), ("shared", ctypes.c_void_p), ("count", ctypes.c_int32)]
+    _fields_ = [("groups", ctypes.c_void_p), ("shared", ctypes.c_void_p), ("count", ctypes.c_int32), ("most_shared", ctypes.c_int32)]
 
 
 class LossTarget(ctypes.Structure):

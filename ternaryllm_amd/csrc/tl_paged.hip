@@ -1379,16 +1379,25 @@ struct SharedPlan {
     bool apart;                                  // the shared keys in a launch of their own; not, the call is one without groups
 };
 
-SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows, int64_t groups)
+SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, const tl_page_batch* batch, int64_t most_rows, const tl_page_prefix* prefix)
 {
     const int group = heads / pages->kv_heads, hd = pages->head_dim;
+    const int64_t groups = prefix->count;
     auto workgroups = [](int each) { return (int)ceil_div(each * compute_units(), 8) * 8; };
     auto plan = [&](int rows) { return Plan{rows, workgroups(rows == 16 && hd == 256 ? 1 : 2), 128, rows == 16 ? 128 : 512, 0}; };
     SharedPlan p;
     const int64_t together = groups > 0 ? ceil_div(tokens, groups) * group : 0;   // rows of a group and a key head, on average
     p.own = plan(most_rows * group <= 16 ? 16 : 64);
     p.prefix = plan(together <= 16 && p.own.rows == 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
-    p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23);
+    // Apart where what need not be read again takes longer than the rows' pieces, which meet in a launch of their own: from 24 MB on, and as much again for every
+    // 2048 rows; not where a sequence has rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32
+    // heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024 (29 MB) 19.8 / 19.1; 2 over 8192 (33 MB) 24.8 / 25.3; 4 over 512, 32 heads on 32 (25 MB) 17.7 / 19.1; 8 over 4096
+    // 20.0 / 32.4; 64 over 64 and up to 500 of their own 28.3 / 16.2; 8 groups of 32 over 256 and up to 500 63 / 50; rows of a key head: 8 sequences of 32 27.2 / 30.0,
+    // 16 of 128 43.7 / 40.0, 4 of 2000 144 / 95.)
+    const int64_t keys = (int64_t)batch->table_pages * pages->page_size, shared = prefix->most_shared < 0 ? keys : prefix->most_shared;
+    const double again = (double)(batch->seqs - groups) * (double)shared * pages->kv_heads * hd * (pages->dtype == TL_F16 ? 4 : 2);
+    p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23) && again >= (24 << 20) + (double)tokens * heads * ((24 << 20) / 2048) && 2 * shared >= keys &&
+              most_rows * group < 128;
     return p;
 }
 
@@ -1477,7 +1486,7 @@ extern "C" int tl_paged_attention_shared_workspace(int64_t tokens, int heads, co
 {
     if (int rc = tl_paged_attention_workspace(tokens, heads, pages, batch, most_rows, bytes)) return rc;
     if (!prefix || prefix->count < 0) return fail(TL_ERR_ARG, "the groups are null or fewer than none");
-    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix->count);
+    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix);
     if (!p.apart) return TL_OK;
     int64_t pieces, ends;
     *bytes = shared_part(p.prefix, tokens, heads, pages, prefix->count, &pieces, &ends) + shared_part(p.own, tokens, heads, pages, batch->seqs, &pieces, &ends);
@@ -1496,7 +1505,7 @@ extern "C" int tl_paged_attention_shared(const void* q, int64_t q_token, int64_t
     if (!prefix || prefix->count < 0 || prefix->count > (1 << 24)) return fail(TL_ERR_ARG, "the groups are null, fewer than none or more than 2^24");
     if (prefix->count > 0 && (!prefix->groups || (a.batch.seqs > 0 && !prefix->shared))) return fail(TL_ERR_ARG, "device pointer is null");
     if (tokens == 0 || a.batch.seqs == 0) return TL_OK;
-    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix->count);
+    const SharedPlan p = shared_plan_of(tokens, heads, pages, batch, most_rows, prefix);
     if (!p.apart) return tl_paged_attention(q, q_token, q_head, dtype, tokens, heads, pages, batch, most_rows, scale, out, workspace, workspace_bytes, stream);
     if (!q || !out || !workspace) return fail(TL_ERR_ARG, "device pointer is null");
     if (most_rows < 0) return fail(TL_ERR_ARG, "most_rows is negative");

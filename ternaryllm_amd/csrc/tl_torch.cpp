@@ -398,12 +398,18 @@ PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t count)
 // Groups of the batch's sequences that begin alike; false where they are none of a plain call.
 bool prefix_of(PyObject* prefix, const tl_page_batch& b, c10::Device device, tl_page_prefix* p)
 {
-    if (!PyTuple_Check(prefix) || PyTuple_GET_SIZE(prefix) != 2) return false;
+    if (!PyTuple_Check(prefix) || PyTuple_GET_SIZE(prefix) != 3) return false;
+    const long long most = absent(PyTuple_GET_ITEM(prefix, 2)) ? -1 : PyLong_AsLongLong(PyTuple_GET_ITEM(prefix, 2));
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
     const at::Tensor *groups = member(prefix, 0), *shared = member(prefix, 1);
     for (const at::Tensor* t : {groups, shared})
         if (!t || t->scalar_type() != at::kInt || t->device() != device || t->numel() == 0 || t->dim() != 1 || !t->is_contiguous()) return false;
     if (shared->numel() != b.seqs || groups->numel() > INT32_MAX) return false;
-    *p = tl_page_prefix{static_cast<const int32_t*>(groups->data_ptr()), static_cast<const int32_t*>(shared->data_ptr()), (int32_t)(groups->numel() - 1)};
+    *p = tl_page_prefix{static_cast<const int32_t*>(groups->data_ptr()), static_cast<const int32_t*>(shared->data_ptr()), (int32_t)(groups->numel() - 1),
+                        (int32_t)std::min<long long>(std::max<long long>(most, -1), INT32_MAX)};
     return true;
 }
 

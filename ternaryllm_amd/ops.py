@@ -645,9 +645,11 @@ class PageBatch(NamedTuple):
 class PagePrefix(NamedTuple):
     """Sequences of a batch that begin with the same tokens, in the same pages.  Group g is the batch's sequences groups[g] .. groups[g + 1] - 1; each of
     them shares its first shared[b] tokens with the others: the same number in all of a group, 0 in sequences of no group, and no more than a sequence
-    has in front of its rows.  Both int32 on the device: groups [groups + 1], shared [seqs]."""
+    has in front of its rows.  Both int32 on the device: groups [groups + 1], shared [seqs].  most_shared: the most tokens that a group shares, where the host
+    knows (it chooses how they are read, results differ by the rounding of sums)."""
     groups: torch.Tensor
     shared: torch.Tensor
+    most_shared: Optional[int] = None
 
 
 _PAGE_CODE = {torch.float16: _lib.TL_F16, torch.float8_e4m3fn: _lib.TL_E4M3}
@@ -690,7 +692,8 @@ def _prefix_args(prefix, batch, device):
             raise RuntimeError(f"{what} is on {t.device}, the rows on {device}")
     if prefix.groups.numel() < 1 or prefix.shared.numel() != batch.table.shape[0]:
         raise ValueError("groups has one entry more than there are groups, shared one for each sequence")
-    return _lib.PagePrefix(prefix.groups.data_ptr(), prefix.shared.data_ptr() or None, prefix.groups.numel() - 1)
+    most = -1 if prefix.most_shared is None else min(int(prefix.most_shared), 2 ** 31 - 1)
+    return _lib.PagePrefix(prefix.groups.data_ptr(), prefix.shared.data_ptr() or None, prefix.groups.numel() - 1, most)
 
 
 def _overlap(x, y):

@@ -167,7 +167,7 @@ class PagedCache:
         # (what stands between groups is a group by itself, of which nothing is shared)
         edges = sorted({0, len(chunks), *(e for g in groups for e in g)})
         both = torch.tensor(edges + shared, dtype=torch.int32).to(self.device)
-        return ops.PagePrefix(both[:len(edges)], both[len(edges):])
+        return ops.PagePrefix(both[:len(edges)], both[len(edges):], max(shared))
 
     def whole(self, sequences):
         """The ops.PageBatch whose rows are all tokens of these sequences (what ops.read_pages reads)."""

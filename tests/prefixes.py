@@ -30,5 +30,6 @@ class Shared(paged.Sequences):
                 if rest and b != first:
                     t[int(self.table[b, at]), :, :rest] = t[int(self.table[first, at]), :, :rest]
 
-    def prefix(self, ops, device="cuda"):
-        return ops.PagePrefix(*(torch.tensor(t, dtype=torch.int32, device=device) for t in (self.groups, self.shared)))
+    def prefix(self, ops, device="cuda", most=1 << 30):
+        """(Said to be so long that they are read apart, however short they are.)"""
+        return ops.PagePrefix(*(torch.tensor(t, dtype=torch.int32, device=device) for t in (self.groups, self.shared)), most)

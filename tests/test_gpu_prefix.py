@@ -63,8 +63,10 @@ def test_the_same_bits_every_time_and_without_groups_what_the_plain_call_gives()
     got = ops.paged_attention(q, dev, batch, prefix=seqs.prefix(ops))
     for _ in range(5):
         assert torch.equal(ops.paged_attention(q, dev, batch, prefix=seqs.prefix(ops)), got)
+    plain = ops.paged_attention(q, dev, batch)
     none = ops.PagePrefix(torch.zeros(1, dtype=torch.int32).cuda(), torch.zeros(12, dtype=torch.int32).cuda())
-    assert torch.equal(ops.paged_attention(q, dev, batch, prefix=none), ops.paged_attention(q, dev, batch))
+    for prefix in (none, seqs.prefix(ops, most=None), seqs.prefix(ops, most=300)):       # (so few that they are not read apart)
+        assert torch.equal(ops.paged_attention(q, dev, batch, prefix=prefix), plain)
 
 
 def test_groups_that_do_not_hold():
@@ -127,7 +129,7 @@ def test_a_captured_call_serves_other_groups():
     q = torch.zeros((12, 8, 64), dtype=torch.float16).cuda()
     i32 = dict(dtype=torch.int32, device="cuda")
     batch = ops.PageBatch(torch.zeros((8, 24), **i32), torch.zeros(9, **i32), torch.zeros(8, **i32), 4)
-    prefix = ops.PagePrefix(torch.zeros(3, **i32), torch.zeros(8, **i32))
+    prefix = ops.PagePrefix(torch.zeros(3, **i32), torch.zeros(8, **i32), 1 << 30)
 
     def fill(i):
         seqs = prefixes.Shared(shapes[i][0], 32, widest=24, seed=i, spare=0)

@@ -98,7 +98,7 @@ def test_a_captured_pass_over_forks(model, cuda):
     tokens = torch.zeros(3, dtype=torch.long, device=cuda)
     batch = ops.PageBatch(torch.zeros((3, 20), dtype=torch.int32, device=cuda), torch.arange(4, dtype=torch.int32, device=cuda),
                           torch.zeros(3, dtype=torch.int32, device=cuda), 1)
-    prefix = ops.PagePrefix(torch.zeros(2, dtype=torch.int32, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda))
+    prefix = ops.PagePrefix(torch.zeros(2, dtype=torch.int32, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda), 1 << 30)
 
     def fill(numbers, token):
         tokens.fill_(token)
