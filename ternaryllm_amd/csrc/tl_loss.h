@@ -5,6 +5,7 @@
 namespace tl {
 
 constexpr int kPieceColumns = 16384;  // columns of P at a time, of many rows (whole units of the transposed codes)
+constexpr int kFewRows = 48;          // whose logits are kept for as long as a call takes
 constexpr int kMostTop = 1024;        // entries of a teacher's row
 
 struct TeacherArgs {

@@ -666,7 +666,7 @@ extern "C" int tl_head_loss_workspace(const tl_layout_header* header, int64_t M,
     if (int rc = check_target(target)) return rc;
     if (!bytes || M < 0 || M > (1 << 24)) return fail(TL_ERR_ARG, "a pointer is null, or %lld rows (0 to 2^24)", (long long)M);
     Parts p{nullptr};
-    if (M > kSmallMaxM) {
+    if (M > kFewRows) {
         many_parts(p, header, M, x_dtype, backward != 0);
     } else {
         int64_t product = 0;
@@ -712,7 +712,7 @@ extern "C" int tl_head_loss(const tl_layout_header* header, const void* blob_dev
     LossArgs a = loss_args(header, M, scale, scale_dtype, target);
     a.loss = loss, a.lse = lse;
     Parts p{static_cast<char*>(workspace)};
-    if (M > kSmallMaxM) {
+    if (M > kFewRows) {
         if (int rc = many_forward(header, blob_dev, x, x_dtype, ldx, a, many_parts(p, header, M, x_dtype, false), st)) return rc;
         return finish_launch();
     }
@@ -742,7 +742,7 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
     Parts p{static_cast<char*>(workspace)};
     float* ds = nullptr;                         // where the scales' gradient is summed up
     auto sum_ds = [&](float* own) { a.ds = ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : own; };
-    if (M > kSmallMaxM) {
+    if (M > kFewRows) {
         const ManyParts f = many_parts(p, header, M, x_dtype, true);
         sum_ds(f.ds);
         if (int rc = many_backward(header, blob_dev, back, x, x_dtype, ldx, a, f, st)) return rc;

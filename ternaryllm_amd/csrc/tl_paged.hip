@@ -1389,6 +1389,14 @@ SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, cons
     const int64_t together = groups > 0 ? ceil_div(tokens, groups) * group : 0;   // rows of a group and a key head, on average
     p.own = plan(most_rows * group <= 16 ? 16 : 64);
     p.prefix = plan(together <= 16 && p.own.rows == 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
+    // As many workgroups as the chip holds, half of them for the shared keys; of many rows, which are most of the work, three quarters.  (us with 512 parts for each /
+    // 256 / 384 and 128: 64 rows over 8192, 32 heads on 8, 43.1 / 35.7 / 41.8; 2 over 32768 37.7 / 32.3 / 33.7; 16 over 2048, 32 heads on 32, 30.9 / 25.1 / 31.4; 8
+    // groups of 8 87.0 / 81.8 / 107.6; 256 over 16384 in 8 bits, 32 heads on 8, 124.3 / 133.3 / 122.2.)
+    if (hd < 256) {
+        const int all = p.prefix.workgroups / 8;     // (of each: the walk has a part of the chip for each eighth of its workgroups)
+        p.prefix.workgroups = (together > 512 ? std::max(all * 3 / 4, 1) : std::max(all / 2, 1)) * 8;
+        p.own.workgroups = std::max(all - p.prefix.workgroups / 8, 1) * 8;
+    }
     // Apart where what need not be read again takes longer than the rows' pieces, which meet in a launch of their own: from 24 MB on, and as much again for every
     // 2048 rows; not where a sequence has rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32
     // heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024 (29 MB) 19.8 / 19.1; 2 over 8192 (33 MB) 24.8 / 25.3; 4 over 512, 32 heads on 32 (25 MB) 17.7 / 19.1; 8 over 4096
