@@ -492,6 +492,13 @@ PieceOfP piece_of_p(const tl_layout_header* h, int64_t M, int x_dtype)
     return PieceOfP{std::min(M, std::min(kForwardRows, std::max<int64_t>(kGradientBytes / (columns * each) / 128 * 128, 128))), columns};
 }
 
+// Rows whose logits are not kept.  (us few / many, fp16: 24 rows of 4096 over 32000 rated 26.7 / 27.1, a step 82 / 83; 33 41.7 / 32.2, 121 / 90; of 1024 24 17.3 / 15.1,
+// 60 / 58; but 33 of 2048 over 5003, whose tiles leave most of the chip idle, 15.6 / 20.7, 43 / 55.  fp32 24 of 4096 over 32000 53 / 57, 179 / 165.)
+bool takes_many(const tl_layout_header* h, int64_t M)
+{
+    return M > kFewRows || (M > kFewRows / 2 && (int64_t)h->columns > 64ll * compute_units());
+}
+
 struct ManyParts {
     int64_t rows;
     void* image;         // of the rows of x
@@ -666,7 +673,7 @@ extern "C" int tl_head_loss_workspace(const tl_layout_header* header, int64_t M,
     if (int rc = check_target(target)) return rc;
     if (!bytes || M < 0 || M > (1 << 24)) return fail(TL_ERR_ARG, "a pointer is null, or %lld rows (0 to 2^24)", (long long)M);
     Parts p{nullptr};
-    if (M > kFewRows) {
+    if (takes_many(header, M)) {
         many_parts(p, header, M, x_dtype, backward != 0);
     } else {
         int64_t product = 0;
@@ -712,7 +719,7 @@ extern "C" int tl_head_loss(const tl_layout_header* header, const void* blob_dev
     LossArgs a = loss_args(header, M, scale, scale_dtype, target);
     a.loss = loss, a.lse = lse;
     Parts p{static_cast<char*>(workspace)};
-    if (M > kFewRows) {
+    if (takes_many(header, M)) {
         if (int rc = many_forward(header, blob_dev, x, x_dtype, ldx, a, many_parts(p, header, M, x_dtype, false), st)) return rc;
         return finish_launch();
     }
@@ -742,7 +749,7 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
     Parts p{static_cast<char*>(workspace)};
     float* ds = nullptr;                         // where the scales' gradient is summed up
     auto sum_ds = [&](float* own) { a.ds = ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : own; };
-    if (M > kFewRows) {
+    if (takes_many(header, M)) {
         const ManyParts f = many_parts(p, header, M, x_dtype, true);
         sum_ds(f.ds);
         if (int rc = many_backward(header, blob_dev, back, x, x_dtype, ldx, a, f, st)) return rc;

@@ -154,6 +154,9 @@ __device__ __forceinline__ void lanes_meet()
     __builtin_amdgcn_wave_barrier();
 }
 
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+
 constexpr int kTeacherRows = 32;                                  // of a wave's, whose teacher's shares stand in LDS at a time
 constexpr int teacher_ld(int columns) { return columns + 4; }
 
@@ -214,9 +217,16 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
         }
         return;
     }
-    float s[GROUPS][C];
+    // a sum times `by` is its logit as an exponent of 2 (the products are with +-2); columns past N are none
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.4028234663852886e38f;
+    float s[GROUPS][C], by[GROUPS][C];
 #pragma unroll
-    for (int group = 0; group < GROUPS; ++group) read_scales(a.w0.scale, a.scale_f16, lane_n0 + group * 4 * C, a.N, 1.0f, s[group]);
+    for (int group = 0; group < GROUPS; ++group) {
+        read_scales(a.w0.scale, a.scale_f16, lane_n0 + group * 4 * C, a.N, 1.0f, s[group]);
+#pragma unroll
+        for (int i = 0; i < C; ++i) by[group][i] = 0.5f * (s[group][i] * l.cool) * kLog2e;
+    }
+    const bool ragged = first_n + COLUMNS > a.N;
     float* wanted = reinterpret_cast<float*>(own);
     auto find_wanted = [&](int row0) {                            // what is wanted of kTeacherRows rows from row0 on, in the wave's columns
         lanes_meet();
@@ -245,8 +255,6 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
     for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
         for (int i = 0; i < C; ++i) ds[group][i] = 0.f;
-    KernelArgs to = a;
-    to.N = l.padded;
 #pragma unroll
     for (int m = 0; m < G; ++m) {
         const int row = lane_m0 + m * 16;
@@ -254,72 +262,112 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
             if (first_m + m * 16 >= a.M) break;                   // (the same for all lanes)
             find_wanted(first_m + m * 16);
         }
-        const long long target = l.targets && row < a.M ? l.targets[row] - l.first : -1;
-        float t[GROUPS][C];
-#pragma unroll
-        for (int group = 0; group < GROUPS; ++group) {
-            const int n = lane_n0 + group * 4 * C;
-            if (l.targets) {
-#pragma unroll
-                for (int i = 0; i < C; ++i) t[group][i] = target == n + i ? 1.f : 0.f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < C / 4; ++i) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(wanted + (m % 2 * 16 + r16) * LD + n - first_n + 4 * i);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) t[group][4 * i + e] = x[e];
-                }
-            }
+        // the row's target among the wave's columns, -1: it is none of them; few waves have one of any row
+        int c = -1;
+        if (l.targets) {
+            const long long target = row < a.M ? l.targets[row] - l.first : -1;
+            if (target >= first_n && target < min(first_n + COLUMNS, a.N) && ((int)target - first_n) / C % 4 == q) c = (int)target - first_n - q * C;
         }
+        const bool some = l.targets && __builtin_amdgcn_ballot_w64(c >= 0) != 0;
+        auto share = [&](int group, float (&t)[C]) {              // of the teacher's
+#pragma unroll
+            for (int i = 0; i < C / 4; ++i) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(wanted + (m % 2 * 16 + r16) * LD + q * C + group * 4 * C + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[4 * i + e] = x[e];
+            }
+        };
         if constexpr (MODE == kLogits) {
             float z[GROUPS][C], top = -__builtin_huge_valf(), sum = 0.f, gap = 0.f;
-            bool wrong = false;
 #pragma unroll
             for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-                for (int i = 0; i < C; ++i) {
-                    float& v = z[group][i];
-                    v = 0.5f * acc[group * CF + i / 4][m][i % 4] * s[group][i] * l.cool;
-                    if (lane_n0 + group * 4 * C + i >= a.N) v = -__builtin_huge_valf();
-                    wrong |= v != v;
-                    top = fmaxf(top, v);
-                    if (t[group][i] > 0.f) gap = fmaf(t[group][i], v, gap);
-                }
-            // (a maximum passes over what is not a number: +inf, which is none either, stands for it)
-            top = with_other_rows(wrong ? __builtin_huge_valf() : top, [](float x, float y) { return fmaxf(x, y); });
+                for (int i = 0; i < C; ++i) z[group][i] = acc[group * CF + i / 4][m][i % 4] * by[group][i];
+            if (ragged) {
+#pragma unroll
+                for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+                    for (int i = 0; i < C; ++i) z[group][i] = lane_n0 + group * 4 * C + i < a.N ? z[group][i] : -__builtin_huge_valf();
+            }
+#pragma unroll
+            for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+                for (int i = 0; i < C; ++i) top = fmaxf(top, z[group][i]);
+            top = with_other_rows(top, [](float x, float y) { return fmaxf(x, y); });
+            // (what is not a number is passed over by the maximum, and comes back in the sum)
             const float base = top == -__builtin_huge_valf() ? 0.f : top;
 #pragma unroll
             for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-                for (int i = 0; i < C; ++i) sum += __expf(z[group][i] - base);
+                for (int i = 0; i < C; ++i) sum += __builtin_amdgcn_exp2f(z[group][i] - base);
             sum = with_other_rows(sum, [](float x, float y) { return x + y; });
             const int part = first_n / COLUMNS, parts = (a.N + COLUMNS - 1) / COLUMNS;
-            if (l.targets) {
-                const long long c = target - first_n;
-                if (row < a.M && c >= 0 && c < COLUMNS && (c / C & 3) == q) l.picks[row] = gap;
-            } else {
-                gap = with_other_rows(gap, [](float x, float y) { return x + y; });
-                if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap;
+            if (some) {
+#pragma unroll
+                for (int group = 0; group < GROUPS; ++group)
+#pragma unroll
+                    for (int i = 0; i < C; ++i)
+                        if (c == group * 4 * C + i) l.picks[row] = z[group][i] * kLn2;
             }
-            if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top, sum);
+            if (!l.targets) {
+#pragma unroll
+                for (int group = 0; group < GROUPS; ++group) {
+                    float t[C];
+                    share(group, t);
+#pragma unroll
+                    for (int i = 0; i < C; ++i) gap = fmaf(t[i], fmaxf(z[group][i], kLowest), gap);   // (0 of what is infinite is 0)
+                }
+                gap = with_other_rows(gap, [](float x, float y) { return x + y; });
+                if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap * kLn2;
+            }
+            if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top * kLn2, sum);
         } else {
             if (row >= a.M) continue;
-            const float lse = l.lse[row], grad = l.grad[row];
+            const float lse = l.lse[row], half_grad = 0.5f * l.grad[row];
             const bool counts = lse_counts(lse);
+            const float base = lse * kLog2e, spoiled = lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
 #pragma unroll
             for (int group = 0; group < GROUPS; ++group) {
                 const int n = lane_n0 + group * 4 * C;
                 float p[C];
+                if (counts) {
+                    float dz[C];
 #pragma unroll
-                for (int i = 0; i < C; ++i) {
-                    const float raw = 0.5f * acc[group * CF + i / 4][m][i % 4];
-                    const float dz = counts && n + i < a.N ? __expf(raw * s[group][i] * l.cool - lse) - t[group][i] : 0.f;
-                    p[i] = dz * s[group][i] * up;
-                    ds[group][i] += counts ? dz * raw * grad : lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
+                    for (int i = 0; i < C; ++i) dz[i] = __builtin_amdgcn_exp2f(fmaf(acc[group * CF + i / 4][m][i % 4], by[group][i], -base));
+                    if (some) {
+#pragma unroll
+                        for (int i = 0; i < C; ++i) dz[i] -= c == group * 4 * C + i ? 1.f : 0.f;
+                    }
+                    if (!l.targets) {
+                        float t[C];
+                        share(group, t);
+#pragma unroll
+                        for (int i = 0; i < C; ++i) dz[i] -= t[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < C; ++i) {
+                        p[i] = dz[i] * (s[group][i] * up);
+                        ds[group][i] = fmaf(dz[i] * half_grad, acc[group * CF + i / 4][m][i % 4], ds[group][i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < C; ++i) p[i] = 0.f, ds[group][i] += spoiled;
                 }
                 if (n >= l.padded) continue;
-                if (a.x_f16) store_piece<C>(to, row, n, l.padded, p);
-                else store_parts<C>(to, row, n, p);
+                if (ragged) {
+#pragma unroll
+                    for (int i = 0; i < C; ++i) p[i] = n + i < a.N ? p[i] : 0.f;
+                }
+                if (a.x_f16) {
+                    u32x4 h[C < 8 ? 1 : C / 8];
+#pragma unroll
+                    for (int i = 0; i < C / 2; ++i) h[i / 4][i % 4] = __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{p[2 * i], p[2 * i + 1]}), half2v));
+                    __half* at = static_cast<__half*>(a.Y) + (long long)row * a.ldy + n;
+                    if constexpr (C == 8) *reinterpret_cast<u32x4*>(at) = h[0];
+                    else *reinterpret_cast<uint2*>(at) = make_uint2(h[0][0], h[0][1]);
+                } else {
+                    store_parts<C>(a, row, n, p);
+                }
             }
         }
     }
