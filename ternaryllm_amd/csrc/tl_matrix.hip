@@ -499,8 +499,10 @@ __device__ __forceinline__ void put_out(const KernelArgs& a, f32x4 (&acc)[F][G],
 // share K out by units, copy for themselves, wait for nobody and add up at the end; or, WN > 1, two groups of waves that share K out
 // and whose waves share what they copy.  PARTS: 1 for fp16 activations, 3 for fp32
 // ones in bf16 parts (a stage's three parts one after the other, with the same codes).
+//
+// (Gradients of fp32 logits in 64 x 128 tiles ask for 170 registers, two more than three workgroups a unit have: 777 x 1111 -> 5003 61 us, 47 with three.)
 template <int PARTS, int WM, int WN, int WK, int FM, int FN, int MODE>
-__global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArgs a)
+__global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients && FN == 1 ? 3 : 2) void tl_matrix_rows(KernelArgs a)
 {
     constexpr int W = WM * WN;                                    // waves that work on the same rows of K, and share what is copied
     constexpr bool SHARED = W > 1;
