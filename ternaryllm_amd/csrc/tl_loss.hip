@@ -15,6 +15,9 @@ constexpr int kFewColumns = 128;                 // of a workgroup of tl_loss_fe
 constexpr int kRowThreads = 1024, kJoinThreads = 256;   // of a workgroup that takes a row of logits, of what is left of them
 constexpr float kNone = -__builtin_huge_valf();
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
 // A maximum and the sum of exponentials against it, joined with another pair.  (Nothing yet: -inf and 0.)
@@ -59,7 +62,7 @@ __device__ __forceinline__ float fold_all(float v, F f)
 // probability 0 and those added elsewhere get id -1.  known: sum t log t; +inf: the row has no teacher; NaN: one of its entries is none.
 __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
 {
-    __shared__ int ids[kMostTop];
+    __shared__ __align__(16) int ids[kMostTop];
     __shared__ float shares[kMostTop];
     const int lane = (int)threadIdx.x;
     const long long row = blockIdx.x;
@@ -88,16 +91,27 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
     wrong = __builtin_amdgcn_ballot_w64(wrong) != 0 || !(fabsf(top) < __builtin_huge_valf() || none);
+    for (int i = a.top + lane; i < (a.top + 3) / 4 * 4; i += 64) ids[i] = -2;
     __syncthreads();
     float known = 0.f;
     for (int i = lane; i < a.top; i += 64) {
-        int id = ids[i];
-        float share = 0.f;
-        for (int j = 0; j < a.top; ++j)
-            if (id >= 0 && ids[j] == id) {
-                if (j < i) id = -1;              // (added where it stands first)
-                share += shares[j];
-            }
+        int id = ids[i], same = 0;
+        // how often it is there, four entries at a time; mostly that is once
+#pragma unroll 4
+        for (int j = 0; j < (a.top + 3) / 4; ++j) {
+            const i32x4 x = reinterpret_cast<const i32x4*>(ids)[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) same += x[e] == id;
+        }
+        float share = shares[i];
+        if (id >= 0 && same > 1) {
+            share = 0.f;
+            for (int j = 0, of = id; j < a.top; ++j)
+                if (ids[j] == of) {
+                    if (j < i) id = -1;          // (added where it stands first)
+                    share += shares[j];
+                }
+        }
         share = id < 0 ? 0.f : share / sum;
         a.entry[row * a.top + i] = wrong ? -1 : id;
         a.share[row * a.top + i] = share;
@@ -144,30 +158,44 @@ __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, 
     if (tid == 0) put_divergence(a, row, lse, gap);
 }
 
-// f(a column's scale), for scales of the call's kind.  (Loads that each ask for the kind are on their way one after the other: they took 30 us of a launch.)
+// f(the scales of four columns from 4 i on, and of a column), for scales of the call's kind.  (Loads that each ask for the kind are on their way one after the
+// other, and those of a value each are many: 32000 of one workgroup's took 30 us, and 7.)
 template <typename F>
 __device__ __forceinline__ void with_scales(const LossArgs& a, F f)
 {
-    if (!a.scale) f([](int) { return 1.0f; });
-    else if (a.scale_f16) f([p = static_cast<const _Float16*>(a.scale)](int n) { return (float)p[n]; });
-    else f([p = static_cast<const float*>(a.scale)](int n) { return p[n]; });
+    auto both = [&](auto type) {
+        using T = decltype(type);
+        typedef T four __attribute__((ext_vector_type(4)));
+        const T* p = static_cast<const T*>(a.scale);
+        auto one = [=](int n) { return (float)p[n]; };
+        if (reinterpret_cast<uintptr_t>(p) % sizeof(four) == 0) f([=](int i) { return __builtin_convertvector(reinterpret_cast<const four*>(p)[i], f32x4); }, one);
+        else f([=](int i) { return f32x4{one(4 * i), one(4 * i + 1), one(4 * i + 2), one(4 * i + 3)}; }, one);
+    };
+    if (!a.scale) f([](int) { return f32x4{1.f, 1.f, 1.f, 1.f}; }, [](int) { return 1.f; });
+    else if (a.scale_f16) both(_Float16{});
+    else both(float{});
 }
 
 // The largest column scale, by one workgroup, where lse ends: what the gradients' fp16 probabilities are raised by goes by it.
 template <int WAVES>
 __device__ __forceinline__ void put_largest_scale(const LossArgs& a)
 {
-    constexpr int U = 16, THREADS = WAVES * 64;
+    constexpr int U = 8, THREADS = WAVES * 64;
     float most = a.scale ? 0.f : 1.f;
     bool wrong = false;
-    with_scales(a, [&](auto scale) {
-        for (int first = (int)threadIdx.x; first < a.N; first += THREADS * U) {
-            float s[U];
+    auto look = [&](float s) { wrong |= !finite(s), most = fmaxf(most, fabsf(s)); };
+    with_scales(a, [&](auto four, auto one) {
+        const int whole = a.N / 4;
+        for (int first = (int)threadIdx.x; first < whole; first += THREADS * U) {
+            f32x4 s[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) s[u] = scale(min(first + u * THREADS, a.N - 1));
+            for (int u = 0; u < U; ++u) s[u] = four(min(first + u * THREADS, whole - 1));
 #pragma unroll
-            for (int u = 0; u < U; ++u) wrong |= !finite(s[u]), most = fmaxf(most, fabsf(s[u]));
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) look(s[u][e]);
         }
+        if ((int)threadIdx.x < a.N - 4 * whole) look(one(4 * whole + (int)threadIdx.x));
     });
     most = fold_all<WAVES>(wrong ? __builtin_huge_valf() : most, [](float x, float y) { return fmaxf(x, y); });
     if (threadIdx.x == 0) a.lse[a.M] = most;
@@ -176,7 +204,7 @@ __device__ __forceinline__ void put_largest_scale(const LossArgs& a)
 // Few rows: their logits are in the workspace, without scales.  A workgroup takes a row, one more the scales.  Bound by latency.
 __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
 {
-    constexpr int WAVES = kRowThreads / 64, U = 8;
+    constexpr int WAVES = kRowThreads / 64, U = 4;
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
     if (row == a.M) {
         put_largest_scale<WAVES>(a);
@@ -186,24 +214,34 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
     auto z = [&](int n) { return raw[n] * load_scale(a.scale, a.scale_f16, n) * a.cool; };
     float top = kNone, sum = 0.f;
     bool wrong = false;
-    with_scales(a, [&](auto scale) {
-        for (int first = tid; first < a.N; first += kRowThreads * U) {
-            float v[U], s[U];
+    with_scales(a, [&](auto four, auto one) {
+        const int whole = a.N / 4;
+        for (int first = tid; first < whole; first += kRowThreads * U) {
+            f32x4 v[U], s[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int n = min(first + u * kRowThreads, a.N - 1);
-                v[u] = raw[n], s[u] = scale(n);
+                const int i = min(first + u * kRowThreads, whole - 1);
+                v[u] = reinterpret_cast<const f32x4*>(raw)[i], s[u] = four(i);
             }
             float most = kNone, part = 0.f;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                v[u] = first + u * kRowThreads < a.N ? v[u] * s[u] * a.cool : kNone;
-                most = fmaxf(most, v[u]), wrong |= v[u] != v[u];
-            }
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[u][e] = first + u * kRowThreads < whole ? v[u][e] * s[u][e] * a.cool : kNone;
+                    most = fmaxf(most, v[u][e]), wrong |= v[u][e] != v[u][e];
+                }
             const float base = most == kNone ? 0.f : most;
 #pragma unroll
-            for (int u = 0; u < U; ++u) part += __expf(v[u] - base);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part += __expf(v[u][e] - base);
             join(top, sum, most, part);
+        }
+        if (tid < a.N - 4 * whole) {
+            const float v = raw[4 * whole + tid] * one(4 * whole + tid) * a.cool;
+            wrong |= v != v;
+            join(top, sum, v, 1.f);
         }
     });
     // (a maximum passes over what is not a number; +inf does not count as a maximum either)

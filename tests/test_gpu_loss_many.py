@@ -92,3 +92,12 @@ def test_weights_whose_rows_repeat():
         dx = x.cuda().requires_grad_()
         loss = ops.cross_entropy(weight, dx, t.cuda(), back=ops.BackWeight(weight))
         check(ref, loss, *torch.autograd.grad(loss, dx, g.cuda()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("top", [0, 7])
+@pytest.mark.parametrize("M", [1, 3, 24, 25])
+def test_few_rows_over_the_longest_vocabularies(M, top, dtype):
+    """And the fewest rows of which logits are not kept."""
+    step(M, 16, 65537 + 5, dtype, top, 2.0 if top else 1.0, seed=M)
+    step(M, 24, 65536, dtype, top, seed=M)
