@@ -4,6 +4,8 @@ import os
 import shutil
 import subprocess
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -23,17 +25,25 @@ def hipcc():
 def build_library(verbose=True):
     """Compiles every translation unit for gfx950 and links the shared library. Always recompiles."""
     csrc = os.path.join(PKG_DIR, "csrc")
-    cmd = [
-        hipcc(), "-shared", "-fPIC", "-O3", "-std=c++17", "--offload-arch=gfx950",
+    flags = [
+        "-fPIC", "-O3", "-std=c++17", "--offload-arch=gfx950",
         # packed-fp32 VALU forms are kept out of the generated code
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-Wall", "-Wno-unused-command-line-argument",
         "-I", os.path.join(ROOT, "include"), "-I", csrc,
-        "-x", "hip",
-    ] + [os.path.join(csrc, s) for s in SOURCES] + ["-o", LIB_PATH]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+    ]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+
+    # a few units at a time: one after the other they take twice as long as the longest of them
+    with tempfile.TemporaryDirectory() as where, ThreadPoolExecutor(max_workers=min(4, os.cpu_count() or 1)) as pool:
+        objects = [os.path.join(where, s + ".o") for s in SOURCES]
+        longest = sorted(range(len(SOURCES)), key=lambda i: -os.path.getsize(os.path.join(csrc, SOURCES[i])))
+        list(pool.map(lambda i: run([hipcc(), "-c", *flags, "-x", "hip", os.path.join(csrc, SOURCES[i]), "-o", objects[i]]), longest))
+        run([hipcc(), "-shared", "-fPIC", "--offload-arch=gfx950", *objects, "-o", LIB_PATH])
     return LIB_PATH
 
 

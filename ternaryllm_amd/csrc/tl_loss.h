@@ -43,7 +43,7 @@ struct LossArgs {
 __device__ __forceinline__ float raise_of(float largest_scale)
 {
     if (!(largest_scale < __builtin_huge_valf())) return __builtin_nanf("");
-    return largest_scale > 0.f ? ldexpf(1.f, min(max(14 - ilogbf(largest_scale), -100), 100)) : 1.f;
+    return largest_scale > 0.f ? ldexpf(1.f, min(max(14 - ilogbf(largest_scale), -126), 126)) : 1.f;
 }
 
 // Whether a row has a gradient of its own: not, it counts for nothing (-inf), or its loss is NaN.

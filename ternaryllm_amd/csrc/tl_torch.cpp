@@ -11,12 +11,14 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 #include <mutex>
@@ -541,6 +543,31 @@ struct HeadLossBackward : torch::autograd::Node {
     }
 };
 
+// What accumulates a leaf's gradient belongs to the stream on which a graph first asked for it, and is the same in every graph of the leaf while one lives: a
+// captured backward pass would wait for that stream, which ends the capture in a thread of the engine's, and the process.  So such a call is refused.
+void refuse_captured(void* stream, std::initializer_list<const at::Tensor*> leaves)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
+    for (const at::Tensor* t : leaves) {
+        if (!t || !t->is_leaf()) continue;
+        const auto held = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto of = held ? held->stream() : std::nullopt;
+        TORCH_CHECK(!held || (of && of->id() == c10::hip::getCurrentHIPStream(t->device().index()).id()),
+                    "a graph of the same leaf lives outside of the captured one: let go of it first, or take a new leaf");
+    }
+}
+
+// capturable(x): raises for a leaf that a captured backward pass must not reach
+PyObject* capturable(PyObject*, PyObject* o)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor* x = plain(o);
+    if (x && x->requires_grad()) refuse_captured(current_stream(x->device()), {x});
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 // head_loss(header address, blob, transposed codes or None, x, scale or None, targets or None, ignore, ids or None, logits or None, temperature)
 // -> losses, None for a call that is not a plain one, or the library's status
 PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t count)
@@ -583,6 +610,7 @@ PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t count)
     }
     const c10::DeviceGuard guard(x->device());
     void* stream = current_stream(x->device());
+    if (by_x || by_scale) refuse_captured(stream, {by_x ? x : nullptr, by_scale ? scale : nullptr});
     const auto floats = x->options().dtype(at::kFloat).requires_grad(false);
     at::Tensor loss = at::empty({rows}, floats), lse = at::empty({rows + 1}, floats);
     const int type = type_code(*x);
@@ -657,6 +685,7 @@ PyMethodDef g_methods[] = {
     {"read_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(read_pages)), METH_FASTCALL, "rows out of pages, or None"},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, "attention over pages, or None"},
     {"head_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(head_loss)), METH_FASTCALL, "what a head's rows are worth, None, or a status"},
+    {"capturable", capturable, METH_O, "refuses a leaf whose gradient must not be captured"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tl_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -263,9 +263,14 @@ class TernaryLinear(nn.Module):
             raise ValueError("targets, ids and logits go with the input's rows")
         w, back = self.device_weight(), None
         if torch.is_grad_enabled() and input.requires_grad:
+            ops.capturable(input)
             back = self._back
             if back is None or back.blob is not w.blob:
-                back = self._back = ops.BackWeight(w)
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first gradient through a head makes its transposed codes: ask for one before a graph is captured")
+                back = ops.BackWeight(w)
+                torch.cuda.current_stream(w.device).synchronize()    # (the next call may be on another stream)
+                self._back = back
         lead, rows = input.dim() - 1, input.shape[:-1].numel()
         return rate(w, input.reshape(rows, self.in_features), [t.reshape(rows, *t.shape[lead:]) for t in wanted], back).view(input.shape[:-1])
 

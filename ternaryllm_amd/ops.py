@@ -1125,6 +1125,11 @@ class BackWeight:
             _lib.check(_lib.lib().tl_back_codes_make(ctypes.byref(weight.header), weight.blob.data_ptr(), self.codes.data_ptr(), _stream_ptr(weight.device)))
 
 
+def capturable(x):
+    """Refuses, while a graph is captured, a leaf that an eager graph holds as well: a captured backward pass must not reach it."""
+    _short().capturable(x)
+
+
 def _loss(weight, x, scale, back, targets, ignore, ids, logits, temperature):
     return _short().head_loss(ctypes.addressof(weight.header), weight.blob, None if back is None else back.codes, x, scale, targets, ignore, ids, logits, temperature)
 

@@ -186,3 +186,27 @@ def test_losses_are_differentiable_once_and_notice_changes(cuda):
     g, = torch.autograd.grad(ops.cross_entropy(weight, plain, t, s, back=back).mean(), plain)
     want = x.detach().t() @ g
     assert ((mix.grad - want).abs() <= 1e-4 * want.abs().max()).all()
+
+
+def test_captures_that_would_meet_an_eager_graph_are_refused(cuda):
+    """On the host, in front of any launch.  The capture goes on with another leaf."""
+    w, s = losses.head(64, 100, torch.float16)
+    linear = TernaryLinear(64, 100, bias=False, weight=w, scale=s, reference_buffers=False).to(cuda)
+    x, t = losses.rows(60, 64, torch.float16).cuda(), torch.arange(60).cuda()
+    leaf = x.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    fresh = linear.__class__(64, 100, bias=False, weight=w, scale=s, reference_buffers=False).to(cuda)
+    alive = linear.cross_entropy(leaf, t)
+    want, = torch.autograd.grad(alive.sum(), leaf, retain_graph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="lives outside"):
+            linear.cross_entropy(leaf, t)
+        with pytest.raises(RuntimeError, match="transposed"):
+            fresh.cross_entropy(x.detach().requires_grad_(), t)
+        other = x.detach().requires_grad_()
+        out, = torch.autograd.grad(linear.cross_entropy(other, t), other, torch.ones(60, device=cuda))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
