@@ -33,9 +33,21 @@ struct LossArgs {
     long long raw_ld;
     const float* grad;                // [M], of the losses
     void* P;                          // [rows][raw_ld], x's type
-    float* ds;                        // [N] or null
+    void* ds;                         // [N] of the scales' type, or null
     void* dx;                         // [M][dx_ld], x's type
     long long dx_ld;
+};
+
+// The gradient of the scales from its parts.
+struct ScaleGradient {
+    const float* parts;               // [count][ld]
+    int count;
+    long long ld;
+    int N;
+    float heat;
+    const float* before;              // null, or [N]: of the rows before
+    void* out;
+    int f16;
 };
 
 // The power of two that fp16 probabilities are raised by, times their columns' scales, so that the largest is 2^15 at most and those that are lost, below

@@ -272,27 +272,29 @@ __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const f
     if (threadIdx.x == 0) put_divergence(a, row, lse_of(top, sum), lse_of(top, sum) - gap);
 }
 
-// ds from its parts, rows one after the other; what rows of the call before have left in it is added to.  64 columns to a workgroup, whose waves share the
-// parts out.
-__global__ __launch_bounds__(256) void tl_loss_ds(float* ds, const float* parts, int count, long long ld, int N, float heat, int more)
+// ds from its parts, rows one after the other, and from what rows of the call before have left; 64 columns to a workgroup of four waves, which share the parts
+// out.
+__device__ __forceinline__ void put_ds(const ScaleGradient& d, int group)
 {
     __shared__ float sums[4][64];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, n = (int)blockIdx.x * 64 + lane;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, n = group * 64 + lane;
     constexpr int U = 8;
     float sum = 0.f;
-    for (int first = wave; first < count; first += 4 * U) {
+    for (int first = wave; first < d.count; first += 4 * U) {
         float v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = first + 4 * u < count && n < N ? parts[(first + 4 * u) * ld + n] : 0.f;
+        for (int u = 0; u < U; ++u) v[u] = first + 4 * u < d.count && n < d.N ? d.parts[(first + 4 * u) * d.ld + n] : 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) sum += v[u];
     }
     sums[wave][lane] = sum;
     __syncthreads();
-    if (wave != 0 || n >= N) return;
-    sum = (sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]) * heat;
-    ds[n] = more ? ds[n] + sum : sum;
+    if (wave != 0 || n >= d.N) return;
+    sum = (sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]) * d.heat;
+    store_out(d.out, d.f16, n, d.before ? d.before[n] + sum : sum);
 }
+
+__global__ __launch_bounds__(256) void tl_loss_ds(ScaleGradient d) { put_ds(d, (int)blockIdx.x); }
 
 // Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after the other.
 template <typename T>
@@ -339,14 +341,19 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
             ds += counts ? dz * raw[u] * grad[u] : lse[u] == kNone ? 0.f : __builtin_nanf("");
         }
     }
-    if (a.ds && there) a.ds[n] = ds * a.heat;
+    if (a.ds && there) store_out(a.ds, a.scale_f16, n, ds * a.heat);
 }
 
-// dx = what a row is multiplied by times the product of P, the sum of `parts` of them.  A thread takes four values of a row.
+// dx = what a row is multiplied by times the product of P, the sum of `parts` of them; a thread takes four values of a row.  The first d_groups workgroups take
+// the gradient of the scales beside it.
 template <typename T>
-__global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float* from, int rows, int parts)
+__global__ __launch_bounds__(256) void tl_loss_out(LossArgs a, const float* from, int rows, int parts, ScaleGradient d, unsigned d_groups)
 {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (blockIdx.x < d_groups) {
+        put_ds(d, (int)blockIdx.x);
+        return;
+    }
+    const long long at = (long long)(blockIdx.x - d_groups) * 256 + threadIdx.x;
     const int pieces = (a.K + 3) / 4, m = (int)(at / pieces), k = (int)(at % pieces) * 4;
     if (m >= rows) return;
     const int row = a.first + m;
@@ -367,12 +374,6 @@ __global__ __launch_bounds__(256) void tl_loss_rows_out(LossArgs a, const float*
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (k + e < a.K) to[e] = (T)settled(counts ? sum[e] * factor : factor);
-}
-
-__global__ __launch_bounds__(256) void tl_loss_scale_out(const float* ds, void* out, int f16, int N)
-{
-    const int n = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (n < N) store_out(out, f16, n, ds[n]);
 }
 
 // The codes of a weight [K][N], transposed: those of a weight of N rows and K columns.  Once for a weight; a thread makes a dword (16 weights).
@@ -466,7 +467,6 @@ struct FewParts {
     void* product;       // workspace of the product of the logits
     void* P;             // backward: [rows][ld]
     float* sums;         // [rows][K]
-    float* ds;           // [N]
 };
 
 FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, bool backward, int64_t product_bytes)
@@ -478,7 +478,6 @@ FewParts few_parts(Parts& p, const tl_layout_header* h, int64_t M, int x_dtype, 
     if (backward) {
         f.P = p.take(rows * ld * (x_dtype == TL_F16 ? 2 : 4));
         f.sums = static_cast<float*>(p.take(rows * h->inners * 4));
-        f.ds = static_cast<float*>(p.take((int64_t)h->columns * 4));
     }
     return f;
 }
@@ -489,11 +488,13 @@ int product_workspace(const tl_layout_header* h, int64_t M, int x_dtype, int64_t
     return M ? tl_spmm_workspace(h, M, x_dtype, TL_X_ROW_MAJOR, bytes) : TL_OK;
 }
 
-void rows_out(const LossArgs& a, int x_dtype, const float* sums, int rows, int parts, hipStream_t st)
+void rows_out(const LossArgs& a, int x_dtype, const float* sums, int rows, int parts, const ScaleGradient* d, hipStream_t st)
 {
-    const dim3 grid((unsigned)ceil_div((int64_t)ceil_div(a.K, 4) * rows, 256));
-    if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_rows_out<_Float16>, grid, dim3(256), 0, st, a, sums, rows, parts);
-    else hipLaunchKernelGGL(tl_loss_rows_out<float>, grid, dim3(256), 0, st, a, sums, rows, parts);
+    const ScaleGradient none{};
+    const unsigned groups = d ? (unsigned)ceil_div(d->N, 64) : 0;
+    const dim3 grid(groups + (unsigned)ceil_div((int64_t)ceil_div(a.K, 4) * rows, 256));
+    if (x_dtype == TL_F16) hipLaunchKernelGGL(tl_loss_out<_Float16>, grid, dim3(256), 0, st, a, sums, rows, parts, d ? *d : none, groups);
+    else hipLaunchKernelGGL(tl_loss_out<float>, grid, dim3(256), 0, st, a, sums, rows, parts, d ? *d : none, groups);
 }
 
 // The product of few rows of P with the transposed weight.
@@ -633,6 +634,8 @@ int many_backward(const tl_layout_header* h, const void* blob, const void* back,
         b.c0 = Codes{static_cast<const unsigned char*>(back), planes};
         b.loss = k.loss;
         b.loss.splits = f.splits;
+        ScaleGradient d{};
+        bool beside = false;                     // the rows' gradient, in one launch with it
         for (int piece = 0; piece < pieces; ++piece) {
             const int64_t n = piece * f.columns, wide = std::min<int64_t>(a.N - n, f.columns), padded = round_up(wide, 8);
             KernelArgs some = k;
@@ -643,9 +646,12 @@ int many_backward(const tl_layout_header* h, const void* blob, const void* back,
             some.loss.first = (int)n, some.loss.padded = (int)padded, some.loss.plane = f.rows * f.columns;
             some.loss.ds = a.ds ? f.ds_parts : nullptr, some.loss.ds_ld = f.columns;
             if (int rc = launch_loss(some, x_dtype, kLossGradients, st)) return rc;
-            if (a.ds)
-                hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 64)), dim3(256), 0, st, a.ds + n, f.ds_parts,
-                                   (int)ceil_div(rows, loss_part(some, x_dtype, kLossGradients)), some.loss.ds_ld, (int)wide, a.heat, (int)(m > 0));
+            // (sums of rows in several parts are kept in fp32 until the last)
+            const bool end = m + rows == a.M;
+            d = ScaleGradient{f.ds_parts, (int)ceil_div(rows, loss_part(some, x_dtype, kLossGradients)), some.loss.ds_ld, (int)wide, a.heat, m > 0 ? f.ds + n : nullptr,
+                              end ? static_cast<char*>(a.ds) + n * (a.scale_f16 ? 2 : 4) : reinterpret_cast<char*>(f.ds + n), end && a.scale_f16};
+            beside = a.ds && a.dx && f.splits > 1 && pieces == 1;
+            if (a.ds && !beside) hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 64)), dim3(256), 0, st, d);
             if (!a.dx) continue;
             // (rows of P begin with column n, those of the transposed weight with column 0: pointers meet where they would be)
             b.K = (int)(n + padded);
@@ -660,7 +666,7 @@ int many_backward(const tl_layout_header* h, const void* blob, const void* back,
         if (a.dx && f.splits > 1) {
             LossArgs some = a;
             some.first = (int)m;
-            rows_out(some, x_dtype, f.sums, rows, pieces * f.splits, st);
+            rows_out(some, x_dtype, f.sums, rows, pieces * f.splits, beside ? &d : nullptr, st);
         }
     }
     return TL_OK;
@@ -785,17 +791,13 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
     a.lse = const_cast<float*>(lse), a.grad = grad;
     a.dx = dx, a.dx_ld = dx_ld;
     Parts p{static_cast<char*>(workspace)};
-    float* ds = nullptr;                         // where the scales' gradient is summed up
-    auto sum_ds = [&](float* own) { a.ds = ds = !dscale ? nullptr : scale_dtype == TL_F32 ? static_cast<float*>(dscale) : own; };
+    a.ds = dscale;
     if (takes_many(header, M)) {
-        const ManyParts f = many_parts(p, header, M, x_dtype, true);
-        sum_ds(f.ds);
-        if (int rc = many_backward(header, blob_dev, back, x, x_dtype, ldx, a, f, st)) return rc;
+        if (int rc = many_backward(header, blob_dev, back, x, x_dtype, ldx, a, many_parts(p, header, M, x_dtype, true), st)) return rc;
     } else {
         int64_t product = 0;
         if (int rc = product_workspace(header, M, x_dtype, &product)) return rc;
         const FewParts f = few_parts(p, header, M, x_dtype, true, product);
-        sum_ds(f.ds);
         a.raw = f.raw, a.raw_ld = round_up(header->columns, 64);
         a.P = f.P;
         const dim3 groups((unsigned)ceil_div(a.raw_ld, kFewColumns));
@@ -804,10 +806,8 @@ extern "C" int tl_head_loss_backward(const tl_layout_header* header, const void*
         else hipLaunchKernelGGL(tl_loss_few_grad<float>, groups, dim3(kFewColumns), 0, st, a);
         if (dx) {
             if (int rc = back_product(header, back, a, x_dtype, f.sums, st)) return rc;
-            rows_out(a, x_dtype, f.sums, a.M, 1, st);
+            rows_out(a, x_dtype, f.sums, a.M, 1, nullptr, st);
         }
     }
-    if (dscale && scale_dtype == TL_F16)
-        hipLaunchKernelGGL(tl_loss_scale_out, dim3((unsigned)ceil_div(header->columns, 256)), dim3(256), 0, st, ds, dscale, 1, a.N);
     return finish_launch();
 }
