@@ -63,7 +63,7 @@ def weight_and_packed(K, N, sparsity, seed, device):
     return _packed[key]
 
 
-KERNEL_SOURCES = ("tl_matrix.hip", "tl_matrix.h", "tl_device.h", "tl_silu.h", "tl_layout.cpp", "tl_common.h")
+KERNEL_SOURCES = ("tl_matrix.hip", "tl_matrix.h", "tl_device.h", "tl_silu.h", "tl_loss.h", "tl_rope.h", "tl_layout.cpp", "tl_common.h")
 
 
 def kernel_source_hash():
