@@ -218,7 +218,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
         return;
     }
     // a sum times `by` is its logit as an exponent of 2 (the products are with +-2); columns past N are none
-    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.4028234663852886e38f;
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     float s[GROUPS][C], by[GROUPS][C];
 #pragma unroll
     for (int group = 0; group < GROUPS; ++group) {
@@ -315,7 +315,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                     float t[C];
                     share(group, t);
 #pragma unroll
-                    for (int i = 0; i < C; ++i) gap = fmaf(t[i], fmaxf(z[group][i], kLowest), gap);   // (0 of what is infinite is 0)
+                    for (int i = 0; i < C; ++i) gap = t[i] != 0.f ? fmaf(t[i], z[group][i], gap) : gap;   // (0 of what is infinite is 0)
                 }
                 gap = with_other_rows(gap, [](float x, float y) { return x + y; });
                 if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap * kLn2;

@@ -101,3 +101,25 @@ def test_few_rows_over_the_longest_vocabularies(M, top, dtype):
     """And the fewest rows of which logits are not kept."""
     step(M, 16, 65537 + 5, dtype, top, 2.0 if top else 1.0, seed=M)
     step(M, 24, 65536, dtype, top, seed=M)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M", [5, 60])
+def test_wanted_columns_of_no_probability(M, dtype):
+    """A column whose scale takes its logits to -inf: rows that want it have an infinite loss, the others what they have without it."""
+    K, N = 64, 300
+    w, _ = losses.head(K, N, dtype, 4)
+    w[:, 7], w[0, 7] = 0, -1
+    x = losses.rows(M, K, dtype, 4).abs().clamp(min=1)
+    s = torch.full((N,), 0.1)
+    s[7] = float("inf")
+    without = s.clone()
+    without[7] = 1e30
+    weight = device_weight(w)
+    ids = torch.arange(M)[:, None] % 5 + torch.tensor([4, 20])           # (some rows' first is 7)
+    logits = torch.randn((M, 2), generator=torch.Generator().manual_seed(1))
+    hit = (ids == 7).any(-1)
+    for rate in (lambda of: ops.distillation(weight, x.cuda(), ids.cuda(), logits.cuda(), of.cuda()), lambda of: ops.cross_entropy(weight, x.cuda(), ids[:, 0].cuda(), of.cuda())):
+        got, want = rate(s).cpu(), rate(without).cpu()
+        assert hit.any() and (got[hit] == float("inf")).all() and (want[hit] > 1e20).all()
+        assert torch.equal(got[~hit], want[~hit]) and got[~hit].isfinite().all()
