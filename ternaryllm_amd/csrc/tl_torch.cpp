@@ -14,6 +14,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -22,6 +23,8 @@
 
 #include <cmath>
 #include <mutex>
+#include <unordered_set>
+#include <vector>
 
 #include "ternary_spmm.h"
 
@@ -544,17 +547,33 @@ struct HeadLossBackward : torch::autograd::Node {
 };
 
 // What accumulates a leaf's gradient belongs to the stream on which a graph first asked for it, and is the same in every graph of the leaf while one lives: a
-// captured backward pass would wait for that stream, which ends the capture in a thread of the engine's, and the process.  So such a call is refused.
-void refuse_captured(void* stream, std::initializer_list<const at::Tensor*> leaves)
+// captured backward pass would wait for that stream, which ends the capture in a thread of the engine's, and the process.  So a call whose operands lead to one of another
+// stream is refused.
+void refuse_captured(void* stream, std::initializer_list<const at::Tensor*> operands)
 {
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
-    for (const at::Tensor* t : leaves) {
-        if (!t || !t->is_leaf()) continue;
-        const auto held = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto of = held ? held->stream() : std::nullopt;
-        TORCH_CHECK(!held || (of && of->id() == c10::hip::getCurrentHIPStream(t->device().index()).id()),
+    std::vector<torch::autograd::Node*> left;
+    std::unordered_set<torch::autograd::Node*> seen;
+    auto look = [&](torch::autograd::Node* node, c10::DeviceIndex device) {
+        if (!node || !seen.insert(node).second) return;
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+            left.push_back(node);
+            return;
+        }
+        const auto of = node->stream();
+        TORCH_CHECK(of && of->id() == c10::hip::getCurrentHIPStream(device).id(),
                     "a graph of the same leaf lives outside of the captured one: let go of it first, or take a new leaf");
+    };
+    for (const at::Tensor* t : operands) {
+        if (!t) continue;
+        const c10::DeviceIndex device = t->device().index();
+        look(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t).get() : t->grad_fn().get(), device);
+        while (!left.empty()) {
+            torch::autograd::Node* node = left.back();
+            left.pop_back();
+            for (const torch::autograd::Edge& e : node->next_edges()) look(e.function.get(), device);
+        }
     }
 }
 

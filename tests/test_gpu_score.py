@@ -210,3 +210,25 @@ def test_captures_that_would_meet_an_eager_graph_are_refused(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_captures_whose_operands_lead_to_an_eager_graph_are_refused(cuda):
+    """Rows that were worked out in the captured graph from a leaf that an eager one holds; a leaf of the captured graph's own goes on."""
+    w, s = losses.head(64, 100, torch.float16)
+    linear = TernaryLinear(64, 100, bias=False, weight=w, scale=s, reference_buffers=False).to(cuda)
+    x, t = losses.rows(60, 64, torch.float16).cuda(), torch.arange(60).cuda()
+    leaf = x.clone().requires_grad_()
+    alive = linear.cross_entropy(leaf * 0.5, t)
+    want, = torch.autograd.grad(alive.sum(), leaf, retain_graph=True)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="lives outside"):
+            linear.cross_entropy(leaf * 0.5, t)
+        other = x.detach().requires_grad_()
+        out, = torch.autograd.grad(linear.cross_entropy(other * 0.5, t), other, torch.ones(60, device=cuda))
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    del alive
