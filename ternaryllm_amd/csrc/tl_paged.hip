@@ -1389,22 +1389,41 @@ SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, cons
     const int64_t together = groups > 0 ? ceil_div(tokens, groups) * group : 0;   // rows of a group and a key head, on average
     p.own = plan(most_rows * group <= 16 ? 16 : 64);
     p.prefix = plan(together <= 16 && p.own.rows == 16 ? 16 : together <= 64 || hd == 256 ? 64 : 128);
-    // As many workgroups as the chip holds, half of them for the shared keys; of many rows, which are most of the work, three quarters.  (us with 512 parts for each /
-    // 256 / 384 and 128: 64 rows over 8192, 32 heads on 8, 43.1 / 35.7 / 41.8; 2 over 32768 37.7 / 32.3 / 33.7; 16 over 2048, 32 heads on 32, 30.9 / 25.1 / 31.4; 8
-    // groups of 8 87.0 / 81.8 / 107.6; 256 over 16384 in 8 bits, 32 heads on 8, 124.3 / 133.3 / 122.2.)
-    if (hd < 256) {
-        const int all = p.prefix.workgroups / 8;     // (of each: the walk has a part of the chip for each eighth of its workgroups)
-        p.prefix.workgroups = (together > 512 ? std::max(all * 3 / 4, 1) : std::max(all / 2, 1)) * 8;
-        p.own.workgroups = std::max(all - p.prefix.workgroups / 8, 1) * 8;
-    }
-    // Apart where what need not be read again takes longer than the rows' pieces, which meet in a launch of their own: from 24 MB on, and as much again for every
-    // 2048 rows; not where a sequence has rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32
-    // heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024 (29 MB) 19.8 / 19.1; 2 over 8192 (33 MB) 24.8 / 25.3; 4 over 512, 32 heads on 32 (25 MB) 17.7 / 19.1; 8 over 4096
-    // 20.0 / 32.4; 64 over 64 and up to 500 of their own 28.3 / 16.2; 8 groups of 32 over 256 and up to 500 63 / 50; rows of a key head: 8 sequences of 32 27.2 / 30.0,
-    // 16 of 128 43.7 / 40.0, 4 of 2000 144 / 95.)
     const int64_t keys = (int64_t)batch->table_pages * pages->page_size, shared = prefix->most_shared < 0 ? keys : prefix->most_shared;
+    // As many workgroups as the chip holds, some eighths of them for the shared keys, so that the longer of the two lists takes least; keys of their own are half as
+    // many on average as they can be, or, where the host does not know that, 256.  (us with half of them for the shared keys / three quarters / so: 64 rows over
+    // 8192, 32 heads on 8, 35.9 / 41.7 / 35.5; 256 over 8192 75.9 / 106.5 / 76.4; 200 over 32768 185 / 170 / 150; 128 over 4096, 32 heads on 32, 97.9 / 171 / 75; 256
+    // over 16384 in 8 bits, 32 heads on 8, 133 / 121 / 121.5.)
+    if (hd < 256 && groups > 0) {
+        // us that a list takes: 4.3 for each unit that a workgroup begins or goes on with, and its keys, of units of many rows 1.3 times as long where two
+        // workgroups share a compute unit; and what the bytes of both take.  (From the same cases with one to seven eighths: off by a tenth.)
+        auto takes = [&](const Plan& of, int64_t lists, int64_t rows, double each, int workgroups) {
+            const int64_t units = lists * pages->kv_heads * std::max<int64_t>(ceil_div(rows, of.rows), 1);
+            const int64_t begun = workgroups < units ? ceil_div(units, workgroups) : workgroups % units ? 2 : 1;
+            const double key = of.rows == 16 ? 0.0055 : (of.rows == 64 ? 0.017 : 0.027) * (workgroups > compute_units() ? 1.3 : 1.0);
+            return 4.3 * (double)begun + (double)units * each / workgroups * key;
+        };
+        const int64_t seqs = std::max(batch->seqs, 1);
+        const double front = (double)std::min(shared, keys), own = prefix->most_shared < 0 ? std::min(0.5 * (double)keys, 256.0) : 0.5 * ((double)keys - front);
+        const double memory = 4.3 + ((double)groups * front + (double)seqs * own) * pages->kv_heads * hd * (pages->dtype == TL_F16 ? 4 : 2) / 8e6;
+        const int eighth = std::max(p.prefix.workgroups / 64, 1) * 8;   // (whole ones of 8: the walk has a part of the chip for each eighth of its workgroups)
+        int best = 4;
+        double least = 1e30;
+        for (int i : {4, 5, 3, 6, 2, 7, 1}) {
+            const double longer = std::max(takes(p.prefix, groups, together, front, i * eighth),
+                                           takes(p.own, seqs, ceil_div(tokens, seqs) * group, own, (8 - i) * eighth));
+            const double t = std::max(longer, memory) + 0.25 * longer;   // (where memory bounds both, the lists hardly matter)
+            if (t < least) best = i, least = t;
+        }
+        p.prefix.workgroups = best * eighth, p.own.workgroups = (8 - best) * eighth;
+    }
+    // Apart where what need not be read again takes longer than the rows' pieces, which meet in a launch of their own: from 23 MB on, and as much again for every
+    // 2048 rows; not where a sequence has rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32
+    // heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024 (29 MB) 19.7 / 18.4; 2 over 8192 (33 MB) 19.4 / 25.2; 4 over 512, 32 heads on 32 (25 MB) 17.1 / 19.0; 8 over 4096
+    // 20.2 / 32.5; 64 over 64 and up to 500 of their own 24.0 / 16.1; 8 groups of 32 over 256 and up to 500 64 / 50; rows of a key head: 8 sequences of 32 26.9 / 29.9,
+    // 16 of 128 43.7 / 40.0, 4 of 2000 144 / 95.)
     const double again = (double)(batch->seqs - groups) * (double)shared * pages->kv_heads * hd * (pages->dtype == TL_F16 ? 4 : 2);
-    p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23) && again >= (24 << 20) + (double)tokens * heads * ((24 << 20) / 2048) && 2 * shared >= keys &&
+    p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23) && again >= (22 << 20) + (double)tokens * heads * ((22 << 20) / 2048) && 2 * shared >= keys &&
               most_rows * group < 128;
     return p;
 }
