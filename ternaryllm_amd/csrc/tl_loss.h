@@ -50,12 +50,16 @@ struct ScaleGradient {
     int f16;
 };
 
-// The power of two that fp16 probabilities are raised by, times their columns' scales, so that the largest is 2^15 at most and those that are lost, below
-// 2^-25, are 2^-40 of it: without it, and with the scales of a head of 4096 rows, all probabilities below 2^-19 would lose bits.
-__device__ __forceinline__ float raise_of(float largest_scale)
+// The power of two that probabilities are raised by, times their columns' scales.  fp16: so that the largest is 2^15 at most and those that are lost, below
+// 2^-25, are 2^-40 of it: without it, and with the scales of a head of 4096 rows, all probabilities below 2^-19 would lose bits.  fp32, which are multiplied in
+// scaled bf16 parts that end at 2^112 (tl_few.hip): so that the largest is 2^101 at most; nothing is lost there but of scales 2^-200 of the largest.
+// NaN where a scale is not finite: so are all gradients of rows then.
+__device__ __forceinline__ float raise_of(float largest_scale, bool f16)
 {
     if (!(largest_scale < __builtin_huge_valf())) return __builtin_nanf("");
-    return largest_scale > 0.f ? ldexpf(1.f, min(max(14 - ilogbf(largest_scale), -126), 126)) : 1.f;
+    if (!(largest_scale > 0.f)) return 1.f;
+    const int e = ilogbf(largest_scale);
+    return ldexpf(1.f, f16 ? min(max(14 - e, -126), 126) : min(100 - e, 0));
 }
 
 // Whether a row has a gradient of its own: not, it counts for nothing (-inf), or its loss is NaN.

@@ -299,7 +299,7 @@ __device__ __forceinline__ void put_ds(const ScaleGradient& d, int group)
 
 __global__ __launch_bounds__(256) void tl_loss_ds(ScaleGradient d) { put_ds(d, (int)blockIdx.x); }
 
-// Few rows, backward: P = dz s 2^e of up to 48 rows (of fp32 rows without the power of two), and ds.  A thread takes a column, all rows one after
+// Few rows, backward: P = dz s 2^e of up to 48 rows, and ds.  A thread takes a column, all rows one after
 // the other.  Bound by latency: 8.6 us for 40 rows of 5003 columns, 10 for 48 fp32 ones of 8000.
 template <typename T>
 __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
     __syncthreads();
     if (n >= a.raw_ld) return;
     const bool there = n < a.N;
-    const float s = there ? load_scale(a.scale, a.scale_f16, n) : 0.f, up = sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f;
+    const float s = there ? load_scale(a.scale, a.scale_f16, n) : 0.f, up = raise_of(a.lse[a.M], sizeof(T) == 2);
     float ds = 0.f;
     constexpr int U = 8;
     for (int m0 = 0; m0 < rows; m0 += U) {
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
             if (m0 + u >= rows) break;
             const bool counts = finite(lse[u]);
             const float dz = counts && there ? __expf(raw[u] * s * a.cool - lse[u]) - wanted[m0 + u][tid] : 0.f;
-            static_cast<T*>(a.P)[(long long)(m0 + u) * a.raw_ld + n] = (T)settled(dz * s * up);
+            static_cast<T*>(a.P)[(long long)(m0 + u) * a.raw_ld + n] = (T)settled(dz * (s * up));
             ds += counts ? dz * raw[u] * grad[u] : lse[u] == kNone ? 0.f : __builtin_nanf("");
         }
     }
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void tl_loss_out(LossArgs a, const float* from
     const int pieces = (a.K + 3) / 4, m = (int)(at / pieces), k = (int)(at % pieces) * 4;
     if (m >= rows) return;
     const int row = a.first + m;
-    const float factor = row_factor(a.lse[row], a.grad[row], a.heat, sizeof(T) == 2 ? raise_of(a.lse[a.M]) : 1.f);
+    const float factor = row_factor(a.lse[row], a.grad[row], a.heat, raise_of(a.lse[a.M], sizeof(T) == 2));
     const bool counts = lse_counts(a.lse[row]);
     float sum[4] = {};
     T* to = static_cast<T*>(a.dx) + row * a.dx_ld + k;
@@ -514,7 +514,7 @@ int back_product(const tl_layout_header* h, const void* back, const LossArgs& a,
     k.planes = (int)h->code_planes, k.units = (int)ceil_div(a.N, TL_CODE_UNIT_ROWS);
     k.c0 = Codes{static_cast<const unsigned char*>(back), k.planes};
     k.x_f16 = x_dtype == TL_F16, k.one = 1.0f;
-    k.tile_rows = 1;                             // (T = 0: there is no index stream to walk, and P's sums are finite)
+    k.tile_rows = 1;                             // (T = 0: there is no index stream to walk; P's sums are finite, or what they are multiplied by is NaN)
     return launch_matrix_few(k, x_dtype, false, st);
 }
 
@@ -634,7 +634,7 @@ int many_backward(const tl_layout_header* h, const void* blob, const void* back,
         const int rows = (int)std::min<int64_t>(a.M - m, f.rows);
         KernelArgs k = rows_product(h, blob, x, x_dtype, ldx, m, rows, a);
         if (int rc = make_loss_image(&k, x_dtype, f.image, st)) return rc;
-        k.loss.lse = a.lse + m, k.loss.grad = a.grad + m, k.loss.largest = x_dtype == TL_F16 ? a.lse + a.M : nullptr;
+        k.loss.lse = a.lse + m, k.loss.grad = a.grad + m, k.loss.largest = a.lse + a.M;
         KernelArgs b = back_args(h, x_dtype, rows);
         b.c0 = Codes{static_cast<const unsigned char*>(back), planes};
         b.loss = k.loss;

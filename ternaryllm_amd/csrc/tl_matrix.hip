@@ -192,7 +192,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
     const int lane = (int)threadIdx.x & 63, q = lane >> 4, r16 = lane & 15;
     const int first_n = lane_n0 - q * C, first_m = lane_m0 - r16;
     if constexpr (MODE == kBack) {
-        const float raised = l.largest ? raise_of(*l.largest) : 1.f;
+        const float raised = raise_of(*l.largest, a.x_f16);
         KernelArgs to = a;                                        // (of several parts each has its own)
         if (l.splits > 1) to.Y = static_cast<float*>(a.Y) + (long long)blockIdx.y * a.M * a.ldy;
 #pragma unroll
@@ -252,7 +252,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
         lanes_meet();
     };
     if (!l.targets) __syncthreads();
-    const float up = MODE == kGradients && a.x_f16 ? raise_of(*l.largest) : 1.f;
+    const float up = MODE == kGradients ? raise_of(*l.largest, a.x_f16) : 1.f;
     float ds[GROUPS][C];
 #pragma unroll
     for (int group = 0; group < GROUPS; ++group)
