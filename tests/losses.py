@@ -79,3 +79,29 @@ class Reference:
         dx = g[:, None] * ((p + U * (self.w.shape[1] + 8) * size) @ a) + half * self.dx.abs() + 2.0 ** -25
         ds = ((dz + U * (self.x.shape[0] + 4) * (self.probabilities - self.wanted).abs()) * g[:, None] * self.raw.abs()).sum(0)
         return dx, ds
+
+
+def thin_head(K, N, entries, seed=0):
+    """A weight int32 [K, N] (numpy) of `entries` weights in every column."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.zeros((K, N), dtype=torch.int32)
+    for _ in range(entries):
+        at = torch.randint(0, K, (1, N), generator=g)
+        w.scatter_(0, at, torch.randint(0, 2, (1, N), generator=g, dtype=torch.int32) * 2 - 1)
+    return w.numpy()
+
+
+def long_rows(M, K, seed=0):
+    """fp32 numbers of up to 22 bits below 4, which take all three of the bf16 parts that such rows are multiplied in: sums of four are exact in fp32 all the same."""
+    return torch.randint(-(1 << 22) + 1, 1 << 22, (M, K), generator=torch.Generator().manual_seed(seed + 6)).float() * 2.0 ** -20
+
+
+def long_scales(N, seed=0):
+    """Column scales that make logits of up to a few tens of sums of those."""
+    return torch.exp2(torch.rand(N, generator=torch.Generator().manual_seed(seed + 7)))
+
+
+def leading_parts(x, parts):
+    """fp32 rows with no more than their first `parts` bf16 parts."""
+    bits = {1: 0xffff0000, 2: 0xffffff00}[parts] - (1 << 32)
+    return (x.contiguous().view(torch.int32) & bits).view(torch.float32)

@@ -128,3 +128,16 @@ def test_the_oracles_gradients_are_those_of_differences():
                 both[i][index] += sign * 1e-5
                 total.append(float((losses.Reference(both[0], w, both[1], wanted, counts, heat=2.0).loss * g.double()).sum()))
             assert abs((total[0] - total[1]) / 2e-5 - float(grad[index])) <= 1e-6 * (1 + abs(float(grad[index])))
+
+
+@pytest.mark.parametrize("M,K,N", [(5, 72, 333), (60, 301, 333), (200, 64, 5003)])
+def test_rows_of_all_bits_would_show_a_part_that_is_lost(M, K, N):
+    """What the GPU's losses of fp32 rows are tried on: sums that are exact, and bounds that the oracle itself passes with none of its rows' bf16 parts left out."""
+    w, x, s = losses.thin_head(K, N, 4, M), losses.long_rows(M, K, M), losses.long_scales(N, M)
+    t, g = torch.randint(0, N, (M,), generator=torch.Generator().manual_seed(M)), torch.rand(M, generator=torch.Generator().manual_seed(1)) + 0.25
+    ref = losses.Reference(x, w, s, *losses.targets(t, N), grad=g)
+    assert torch.equal(ref.raw, ref.raw.float().double()) and float(ref.raw.abs().max()) < 16
+    dx_bound, ds_bound = ref.gradient_bounds()
+    for parts in (1, 2):
+        less = losses.Reference(losses.leading_parts(x, parts), w, s, *losses.targets(t, N), grad=g)
+        assert ((less.loss - ref.loss).abs() > 2 * ref.loss_bound()).any() and ((less.ds - ref.ds).abs() > 2 * ds_bound).any()
