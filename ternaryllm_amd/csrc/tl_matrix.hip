@@ -177,13 +177,78 @@ __device__ __forceinline__ void store_parts(const KernelArgs& a, int m, int n, c
     }
 }
 
+// Whether all of a row's activations are.
+__device__ __forceinline__ bool finite_row(const KernelArgs& a, int m)
+{
+    const CallersX x = callers_x(a, m);
+    bool fine = true;
+#pragma unroll 8
+    for (int k = 0; k < a.K; ++k) fine &= fabsf(x(k)) < __builtin_huge_valf();
+    return fine;
+}
+
+// A sum that is not finite is worked out again by the lane that holds it, before anything is stored: the outputs of
+// finite rows keep their bits whatever another row of the tile holds.  (The sums that need it go into a mask that a
+// loop takes bit by bit, so that the walk stands here once and the sums stay in registers.)  put_out's arguments; returns what the sums, and all others of
+// the lane, are to be multiplied by.
+template <int CF, int FW, int F, int G, int MODE>
+__device__ __forceinline__ float finite_sums(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0)
+{
+    constexpr int C = 4 * CF, GROUPS = FW / CF, ALL = F / CF * G;
+    bool fine = true;
+    float half = 0.5f;                                            // (the products are with +-2)
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int m = 0; m < G; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[f][m][e]) < __builtin_huge_valf();
+    if (!fine) {
+        half = 1.0f;
+#pragma unroll 1
+        for (int i = 0; i < ALL; ++i) {
+            const int group = i / G, m = i % G, n = lane_n0 + group % GROUPS * 4 * C;
+            float v[C];
+            uint32_t redo = 0;
+#pragma unroll
+            for (int e = 0; e < C; ++e) {
+                v[e] = acc[e / 4][0][e % 4];
+#pragma unroll
+                for (int o = 1; o < ALL; ++o) v[e] = o == i ? acc[o / G * CF + e / 4][o % G][e % 4] : v[e];
+                const bool mine = lane_m0 + m * 16 < a.M && n + e < a.N;
+                redo |= mine && !(fabsf(v[e]) < __builtin_huge_valf()) ? 1u << e : 0u;
+                v[e] *= 0.5f;                                     // (twice what is worked out again might overflow)
+            }
+            if constexpr (MODE >= kLogits) {                      // (a row that is not finite is to be NaN: it need not be walked, a long way for all of its columns)
+                if (redo != 0 && !finite_row(a, lane_m0 + m * 16)) {
+#pragma unroll
+                    for (int e = 0; e < C; ++e) v[e] = __builtin_nanf("");
+                    redo = 0;
+                }
+            }
+            while (redo != 0) {
+                const int at = __builtin_ctz(redo);
+                redo &= redo - 1;
+                const float y = exact_output(a, group >= GROUPS ? a.w1 : a.w0, lane_m0 + m * 16, n + at + (MODE >= kLogits ? a.loss.first : 0));
+#pragma unroll
+                for (int e = 0; e < C; ++e) v[e] = e == at ? y : v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < C; ++e)
+#pragma unroll
+                for (int o = 0; o < ALL; ++o) acc[o / G * CF + e / 4][o % G][e % 4] = o == i ? v[e] : acc[o / G * CF + e / 4][o % G][e % 4];
+        }
+    }
+    return half;
+}
+
 // The last steps of a head's losses (put_out's arguments; own: LDS of the wave's own, kTeacherRows * teacher_ld floats of it, once every wave of the
 // workgroup is done with its buffers).  A row's logits lie with four lanes; a wave leaves their maximum and sum for its columns.  Its teacher's entries are
 // few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.
 // Measured (fp16, 128 x 256 tiles, whole kernels): 4096 rows of 4096 over 32000 columns, logits 618 to 690 us with the clock (1.56 to 1.74 PFLOP/s; 32000 logits of a row are
 // 500 pairs of 8 bytes), gradients 748 in two launches, the product of P 688; with 32 entries of a teacher 2048 rows' logits take 394, gradients 415, the
 // product 380.  Each kernel is its product: the exponentials (two a logit in all) and what is stored are beside other workgroups' products.
-template <int CF, int FW, int F, int G, int MODE>
+template <int CF, int FW, int F, int G, int MODE, bool F32>
 __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0, unsigned char* own)
 {
     constexpr int C = 4 * CF, GROUPS = FW / CF, COLUMNS = 16 * FW, LD = teacher_ld(COLUMNS);
@@ -220,14 +285,17 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
         }
         return;
     }
-    // a sum times `by` is its logit as an exponent of 2 (the products are with +-2); columns past N are none
+    // (the products are with +-2; of fp16 rows only those that are not finite have sums that are not)
+    float half = 0.5f;
+    if constexpr (F32) half = finite_sums<CF, FW, F, G, MODE>(a, acc, lane_m0, lane_n0);
+    // a sum times `by` is its logit as an exponent of 2; columns past N are none
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     float s[GROUPS][C], by[GROUPS][C];
 #pragma unroll
     for (int group = 0; group < GROUPS; ++group) {
         read_scales(a.w0.scale, a.scale_f16, lane_n0 + group * 4 * C, a.N, 1.0f, s[group]);
 #pragma unroll
-        for (int i = 0; i < C; ++i) by[group][i] = 0.5f * (s[group][i] * l.cool) * kLog2e;
+        for (int i = 0; i < C; ++i) by[group][i] = half * (s[group][i] * l.cool) * kLog2e;
     }
     const bool ragged = first_n + COLUMNS > a.N;
     float* wanted = reinterpret_cast<float*>(own);
@@ -326,7 +394,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
             if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top * kLn2, sum);
         } else {
             if (row >= a.M) continue;
-            const float lse = l.lse[row], half_grad = 0.5f * l.grad[row];
+            const float lse = l.lse[row], half_grad = half * l.grad[row];
             const bool counts = lse_counts(lse);
             const float base = lse * kLog2e, spoiled = lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
 #pragma unroll
@@ -392,51 +460,12 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
 
 // A lane's sums of G rows on their way out: C = 4 * CF neighbouring columns of each row from each CF fragments, of one weight or of
 // two (fragments FW and on).  lane_m0 and lane_n0: its first row, of rows 16 apart, and its first column, of groups 4 * C apart.
-// A sum that is not finite is worked out again by the lane that holds it, before anything is stored: the outputs of
-// finite rows keep their bits whatever another row of the tile holds.  (The sums that need it go into a mask that a
-// loop takes bit by bit, so that the walk stands here once and the sums stay in registers.)
 template <int CF, int FW, int F, int G, int MODE>
 __device__ __forceinline__ void put_out(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0)
 {
-    constexpr int C = 4 * CF, GROUPS = FW / CF, ALL = F / CF * G;
+    constexpr int C = 4 * CF, GROUPS = FW / CF;
     static_assert(F == (MODE == kTwoWeights ? 2 : 1) * FW && FW % CF == 0);
-    bool fine = true;
-    float half = 0.5f;                                            // (the products are with +-2)
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int m = 0; m < G; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[f][m][e]) < __builtin_huge_valf();
-    if (!fine) {
-        half = 1.0f;
-#pragma unroll 1
-        for (int i = 0; i < ALL; ++i) {
-            const int group = i / G, m = i % G, n = lane_n0 + group % GROUPS * 4 * C;
-            float v[C];
-            uint32_t redo = 0;
-#pragma unroll
-            for (int e = 0; e < C; ++e) {
-                v[e] = acc[e / 4][0][e % 4];
-#pragma unroll
-                for (int o = 1; o < ALL; ++o) v[e] = o == i ? acc[o / G * CF + e / 4][o % G][e % 4] : v[e];
-                const bool mine = lane_m0 + m * 16 < a.M && n + e < a.N;
-                redo |= mine && !(fabsf(v[e]) < __builtin_huge_valf()) ? 1u << e : 0u;
-                v[e] *= 0.5f;                                     // (twice what is worked out again might overflow)
-            }
-            while (redo != 0) {
-                const int at = __builtin_ctz(redo);
-                redo &= redo - 1;
-                const float y = exact_output(a, group >= GROUPS ? a.w1 : a.w0, lane_m0 + m * 16, n + at);
-#pragma unroll
-                for (int e = 0; e < C; ++e) v[e] = e == at ? y : v[e];
-            }
-#pragma unroll
-            for (int e = 0; e < C; ++e)
-#pragma unroll
-                for (int o = 0; o < ALL; ++o) acc[o / G * CF + e / 4][o % G][e % 4] = o == i ? v[e] : acc[o / G * CF + e / 4][o % G][e % 4];
-        }
-    }
+    const float half = finite_sums<CF, FW, F, G, MODE>(a, acc, lane_m0, lane_n0);   // (the products are with +-2)
     float s0[GROUPS][C], s1[MODE == kTwoWeights ? GROUPS : 1][C];
 #pragma unroll
     for (int group = 0; group < GROUPS; ++group) {
@@ -756,7 +785,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients
                     for (int e = 0; e < 4; ++e) v[f][g][e] += high[e];
                 }
             }
-        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, HALF, MODE>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
+        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, HALF, MODE, F32>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
         else put_out<CF, FW, F, HALF, MODE>(a, v, m0 + wk * HALF * 16 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
     } else if constexpr (WK > 1) {
         // every wave has sums of the whole tile, of its own rows of K: they meet in LDS (a wave's in its own part, which it is
@@ -804,7 +833,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients
 #pragma unroll
                 for (int m = 0; m < G; ++m) add_low(acc[f][m], low[f][m]);
         }
-        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, G, MODE>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
+        if constexpr (MODE >= kLogits) put_loss<CF, FW, F, G, MODE, F32>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF, teacher);
         else put_out<CF, FW, F, G, MODE>(a, acc, m0 + wm * FM * 32 + r16, nb0 * 16 + wn * WAVE_N + q * 4 * CF);
     }
 }

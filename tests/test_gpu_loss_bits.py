@@ -44,3 +44,24 @@ def test_rows_of_all_bits(M, K, N, top):
 def test_rows_of_all_bits_in_parts():
     """More rows than the workspace of a backward pass takes at a time."""
     step(1700, 16, 16500, losses.long_rows(1700, 16), losses.long_scales(16500))
+
+
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("M,K,N", SIZES[:4])
+def test_rows_near_the_end_of_the_range(M, K, N, top):
+    """Up to 2^120, where scaled bf16 parts leave fp32's range, with scales that make ordinary logits of them."""
+    step(M, K, N, losses.long_rows(M, K, M), losses.long_scales(N, M), 2.0 ** 118, top)
+
+
+@pytest.mark.parametrize("M,K,N", [(6, 72, 333), (70, 72, 333), (70, 72, 5003)])
+def test_rows_beside_such_rows_keep_their_bits(M, K, N):
+    w, s = losses.thin_head(K, N, 4, M), losses.long_scales(N, M) * 2.0 ** -118
+    x, t, g, weight = losses.long_rows(M, K, M), some_targets(M, N, K), spread(M, N), device_weight(w)
+    plain = graded(weight, x, t, s, g)
+    large = [3, M - 2]
+    x[large] *= 2.0 ** 118
+    got = graded(weight, x, t, s, g)
+    others = [m for m in range(M) if m not in large]
+    assert torch.equal(got[0][others], plain[0][others]) and torch.equal(got[1][others], plain[1][others])
+    alone = graded(weight, x[large], t[large], s, g[large])
+    assert ((got[0][large] - alone[0]).abs() <= 1e-4).all() and got[1][large].isfinite().all() and got[2].isfinite().all()
