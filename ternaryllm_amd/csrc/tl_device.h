@@ -48,10 +48,10 @@ struct LossRows {
     unsigned top_magic;          // ceil(2^32 / top)
     int first;                   // the weight's first column among all of the head's
     float cool, heat;            // 1 / temperature, and it
-    float2* parts;               // logits: [M][parts of the columns]: maximum, sum of exponentials against it
+    float2* parts;               // logits, as exponents of 2: [M][parts of the columns]: maximum, sum of exponentials against it
     float* gaps;                 // ... [M][parts]: sum of t z
     float* picks;                // ... [M]: the target's logit
-    const float *lse, *grad;     // gradients: [M]
+    const float *lse, *grad;     // gradients: [M], lse as an exponent of 2
     const float* largest;        // ... the largest column scale
     int padded;                  // ... columns of P, the last ones 0
     long long plane;             // ... of fp32 rows: between the parts of P

@@ -28,7 +28,8 @@ struct LossArgs {
     long long ignore;
     const int* entry;                 // [M][top], -1: none
     const float *share, *known;
-    float *loss, *lse;                // [M], [M + 1]: what the backward pass keeps, and the largest column scale
+    float *loss, *lse;                // [M], [M + 1]: what the backward pass keeps (of many rows as an exponent of 2, as their product takes it), and the largest
+                                      // column scale
     const float* raw;                 // [rows][raw_ld]: products without scales
     long long raw_ld;
     const float* grad;                // [M], of the losses
@@ -60,6 +61,14 @@ __device__ __forceinline__ float raise_of(float largest_scale, bool f16)
     if (!(largest_scale > 0.f)) return 1.f;
     const int e = ilogbf(largest_scale);
     return ldexpf(1.f, f16 ? min(max(14 - e, -126), 126) : min(100 - e, 0));
+}
+
+// A product that is rounded before anything is taken off it.  (A large logit less one that the same was made of is 0, and its exponential 1; as one
+// instruction with the subtraction it would be what the rounding had dropped, from 2^24 on whole numbers, and its exponential 0 or infinite.)
+__device__ __forceinline__ float rounded_product(float x, float y)
+{
+#pragma clang fp contract(off)
+    return x * y;
 }
 
 // Whether a row has a gradient of its own: not, it counts for nothing (-inf), or its loss is NaN.

@@ -13,33 +13,35 @@ namespace {
 
 constexpr int kFewColumns = 128;                 // of a workgroup of tl_loss_few_grad
 constexpr int kRowThreads = 1024, kJoinThreads = 256;   // of a workgroup that takes a row of logits, of what is left of them
-constexpr float kNone = -__builtin_huge_valf();
+constexpr float kNone = -__builtin_huge_valf(), kLn2 = 0.6931471805599453f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
-// A maximum and the sum of exponentials against it, joined with another pair.  (Nothing yet: -inf and 0.)
+// A maximum and the sum of exponentials against it (E2: of 2), joined with another pair.  (Nothing yet: -inf and 0.)
+template <bool E2>
 __device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2)
 {
     const float now = fmaxf(top, top2), base = now == kNone ? 0.f : now;
-    sum = sum * __expf(top - base) + sum2 * __expf(top2 - base);
+    auto power = [](float x) { return E2 ? __builtin_amdgcn_exp2f(x) : __expf(x); };
+    sum = sum * power(top - base) + sum2 * power(top2 - base);
     top = now;
 }
 
 // The same over a workgroup of WAVES waves; the result in all threads.
-template <int WAVES>
+template <int WAVES, bool E2>
 __device__ __forceinline__ void join_all(float& top, float& sum)
 {
     __shared__ float tops[WAVES], sums[WAVES];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) join(top, sum, __shfl_xor(top, off, 64), __shfl_xor(sum, off, 64));
+    for (int off = 1; off < 64; off <<= 1) join<E2>(top, sum, __shfl_xor(top, off, 64), __shfl_xor(sum, off, 64));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, sums[threadIdx.x >> 6] = sum;
     __syncthreads();
     top = kNone, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) join(top, sum, tops[i], sums[i]);
+    for (int i = 0; i < WAVES; ++i) join<E2>(top, sum, tops[i], sums[i]);
     __syncthreads();
 }
 
@@ -123,9 +125,10 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
     if (lane == 0) a.known[row] = wrong ? __builtin_nanf("") : none ? __builtin_huge_valf() : known;
 }
 
-__device__ __forceinline__ float lse_of(float top, float sum) { return finite(top) ? top + logf(sum) : __builtin_nanf(""); }
+template <bool E2>
+__device__ __forceinline__ float lse_of(float top, float sum) { return finite(top) ? top + (E2 ? log2f(sum) : logf(sum)) : __builtin_nanf(""); }
 
-// A row's divergence from sum t (lse - z), by one thread.
+// A row's divergence from sum t (lse - z), by one thread; lse: as it is kept.
 __device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float lse, float gap)
 {
     const float known = a.known[row];
@@ -134,18 +137,18 @@ __device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float
     a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
 }
 
-// A row's loss from its lse and its entries' logits (z(entry), each asked for by one thread of the workgroup), and what the backward pass wants of it: lse,
-// NaN where the loss is, -inf for a row that counts for nothing.
-template <int WAVES, typename Z>
+// A row's loss from its lse and its entries' logits (z(entry), each asked for by one thread of the workgroup; E2: all as exponents of 2), and what the backward
+// pass wants of it: lse, NaN where the loss is, -inf for a row that counts for nothing.
+template <int WAVES, bool E2, typename Z>
 __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, float sum, Z z)
 {
     const int tid = (int)threadIdx.x;
-    const float lse = lse_of(top, sum);
+    const float lse = lse_of<E2>(top, sum);
     if (a.targets) {
         if (tid != 0) return;
         const long long target = a.targets[row];
         const bool counts = target != a.ignore, there = target >= 0 && target < a.N;
-        const float loss = !counts ? 0.f : there ? lse - z((int)target, 0) : __builtin_nanf("");
+        const float loss = !counts ? 0.f : there ? (lse - z((int)target, 0)) * (E2 ? kLn2 : 1.f) : __builtin_nanf("");
         a.loss[row] = loss;
         a.lse[row] = !counts ? kNone : there ? lse : __builtin_nanf("");
         return;
@@ -156,7 +159,7 @@ __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, 
         if (id >= 0) gap = fmaf(a.share[(long long)row * a.top + i], lse - z(id, i), gap);
     }
     gap = fold_all<WAVES>(gap, [](float x, float y) { return x + y; });
-    if (tid == 0) put_divergence(a, row, lse, gap);
+    if (tid == 0) put_divergence(a, row, lse, gap * (E2 ? kLn2 : 1.f));
 }
 
 // f(the scales of four columns from 4 i on, and of a column), for scales of the call's kind.  (Loads that each ask for the kind are on their way one after the
@@ -176,6 +179,9 @@ __device__ __forceinline__ void with_scales(const LossArgs& a, F f)
     else if (a.scale_f16) both(_Float16{});
     else both(float{});
 }
+
+// A logit from its product, as it is rounded in both passes.
+__device__ __forceinline__ float logit_of(const LossArgs& a, float raw, float scale) { return rounded_product(rounded_product(raw, scale), a.cool); }
 
 // The largest column scale, by one workgroup, where lse ends: what the gradients' fp16 probabilities are raised by goes by it.
 template <int WAVES>
@@ -213,7 +219,7 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
         return;
     }
     const float* raw = a.raw + (long long)blockIdx.x * a.raw_ld;
-    auto z = [&](int n) { return raw[n] * load_scale(a.scale, a.scale_f16, n) * a.cool; };
+    auto z = [&](int n) { return logit_of(a, raw[n], load_scale(a.scale, a.scale_f16, n)); };
     float top = kNone, sum = 0.f;
     bool wrong = false;
     with_scales(a, [&](auto four, auto one) {
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[u][e] = first + u * kRowThreads < whole ? v[u][e] * s[u][e] * a.cool : kNone;
+                    v[u][e] = first + u * kRowThreads < whole ? logit_of(a, v[u][e], s[u][e]) : kNone;
                     most = fmaxf(most, v[u][e]), wrong |= v[u][e] != v[u][e];
                 }
             const float base = most == kNone ? 0.f : most;
@@ -238,21 +244,21 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) part += __expf(v[u][e] - base);
-            join(top, sum, most, part);
+            join<false>(top, sum, most, part);
         }
         if (tid < a.N - 4 * whole) {
-            const float v = raw[4 * whole + tid] * one(4 * whole + tid) * a.cool;
+            const float v = logit_of(a, raw[4 * whole + tid], one(4 * whole + tid));
             wrong |= v != v;
-            join(top, sum, v, 1.f);
+            join<false>(top, sum, v, 1.f);
         }
     });
     // (a maximum passes over what is not a number; +inf does not count as a maximum either)
     if (wrong) top = __builtin_huge_valf();
-    join_all<WAVES>(top, sum);
-    put_loss<WAVES>(a, row, top, sum, [&](int n, int) { return z(n); });
+    join_all<WAVES, false>(top, sum);
+    put_loss<WAVES, false>(a, row, top, sum, [&](int n, int) { return z(n); });
 }
 
-// Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted.  A workgroup takes a row, one more the scales.
+// Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted, all as exponents of 2.  A workgroup takes a row, one more the scales.
 // 5 us for 40 rows of 500 parts, 12 for 4096 (16 MB).
 __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
 {
@@ -263,16 +269,17 @@ __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const f
     }
     const float2* own = parts + (long long)blockIdx.x * count;
     float top = kNone, sum = 0.f;
-    for (int i = (int)threadIdx.x; i < count; i += 256) join(top, sum, own[i].x, own[i].y);
-    join_all<4>(top, sum);
+    for (int i = (int)threadIdx.x; i < count; i += 256) join<true>(top, sum, own[i].x, own[i].y);
+    join_all<4, true>(top, sum);
     if (a.targets) {
-        put_loss<4>(a, row, top, sum, [&](int, int) { return picks[blockIdx.x]; });
+        put_loss<4, true>(a, row, top, sum, [&](int, int) { return picks[blockIdx.x]; });
         return;
     }
     float gap = 0.f;
     for (int i = (int)threadIdx.x; i < count; i += 256) gap += gaps[(long long)blockIdx.x * count + i];
     gap = fold_all<4>(gap, [](float x, float y) { return x + y; });
-    if (threadIdx.x == 0) put_divergence(a, row, lse_of(top, sum), lse_of(top, sum) - gap);
+    const float lse = lse_of<true>(top, sum);
+    if (threadIdx.x == 0) put_divergence(a, row, lse, (lse - gap) * kLn2);
 }
 
 // ds from its parts, rows one after the other, and from what rows of the call before have left; 64 columns to a workgroup of four waves, which share the parts
@@ -340,7 +347,7 @@ __global__ __launch_bounds__(kFewColumns) void tl_loss_few_grad(LossArgs a)
         for (int u = 0; u < U; ++u) {
             if (m0 + u >= rows) break;
             const bool counts = finite(lse[u]);
-            const float dz = counts && there ? __expf(raw[u] * s * a.cool - lse[u]) - wanted[m0 + u][tid] : 0.f;
+            const float dz = counts && there ? __expf(logit_of(a, raw[u], s) - lse[u]) - wanted[m0 + u][tid] : 0.f;
             static_cast<T*>(a.P)[(long long)(m0 + u) * a.raw_ld + n] = (T)settled(dz * (s * up));
             ds += counts ? dz * raw[u] * grad[u] : lse[u] == kNone ? 0.f : __builtin_nanf("");
         }

@@ -289,7 +289,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
     float half = 0.5f;
     if constexpr (F32) half = finite_sums<CF, FW, F, G, MODE>(a, acc, lane_m0, lane_n0);
     // a sum times `by` is its logit as an exponent of 2; columns past N are none
-    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+    constexpr float kLog2e = 1.4426950408889634f;
     float s[GROUPS][C], by[GROUPS][C];
 #pragma unroll
     for (int group = 0; group < GROUPS; ++group) {
@@ -353,7 +353,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
 #pragma unroll
             for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-                for (int i = 0; i < C; ++i) z[group][i] = acc[group * CF + i / 4][m][i % 4] * by[group][i];
+                for (int i = 0; i < C; ++i) z[group][i] = rounded_product(acc[group * CF + i / 4][m][i % 4], by[group][i]);
             if (ragged) {
 #pragma unroll
                 for (int group = 0; group < GROUPS; ++group)
@@ -378,7 +378,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                 for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
                     for (int i = 0; i < C; ++i)
-                        if (c == group * 4 * C + i) l.picks[row] = z[group][i] * kLn2;
+                        if (c == group * 4 * C + i) l.picks[row] = z[group][i];
             }
             if (!l.targets) {
 #pragma unroll
@@ -389,14 +389,14 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                     for (int i = 0; i < C; ++i) gap = t[i] != 0.f ? fmaf(t[i], z[group][i], gap) : gap;   // (0 of what is infinite is 0)
                 }
                 gap = with_other_rows(gap, [](float x, float y) { return x + y; });
-                if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap * kLn2;
+                if (q == 0 && row < a.M && part < parts) l.gaps[(long long)row * parts + part] = gap;
             }
-            if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top * kLn2, sum);
+            if (q == 0 && row < a.M && part < parts) l.parts[(long long)row * parts + part] = make_float2(top, sum);
         } else {
             if (row >= a.M) continue;
             const float lse = l.lse[row], half_grad = half * l.grad[row];
             const bool counts = lse_counts(lse);
-            const float base = lse * kLog2e, spoiled = lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
+            const float spoiled = lse == -__builtin_huge_valf() ? 0.f : __builtin_nanf("");
 #pragma unroll
             for (int group = 0; group < GROUPS; ++group) {
                 const int n = lane_n0 + group * 4 * C;
@@ -404,7 +404,7 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
                 if (counts) {
                     float dz[C];
 #pragma unroll
-                    for (int i = 0; i < C; ++i) dz[i] = __builtin_amdgcn_exp2f(fmaf(acc[group * CF + i / 4][m][i % 4], by[group][i], -base));
+                    for (int i = 0; i < C; ++i) dz[i] = __builtin_amdgcn_exp2f(rounded_product(acc[group * CF + i / 4][m][i % 4], by[group][i]) - lse);
                     if (some) {
 #pragma unroll
                         for (int i = 0; i < C; ++i) dz[i] -= c == group * 4 * C + i ? 1.f : 0.f;

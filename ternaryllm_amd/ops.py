@@ -1169,8 +1169,8 @@ def _loss_result(y):
 def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
     """-log softmax((x @ W) * scale)[row, targets[row]] for every row of x [rows, K], float32 [rows], without keeping the logits [rows, N].  targets: int64
     [rows]; a row whose target is `ignore` has loss and gradient 0, one whose target is no column NaN.  x and scale [N]: float16 or float32.
-    Differentiable once by x, with back = BackWeight(weight), and by scale; logits, sums and what is kept are fp32, x's gradient takes the
-    distribution's in x's type.  A row with a logit that is NaN or +inf has loss NaN, one that is not finite may
+    Differentiable once by x, with back = BackWeight(weight), and by scale; logits, sums and what is kept are fp32 (a row's logarithm of its sum is: the
+    gradients' probabilities are off by 2^-23 of its largest logit, relative), x's gradient takes the distribution's in x's type.  A row with a logit that is NaN or +inf has loss NaN, one that is not finite may
     have (which makes the scales' gradient NaN), and no other row has it of it; one that wants a column of logit -inf has an infinite loss."""
     if back is None or back.blob is weight.blob:
         y = _loss(weight, x, scale, back, targets, ignore, None, None, 1.0)
