@@ -716,6 +716,7 @@ typedef struct tl_loss_target {
 /* A teacher's top logits as the losses take them: probabilities t = softmax(logits / temperature) over the `top` (1 to 1024) entries of a row, ids
  * [M][ids_ld] naming columns of the head.  An entry of logit -inf is none, whatever its id; a repeated id's probabilities add up; a row of -inf alone
  * has no teacher (loss and gradient 0); a row with a logit that is NaN or +inf, or with an id that is no column, is NaN.
+ *   temperature  1e-6 to 1e6
  *   entries, shares [M][top], known [M]: the columns that are named (-1: none), each once, their probabilities, and sum t log t */
 int tl_teacher_entries(const int64_t* ids, int64_t ids_ld, const void* logits, int dtype, int64_t logits_ld, int64_t M, int top, int columns,
                        float temperature, int32_t* entries, float* shares, float* known, void* stream);

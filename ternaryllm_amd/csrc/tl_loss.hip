@@ -427,10 +427,16 @@ int check_weight(const tl_layout_header* h, const void* blob)
     return TL_OK;
 }
 
+// (Its square and its reciprocal are factors of results, and the reciprocal of logits: all of them fp32 numbers of full precision.)
+int check_temperature(float t)
+{
+    return t >= 1e-6f && t <= 1e6f ? TL_OK : fail(TL_ERR_ARG, "temperature=%g is no number from 1e-6 to 1e6", (double)t);
+}
+
 int check_target(const tl_loss_target* t)
 {
     if (!t) return fail(TL_ERR_ARG, "null pointer");
-    if (!(t->temperature > 0.f) || t->temperature > 1e6f) return fail(TL_ERR_ARG, "temperature=%g is not a positive number up to 1e6", (double)t->temperature);
+    if (int rc = check_temperature(t->temperature)) return rc;
     if ((t->targets != nullptr) == (t->entries != nullptr)) return fail(TL_ERR_ARG, "either targets or a teacher's entries");
     if (t->targets && t->temperature != 1.f) return fail(TL_ERR_ARG, "cross entropy has no temperature");
     if (t->entries && (t->top < 1 || t->top > kMostTop)) return fail(TL_ERR_ARG, "%d entries of a teacher (1 to %d)", t->top, kMostTop);
@@ -692,7 +698,7 @@ extern "C" int tl_teacher_entries(const int64_t* ids, int64_t ids_ld, const void
     if (int rc = check_dtype(dtype, "logits")) return rc;
     if (M < 0 || M > (1 << 24) || columns < 1) return fail(TL_ERR_SHAPE, "%lld rows over %d columns", (long long)M, columns);
     if (top < 1 || top > kMostTop) return fail(TL_ERR_ARG, "%d entries of a teacher (1 to %d)", top, kMostTop);
-    if (!(temperature > 0.f) || temperature > 1e6f) return fail(TL_ERR_ARG, "temperature=%g is not a positive number up to 1e6", (double)temperature);
+    if (int rc = check_temperature(temperature)) return rc;
     if (M == 0) return TL_OK;
     if (!ids || !logits || !entries || !shares || !known) return fail(TL_ERR_ARG, "device pointer is null");
     if (ids_ld < top || logits_ld < top) return fail(TL_ERR_SHAPE, "rows of ids or logits are shorter than %d", top);

@@ -1188,7 +1188,7 @@ def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
 def distillation(weight, x, ids, logits, scale=None, *, temperature=1.0, back=None):
     """temperature^2 * KL(teacher || softmax((x @ W) * scale / temperature)) for every row of x [rows, K], float32 [rows], without keeping the student's
     logits.  The teacher is known by its top logits: ids int64 [rows, top] (columns of W, in any order) and logits [rows, top], float16 or float32, top 1
-    to 1024; its probabilities are softmax(logits / temperature) over them.  A logit of -inf names nothing, whatever its id; a repeated id's probabilities
+    to 1024; its probabilities are softmax(logits / temperature) over them (temperature: 1e-6 to 1e6).  A logit of -inf names nothing, whatever its id; a repeated id's probabilities
     add up; a row of -inf alone has loss and gradient 0; one with NaN, +inf or an id that is no column is NaN.  Differentiable as cross_entropy is,
     by the student alone."""
     if back is None or back.blob is weight.blob:
@@ -1202,8 +1202,8 @@ def distillation(weight, x, ids, logits, scale=None, *, temperature=1.0, back=No
     _code(logits.dtype, "logits")
     if (logits.requires_grad and torch.is_grad_enabled()) or (torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(logits).tangent is not None):
         raise RuntimeError("a teacher's logits have no gradient here: detach them")
-    if not 0.0 < float(temperature) <= 1e6:
-        raise ValueError(f"temperature={temperature} is not a positive number up to 1e6")
+    if not 1e-6 <= float(temperature) <= 1e6:
+        raise ValueError(f"temperature={temperature} is no number from 1e-6 to 1e6")
     if not 1 <= ids.shape[1] <= 1024:
         raise ValueError(f"a teacher has 1 to 1024 entries to a row, not {ids.shape[1]}")
     _cuda(x, "x")

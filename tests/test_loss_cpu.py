@@ -141,3 +141,15 @@ def test_rows_of_all_bits_would_show_a_part_that_is_lost(M, K, N):
     for parts in (1, 2):
         less = losses.Reference(losses.leading_parts(x, parts), w, s, *losses.targets(t, N), grad=g)
         assert ((less.loss - ref.loss).abs() > 2 * ref.loss_bound()).any() and ((less.ds - ref.ds).abs() > 2 * ds_bound).any()
+
+
+@pytest.mark.parametrize("temperature", [1e-7, 1e-20, 1e-39, 1e-45, 2e6, float("inf")])
+def test_temperatures_whose_reciprocal_or_square_fp32_does_not_hold(temperature):
+    w, x, _, s = operands()
+    ids, logits = torch.zeros((3, 5), dtype=torch.int64), torch.zeros((3, 5))
+    with pytest.raises(ValueError, match="temperature"):
+        ops.distillation(w, x, ids, logits, s, temperature=temperature)
+    at, size = ctypes.c_void_p(256), ctypes.c_int64(0)
+    t = target(targets=None, entries=at, shares=at, known=at, top=4, temperature=temperature)
+    assert _lib.lib().tl_head_loss_workspace(w.header, 10, _lib.TL_F16, t, 0, size) == -1
+    assert _lib.lib().tl_teacher_entries(256, 4, 256, _lib.TL_F32, 4, 3, 4, 100, temperature, 256, 256, 256, None) == -1
