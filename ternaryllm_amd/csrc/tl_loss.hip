@@ -83,10 +83,10 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
     const bool none = top == kNone;
     float sum = 0.f;
     for (int i = lane; i < a.top; i += 64) {
-        const float e = none ? 0.f : expf(logit(i) - top);
+        const float v = logit(i), e = none ? 0.f : expf(v - top);
         const long long id = from[i];
         const bool outside = id < 0 || id >= a.N;
-        wrong |= e > 0.f && outside;
+        wrong |= v > kNone && outside;           // (however little its probability)
         ids[i] = e > 0.f && !outside ? (int)id : -1;
         shares[i] = e;
         sum += e;

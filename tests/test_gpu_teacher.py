@@ -29,3 +29,18 @@ def test_temperatures_far_from_one(M, K, N, dtype, heat):
     scales, most, bound = scales.cpu().double(), torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4), ref.gradient_bounds()[1]
     past = (scales.abs() == math.inf) & (scales.sign() == ref.ds.sign()) & (ref.ds.abs() + bound >= most)
     assert (past | ((scales - ref.ds).abs() <= bound + torch.finfo(dtype).eps / 2 * ref.ds.abs() + 2.0 ** -25)).all()
+
+
+@pytest.mark.parametrize("M", [6, 70])
+def test_an_unlikely_entry_that_is_no_column(M):
+    """Its probability is 0 in fp32, and the row has no loss all the same; an entry of -inf may have any id."""
+    w, s = losses.head(64, 200, torch.float16)
+    weight = device_weight(w)
+    back = ops.BackWeight(weight)
+    x = losses.rows(M, 64, torch.float16).cuda().requires_grad_()
+    ids, logits = torch.randint(0, 200, (M, 4), generator=torch.Generator().manual_seed(1)), torch.randn((M, 4), generator=torch.Generator().manual_seed(2))
+    for row, (number, logit) in enumerate([(200, -1000.0), (-1, -200.0), (1 << 40, -3e38), (-5, -math.inf), (7, -1000.0)]):
+        ids[row, 2], logits[row, 2] = number, logit
+    loss = ops.distillation(weight, x, ids.cuda(), logits.cuda(), s.cuda(), back=back)
+    gx, = torch.autograd.grad(loss.sum(), x)
+    assert loss[:3].isnan().all() and gx[:3].isnan().all() and loss[3:].isfinite().all() and gx[3:].isfinite().all()
