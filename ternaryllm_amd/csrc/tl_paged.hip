@@ -42,6 +42,7 @@ struct PagedAttn {
     int fixed;                                   // cost of a unit beside its keys
     int least;                                   // cost of a workgroup's part, 1 or more
     int uncut;                                   // units go to one workgroup whole
+    int workgroups, rows;                        // of the launch, of a unit
     float* pieces;                               // [workgroups][2][rows][head_dim + 4]
     Shared* shared;                              // [workgroups]
     // groups of sequences that begin alike (kPrefix, kOwn)
@@ -50,7 +51,6 @@ struct PagedAttn {
     float* firsts;                               // [tokens][heads][head_dim + 4]: of every row the piece of the workgroup in which its unit begins; pieces then
                                                  // are [workgroups][rows][head_dim + 4], of units that began before
     int2* ends;                                  // of every unit the workgroups in which it begins and ends
-    int workgroups, rows;                        // of the launch, of a unit
 };
 
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -788,8 +788,9 @@ __device__ __forceinline__ void tl_paged_rows(const PagedAttn& a, int block, int
             }
             behind(may_mix, t);
         };
-        // (the loop at the beginning of a line of the instruction cache: 4096 rows over 4096 take 418 us so, 425 where it begins somewhere inside one)
-        asm volatile(".p2align 6");
+        // (Where the loop stands among the 32 bytes that are fetched at a time: 4096 rows over 4096 take 409 us with its first instruction 8 bytes behind their
+        // beginning, as here, 415 at it, 417 16 bytes behind, 420 24, and 425 4 bytes beside any of those but the first.)
+        asm volatile(".p2align 6\n\ts_nop 0\n\ts_nop 0");
         int t = first_tile;
         for (; t < min(seen_tiles, first_mixed - 1) && !far; ++t) work(std::false_type{}, t);   // (nor is the next one mixed)
         for (; t < seen_tiles; ++t) work(std::true_type{}, t);
@@ -1068,10 +1069,10 @@ __global__ __launch_bounds__(256, HD == 256 && ROWS == 16 ? 1 : 2) void tl_paged
 {
     if constexpr (ROWS == 16) {
         __shared__ __align__(16) unsigned char lds[kFewLds<HD>];
-        tl_paged_few<HD, BYTES, SET>(a, (int)blockIdx.x, (int)gridDim.x, lds);
+        tl_paged_few<HD, BYTES, SET>(a, (int)blockIdx.x, a.workgroups, lds);
     } else {
         __shared__ __align__(16) unsigned char lds[kRowsLdsOf<HD>];
-        tl_paged_rows<HD, ROWS / 64, BYTES, SET>(a, (int)blockIdx.x, (int)gridDim.x, lds);
+        tl_paged_rows<HD, ROWS / 64, BYTES, SET>(a, (int)blockIdx.x, a.workgroups, lds);
     }
 }
 
@@ -1099,6 +1100,8 @@ __global__ __launch_bounds__(256, 2) void tl_paged_both(PagedAttn a, PagedAttn b
 // groups of lanes, which share the pieces out.
 template <int ROWS>
 constexpr int kJoinThreads = ROWS > 16 ? 512 : 256;
+constexpr int kJoinParts = 8;                    // workgroups that share out a unit's rows.  (Not read from the grid, which stands behind all of PagedAttn, in a
+                                                 // line of its own and a trip to memory more: 0.4 us of 14.9.)
 
 template <int HD, int ROWS>
 __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
@@ -1149,7 +1152,7 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
         *reinterpret_cast<uint2*>(a.out + ((long long)(w.s.start + x.token) * a.heads + x.head) * HD + lane * 4) = *reinterpret_cast<const uint2*>(h);
     };
     if (count <= FEW) {
-        for (int r = (int)blockIdx.y * AT_ONCE + own; r < ROWS; r += (int)gridDim.y * AT_ONCE) {
+        for (int r = (int)blockIdx.y * AT_ONCE + own; r < ROWS; r += kJoinParts * AT_ONCE) {
             const Row x = row_of(a, w, u, r);
             if (!x.there) continue;
             start();
@@ -1158,7 +1161,7 @@ __global__ __launch_bounds__(kJoinThreads<ROWS>) void tl_paged_join(PagedAttn a)
         }
         return;
     }
-    for (int r = (int)blockIdx.y; r < ROWS; r += (int)gridDim.y) {
+    for (int r = (int)blockIdx.y; r < ROWS; r += kJoinParts) {
         const Row x = row_of(a, w, u, r);
         if (!x.there) continue;                                   // (the same for all)
         start();
@@ -1322,7 +1325,7 @@ int check_heads(int heads, const tl_pages* pages)
 template <int HD, int ROWS>
 void launch_join(const PagedAttn& a, const Plan& p, hipStream_t st)
 {
-    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, 8), dim3(kJoinThreads<ROWS>), 0, st, a);
+    if (!p.uncut) hipLaunchKernelGGL((tl_paged_join<HD, ROWS>), dim3((unsigned)p.workgroups, kJoinParts), dim3(kJoinThreads<ROWS>), 0, st, a);
 }
 
 template <int HD, bool BYTES, Keys SET>
