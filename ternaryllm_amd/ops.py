@@ -646,7 +646,8 @@ class PagePrefix(NamedTuple):
     """Sequences of a batch that begin with the same tokens, in the same pages.  Group g is the batch's sequences groups[g] .. groups[g + 1] - 1; each of
     them shares its first shared[b] tokens with the others: the same number in all of a group, 0 in sequences of no group, and no more than a sequence
     has in front of its rows.  Both int32 on the device: groups [groups + 1], shared [seqs].  most_shared: the most tokens that a group shares, where the host
-    knows (it chooses how they are read, results differ by the rounding of sums)."""
+    knows (it chooses how they are read, results differ by the rounding of sums; None stands for all that the table holds, and a batch that shares little of it may
+    then take a third longer than without groups)."""
     groups: torch.Tensor
     shared: torch.Tensor
     most_shared: Optional[int] = None

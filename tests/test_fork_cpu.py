@@ -1,10 +1,11 @@
 """Sequences of a paged cache that go on from the same tokens, on the host alone: which pages they hold, which are copied, which stand in a group."""
+import ctypes
 import random
 
 import pytest
 import torch
 
-from ternaryllm_amd import PagedCache, ops
+from ternaryllm_amd import PagedCache, _lib, ops
 
 
 def stamp(cache, batch, seq, first, last, value):
@@ -124,3 +125,18 @@ def test_prefixes_that_are_none():
             ops.paged_attention(q, pages, batch, prefix=bad)
     with pytest.raises(RuntimeError, match="GPU"):               # taken, up to the GPU that is not there
         ops.paged_attention(q, pages, batch, prefix=good)
+
+
+@pytest.mark.parametrize("seqs,shared,heads,kv,apart", [
+    (4, 512, 32, 32, True), (64, 8192, 32, 8, True), (64, 600, 32, 8, True), (32, 1400, 32, 8, True), (16, 1400, 32, 8, True),
+    (32, 600, 32, 8, False), (32, 256, 32, 8, False), (2, 512, 32, 8, False), (64, 64, 32, 8, False)])
+def test_shared_tokens_are_read_apart_where_that_takes_less(seqs, shared, heads, kv, apart):
+    """What the two forms took is in the comment of the rule; the workspace shows which is chosen."""
+    at = ctypes.c_void_p(256)
+    pages = _lib.Pages(at, at, None, None, kv * 32 * 128, 32 * 128, 128, 10000, 32, kv, 128, _lib.TL_F16)
+    batch = _lib.PageBatch(at, at, at, shared // 32 + 3, shared // 32 + 3, seqs)
+    prefix = _lib.PagePrefix(at, at, 1, shared)
+    need = [ctypes.c_int64(0), ctypes.c_int64(0)]
+    assert _lib.lib().tl_paged_attention_workspace(seqs, heads, pages, batch, 1, need[0]) == 0
+    assert _lib.lib().tl_paged_attention_shared_workspace(seqs, heads, pages, batch, prefix, 1, need[1]) == 0
+    assert (need[1].value != need[0].value) == apart
