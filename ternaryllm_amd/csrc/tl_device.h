@@ -59,7 +59,7 @@ struct LossRows {
     long long ds_ld;
     const float* sums;           // product of P: null, or the sums of the pieces before, [M][ldy of theirs = N]
     int last;                    // ... the last piece: times what the row is multiplied by
-    int unit0, units;            // ... units of K that the launch multiplies, planes one after the other
+    int unit0, units;            // ... units of K that the launch multiplies, planes one after the other; the image's rows begin with the first
     int splits;                  // ... shared out among workgroups: each its own [M][ldy] of Y
 };
 

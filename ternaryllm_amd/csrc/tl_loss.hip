@@ -671,9 +671,9 @@ int many_backward(const tl_layout_header* h, const void* blob, const void* back,
             beside = a.ds && a.dx && f.splits > 1 && pieces == 1;
             if (a.ds && !beside) hipLaunchKernelGGL(tl_loss_ds, dim3((unsigned)ceil_div(wide, 64)), dim3(256), 0, st, d);
             if (!a.dx) continue;
-            // (rows of P begin with column n, those of the transposed weight with column 0: pointers meet where they would be)
+            // (rows of P begin with column n, a whole unit, those of the transposed weight with column 0)
             b.K = (int)(n + padded);
-            b.image = static_cast<const char*>(f.P) - n * 2, b.image_ld = f.columns, b.image_plane = some.loss.plane;
+            b.image = f.P, b.image_ld = f.columns, b.image_plane = some.loss.plane;
             b.loss.unit0 = (int)(n / TL_CODE_UNIT_ROWS), b.loss.units = planes > 1 ? planes * b.units : (int)ceil_div(wide, TL_CODE_UNIT_ROWS);
             const bool last = f.splits == 1 && piece + 1 == pieces;
             b.loss.sums = f.splits == 1 && piece > 0 ? f.sums : nullptr, b.loss.last = last;

@@ -571,7 +571,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients
     // ---- what this wave copies ----
     // activations: its load i covers rows (i * W + wave) * 8 .. + 7 of the tile; lane -> row lane / 8, place lane % 8
     uint32_t xrow[XL];                                            // byte offset of this lane's row from the tile's base
-    const uint32_t limit = (uint32_t)((a.K + 7) / 8 * 16 - 16);          // last whole piece of a row: pieces past it meet zero weights
+    const uint32_t row_at = MODE == kBack ? (uint32_t)(a.loss.unit0 * TL_CODE_UNIT_ROWS * 2) : 0u;   // what a row of the image begins with, of K's bytes
+    const uint32_t limit = (uint32_t)((a.K + 7) / 8 * 16 - 16) - row_at;          // last whole piece of a row: pieces past it meet zero weights
     const int lane_row = lane >> 3;
 
     const uint32_t piece = (uint32_t)piece_place(wave * 8 + lane_row, lane & 7) * 16;
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients
     auto issue_x = [&](auto turn_tag, auto whole_tag) {
         constexpr int TURN = decltype(turn_tag)::value, STAGE = TURN / PARTS;
         constexpr bool WHOLE = decltype(whole_tag)::value;
-        const uint32_t k_bytes = (uint32_t)(lk * TL_CODE_UNIT_ROWS + STAGE * kStageRows) * 2;
+        const uint32_t k_bytes = (uint32_t)(lk * TL_CODE_UNIT_ROWS + STAGE * kStageRows) * 2 - row_at;
         const unsigned char* src = part_image[TURN % PARTS] + (WHOLE ? k_bytes : 0);
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
