@@ -42,7 +42,6 @@ struct PagedAttn {
     int fixed;                                   // cost of a unit beside its keys
     int least;                                   // cost of a workgroup's part, 1 or more
     int uncut;                                   // units go to one workgroup whole
-    int workgroups, rows;                        // of the launch, of a unit
     float* pieces;                               // [workgroups][2][rows][head_dim + 4]
     Shared* shared;                              // [workgroups]
     // groups of sequences that begin alike (kPrefix, kOwn)
@@ -51,6 +50,7 @@ struct PagedAttn {
     float* firsts;                               // [tokens][heads][head_dim + 4]: of every row the piece of the workgroup in which its unit begins; pieces then
                                                  // are [workgroups][rows][head_dim + 4], of units that began before
     int2* ends;                                  // of every unit the workgroups in which it begins and ends
+    int workgroups, rows;                        // of the launch, of a unit
 };
 
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -1354,7 +1354,9 @@ void launch_attention(const PagedAttn& a, const Plan& p, hipStream_t st)
     else launch_join<HD, 64>(a, p, st);
 }
 
-constexpr int64_t kRowsOfFourWaves = 1024;
+// Rows of heads, up to which four waves join one's pieces, which are many where rows are few.  (us a call with four / one: 128 rows over 512 keys 17.7 / 18.0, 256 over
+// 30000 32.9 / 36.3, over 6000 20.3 / 20.8; 512 over 6000 22.7 / 22.3, 560 over 8000 26.3 / 24.7, 1024 over 6000 29.7 / 28.1, 2048 39.3 / 35.1.)
+constexpr int64_t kRowsOfFourWaves = 256;
 
 template <int HD, bool BYTES>
 void launch_shared(const PagedAttn& a, const Plan& pa, const PagedAttn& b, const Plan& pb, hipStream_t st)
