@@ -244,10 +244,12 @@ __device__ __forceinline__ float finite_sums(const KernelArgs& a, f32x4 (&acc)[F
 
 // The last steps of a head's losses (put_out's arguments; own: LDS of the wave's own, kTeacherRows * teacher_ld floats of it, once every wave of the
 // workgroup is done with its buffers).  A row's logits lie with four lanes; a wave leaves their maximum and sum for its columns.  Its teacher's entries are
-// few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.
+// few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.  (Rows times entries
+// times waves of columns: a step of 2048 rows of 4096 over 32000 columns takes 960 us without a teacher, 990 with 8 entries, 1011 with 32, 1095 with 128, 1722 with
+// 512 and 2490 with 1024.)
 // Measured (fp16, 128 x 256 tiles, whole kernels): 4096 rows of 4096 over 32000 columns, logits 618 to 690 us with the clock (1.56 to 1.74 PFLOP/s; 32000 logits of a row are
-// 500 pairs of 8 bytes), gradients 748 in two launches, the product of P 688; with 32 entries of a teacher 2048 rows' logits take 394, gradients 415, the
-// product 380.  Each kernel is its product: the exponentials (two a logit in all) and what is stored are beside other workgroups' products.
+// 500 pairs of 8 bytes), gradients 740 in two launches, the product of P 672; with 32 entries of a teacher 2048 rows' logits take 394, gradients 406, the
+// product 370; 777 fp32 rows of 1111 over 5003 columns 40, 48 and 32.  Each kernel is its product: the exponentials (two a logit in all) and what is stored are beside other workgroups' products.
 template <int CF, int FW, int F, int G, int MODE, bool F32>
 __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0, unsigned char* own)
 {
@@ -531,10 +533,8 @@ __device__ __forceinline__ void put_out(const KernelArgs& a, f32x4 (&acc)[F][G],
 // share K out by units, copy for themselves, wait for nobody and add up at the end; or, WN > 1, two groups of waves that share K out
 // and whose waves share what they copy.  PARTS: 1 for fp16 activations, 3 for fp32
 // ones in bf16 parts (a stage's three parts one after the other, with the same codes).
-//
-// (Gradients of fp32 logits in 64 x 128 tiles ask for 170 registers, two more than three workgroups a unit have: 777 x 1111 -> 5003 61 us, 47 with three.)
 template <int PARTS, int WM, int WN, int WK, int FM, int FN, int MODE>
-__global__ __launch_bounds__(WM * WN * WK * 64, PARTS == 3 && MODE == kGradients && FN == 1 ? 3 : 2) void tl_matrix_rows(KernelArgs a)
+__global__ __launch_bounds__(WM * WN * WK * 64, 2) void tl_matrix_rows(KernelArgs a)
 {
     constexpr int W = WM * WN;                                    // waves that work on the same rows of K, and share what is copied
     constexpr bool SHARED = W > 1;
