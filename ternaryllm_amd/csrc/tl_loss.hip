@@ -125,8 +125,10 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
     if (lane == 0) a.known[row] = wrong ? __builtin_nanf("") : none ? __builtin_huge_valf() : known;
 }
 
+// The logarithm of a row's sum against its maximum, which differences from the maximum are added to: a large maximum would round most of it away.  NaN: no row
+// has such a maximum.
 template <bool E2>
-__device__ __forceinline__ float lse_of(float top, float sum) { return finite(top) ? top + (E2 ? log2f(sum) : logf(sum)) : __builtin_nanf(""); }
+__device__ __forceinline__ float log_of(float top, float sum) { return finite(top) ? E2 ? log2f(sum) : logf(sum) : __builtin_nanf(""); }
 
 // A row's divergence from sum t (lse - z), by one thread; lse: as it is kept.
 __device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float lse, float gap)
@@ -137,18 +139,18 @@ __device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float
     a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
 }
 
-// A row's loss from its lse and its entries' logits (z(entry), each asked for by one thread of the workgroup; E2: all as exponents of 2), and what the backward
+// A row's loss from its maximum, its sum and its entries' logits (z(entry), each asked for by one thread of the workgroup; E2: all as exponents of 2), and what the backward
 // pass wants of it: lse, NaN where the loss is, -inf for a row that counts for nothing.
 template <int WAVES, bool E2, typename Z>
 __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, float sum, Z z)
 {
     const int tid = (int)threadIdx.x;
-    const float lse = lse_of<E2>(top, sum);
+    const float above = log_of<E2>(top, sum), lse = top + above;
     if (a.targets) {
         if (tid != 0) return;
         const long long target = a.targets[row];
         const bool counts = target != a.ignore, there = target >= 0 && target < a.N;
-        const float loss = !counts ? 0.f : there ? (lse - z((int)target, 0)) * (E2 ? kLn2 : 1.f) : __builtin_nanf("");
+        const float loss = !counts ? 0.f : there ? (top - z((int)target, 0) + above) * (E2 ? kLn2 : 1.f) : __builtin_nanf("");
         a.loss[row] = loss;
         a.lse[row] = !counts ? kNone : there ? lse : __builtin_nanf("");
         return;
@@ -156,7 +158,7 @@ __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, 
     float gap = 0.f;
     for (int i = tid; i < a.top; i += WAVES * 64) {
         const int id = a.entry[(long long)row * a.top + i];
-        if (id >= 0) gap = fmaf(a.share[(long long)row * a.top + i], lse - z(id, i), gap);
+        if (id >= 0) gap = fmaf(a.share[(long long)row * a.top + i], top - z(id, i) + above, gap);
     }
     gap = fold_all<WAVES>(gap, [](float x, float y) { return x + y; });
     if (tid == 0) put_divergence(a, row, lse, gap * (E2 ? kLn2 : 1.f));
@@ -278,8 +280,8 @@ __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const f
     float gap = 0.f;
     for (int i = (int)threadIdx.x; i < count; i += 256) gap += gaps[(long long)blockIdx.x * count + i];
     gap = fold_all<4>(gap, [](float x, float y) { return x + y; });
-    const float lse = lse_of<true>(top, sum);
-    if (threadIdx.x == 0) put_divergence(a, row, lse, (lse - gap) * kLn2);
+    const float above = log_of<true>(top, sum);
+    if (threadIdx.x == 0) put_divergence(a, row, top + above, (top - gap + above) * kLn2);
 }
 
 // ds from its parts, rows one after the other, and from what rows of the call before have left; 64 columns to a workgroup of four waves, which share the parts

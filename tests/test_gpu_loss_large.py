@@ -54,3 +54,24 @@ def test_one_logit_leads(M, K, N, dtype, up, heat):
     dx_bound, ds_bound = ref.gradient_bounds()
     assert ((got[1] - ref.dx).abs() <= dx_bound).all()
     assert ((got[2] - ref.ds).abs() <= ds_bound + losses.U * ref.ds.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("up", [2.0 ** 3, 2.0 ** 14, 2.0 ** 20])
+@pytest.mark.parametrize("M", [3, 60])
+def test_two_logits_share_the_lead(M, up, dtype):
+    """Two columns that are alike, far above all others: half of the probability is each one's, and a row that wants either has lost the logarithm of 2 and no more."""
+    K, N = 64, 500
+    w = losses.head(K, N, F32, M)[0]
+    w[:, 7], w[:, 400] = 1, 1
+    x = losses.rows(M, K, dtype, M).abs() + 1
+    weight, s = device_weight(w), torch.full((N,), up).cuda()
+    t = torch.tensor([7, 400] * M)[:M].cuda()
+    with torch.no_grad():
+        loss = ops.cross_entropy(weight, x.cuda(), t, s).cpu().double()
+        one = ops.distillation(weight, x.cuda(), t[:, None], torch.zeros((M, 1)).cuda(), s).cpu().double()
+    z = (x.double() @ torch.as_tensor(w).double()) * up
+    most = z.topk(3, -1).values
+    assert (most[:, 0] == most[:, 1]).all() and (most[:, 1] - most[:, 2] > 100).all()
+    # (both passes' sums and logits are exact but for the factor that makes exponents of 2 of them, the same for both columns; a logarithm and a product are left)
+    assert ((loss - 0.6931471805599453).abs() <= 8 * losses.U).all() and torch.equal(one, loss)
