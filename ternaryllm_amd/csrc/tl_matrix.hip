@@ -189,8 +189,8 @@ __device__ __forceinline__ bool finite_row(const KernelArgs& a, int m)
 
 // A sum that is not finite is worked out again by the lane that holds it, before anything is stored: the outputs of
 // finite rows keep their bits whatever another row of the tile holds.  (The sums that need it go into a mask that a
-// loop takes bit by bit, so that the walk stands here once and the sums stay in registers.)  put_out's arguments, and the lane's rows whose sums are to be
-// NaN instead, a bit to each; returns what the sums, and all others of the lane, are to be multiplied by.
+// loop takes bit by bit, so that the walk stands here once and the sums stay in registers.)  put_out's arguments, and the lane's
+// rows whose sums are to be NaN instead, a bit to each; returns what the sums, and all others of the lane, are to be multiplied by.
 template <int CF, int FW, int F, int G, int MODE>
 __device__ __forceinline__ float finite_sums(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0, uint32_t spoiled = 0)
 {
@@ -244,12 +244,13 @@ __device__ __forceinline__ float finite_sums(const KernelArgs& a, f32x4 (&acc)[F
 
 // The last steps of a head's losses (put_out's arguments; own: LDS of the wave's own, kTeacherRows * teacher_ld floats of it, once every wave of the
 // workgroup is done with its buffers).  A row's logits lie with four lanes; a wave leaves their maximum and sum for its columns.  Its teacher's entries are
-// few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.  (Rows times entries
-// times waves of columns: a step of 2048 rows of 4096 over 32000 columns takes 960 us without a teacher, 990 with 8 entries, 1011 with 32, 1095 with 128, 1722 with
-// 512 and 2490 with 1024.)
+// few among all columns: a wave looks through all of its rows' and puts those of its own columns into LDS, where they stand as the logits do.  (Rows times
+// entries times waves of columns: a step of 2048 rows of 4096 over 32000 columns takes 960 us without a teacher, 990 with 8 entries, 1011 with 32, 1095 with 128,
+// 1722 with 512 and 2490 with 1024.)
 // Measured (fp16, 128 x 256 tiles, whole kernels): 4096 rows of 4096 over 32000 columns, logits 618 to 690 us with the clock (1.56 to 1.74 PFLOP/s; 32000 logits of a row are
 // 500 pairs of 8 bytes), gradients 740 in two launches, the product of P 672; with 32 entries of a teacher 2048 rows' logits take 394, gradients 406, the
-// product 370; 777 fp32 rows of 1111 over 5003 columns 40, 48 and 32.  Each kernel is its product: the exponentials (two a logit in all) and what is stored are beside other workgroups' products.
+// product 370; 777 fp32 rows of 1111 over 5003 columns 40, 48 and 32.  Each kernel is its product: the exponentials (two a logit in all) and what is stored are
+// beside other workgroups' products.
 template <int CF, int FW, int F, int G, int MODE, bool F32>
 __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G], int lane_m0, int lane_n0, unsigned char* own)
 {
@@ -287,20 +288,20 @@ __device__ __forceinline__ void put_loss(const KernelArgs& a, f32x4 (&acc)[F][G]
         }
         return;
     }
-    // The products are with +-2.  Of fp16 rows only those that are not finite have sums that are not.  Of fp32 rows these are found by the wave together, or by what
-    // the forward pass made of them, and stay as they are: a walk of all of a row's columns is a long way.  (us, a step of 2000 rows of 2048 over 16000 columns:
-    // 918, with a NaN in 20 of them 1104, in all 1507; 20 finite ones that have to be walked take it to 27 ms.)
+    // The products are with +-2.  Of fp16 rows only those that are not finite have sums that are not.  Of fp32 rows these are found by the wave together, or by
+    // what the forward pass made of them, and stay as they are: a walk of all of a row's columns is a long way.  (us, a step of 2000 rows of 2048 over 16000
+    // columns: 918, 4 of them for looking at all sums; with a NaN in 20 rows 1104, in all 1507; 20 finite ones that have to be walked take it to 27 ms.)
     float half = 0.5f;
     if constexpr (F32) {
         uint32_t bad = 0, spoiled = 0;                            // this lane's rows that have such a sum, that are not finite
 #pragma unroll
         for (int m = 0; m < G; ++m) {
-            bool fine = true;
+            float none = 0.f;                                     // (NaN of what is not finite: one instruction to a sum, not two)
 #pragma unroll
             for (int f = 0; f < F; ++f)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[f][m][e]) < __builtin_huge_valf();
-            bad |= !fine && lane_m0 + m * 16 < a.M ? 1u << m : 0u;
+                for (int e = 0; e < 4; ++e) none = fmaf(acc[f][m][e], 0.f, none);
+            bad |= none != 0.f && lane_m0 + m * 16 < a.M ? 1u << m : 0u;
         }
         if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
 #pragma unroll 1
