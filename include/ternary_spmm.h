@@ -728,8 +728,9 @@ int tl_back_codes_make(const tl_layout_header* header, const void* blob_dev, voi
 /* loss[m] = temperature^2 * sum_v t_v (log t_v - log softmax(z_m / temperature)_v): cross entropy where t is one entry.  x is [M][ldx] of x_dtype, row-major.
  *   lse        [M + 1] float: what the backward pass wants of the forward one
  *   workspace  device, 256-byte aligned, of tl_head_loss_workspace bytes at least; calls that share it must not overlap
- * A row with a logit that is NaN or +inf has loss NaN, and any row of x that is not finite may have; it does not reach other rows' (it does reach dscale); one
- * that wants a column whose logit is -inf has an infinite loss.  Logits, as exponents of 2 too, and the products that they are scales times, are fp32 numbers.  The reference has no counterpart: it runs a model's forward pass alone (TernaryLLM/TernaryLlama.py:69-75). */
+ * A row with a logit that is NaN or +inf has loss NaN, and any row of x that is not finite may have; it does not reach other rows' (it does reach dscale);
+ * one that wants a column whose logit is -inf has an infinite loss.  Logits, as exponents of 2 too, and the sums that they are scales times, are fp32.  The
+ * reference has no counterpart: it runs a model's forward pass alone (TernaryLLM/TernaryLlama.py:69-75). */
 int tl_head_loss_workspace(const tl_layout_header* header, int64_t M, int x_dtype, const tl_loss_target* target, int backward, int64_t* bytes);
 int tl_head_loss(const tl_layout_header* header, const void* blob_dev, const void* x, int x_dtype, int64_t ldx, int64_t M, const void* scale, int scale_dtype,
                  const tl_loss_target* target, float* loss, float* lse, void* workspace, int64_t workspace_bytes, void* stream);

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64) void tl_teacher(TeacherArgs a)
 }
 
 // The logarithm of a row's sum against its maximum, which differences from the maximum are added to: a large maximum would round most of it away.  NaN: no row
-// has such a maximum.
+// of finite logits has such a maximum.
 template <bool E2>
 __device__ __forceinline__ float log_of(float top, float sum) { return finite(top) ? E2 ? log2f(sum) : logf(sum) : __builtin_nanf(""); }
 
@@ -139,8 +139,8 @@ __device__ __forceinline__ void put_divergence(const LossArgs& a, int row, float
     a.lse[row] = none ? kNone : known == known ? lse : __builtin_nanf("");
 }
 
-// A row's loss from its maximum, its sum and its entries' logits (z(entry), each asked for by one thread of the workgroup; E2: all as exponents of 2), and what the backward
-// pass wants of it: lse, NaN where the loss is, -inf for a row that counts for nothing.
+// A row's loss from its maximum, its sum and its entries' logits (z(entry), each asked for by one thread of the workgroup; E2: all as exponents of 2), and what
+// the backward pass wants of it: lse, NaN where the loss is, -inf for a row that counts for nothing.
 template <int WAVES, bool E2, typename Z>
 __device__ __forceinline__ void put_loss(const LossArgs& a, int row, float top, float sum, Z z)
 {
@@ -260,7 +260,8 @@ __global__ __launch_bounds__(kRowThreads) void tl_loss_few(LossArgs a)
     put_loss<WAVES, false>(a, row, top, sum, [&](int n, int) { return z(n); });
 }
 
-// Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted, all as exponents of 2.  A workgroup takes a row, one more the scales.
+// Many rows: a product has left maxima and sums of parts of their columns, and the logits that are wanted, all as exponents of 2.  A workgroup takes a row, one
+// more the scales.
 // 5 us for 40 rows of 500 parts, 12 for 4096 (16 MB).
 __global__ __launch_bounds__(kJoinThreads) void tl_loss_join(LossArgs a, const float2* parts, const float* gaps, const float* picks, int count)
 {

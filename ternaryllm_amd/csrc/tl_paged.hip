@@ -1424,12 +1424,12 @@ SharedPlan shared_plan_of(int64_t tokens, int heads, const tl_pages* pages, cons
         p.prefix.workgroups = best * eighth, p.own.workgroups = (8 - best) * eighth;
     }
     // Apart where what need not be read again takes longer than the rows' pieces, which meet in a launch of their own: from 22 MB on, and as much again for every
-    // 2048 rows, where units of the shared keys have up to 64 rows, and from 100 MB on where they have 128, whose launch takes 24 us at least (us apart / not, 32 heads
-    // on 8: 32 rows over 600 (73 MB) 27.9 / 20.6, over 1000 29.4 / 27.0, over 1400 26.4 / 30.9; 64 over 600 27.0 / 29.5; of 418 such shapes, 4 to 256 sequences over 256
-    // to 5000 tokens in both types, 7 take a tenth longer than the better of the two); not where a sequence has rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32
-    // heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024 (29 MB) 19.7 / 18.4; 2 over 8192 (33 MB) 19.4 / 25.2; 4 over 512, 32 heads on 32 (25 MB) 17.1 / 19.0; 8 over 4096
-    // 20.2 / 32.5; 64 over 64 and up to 500 of their own 24.0 / 16.1; 8 groups of 32 over 256 and up to 500 64 / 50; rows of a key head: 8 sequences of 32 26.9 / 29.9,
-    // 16 of 128 43.7 / 40.0, 4 of 2000 144 / 95.)
+    // 2048 rows, where units of the shared keys have up to 64 rows, and from 100 MB on where they have 128, whose launch takes 24 us at least; not where a sequence has
+    // rows enough to fill a unit by itself, or mostly keys of its own.  (us apart / not: 2 rows over 512 shared tokens, 32 heads on 8 (2 MB) 16.1 / 12.8; 8 over 1024
+    // (29 MB) 19.7 / 18.4; 2 over 8192 (33 MB) 19.4 / 25.2; 4 over 512, 32 heads on 32 (25 MB) 17.1 / 19.0; 8 over 4096 20.2 / 32.5; 32 over 600, 32 heads on 8 (73 MB)
+    // 27.9 / 20.6, over 1000 29.4 / 27.0, over 1400 26.4 / 30.9; 64 over 600 27.0 / 29.5; 64 over 64 and up to 500 of their own 24.0 / 16.1; 8 groups of 32 over 256 and
+    // up to 500 64 / 50; rows of a key head: 8 sequences of 32 26.9 / 29.9, 16 of 128 43.7 / 40.0, 4 of 2000 144 / 95.  Of 418 shapes, 4 to 256 sequences over 256 to
+    // 5000 tokens in both types, 7 take a tenth longer than the better of the two.)
     const double again = (double)(batch->seqs - groups) * (double)shared * pages->kv_heads * hd * (pages->dtype == TL_F16 ? 4 : 2);
     const double least = ((p.prefix.rows > 64 ? 100 : 22) << 20) + (double)tokens * heads * ((22 << 20) / 2048);
     p.apart = groups > 0 && tokens > 0 && tokens * heads <= (1 << 23) && again >= least && 2 * shared >= keys && most_rows * group < 128;

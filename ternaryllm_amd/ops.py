@@ -1171,8 +1171,9 @@ def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
     """-log softmax((x @ W) * scale)[row, targets[row]] for every row of x [rows, K], float32 [rows], without keeping the logits [rows, N].  targets: int64
     [rows]; a row whose target is `ignore` has loss and gradient 0, one whose target is no column NaN.  x and scale [N]: float16 or float32.
     Differentiable once by x, with back = BackWeight(weight), and by scale; logits, sums and what is kept are fp32 (a row's logarithm of its sum is: the
-    gradients' probabilities are off by 2^-23 of its largest logit, relative), x's gradient takes the distribution's in x's type.  A row with a logit that is NaN or +inf has loss NaN, one that is not finite may
-    have (which makes the scales' gradient NaN), and no other row has it of it; one that wants a column of logit -inf has an infinite loss."""
+    gradients' probabilities are off by 2^-23 of its largest logit, relative), x's gradient takes the distribution's in x's type.  A row with a logit that
+    is NaN or +inf has loss NaN, one that is not finite may have (which makes the scales' gradient NaN), and no other row has it of it; one that wants a
+    column of logit -inf has an infinite loss."""
     if back is None or back.blob is weight.blob:
         y = _loss(weight, x, scale, back, targets, ignore, None, None, 1.0)
         if torch.is_tensor(y):
@@ -1189,8 +1190,8 @@ def cross_entropy(weight, x, targets, scale=None, *, ignore=-100, back=None):
 def distillation(weight, x, ids, logits, scale=None, *, temperature=1.0, back=None):
     """temperature^2 * KL(teacher || softmax((x @ W) * scale / temperature)) for every row of x [rows, K], float32 [rows], without keeping the student's
     logits.  The teacher is known by its top logits: ids int64 [rows, top] (columns of W, in any order) and logits [rows, top], float16 or float32, top 1
-    to 1024; its probabilities are softmax(logits / temperature) over them (temperature: 1e-6 to 1e6).  A logit of -inf names nothing, whatever its id; a repeated id's probabilities
-    add up; a row of -inf alone has loss and gradient 0; one with NaN, +inf or an id that is no column is NaN.  Differentiable as cross_entropy is,
+    to 1024; its probabilities are softmax(logits / temperature) over them (temperature: 1e-6 to 1e6).  A logit of -inf names nothing, whatever its id; a
+    repeated id's probabilities add up; a row of -inf alone has loss and gradient 0; one with NaN, +inf or an id that is no column is NaN.  Differentiable as cross_entropy is,
     by the student alone."""
     if back is None or back.blob is weight.blob:
         y = _loss(weight, x, scale, back, None, 0, ids, logits, temperature)
